@@ -354,6 +354,92 @@ int wpt_cache_append(const void* src, int64_t src_stride_b, int64_t src_stride_n
                      int64_t dst_stride_n, const int64_t* first, const int64_t* counts, int B, int n, int row_bytes,
                      int64_t capacity, void* stream);
 
+/*
+ * The attention weight that each cached row collects from a pass of queries:
+ *   weights[b, n] += sum over t, h of exp(scale * q[b, t, h] . k[b, n] - lse[b, t, h])
+ * over the queries that read row n: max(0, p - window + 1, floor) <= n <=
+ * min(p, N - 1), p = positions[b, t] (window 0: no window). lse is the
+ * forward pass's (with a sink, the sink is in it; a query that reads no row
+ * has -inf and adds nothing). Rows that no query reads are not touched, and
+ * what they hold (NaN too) reaches no other row. Each row's sum is taken in
+ * a fixed order: repeated calls agree bit for bit.
+ *   q          bf16 (B, T, H, C), contiguous, 16-byte aligned; C 64 or 128
+ *   k          bf16 (B, N, C) at the given strides in elements (multiples of 8)
+ *   positions  int64 (B, T);  floor  int64 (B, T) or NULL
+ *   lse        fp32 (B, T, H);  weights  fp32 (B, N), row stride weights_ld
+ *   scratch    wpt_attn_weights_scratch_bytes(B, T, H, N) bytes, 16-byte
+ *              aligned (none is needed, and NULL taken, up to 256 columns T * H)
+ */
+int wpt_attn_weights(const void* q, const void* k, int64_t k_stride_b, int64_t k_stride_n, const int64_t* positions,
+                     const int64_t* floor, const float* lse, float* weights, int64_t weights_ld, void* scratch, int B,
+                     int T, int H, int C, int N, int window, float scale, void* stream);
+
+/* Bytes of scratch wpt_attn_weights needs (0: none, or a bad shape). */
+size_t wpt_attn_weights_scratch_bytes(int B, int T, int H, int N);
+
+/*
+ * Eviction by accumulated weight. Row b of the cache has lengths[b] live
+ * table rows (clamped to 0 .. N). If they are more than `keep`, it keeps the
+ * first `first`, the last `recent` (first + recent <= keep) and, of the
+ * others, those with the largest weights (equal weights: the lowest row; NaN
+ * ranks as -inf), `keep` in all; otherwise all of them. The kept rows go, in
+ * their order, to the front of the new tables; the places after them are
+ * zeroed.
+ *   held          (B, N, row_bytes) at the given strides in BYTES; row_bytes
+ *                 a multiple of 4, as bases and strides (16: faster)
+ *   weights       fp32 (B, N), row stride weights_ld
+ *   kept          (B, capacity, row_bytes), contiguous; must not overlap held
+ *   kept_weights  fp32 (B, capacity), contiguous
+ *   rows          int64 (B, keep): the kept rows' old places, -1 padded
+ *   counts        int64 (B,): rows kept
+ */
+int wpt_cache_evict(const void* held, int64_t held_stride_b, int64_t held_stride_n, const float* weights,
+                    int64_t weights_ld, const int64_t* lengths, void* kept, float* kept_weights, int64_t* rows,
+                    int64_t* counts, int B, int N, int row_bytes, int keep, int recent, int first, int capacity,
+                    void* stream);
+
+/*
+ * Beam search's selection. Text r has W beams with the running totals
+ * totals[r] and the scores (logits) scores[r, w] over V tokens; the value of
+ * (beam w, token v) is
+ *   totals[r, w] + ((x - m) - log(sum over v of exp(x - m))),  m the beam's
+ *   largest score,
+ * and the K largest win (equal values: the lowest w * V + v), best first. An
+ * ended beam (done) offers one candidate: itself, its total unchanged, with
+ * the token `end`; its scores are not read. A value that is -inf or NaN is
+ * no candidate (so a score of NaN or +inf takes its whole beam out); places
+ * without a candidate get total -inf, parent and token -1.
+ *   scores   fp32, or bf16 when bf16 is 1; (R, W, V), last dimension
+ *            contiguous, the others at strides in elements (any alignment)
+ *   totals   fp32 (R, W);  done  bytes (R, W) or NULL
+ *   scratch  wpt_beam_scratch_bytes(R, W, V, K) bytes, 8-byte aligned
+ *   out_totals fp32, parents and tokens int64: (R, K)
+ * W and K up to 64, W * V under 2^32.
+ */
+int wpt_beam_select(const void* scores, int bf16, int64_t stride_r, int64_t stride_w, const float* totals,
+                    const uint8_t* done, int end, void* scratch, float* out_totals, int64_t* parents, int64_t* tokens,
+                    int R, int W, int V, int K, void* stream);
+
+/* Bytes of scratch wpt_beam_select needs (0 for a bad shape). */
+size_t wpt_beam_scratch_bytes(int R, int W, int V, int K);
+
+/*
+ * Reordering of the beams' cached rows, in place. Table i holds R * W rows of
+ * (capacity[i], row_bytes[i]) bytes, beam w of text r at r * W + w; for every
+ * table, beam w of text r takes the table rows first[r] (0 when first is
+ * NULL) .. lengths[r * W + parent] - 1 of beam parent = parents[r, w] as they
+ * were before the call. A parent of -1, or w itself, leaves the beam as it
+ * is; one of W or above does too and sets the status word's shape bit.
+ *   tables, stride_b, stride_n (bytes), row_bytes, capacity: `count` entries
+ *            on the host, up to 32; all multiples of 4 bytes (16: faster),
+ *            no two places of the tables overlapping
+ *   parents  int64 (R, W);  lengths  int64 (R * W,);  first  int64 (R,) or NULL
+ * W up to 64.
+ */
+int wpt_cache_reorder(void* const* tables, const int64_t* stride_b, const int64_t* stride_n, const int* row_bytes,
+                      const int64_t* capacity, int count, const int64_t* parents, const int64_t* lengths,
+                      const int64_t* first, int R, int W, void* stream);
+
 /* Bytes of scratch wpt_accept needs for R rows of n drafts over V entries
  * (0 for a bad shape). */
 size_t wpt_accept_scratch_bytes(int R, int n, int V);

@@ -17,6 +17,14 @@ makes WPT's exact and sparse layers run on these kernels. It exposes
     tree_attention(q, k, v, cache_len, parents, scale, sink=None) -> (out, lse)
     accept(scores, drafted, q, uniforms, resample, temperature, top_k)
 
+and, for a generation cache between two steps,
+
+    cache_append(held, new, first, counts)
+    attention_weights(q, k, positions, lse, scale, weights)
+    cache_evict(held, weights, lengths, keep)
+    beam_select(scores, totals, beams)
+    cache_reorder(tables, parents, lengths)
+
 with the reference's argument meanings, dtypes, -1 conventions and errors.
 Forward passes run hand-written CUDA kernels (libwpt_b200.so, C ABI in
 include/wpt_attn.h); there is no CPU path and no other backend: a missing
@@ -288,6 +296,61 @@ def cache_append(held, new, first, counts, need=None):
     return ops.cache_append(held, new, first, counts, need)
 
 
+# ------------------------------------------------ eviction from the cache
+
+def attention_weights(q, k, positions, lse, scale, weights=None, window=0, floor=None):
+    """The attention weight that each cached row collects, for eviction by it:
+    adds to weights (B, N) fp32, in place (None: new zeros), the sum over the
+    pass's queries and heads of exp(scale q.k - lse), the softmax weights of
+    the rows each query reads. q (B, T, H, c) at positions (T,) or (B, T), k
+    (B, N, c) the cache's keys, lse (B, T, H) as forward_with_lse returns it
+    for the same rows (a sink's share is then in lse and goes to no row);
+    window and floor as there. Returns weights. Not differentiable."""
+    _bf16_only(q, k)
+    if weights is None:
+        weights = torch.zeros(q.shape[0], k.shape[1], dtype=torch.float32, device=q.device)
+    return ops.attention_weights(q, k, _positions(positions, q.shape[0]), lse, scale, weights, window, floor)
+
+
+def cache_evict(held, weights, lengths, keep, recent=0, first=0, capacity=None):
+    """Cuts the generation cache to a budget of `keep` rows a text by their
+    accumulated attention weight (attention_weights): of held (B, N, ...),
+    with lengths (B,) live rows, each text keeps its first `first` and last
+    `recent` rows and, of the others, those with the largest weights (B, N)
+    (equal weights: the lowest row; NaN as -inf), in their order. Returns new
+    tables with room for `capacity` rows (default `keep`), zeros after the
+    kept ones: (held (B, capacity, ...), weights (B, capacity), rows (B, keep)
+    int64, the kept rows' old places, -1 padded, counts (B,) int64). A text
+    with no more than `keep` rows keeps them all. Nothing is read back to the
+    host."""
+    return ops.cache_evict(held, weights, lengths, keep, recent, first, capacity)
+
+
+# -------------------------------------------------------------- beam search
+
+def beam_select(scores, totals, beams, done=None, end=None):
+    """One step of beam search over R texts of W beams: the `beams` best of
+    totals (R, W) + log_softmax(scores (R, W, V)) of each text, best first
+    (equal values: the lowest beam, then the lowest token). scores fp32 or
+    bf16 (head_scores' output viewed as (R, W, V)), up to 64 beams in and out.
+    A beam in done (R, W) has ended: it offers itself alone, its total
+    unchanged, with the token `end` (so `tokens == end` is the next done).
+    Returns (totals (R, beams) fp32, parents (R, beams) int64, tokens
+    (R, beams) int64), -inf and -1 where there are fewer candidates."""
+    return ops.beam_select(scores, totals, beams, done, end)
+
+
+def cache_reorder(tables, parents, lengths, first=None):
+    """Makes each beam's cached rows its parent's, in place: for every table
+    (R * W, N, ...) of the list `tables` (or the one), beam w of text r takes
+    the rows first[r] (default 0) .. lengths[r * W + p] - 1 of beam p =
+    parents[r, w] (R, W), as beam_select returns them; a parent of -1 leaves
+    the beam as it is. first: the rows before it are the same in all beams of
+    a text (its prompt) and are not moved. Tables of any shape and dtype
+    (accumulated weights (R * W, N) too). Returns `tables`."""
+    return ops.cache_reorder(tables, parents, lengths, first)
+
+
 # ------------------------------------------------------------- installation
 
 def install(kernels, attention=None, device=None, check=True):
@@ -317,6 +380,7 @@ def install(kernels, attention=None, device=None, check=True):
     return me
 
 
-__all__ = ["install", "drafter_attention", "cache_append", "sample", "accept", "NAME", "WINDOW", "chosen_columns", "exact_attention", "sparse_attention", "window_attention",
-           "tree_attention",
+__all__ = ["install", "drafter_attention", "cache_append", "attention_weights", "cache_evict", "beam_select",
+           "cache_reorder", "sample", "accept", "NAME",
+           "WINDOW", "chosen_columns", "exact_attention", "sparse_attention", "window_attention", "tree_attention",
            "forward_with_lse", "device_status", "LibraryMissing"]

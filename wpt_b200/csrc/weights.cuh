@@ -1,0 +1,718 @@
+// The attention weight that each cached row collects: for a pass of queries
+// q (B, T, H, C) over keys k (B, N, C) with the forward pass's log-sum-exp,
+//
+//   weights[b, n] += sum over t, h of exp(scale q_bth . k_bn - lse_bth)
+//
+// over the queries that read row n (max(0, p - window + 1, floor) <= n <=
+// min(p, N - 1), p the query's position). With lse known there is no running
+// maximum: a key's weight is a plain sum over the (query, head) columns, so
+// the keys are the product's M (S^T = K Q^T), thread r owns key r and no sum
+// crosses threads. Every key's columns are summed in a fixed order, so
+// repeated calls agree bit for bit.
+//
+// weights_stream_kernel (T * H up to 256 columns, one decode step): the
+// queries stay in shared memory and the keys stream through it. The rows'
+// live key tiles are laid end to end and cut into one equal range a CTA, so
+// rows of any lengths keep the SMs equally busy. Bound: HBM (2 C bytes a key).
+//
+// weights_tile_kernel (more columns, a prompt): 256 keys stay in shared
+// memory and the queries stream past them, 128 columns at a time, S^T
+// double-buffered in TMEM for each 128 keys. Items of (256 keys, a run of
+// column tiles) are handed out by an atomic ticket; where a key's columns
+// are cut into several runs, their sums go to scratch and
+// weights_reduce_kernel adds them in order. Bound: the exponentials (16 a
+// clock an SM against 32 columns' products of 128 terms).
+#pragma once
+
+#include <climits>
+
+#include "common.cuh"
+
+namespace wpt {
+
+// The rows [lo, hi] that the query at `pos` reads; hi < lo for none.
+__device__ __forceinline__ int2 weights_range(int64_t pos, const int64_t* floor, int64_t at, int window, int N) {
+  int64_t hi = pos < N - 1 ? pos : N - 1;
+  int64_t lo = window > 0 ? pos - window + 1 : 0;
+  if (floor != nullptr && floor[at] > lo) lo = floor[at];
+  if (lo < 0) lo = 0;
+  if (hi < lo) return make_int2(INT_MAX, -1);
+  return make_int2(static_cast<int>(lo), static_cast<int>(hi));
+}
+
+// The exponent's constant of a column: exp(x - lse) = 2^(x log2e + this). A
+// query without rows has lse -inf; it adds nothing.
+__device__ __forceinline__ float weights_offset(float lse) { return lse == -INFINITY ? -INFINITY : -lse * LOG2E; }
+
+// ------------------------------------------------------------- key stream
+
+constexpr int WEIGHTS_BAL_ROWS = 1024;  // most batch rows whose tiles are laid end to end
+constexpr int WEIGHTS_STREAM_THREADS = 192;  // warps 0-3 epilogue, 4 MMA, 5 loader
+
+struct WeightsParams {
+  const int64_t* positions;  // (B, T)
+  const int64_t* floor;      // (B, T) or NULL
+  const float* lse;          // (B, T, H)
+  float* weights;            // (B, N), row stride weights_ld
+  int64_t weights_ld;
+  unsigned* status;
+  int B, T, H, N, window;
+  float scale_log2;  // scale * log2(e)
+};
+
+template <int C, int NCOL, int STAGES>
+struct WeightsStreamLayout {
+  static constexpr int Q_BYTES = NCOL * C * 2, K_BYTES = 128 * C * 2;
+  static constexpr int OFF_Q = 0;  // two buffers
+  static constexpr int OFF_K = 2 * Q_BYTES;
+  static constexpr int OFF_COL = OFF_K + STAGES * K_BYTES;  // float offset, int lo, int hi of each column
+  static constexpr int OFF_PRE = OFF_COL + NCOL * 12;
+  static constexpr int OFF_FIRST = OFF_PRE + (WEIGHTS_BAL_ROWS + 2) * 4;
+  static constexpr int OFF_BAR = OFF_FIRST + WEIGHTS_BAL_ROWS * 4;
+  // q_full[2], q_empty[2], s_full[2], s_free[2], drained, k_full[STAGES], k_empty[STAGES]
+  static constexpr int NBAR = 9 + 2 * STAGES;
+  static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
+  static constexpr int BYTES = OFF_MISC + 64 + 1024;
+  static constexpr int TMEM_COLS = 2 * NCOL <= 32 ? 32 : 2 * NCOL;
+};
+
+// The key tiles [first, first + n) that batch row b's queries read.
+__device__ __forceinline__ int2 weights_row_tiles(const WeightsParams& p, int b) {
+  int lo = INT_MAX, hi = -1;
+  for (int t = 0; t < p.T; ++t) {
+    const int64_t at = static_cast<int64_t>(b) * p.T + t;
+    const int2 r = weights_range(p.positions[at], p.floor, at, p.window, p.N);
+    lo = min(lo, r.x);
+    hi = max(hi, r.y);
+  }
+  return hi < lo ? make_int2(0, 0) : make_int2(lo / 128, hi / 128 - lo / 128 + 1);
+}
+
+// A role's walk over its CTA's work: segments of (batch row, key tiles).
+struct WeightsWalk {
+  int b, tile0, ntiles;
+  const int *pre, *first;  // balanced: live tiles of the rows before each row, and each row's first
+  int64_t lo, hi;          // balanced: the CTA's range of the tiles laid end to end
+  bool balanced;
+  int next;
+
+  __device__ __forceinline__ void start(const WeightsParams& p, const int* s_pre, const int* s_first) {
+    pre = s_pre;
+    first = s_first;
+    balanced = p.B <= WEIGHTS_BAL_ROWS;
+    if (balanced) {
+      const int64_t total = pre[p.B];
+      lo = total * blockIdx.x / gridDim.x;
+      hi = total * (blockIdx.x + 1) / gridDim.x;
+      // the first row that ends after lo
+      int a = 0, z = p.B;
+      while (a < z) {
+        const int m = (a + z) >> 1;
+        if (pre[m + 1] > lo)
+          z = m;
+        else
+          a = m + 1;
+      }
+      next = a;
+    } else {
+      next = blockIdx.x;
+    }
+  }
+  __device__ __forceinline__ bool step(const WeightsParams& p) {
+    if (balanced) {
+      while (next < p.B && pre[next + 1] == pre[next]) ++next;
+      if (next >= p.B || pre[next] >= hi || lo >= hi) return false;
+      b = next++;
+      const int64_t a = max(lo, static_cast<int64_t>(pre[b])), z = min(hi, static_cast<int64_t>(pre[b + 1]));
+      tile0 = first[b] + static_cast<int>(a - pre[b]);
+      ntiles = static_cast<int>(z - a);
+      return true;
+    }
+    for (; next < p.B; next += gridDim.x) {
+      const int2 t = weights_row_tiles(p, next);
+      if (t.y > 0) {
+        b = next;
+        tile0 = t.x;
+        ntiles = t.y;
+        next += gridDim.x;
+        return true;
+      }
+    }
+    return false;
+  }
+};
+
+template <int C, int NCOL, int STAGES>
+__global__ void __launch_bounds__(WEIGHTS_STREAM_THREADS, 1)
+    weights_stream_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                          const WeightsParams p) {
+  using L = WeightsStreamLayout<C, NCOL, STAGES>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* s_off = reinterpret_cast<float*>(smem + L::OFF_COL);
+  int* s_lo = reinterpret_cast<int*>(smem + L::OFF_COL + NCOL * 4);
+  int* s_hi = reinterpret_cast<int*>(smem + L::OFF_COL + NCOL * 8);
+  int* s_pre = reinterpret_cast<int*>(smem + L::OFF_PRE);
+  int* s_first = reinterpret_cast<int*>(smem + L::OFF_FIRST);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
+  uint64_t* q_full = bars;
+  uint64_t* q_empty = bars + 2;
+  uint64_t* s_full = bars + 4;
+  uint64_t* s_free = bars + 6;
+  uint64_t* drained = bars + 8;
+  uint64_t* k_full = bars + 9;
+  uint64_t* k_empty = k_full + STAGES;
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC);
+  int* s_scan = reinterpret_cast<int*>(smem + L::OFF_MISC + 16);  // 6 warp totals
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    mbar_init(drained, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(q_full + i, 1);
+      mbar_init(q_empty + i, 1);
+      mbar_init(s_full + i, 1);
+      mbar_init(s_free + i, 4);
+    }
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(k_full + s, 1);
+      mbar_init(k_empty + s, 1);
+    }
+    fence_mbar_init();
+  }
+  if (warp == 4) {
+    tmem_alloc(s_tmem, L::TMEM_COLS);
+    tmem_relinquish();
+  }
+  if (warp == 5 && lane == 0) {
+    tma_prefetch(&tm_q);
+    tma_prefetch(&tm_k);
+  }
+  griddep_wait();
+  if (p.B <= WEIGHTS_BAL_ROWS) {
+    // live tiles of the rows before each row
+    const int per = (p.B + WEIGHTS_STREAM_THREADS - 1) / WEIGHTS_STREAM_THREADS;
+    const int b0 = min(p.B, static_cast<int>(threadIdx.x) * per), b1 = min(p.B, b0 + per);
+    int sum = 0;
+    for (int b = b0; b < b1; ++b) {
+      const int2 tiles = weights_row_tiles(p, b);
+      s_first[b] = tiles.x;
+      s_pre[b + 1] = tiles.y;
+      sum += tiles.y;
+    }
+    int incl = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
+    }
+    if (lane == 31) s_scan[warp] = incl;
+    __syncthreads();
+    int at = incl - sum;
+    for (int w = 0; w < warp; ++w) at += s_scan[w];
+    for (int b = b0; b < b1; ++b) {
+      at += s_pre[b + 1];
+      s_pre[b + 1] = at;
+    }
+    if (threadIdx.x == 0) s_pre[0] = 0;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *s_tmem;
+  WeightsWalk walk;
+  walk.start(p, s_pre, s_first);
+
+  if (warp == 5) {
+    if (lane == 0) {
+      bool ok = true;
+      int j = 0;
+      for (int seg = 0; ok && walk.step(p); ++seg) {
+        uint8_t* sQ = smem + L::OFF_Q + (seg & 1) * L::Q_BYTES;
+        if (seg >= 2 && !(ok = mbar_wait(q_empty + (seg & 1), ((seg >> 1) & 1) ^ 1, p.status))) break;
+        mbar_expect_tx(q_full + (seg & 1), L::Q_BYTES);
+#pragma unroll
+        for (int c = 0; c < C / 64; ++c)
+          tma_load_3d(sQ + c * NCOL * 128, &tm_q, q_full + (seg & 1), c * 64, 0, walk.b);
+        for (int jj = 0; jj < walk.ntiles; ++jj, ++j) {
+          const int st = j % STAGES;
+          if (j >= STAGES && !(ok = mbar_wait(k_empty + st, ((j / STAGES) & 1) ^ 1, p.status))) break;
+          uint8_t* sK = smem + L::OFF_K + st * L::K_BYTES;
+          mbar_expect_tx(k_full + st, L::K_BYTES);
+#pragma unroll
+          for (int c = 0; c < C / 64; ++c)
+            tma_load_3d(sK + c * 128 * 128, &tm_k, k_full + st, c * 64, (walk.tile0 + jj) * 128, walk.b);
+        }
+      }
+      // after a wait that ran out: the copies in flight land before the block leaves
+      for (int st = 0; !ok && st < STAGES && st < j; ++st)
+        mbar_wait(k_full + st, ((j - 1 - st) / STAGES) & 1, p.status);
+    }
+    __syncwarp();
+  } else if (warp == 4) {
+    if (lane == 0) {
+      constexpr uint32_t IDESC = idesc_bf16(128, NCOL, 0, 0);
+      bool ok = true;
+      int j = 0;
+      for (int seg = 0; ok && walk.step(p); ++seg) {
+        const uint32_t q_addr = smem_u32(smem + L::OFF_Q + (seg & 1) * L::Q_BYTES);
+        if (!(ok = mbar_wait(q_full + (seg & 1), (seg >> 1) & 1, p.status))) break;
+        for (int jj = 0; jj < walk.ntiles; ++jj, ++j) {
+          const int st = j % STAGES, buf = j & 1;
+          if (!(ok = mbar_wait(k_full + st, (j / STAGES) & 1, p.status))) break;
+          if (j >= 2 && !(ok = mbar_wait(s_free + buf, ((j >> 1) & 1) ^ 1, p.status))) break;
+          tc_fence_after();
+          const uint32_t k_addr = smem_u32(smem + L::OFF_K + st * L::K_BYTES);
+#pragma unroll
+          for (int kk = 0; kk < C / 16; ++kk)
+            mma_ss(tmem + buf * NCOL, sdesc_sw128(k_addr + (kk >> 2) * (128 * 128) + (kk & 3) * 32, 16, 1024),
+                   sdesc_sw128(q_addr + (kk >> 2) * (NCOL * 128) + (kk & 3) * 32, 16, 1024), IDESC, kk > 0 ? 1u : 0u);
+          mma_commit(k_empty + st);
+          mma_commit(s_full + buf);
+        }
+        if (ok) mma_commit(q_empty + (seg & 1));
+      }
+      mma_commit(drained);  // TMEM is freed with no product in flight
+      mbar_wait(drained, 0, p.status);
+    }
+    __syncwarp();
+  } else {
+    const int r = threadIdx.x;
+    const uint32_t lane_addr = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+    bool ok = true;
+    int j = 0;
+    while (walk.step(p)) {
+      const int b = walk.b;
+      // the previous segment's columns were read; a wait that ran out stops all four warps
+      if (!named_barrier_and(1, 128, ok)) break;
+      for (int c = r; c < NCOL; c += 128) {
+        const int t = c / p.H;
+        float off = -INFINITY;  // a padding column adds nothing
+        int2 range = make_int2(0, INT_MAX);
+        if (t < p.T) {
+          const int64_t at = static_cast<int64_t>(b) * p.T + t;
+          range = weights_range(p.positions[at], p.floor, at, p.window, p.N);
+          off = weights_offset(p.lse[at * p.H + (c - t * p.H)]);
+        }
+        s_off[c] = off;
+        s_lo[c] = range.x;
+        s_hi[c] = range.y;
+      }
+      named_barrier(1, 128);
+      // rows that every column reads, and that any does
+      int all_lo = 0, all_hi = INT_MAX, any_lo = INT_MAX, any_hi = -1;
+      for (int c = 0; c < p.T * p.H; c += p.H) {
+        all_lo = max(all_lo, s_lo[c]);
+        all_hi = min(all_hi, s_hi[c]);
+        any_lo = min(any_lo, s_lo[c]);
+        any_hi = max(any_hi, s_hi[c]);
+      }
+      for (int jj = 0; jj < walk.ntiles; ++jj, ++j) {
+        const int n0 = (walk.tile0 + jj) * 128, n = n0 + r, buf = j & 1;
+        const bool mine = n >= any_lo && n <= any_hi;
+        float* to = p.weights + static_cast<int64_t>(b) * p.weights_ld + n;
+        const float before = mine ? *to : 0.f;
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(s_full + buf, (j >> 1) & 1, p.status)))) break;
+        tc_fence_after();
+        const bool whole = n0 >= all_lo && n0 + 127 <= all_hi;
+        float sum = 0.f;
+#pragma unroll
+        for (int c0 = 0; c0 < NCOL; c0 += 32) {
+          constexpr int W = NCOL < 32 ? NCOL : 32;
+          uint32_t x[W];
+          if constexpr (W == 32)
+            tmem_ld32(lane_addr + buf * NCOL + c0, x);
+          else
+            tmem_ld16(lane_addr + buf * NCOL + c0, x);
+          float part[4] = {0.f, 0.f, 0.f, 0.f};
+          if (whole) {
+#pragma unroll
+            for (int c = 0; c < W; ++c)
+              part[c & 3] += fast_exp2(fmaf(__uint_as_float(x[c]), p.scale_log2, s_off[c0 + c]));
+          } else {
+#pragma unroll
+            for (int c = 0; c < W; ++c) {
+              const float e = fast_exp2(fmaf(__uint_as_float(x[c]), p.scale_log2, s_off[c0 + c]));
+              part[c & 3] += n >= s_lo[c0 + c] && n <= s_hi[c0 + c] ? e : 0.f;
+            }
+          }
+          sum += (part[0] + part[1]) + (part[2] + part[3]);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(s_free + buf);
+        if (mine) *to = before + sum;
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 4) {
+    tc_fence_after();
+    tmem_dealloc(tmem, L::TMEM_COLS);
+  }
+}
+
+// ------------------------------------------------------------ query stream
+
+constexpr int WEIGHTS_TILE_THREADS = 320;  // warps 0-7 epilogue, 8 MMA, 9 loader
+constexpr int WEIGHTS_TILE_KEYS = 256;
+constexpr int WEIGHTS_TILE_COLS = 128;
+
+struct WeightsTileParams {
+  float* weights;      // (B, N), row stride weights_ld
+  int64_t weights_ld;
+  const int4* meta;    // (B, tiles): lowest and highest row any column reads, then that all of them read
+  const float* offset; // (B, tiles, 128): each column's exponent constant
+  const int2* range;   // (B, tiles, 128): each column's rows
+  float* partial;      // (chunks, B, N) when chunks > 1
+  unsigned* ticket;
+  unsigned* status;
+  int B, N, tiles, key_blocks, chunks, chunk_tiles, items;
+  float scale_log2;
+};
+
+// One CTA a column tile: its columns' constants and rows, and the tile's.
+__global__ void __launch_bounds__(WEIGHTS_TILE_COLS)
+    weights_prep_kernel(const WeightsParams p, int tiles, int4* meta, float* offset, int2* range, unsigned* ticket) {
+  __shared__ int s_red[4][4];
+  const int b = blockIdx.x / tiles, tile = blockIdx.x - b * tiles;
+  griddep_wait();
+  if (blockIdx.x == 0 && threadIdx.x == 0) *ticket = 0;
+  const int64_t c = static_cast<int64_t>(tile) * WEIGHTS_TILE_COLS + threadIdx.x;
+  const int t = static_cast<int>(c / p.H);
+  float off = -INFINITY;
+  int2 r = make_int2(INT_MAX, -1);
+  int4 m = make_int4(INT_MAX, -1, 0, INT_MAX);  // a column past the last changes nothing
+  if (t < p.T) {
+    const int64_t at = static_cast<int64_t>(b) * p.T + t;
+    r = weights_range(p.positions[at], p.floor, at, p.window, p.N);
+    off = weights_offset(p.lse[at * p.H + (c - static_cast<int64_t>(t) * p.H)]);
+    m = make_int4(r.x, r.y, r.x, r.y);
+  }
+  const int64_t to = (static_cast<int64_t>(b) * tiles + tile) * WEIGHTS_TILE_COLS + threadIdx.x;
+  offset[to] = off;
+  range[to] = r;
+  m.x = __reduce_min_sync(0xffffffffu, m.x);
+  m.y = __reduce_max_sync(0xffffffffu, m.y);
+  m.z = __reduce_max_sync(0xffffffffu, m.z);
+  m.w = __reduce_min_sync(0xffffffffu, m.w);
+  const int warp = threadIdx.x >> 5;
+  if ((threadIdx.x & 31) == 0) {
+    s_red[0][warp] = m.x;
+    s_red[1][warp] = m.y;
+    s_red[2][warp] = m.z;
+    s_red[3][warp] = m.w;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 4; ++w) {
+      m.x = min(m.x, s_red[0][w]);
+      m.y = max(m.y, s_red[1][w]);
+      m.z = max(m.z, s_red[2][w]);
+      m.w = min(m.w, s_red[3][w]);
+    }
+    meta[static_cast<int64_t>(b) * tiles + tile] = m;
+  }
+}
+
+template <int C, int STAGES>
+struct WeightsTileLayout {
+  static constexpr int K_BYTES = WEIGHTS_TILE_KEYS * C * 2;
+  static constexpr int Q_BYTES = WEIGHTS_TILE_COLS * C * 2, OFF_BYTES = WEIGHTS_TILE_COLS * 4;
+  static constexpr int OFF_K = 0;
+  static constexpr int OFF_Q = K_BYTES;
+  static constexpr int OFF_COL = OFF_Q + STAGES * Q_BYTES;
+  static constexpr int OFF_BAR = OFF_COL + STAGES * OFF_BYTES;
+  // k_full, k_empty, item_full[2], item_empty[2], s_full[2][2], s_free[2][2], drained, q_full[STAGES],
+  // q_empty[STAGES]
+  static constexpr int NBAR = 15 + 2 * STAGES;
+  static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
+  static constexpr int BYTES = OFF_MISC + 32 + 1024;
+};
+
+// The column tiles of an item that read any of its keys, found 32 at a time
+// by the warp: step() gives the next one, or -1.
+struct WeightsTiles {
+  const int4* meta;
+  int at, end, n0, n1;
+  unsigned mask;
+  __device__ __forceinline__ void start(const int4* m, int first, int last, int lo, int hi) {
+    meta = m;
+    at = first - 32;
+    end = last;
+    n0 = lo;
+    n1 = hi;
+    mask = 0;
+  }
+  __device__ __forceinline__ int step() {
+    while (mask == 0) {
+      at += 32;
+      if (at >= end) return -1;
+      const int i = at + (threadIdx.x & 31);
+      bool live = false;
+      if (i < end) {
+        const int4 m = meta[i];
+        live = m.x <= n1 && m.y >= n0;
+      }
+      mask = __ballot_sync(0xffffffffu, live);
+    }
+    const int i = __ffs(mask) - 1;
+    mask &= mask - 1;
+    return at + i;
+  }
+};
+
+template <int C, int STAGES>
+__global__ void __launch_bounds__(WEIGHTS_TILE_THREADS, 1)
+    weights_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                        const WeightsTileParams p) {
+  using L = WeightsTileLayout<C, STAGES>;
+  constexpr int KEYS = WEIGHTS_TILE_KEYS, COLS = WEIGHTS_TILE_COLS;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
+  uint64_t* k_full = bars;
+  uint64_t* k_empty = bars + 1;
+  uint64_t* item_full = bars + 2;
+  uint64_t* item_empty = bars + 4;
+  uint64_t* s_full = bars + 6;   // [buffer][key tile]
+  uint64_t* s_free = bars + 10;  // [buffer][key tile]
+  uint64_t* drained = bars + 14;
+  uint64_t* q_full = bars + 15;
+  uint64_t* q_empty = q_full + STAGES;
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC);
+  volatile int* s_item = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 8);  // two slots
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    mbar_init(k_full, 1);
+    mbar_init(k_empty, 1);
+    mbar_init(drained, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(item_full + i, 1);
+      mbar_init(item_empty + i, 9);  // the MMA warp and the eight epilogue warps
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(s_full + i, 1);
+      mbar_init(s_free + i, 4);
+    }
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(q_full + s, 1);
+      mbar_init(q_empty + s, 9);  // the products and the epilogue warps' reads of the constants
+    }
+    fence_mbar_init();
+  }
+  if (warp == 8) {
+    tmem_alloc(s_tmem, 512);
+    tmem_relinquish();
+  }
+  if (warp == 9 && lane == 0) {
+    tma_prefetch(&tm_q);
+    tma_prefetch(&tm_k);
+  }
+  griddep_wait();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *s_tmem;
+
+  // an item: keys [n0, n0 + 256) of row b against column tiles [c0, c1)
+  struct Item {
+    int b, n0, chunk;
+    WeightsTiles tiles;
+  };
+  auto open = [&](int item, Item& it) {
+    const int per = p.B * p.key_blocks;
+    it.chunk = p.chunks - 1 - item / per;  // a causal pass's last columns read the most keys: first
+    const int rest = item % per;
+    it.b = rest % p.B;
+    it.n0 = rest / p.B * KEYS;
+    const int c0 = it.chunk * p.chunk_tiles;
+    it.tiles.start(p.meta + static_cast<int64_t>(it.b) * p.tiles, c0, min(p.tiles, c0 + p.chunk_tiles), it.n0,
+                   it.n0 + KEYS - 1);
+  };
+  auto wait = [&](uint64_t* bar, int parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status)); };
+
+  if (warp == 9) {
+    // ------------------------------------------------------------ loader
+    bool ok = true;
+    int u = 0, k_uses = 0;
+    for (int i = 0; ok; ++i) {
+      int item = 0;
+      if (lane == 0) item = static_cast<int>(atomicAdd(p.ticket, 1u));
+      item = __shfl_sync(0xffffffffu, item, 0);
+      if (item >= p.items) item = -1;
+      if (i >= 2 && !(ok = wait(item_empty + (i & 1), ((i >> 1) & 1) ^ 1))) break;
+      if (lane == 0) {
+        s_item[i & 1] = item;
+        mbar_arrive(item_full + (i & 1));
+      }
+      if (item < 0) break;
+      Item it;
+      open(item, it);
+      bool first = true;
+      for (int ct = it.tiles.step(); ok && ct >= 0; ct = it.tiles.step(), ++u) {
+        if (first) {
+          first = false;
+          if (k_uses > 0 && !(ok = wait(k_empty, (k_uses - 1) & 1))) break;
+          ++k_uses;
+          if (lane == 0) {
+            mbar_expect_tx(k_full, L::K_BYTES);
+#pragma unroll
+            for (int g = 0; g < 2; ++g)
+#pragma unroll
+              for (int c = 0; c < C / 64; ++c)
+                tma_load_3d(smem + L::OFF_K + (g * (C / 64) + c) * 128 * 128, &tm_k, k_full, c * 64, it.n0 + g * 128,
+                            it.b);
+          }
+        }
+        const int st = u % STAGES;
+        if (u >= STAGES && !(ok = wait(q_empty + st, ((u / STAGES) & 1) ^ 1))) break;
+        if (lane == 0) {
+          mbar_expect_tx(q_full + st, L::Q_BYTES + L::OFF_BYTES);
+#pragma unroll
+          for (int c = 0; c < C / 64; ++c)
+            tma_load_3d(smem + L::OFF_Q + st * L::Q_BYTES + c * COLS * 128, &tm_q, q_full + st, c * 64, ct * COLS, it.b);
+          bulk_load(smem + L::OFF_COL + st * L::OFF_BYTES,
+                    p.offset + (static_cast<int64_t>(it.b) * p.tiles + ct) * COLS, L::OFF_BYTES, q_full + st);
+        }
+        __syncwarp();
+      }
+    }
+    // after a wait that ran out: the copies in flight land before the block leaves
+    if (!ok) {
+      if (k_uses > 0) mbar_wait(k_full, (k_uses - 1) & 1, p.status);
+      for (int st = 0; st < STAGES && st < u; ++st) mbar_wait(q_full + st, ((u - 1 - st) / STAGES) & 1, p.status);
+    }
+  } else if (warp == 8) {
+    // ------------------------------------------------------- MMA issuer
+    constexpr uint32_t IDESC = idesc_bf16(128, COLS, 0, 0);
+    const uint32_t k_addr = smem_u32(smem + L::OFF_K);
+    bool ok = true;
+    int u = 0, k_uses = 0;
+    for (int i = 0; ok; ++i) {
+      if (!(ok = wait(item_full + (i & 1), (i >> 1) & 1))) break;
+      const int item = s_item[i & 1];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(item_empty + (i & 1));
+      if (item < 0) break;
+      Item it;
+      open(item, it);
+      bool any = false;
+      for (int ct = it.tiles.step(); ok && ct >= 0; ct = it.tiles.step(), ++u) {
+        if (!any) {
+          any = true;
+          if (!(ok = wait(k_full, k_uses & 1))) break;
+          ++k_uses;
+        }
+        const int st = u % STAGES, buf = u & 1;
+        if (!(ok = wait(q_full + st, (u / STAGES) & 1))) break;
+        const uint32_t q_addr = smem_u32(smem + L::OFF_Q + st * L::Q_BYTES);
+        for (int g = 0; g < 2; ++g) {
+          if (u >= 2 && !(ok = wait(s_free + buf * 2 + g, ((u >> 1) & 1) ^ 1))) break;
+          tc_fence_after();
+          if (lane == 0) {
+#pragma unroll
+            for (int kk = 0; kk < C / 16; ++kk)
+              mma_ss(tmem + (buf * 2 + g) * COLS,
+                     sdesc_sw128(k_addr + (g * (C / 64) + (kk >> 2)) * (128 * 128) + (kk & 3) * 32, 16, 1024),
+                     sdesc_sw128(q_addr + (kk >> 2) * (COLS * 128) + (kk & 3) * 32, 16, 1024), IDESC,
+                     kk > 0 ? 1u : 0u);
+            mma_commit(s_full + buf * 2 + g);
+            if (g == 1) mma_commit(q_empty + st);
+          }
+          __syncwarp();
+        }
+      }
+      if (ok && any && lane == 0) mma_commit(k_empty);
+      __syncwarp();
+    }
+    if (lane == 0) {  // TMEM is freed with no product in flight
+      mma_commit(drained);
+      mbar_wait(drained, 0, p.status);
+    }
+    __syncwarp();
+  } else {
+    // ----------------------------------------------------------- epilogue
+    const int g = warp >> 2, r = threadIdx.x & 127;
+    const uint32_t lane_addr = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + g * COLS;
+    bool ok = true;
+    int u = 0;
+    for (int i = 0; ok; ++i) {
+      if (!(ok = wait(item_full + (i & 1), (i >> 1) & 1))) break;
+      const int item = s_item[i & 1];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(item_empty + (i & 1));
+      if (item < 0) break;
+      Item it;
+      open(item, it);
+      const int n0 = it.n0 + g * 128, n = n0 + r;
+      float sum = 0.f;
+      for (int ct = it.tiles.step(); ok && ct >= 0; ct = it.tiles.step(), ++u) {
+        const int st = u % STAGES, buf = u & 1;
+        const int4 m = it.tiles.meta[ct];
+        const bool none = m.x > n0 + 127 || m.y < n0;  // the item's other 128 keys are read, these are not
+        const bool whole = n0 >= m.z && n0 + 127 <= m.w;
+        const int2* range = p.range + (static_cast<int64_t>(it.b) * p.tiles + ct) * COLS;
+        const float* off = reinterpret_cast<const float*>(smem + L::OFF_COL + st * L::OFF_BYTES);
+        if (!(ok = wait(s_full + buf * 2 + g, (u >> 1) & 1))) break;
+        // the constants came by a copy that the products do not order for this thread
+        if (!(ok = wait(q_full + st, (u / STAGES) & 1))) break;
+        tc_fence_after();
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
+        if (!none) {
+#pragma unroll 1
+          for (int c0 = 0; c0 < COLS; c0 += 32) {
+            uint32_t x[32];
+            tmem_ld32(lane_addr + buf * 2 * COLS + c0, x);
+            if (whole) {
+#pragma unroll
+              for (int c = 0; c < 32; ++c)
+                part[c & 3] += fast_exp2(fmaf(__uint_as_float(x[c]), p.scale_log2, off[c0 + c]));
+            } else {
+#pragma unroll
+              for (int c = 0; c < 32; ++c) {
+                const float e = fast_exp2(fmaf(__uint_as_float(x[c]), p.scale_log2, off[c0 + c]));
+                const int2 rows = __ldg(range + c0 + c);
+                part[c & 3] += n >= rows.x && n <= rows.y ? e : 0.f;
+              }
+            }
+          }
+        }
+        sum += (part[0] + part[1]) + (part[2] + part[3]);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(s_free + buf * 2 + g);
+          mbar_arrive(q_empty + st);
+        }
+      }
+      if (!ok || n >= p.N) continue;
+      if (p.chunks > 1)
+        p.partial[(static_cast<int64_t>(it.chunk) * p.B + it.b) * p.N + n] = sum;
+      else
+        p.weights[static_cast<int64_t>(it.b) * p.weights_ld + n] += sum;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// weights += the chunks' sums, in their order.
+__global__ void __launch_bounds__(256)
+    weights_reduce_kernel(const float* partial, float* weights, int64_t weights_ld, int chunks, int B, int N) {
+  griddep_wait();
+  const int64_t rows = static_cast<int64_t>(B) * N;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= rows) return;
+  float sum = 0.f;
+  for (int c = 0; c < chunks; ++c) sum += partial[c * rows + i];
+  weights[i / N * weights_ld + i % N] += sum;
+}
+
+}  // namespace wpt

@@ -2,6 +2,7 @@
 // this file) and the extern "C" launchers declared in include/wpt_attn.h.
 #include <algorithm>
 #include <atomic>
+#include <climits>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -14,8 +15,10 @@
 #include "../../include/wpt_attn.h"
 #include "accept.cuh"
 #include "backward.cuh"
+#include "beam.cuh"
 #include "cache.cuh"
 #include "common.cuh"
+#include "evict.cuh"
 #include "exchange.cuh"
 #include "head.cuh"
 #include "merge.cuh"
@@ -23,6 +26,7 @@
 #include "select.cuh"
 #include "stream.cuh"
 #include "tree.cuh"
+#include "weights.cuh"
 
 namespace {
 
@@ -1306,4 +1310,374 @@ extern "C" int wpt_attn_decode_noalloc(const void* q, const void* k, const void*
   }
   return wpt_attn_decode(q, k, v, k_stride_b, k_stride_n, v_stride_b, v_stride_n, positions, floor_rows, idx, K, sink,
                          out, lse, part_o, part_lse, splits, chunk_tiles, B, T, H, C, N, window, scale, stream);
+}
+
+// ----------------------------------------- the cache between two decode steps
+
+namespace {
+
+// A launch as a programmatic dependent of the kernel before it on the stream
+// (every kernel launched so waits for it on the device before its first
+// global access), with a cluster of `cluster` CTAs when that is above 1.
+template <typename Kernel, typename... Args>
+int launch_dependent(const char* what, Kernel kernel, int64_t grid, int threads, int smem, int cluster,
+                     cudaStream_t stream, const Args&... args) {
+  if (grid >= (int64_t(1) << 31)) return fail(WPT_ERR_UNSUPPORTED, "%s: too large a grid", what);
+  if (smem > 0)
+    if (int rc = allow_smem(kernel, smem)) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  if (e != cudaSuccess) return cuda_fail(e, what);
+  return WPT_OK;
+}
+
+// Scratch of the query-stream form, in bytes from its start.
+struct WeightsPlan {
+  int tiles, key_blocks, chunks, chunk_tiles;
+  int64_t meta, offset, range, partial, ticket, bytes;
+};
+
+WeightsPlan weights_plan(int64_t B, int64_t T, int64_t H, int64_t N) {
+  WeightsPlan w = {};
+  const int64_t cols = T * H;
+  if (cols <= 256) return w;  // the key-stream form needs none
+  w.tiles = static_cast<int>((cols + wpt::WEIGHTS_TILE_COLS - 1) / wpt::WEIGHTS_TILE_COLS);
+  w.key_blocks = static_cast<int>((N + wpt::WEIGHTS_TILE_KEYS - 1) / wpt::WEIGHTS_TILE_KEYS);
+  // runs of at most 32 column tiles, shorter ones (not under 4) while that gives every SM work
+  int64_t per = 32;
+  while (per > 4 && B * w.key_blocks * ((w.tiles + per - 1) / per) < 4 * 148) per /= 2;
+  w.chunk_tiles = static_cast<int>(per < w.tiles ? per : w.tiles);
+  w.chunks = (w.tiles + w.chunk_tiles - 1) / w.chunk_tiles;
+  int64_t at = 0;
+  const int64_t n = B * w.tiles;
+  w.meta = at, at += n * 16;
+  w.offset = at, at += n * wpt::WEIGHTS_TILE_COLS * 4;
+  w.range = at, at += n * wpt::WEIGHTS_TILE_COLS * 8;
+  w.partial = at, at += w.chunks > 1 ? (w.chunks * B * N * 4 + 15) / 16 * 16 : 0;
+  w.ticket = at, at += 16;
+  w.bytes = at;
+  return w;
+}
+
+template <int C, int NCOL, int STAGES>
+int launch_weights_stream(const CUtensorMap& tq, const CUtensorMap& tk, const wpt::WeightsParams& p,
+                          cudaStream_t stream) {
+  using L = wpt::WeightsStreamLayout<C, NCOL, STAGES>;
+  static_assert(L::BYTES <= 232448, "attention-weight kernel shared memory exceeds 227 KB");
+  int sms = 148;
+  current_device(&sms);
+  return launch_dependent("weights_stream_kernel launch", wpt::weights_stream_kernel<C, NCOL, STAGES>, sms,
+                          wpt::WEIGHTS_STREAM_THREADS, L::BYTES, 1, stream, tq, tk, p);
+}
+
+template <int C>
+int weights_call(const void* q, const CUtensorMap& tk, const wpt::WeightsParams& p, uint8_t* scratch,
+                 cudaStream_t stream) {
+  const int64_t cols = static_cast<int64_t>(p.T) * p.H;
+  const bool few = cols <= 256;
+  const int ncol = !few ? 128 : cols <= 16 ? 16 : cols <= 32 ? 32 : cols <= 64 ? 64 : cols <= 128 ? 128 : 256;
+  CUtensorMap tq;
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(C), static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(p.B)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(C) * 2, static_cast<cuuint64_t>(cols) * C * 2};
+  cuuint32_t box[3] = {64, static_cast<cuuint32_t>(ncol), 1};
+  if (int rc = tensor_map(&tq, q, 3, dims, strides, box)) return rc;
+  if (few) {
+    switch (ncol) {
+      case 16: return launch_weights_stream<C, 16, 6>(tq, tk, p, stream);
+      case 32: return launch_weights_stream<C, 32, 6>(tq, tk, p, stream);
+      case 64: return launch_weights_stream<C, 64, 5>(tq, tk, p, stream);
+      case 128: return launch_weights_stream<C, 128, 4>(tq, tk, p, stream);
+      default: return launch_weights_stream<C, 256, 2>(tq, tk, p, stream);
+    }
+  }
+  const WeightsPlan w = weights_plan(p.B, p.T, p.H, p.N);
+  constexpr int STAGES = C == 128 ? 4 : 8;
+  using L = wpt::WeightsTileLayout<C, STAGES>;
+  static_assert(L::BYTES <= 232448, "attention-weight kernel shared memory exceeds 227 KB");
+  wpt::WeightsTileParams t;
+  t.weights = p.weights;
+  t.weights_ld = p.weights_ld;
+  int4* meta = reinterpret_cast<int4*>(scratch + w.meta);
+  float* offset = reinterpret_cast<float*>(scratch + w.offset);
+  int2* range = reinterpret_cast<int2*>(scratch + w.range);
+  t.meta = meta;
+  t.offset = offset;
+  t.range = range;
+  t.partial = reinterpret_cast<float*>(scratch + w.partial);
+  t.ticket = reinterpret_cast<unsigned*>(scratch + w.ticket);
+  t.status = p.status;
+  t.B = p.B;
+  t.N = p.N;
+  t.tiles = w.tiles;
+  t.key_blocks = w.key_blocks;
+  t.chunks = w.chunks;
+  t.chunk_tiles = w.chunk_tiles;
+  t.scale_log2 = p.scale_log2;
+  const int64_t items = static_cast<int64_t>(p.B) * w.key_blocks * w.chunks;
+  if (items >= (int64_t(1) << 30)) return fail(WPT_ERR_UNSUPPORTED, "attention weights: too many keys and queries");
+  t.items = static_cast<int>(items);
+  if (int rc = launch_dependent("weights_prep_kernel launch", wpt::weights_prep_kernel,
+                                static_cast<int64_t>(p.B) * w.tiles, wpt::WEIGHTS_TILE_COLS, 0, 1, stream, p, w.tiles,
+                                meta, offset, range, t.ticket))
+    return rc;
+  int sms = 148;
+  current_device(&sms);
+  if (int rc = launch_dependent("weights_tile_kernel launch", wpt::weights_tile_kernel<C, STAGES>,
+                                std::min<int64_t>(items, sms), wpt::WEIGHTS_TILE_THREADS, L::BYTES, 1, stream, tq, tk,
+                                t))
+    return rc;
+  if (w.chunks == 1) return WPT_OK;
+  return launch_dependent("weights_reduce_kernel launch", wpt::weights_reduce_kernel,
+                          (static_cast<int64_t>(p.B) * p.N + 255) / 256, 256, 0, 1, stream,
+                          static_cast<const float*>(t.partial), p.weights, p.weights_ld, w.chunks, p.B, p.N);
+}
+
+}  // namespace
+
+extern "C" size_t wpt_attn_weights_scratch_bytes(int B, int T, int H, int N) {
+  if (B < 1 || T < 1 || H < 1 || N < 1 || static_cast<int64_t>(T) * H >= (int64_t(1) << 31)) return 0;
+  return static_cast<size_t>(weights_plan(B, T, H, N).bytes);
+}
+
+extern "C" int wpt_attn_weights(const void* q, const void* k, int64_t k_stride_b, int64_t k_stride_n,
+                                const int64_t* positions, const int64_t* floor, const float* lse, float* weights,
+                                int64_t weights_ld, void* scratch, int B, int T, int H, int C, int N, int window,
+                                float scale, void* stream) {
+  if (C != 64 && C != 128)
+    return fail(WPT_ERR_UNSUPPORTED, "head width %d: the attention-weight kernels take 64 and 128", C);
+  if (B < 0 || T < 0 || H < 1 || N < 0 || window < 0)
+    return fail(WPT_ERR_INVALID, "bad shape B=%d T=%d H=%d N=%d window=%d", B, T, H, N, window);
+  if (B == 0 || T == 0 || N == 0) return WPT_OK;
+  if (static_cast<int64_t>(T) * H >= (int64_t(1) << 31) || B >= (1 << 24) || N > INT_MAX - 512)
+    return fail(WPT_ERR_UNSUPPORTED, "attention weights: shape too large");
+  if (static_cast<int64_t>(B) * ((static_cast<int64_t>(T) * H + 127) / 128) >= (int64_t(1) << 31))
+    return fail(WPT_ERR_UNSUPPORTED, "attention weights: B*T*H too large");
+  if (!q || !k || !positions || !lse || !weights) return fail(WPT_ERR_INVALID, "a required pointer is NULL");
+  if (weights_ld < N && B > 1) return fail(WPT_ERR_INVALID, "the weights' row stride is under N");
+  if (!aligned16(q)) return fail(WPT_ERR_INVALID, "q must be 16-byte aligned");
+  if (static_cast<int64_t>(T) * H > 256 && (!scratch || !aligned16(scratch)))
+    return fail(WPT_ERR_INVALID, "attention weights: scratch is missing or not 16-byte aligned");
+  CUtensorMap tk;
+  if (int rc = table_map(&tk, k, k_stride_b, k_stride_n, B, N, C)) return rc;
+  wpt::WeightsParams p;
+  p.positions = positions;
+  p.floor = floor;
+  p.lse = lse;
+  p.weights = weights;
+  p.weights_ld = weights_ld;
+  if (int rc = status_word(&p.status)) return rc;
+  p.B = B;
+  p.T = T;
+  p.H = H;
+  p.N = N;
+  p.window = window;
+  p.scale_log2 = scale * wpt::LOG2E;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  uint8_t* at = static_cast<uint8_t*>(scratch);
+  return C == 64 ? weights_call<64>(q, tk, p, at, s) : weights_call<128>(q, tk, p, at, s);
+}
+
+extern "C" int wpt_cache_evict(const void* held, int64_t held_stride_b, int64_t held_stride_n, const float* weights,
+                               int64_t weights_ld, const int64_t* lengths, void* kept, float* kept_weights,
+                               int64_t* rows, int64_t* counts, int B, int N, int row_bytes, int keep, int recent,
+                               int first, int capacity, void* stream) {
+  if (B < 0 || N < 0 || row_bytes < 0 || keep < 0 || capacity < keep || recent < 0 || first < 0)
+    return fail(WPT_ERR_INVALID, "bad eviction shape B=%d N=%d keep=%d recent=%d first=%d capacity=%d", B, N, keep,
+                recent, first, capacity);
+  if (static_cast<int64_t>(recent) + first > keep)
+    return fail(WPT_ERR_INVALID, "%d first and %d recent rows do not fit in the %d kept", first, recent, keep);
+  if (row_bytes % 4)
+    return fail(WPT_ERR_UNSUPPORTED, "cache rows of %d bytes: the eviction kernel copies multiples of 4", row_bytes);
+  if (N > INT_MAX - (1 << 20) || capacity > INT_MAX - (1 << 20))
+    return fail(WPT_ERR_UNSUPPORTED, "eviction: table too long");
+  if (B == 0) return WPT_OK;
+  const bool copies = capacity > 0 && row_bytes > 0;
+  if (!lengths || !counts || (N > 0 && !weights) || (keep > 0 && !rows) || (capacity > 0 && !kept_weights) ||
+      (copies && (!kept || (N > 0 && !held))))
+    return fail(WPT_ERR_INVALID, "a required pointer is NULL");
+  if (weights_ld < N && B > 1) return fail(WPT_ERR_INVALID, "the weights' row stride is under N");
+  const auto at = reinterpret_cast<uintptr_t>(held) | reinterpret_cast<uintptr_t>(kept) |
+                  static_cast<uintptr_t>(held_stride_b) | static_cast<uintptr_t>(held_stride_n) |
+                  static_cast<uintptr_t>(row_bytes);
+  if (at % 4) return fail(WPT_ERR_INVALID, "cache tables and strides must be multiples of 4 bytes");
+  int sms = 148;
+  current_device(&sms);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  wpt::EvictParams p;
+  p.weights = weights;
+  p.weights_ld = weights_ld;
+  p.lengths = lengths;
+  p.rows = rows;
+  p.weights_out = kept_weights;
+  p.counts = counts;
+  p.N = N;
+  p.keep = keep;
+  p.recent = recent;
+  p.first = first;
+  p.capacity = capacity;
+  p.slices = 1;
+  while (p.slices < 8 && N > 8192 * p.slices && static_cast<int64_t>(B) * p.slices * 2 <= sms) p.slices *= 2;
+  const int slice = (N / p.slices + 1024) / 1024 * 1024;
+  p.cache_cap = slice < 49152 ? slice : 49152;
+  if (int rc = launch_dependent("evict_rows_kernel launch", wpt::evict_rows_kernel, static_cast<int64_t>(B) * p.slices,
+                                wpt::EVICT_THREADS, p.cache_cap * 4, p.slices, s, p))
+    return rc;
+  if (!copies) return WPT_OK;
+  wpt::GatherParams g;
+  g.src = static_cast<const uint8_t*>(held);
+  g.src_sb = held_stride_b;
+  g.src_sn = held_stride_n;
+  g.dst = static_cast<uint8_t*>(kept);
+  g.rows = rows;
+  g.keep = keep;
+  g.capacity = capacity;
+  const bool wide = at % 16 == 0;
+  g.units = row_bytes / (wide ? 16 : 4);
+  const int64_t blocks = (static_cast<int64_t>(capacity) * g.units + 255) / 256;
+  g.chunks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(blocks, (int64_t(8) * sms + B - 1) / B)));
+  if (wide)
+    return launch_dependent("evict_gather_kernel launch", wpt::evict_gather_kernel<uint4>,
+                            static_cast<int64_t>(B) * g.chunks, 256, 0, 1, s, g);
+  return launch_dependent("evict_gather_kernel launch", wpt::evict_gather_kernel<uint32_t>,
+                          static_cast<int64_t>(B) * g.chunks, 256, 0, 1, s, g);
+}
+
+namespace {
+// Runs a beam's scores are cut into, and tiles a run.
+void beam_plan(int64_t R, int64_t W, int64_t V, int sms, int* splits, int* tiles) {
+  const int64_t all = (V + 8 + wpt::BEAM_TILE - 1) / wpt::BEAM_TILE;  // a row may start 7 scores into its first tile
+  int64_t want = (4 * static_cast<int64_t>(sms) + R * W - 1) / (R * W);
+  if (want > all) want = all;
+  if (want < 1) want = 1;
+  *tiles = static_cast<int>((all + want - 1) / want);
+  *splits = static_cast<int>((all + *tiles - 1) / *tiles);
+}
+}  // namespace
+
+extern "C" size_t wpt_beam_scratch_bytes(int R, int W, int V, int K) {
+  if (R < 1 || W < 1 || V < 1 || K < 1) return 0;
+  int sms = 148, splits, tiles;
+  current_device(&sms);
+  beam_plan(R, W, V, sms, &splits, &tiles);
+  return static_cast<size_t>(R) * W * splits * (8 + 8 * static_cast<size_t>(K));
+}
+
+extern "C" int wpt_beam_select(const void* scores, int bf16, int64_t stride_r, int64_t stride_w, const float* totals,
+                               const uint8_t* done, int end, void* scratch, float* out_totals, int64_t* parents,
+                               int64_t* tokens, int R, int W, int V, int K, void* stream) {
+  if (R < 0 || W < 1 || V < 1 || K < 1) return fail(WPT_ERR_INVALID, "bad shape R=%d W=%d V=%d beams=%d", R, W, V, K);
+  if (W > wpt::BEAM_MAX || K > wpt::BEAM_MAX)
+    return fail(WPT_ERR_UNSUPPORTED, "%d beams in, %d out: the selection kernels take up to %d", W, K, wpt::BEAM_MAX);
+  if (V > INT_MAX - (1 << 20) || static_cast<int64_t>(W) * V > UINT_MAX)
+    return fail(WPT_ERR_UNSUPPORTED, "%d beams of %d scores are too many", W, V);
+  if (R == 0) return WPT_OK;
+  if (!scores || !totals || !scratch || !out_totals || !parents || !tokens)
+    return fail(WPT_ERR_INVALID, "a required pointer is NULL");
+  if (done && (end < 0 || end >= V)) return fail(WPT_ERR_INVALID, "end token %d of a vocabulary of %d", end, V);
+  if (reinterpret_cast<uintptr_t>(scratch) & 7) return fail(WPT_ERR_INVALID, "scratch must be 8-byte aligned");
+  if (reinterpret_cast<uintptr_t>(scores) & (bf16 ? 1 : 3)) return fail(WPT_ERR_INVALID, "scores are misaligned");
+  int sms = 148;
+  current_device(&sms);
+  wpt::BeamParams p;
+  beam_plan(R, W, V, sms, &p.splits, &p.tiles);
+  p.scores = scores;
+  p.stride_r = stride_r;
+  p.stride_w = stride_w;
+  p.totals = totals;
+  p.done = done;
+  p.stats = static_cast<float2*>(scratch);
+  p.cand = reinterpret_cast<uint64_t*>(p.stats + static_cast<int64_t>(R) * W * p.splits);
+  p.out_totals = out_totals;
+  p.parents = parents;
+  p.tokens = tokens;
+  p.R = R;
+  p.W = W;
+  p.V = V;
+  p.K = K;
+  p.end = end;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int64_t runs = static_cast<int64_t>(R) * W * p.splits;
+  const int rc = bf16 ? launch_dependent("beam_scan_kernel launch", wpt::beam_scan_kernel<__nv_bfloat16>, runs,
+                                         wpt::BEAM_THREADS, 0, 1, s, p)
+                      : launch_dependent("beam_scan_kernel launch", wpt::beam_scan_kernel<float>, runs,
+                                         wpt::BEAM_THREADS, 0, 1, s, p);
+  if (rc) return rc;
+  return launch_dependent("beam_merge_kernel launch", wpt::beam_merge_kernel, R, wpt::BEAM_THREADS, 0, 1, s, p);
+}
+
+namespace {
+template <typename Unit, int MAXW>
+int launch_reorder(const wpt::ReorderParams& p, int tables, cudaStream_t stream) {
+  return launch_dependent("reorder_kernel launch", wpt::reorder_kernel<Unit, MAXW>,
+                          static_cast<int64_t>(tables) * p.R * p.chunks, wpt::REORDER_THREADS, 0, 1, stream, p);
+}
+}  // namespace
+
+extern "C" int wpt_cache_reorder(void* const* tables, const int64_t* stride_b, const int64_t* stride_n,
+                                 const int* row_bytes, const int64_t* capacity, int count, const int64_t* parents,
+                                 const int64_t* lengths, const int64_t* first, int R, int W, void* stream) {
+  if (count < 0 || R < 0 || W < 1) return fail(WPT_ERR_INVALID, "bad reorder shape");
+  if (W > wpt::BEAM_MAX)
+    return fail(WPT_ERR_UNSUPPORTED, "%d beams: the reordering kernel takes up to %d", W, wpt::BEAM_MAX);
+  if (count > wpt::REORDER_TABLES)
+    return fail(WPT_ERR_UNSUPPORTED, "%d tables: a call takes up to %d", count, wpt::REORDER_TABLES);
+  if (count == 0 || R == 0) return WPT_OK;
+  if (!tables || !stride_b || !stride_n || !row_bytes || !capacity || !parents || !lengths)
+    return fail(WPT_ERR_INVALID, "a required pointer is NULL");
+  wpt::ReorderParams p;
+  uintptr_t all = 0;
+  for (int i = 0; i < count; ++i) {
+    if (row_bytes[i] < 0 || capacity[i] < 0 || capacity[i] > INT_MAX)
+      return fail(WPT_ERR_INVALID, "bad table %d", i);
+    if (row_bytes[i] > 0 && capacity[i] > 0 && !tables[i]) return fail(WPT_ERR_INVALID, "table %d is NULL", i);
+    all |= reinterpret_cast<uintptr_t>(tables[i]) | static_cast<uintptr_t>(stride_b[i]) |
+           static_cast<uintptr_t>(stride_n[i]) | static_cast<uintptr_t>(row_bytes[i]);
+  }
+  if (all % 4)
+    return fail(WPT_ERR_UNSUPPORTED, "the reordering kernel moves units of 4 bytes: tables, strides and rows must be "
+                                     "multiples of 4 bytes");
+  if (int rc = status_word(&p.status)) return rc;
+  // 16-byte units, one register quad a beam; above 32 beams, or for rows that
+  // are not 16-byte multiples, 4-byte units
+  const bool wide = all % 16 == 0 && W <= 32;
+  int64_t most = 0;
+  for (int i = 0; i < count; ++i) {
+    p.table[i].base = static_cast<uint8_t*>(tables[i]);
+    p.table[i].stride_b = stride_b[i];
+    p.table[i].stride_n = stride_n[i];
+    p.table[i].units = row_bytes[i] / (wide ? 16 : 4);
+    p.table[i].capacity = static_cast<int>(capacity[i]);
+    most = std::max(most, capacity[i] * p.table[i].units);
+  }
+  p.parents = parents;
+  p.lengths = lengths;
+  p.first = first;
+  p.R = R;
+  p.W = W;
+  int sms = 148;
+  current_device(&sms);
+  const int64_t blocks = (most + wpt::REORDER_THREADS - 1) / wpt::REORDER_THREADS;
+  const int64_t groups = static_cast<int64_t>(count) * R;
+  p.chunks = static_cast<int>(std::max<int64_t>(1, std::min(blocks, (int64_t(8) * sms + groups - 1) / groups)));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (wide) {
+    if (W <= 8) return launch_reorder<uint4, 8>(p, count, s);
+    if (W <= 16) return launch_reorder<uint4, 16>(p, count, s);
+    return launch_reorder<uint4, 32>(p, count, s);
+  }
+  if (W <= 16) return launch_reorder<uint32_t, 16>(p, count, s);
+  return launch_reorder<uint32_t, 64>(p, count, s);
 }
