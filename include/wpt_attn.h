@@ -423,21 +423,25 @@ int wpt_beam_select(const void* scores, int bf16, int64_t stride_r, int64_t stri
 /* Bytes of scratch wpt_beam_select needs (0 for a bad shape). */
 size_t wpt_beam_scratch_bytes(int R, int W, int V, int K);
 
+/* A cache table: the address on the device, then bytes (capacity in rows). */
+typedef struct {
+  int64_t address, stride_b, stride_n, row_bytes, capacity;
+} wpt_cache_table;
+
 /*
- * Reordering of the beams' cached rows, in place. Table i holds R * W rows of
- * (capacity[i], row_bytes[i]) bytes, beam w of text r at r * W + w; for every
+ * Reordering of the beams' cached rows, in place. A table holds R * W rows of
+ * (capacity, row_bytes) bytes, beam w of text r at r * W + w; for every
  * table, beam w of text r takes the table rows first[r] (0 when first is
  * NULL) .. lengths[r * W + parent] - 1 of beam parent = parents[r, w] as they
  * were before the call. A parent of -1, or w itself, leaves the beam as it
  * is; one of W or above does too and sets the status word's shape bit.
- *   tables, stride_b, stride_n (bytes), row_bytes, capacity: `count` entries
- *            on the host, up to 32; all multiples of 4 bytes (16: faster),
- *            no two places of the tables overlapping
+ *   tables   `count` descriptions on the host, up to 32 (strides and rows in
+ *            bytes); addresses, strides and rows multiples of 4 bytes (16:
+ *            faster), no two places of the tables overlapping
  *   parents  int64 (R, W);  lengths  int64 (R * W,);  first  int64 (R,) or NULL
  * W up to 64.
  */
-int wpt_cache_reorder(void* const* tables, const int64_t* stride_b, const int64_t* stride_n, const int* row_bytes,
-                      const int64_t* capacity, int count, const int64_t* parents, const int64_t* lengths,
+int wpt_cache_reorder(const wpt_cache_table* tables, int count, const int64_t* parents, const int64_t* lengths,
                       const int64_t* first, int R, int W, void* stream);
 
 /* Bytes of scratch wpt_accept needs for R rows of n drafts over V entries

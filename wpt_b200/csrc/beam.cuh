@@ -29,6 +29,7 @@ constexpr int BEAM_MAX = 64;  // beams in and out
 constexpr int BEAM_THREADS = 256;
 constexpr int BEAM_PER = 16;  // scores a thread holds at once
 constexpr int BEAM_TILE = BEAM_THREADS * BEAM_PER;
+constexpr int BEAM_ROOM = 1024;  // candidates of a run above its bound, before they are ranked
 constexpr int BEAM_GROUPS = 64;  // groups of threads whose maxima give the gather's bound
 
 struct BeamParams {
@@ -86,18 +87,13 @@ struct BeamShared {
   int count, listed;
 };
 
-template <int PER, class Key>
-__device__ __forceinline__ void beam_keep_best(BeamShared& s, int K, Key key) {
-  // A bound: the K-th largest of the maxima of BEAM_GROUPS groups of threads.
-  // At least K offered keys reach it, so the K best do.
-  uint32_t top = 0;
-#pragma unroll
-  for (int j = 0; j < PER; ++j) top = max(top, static_cast<uint32_t>(key(j) >> 32));
+// A bound that the K best of the threads' keys reach: the K-th largest of the
+// maxima of BEAM_GROUPS groups of threads (top: a thread's largest key's
+// upper half, 0 for none). Ends after a barrier.
+__device__ __forceinline__ uint32_t beam_bound(BeamShared& s, int K, uint32_t top) {
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
   if ((threadIdx.x & 3) == 0) s.group[threadIdx.x >> 2] = top;
-  if (threadIdx.x < s.listed) s.buf[threadIdx.x] = s.list[threadIdx.x];
-  if (threadIdx.x == 0) s.count = s.listed;
   __syncthreads();
   if (threadIdx.x < 32) {
     const uint32_t a = s.group[threadIdx.x], b = s.group[threadIdx.x + 32];
@@ -110,15 +106,11 @@ __device__ __forceinline__ void beam_keep_best(BeamShared& s, int K, Key key) {
     if (threadIdx.x == 0) s.bound = bound;
   }
   __syncthreads();
-  const uint32_t bound = s.bound;
-  const uint64_t worst = s.listed == K ? s.list[K - 1] : 0;
-#pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    const uint64_t k = key(j);
-    if (k > worst && static_cast<uint32_t>(k >> 32) >= bound) s.buf[atomicAdd(&s.count, 1)] = k;
-  }
-  __syncthreads();
-  const int n = s.count;
+  return s.bound;
+}
+
+// s.list = the K best of the n unique keys in s.buf, best first.
+__device__ __forceinline__ void beam_rank(BeamShared& s, int K, int n) {
   for (int i = threadIdx.x; i < n; i += BEAM_THREADS) {
     const uint64_t mine = s.buf[i];
     int rank = 0;
@@ -129,9 +121,47 @@ __device__ __forceinline__ void beam_keep_best(BeamShared& s, int K, Key key) {
   __syncthreads();
 }
 
+template <int PER, class Key>
+__device__ __forceinline__ void beam_keep_best(BeamShared& s, int K, Key key) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) top = max(top, static_cast<uint32_t>(key(j) >> 32));
+  if (threadIdx.x < s.listed) s.buf[threadIdx.x] = s.list[threadIdx.x];
+  if (threadIdx.x == 0) s.count = s.listed;
+  const uint32_t bound = beam_bound(s, K, top);
+  const uint64_t worst = s.listed == K ? s.list[K - 1] : 0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const uint64_t k = key(j);
+    if (k > worst && static_cast<uint32_t>(k >> 32) >= bound) s.buf[atomicAdd(&s.count, 1)] = k;
+  }
+  __syncthreads();
+  beam_rank(s, K, s.count);
+}
+
+// A thread's BEAM_PER scores of the tile at e0 (positions are counted from the
+// 16-byte boundary at or before the row; off: the row's first): -inf outside it.
 template <typename T>
-__global__ void __launch_bounds__(BEAM_THREADS) beam_scan_kernel(const BeamParams p) {
-  constexpr int VEC = 16 / sizeof(T), LOADS = BEAM_PER / VEC;
+__device__ __forceinline__ void beam_load_tile(const T* from, int64_t e0, int off, int64_t end, float (&x)[BEAM_PER]) {
+  constexpr int VEC = 16 / sizeof(T);
+#pragma unroll
+  for (int l = 0; l < BEAM_PER / VEC; ++l) {
+    const int64_t e = e0 + (l * BEAM_THREADS + threadIdx.x) * VEC;
+    float f[VEC];
+    if (e >= off && e + VEC <= end) {
+      beam_load16(from + e, f);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) f[i] = e + i >= off && e + i < end ? beam_load(from + e + i) : -INFINITY;
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) x[l * VEC + i] = f[i];
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(BEAM_THREADS, 4) beam_scan_kernel(const BeamParams p) {
+  constexpr int VEC = 16 / sizeof(T);
   __shared__ BeamShared s;
   __shared__ float s_m[BEAM_THREADS / 32], s_s[BEAM_THREADS / 32];
   const int split = blockIdx.x % p.splits;
@@ -140,54 +170,53 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_scan_kernel(const BeamParam
   griddep_wait();
   if (p.done != nullptr && p.done[rw]) return;  // an ended beam's scores are not read
   const T* row = static_cast<const T*>(p.scores) + r * p.stride_r + w * p.stride_w;
-  // positions are counted from the 16-byte boundary at or before the row
   const int off = static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
   const int64_t end = static_cast<int64_t>(off) + p.V;
   const T* from = row - off;
-  if (threadIdx.x == 0) s.listed = 0;
-  __syncthreads();
-  float m = -INFINITY, sum = 0.f;
-  bool bad = false;  // a NaN or +inf was met
-  for (int tile = 0; tile < p.tiles; ++tile) {
-    const int64_t e0 = (static_cast<int64_t>(split) * p.tiles + tile) * BEAM_TILE;
-    if (e0 >= end) break;
-    float x[BEAM_PER];
-#pragma unroll
-    for (int l = 0; l < LOADS; ++l) {
-      const int64_t e = e0 + (l * BEAM_THREADS + threadIdx.x) * VEC;
-      float f[VEC];
-      if (e >= off && e + VEC <= end) {
-        beam_load16(from + e, f);
-      } else {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) f[i] = e + i >= off && e + i < end ? beam_load(from + e + i) : -INFINITY;
-      }
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) x[l * VEC + i] = f[i];
-    }
+  const int64_t run0 = static_cast<int64_t>(split) * p.tiles * BEAM_TILE;
+  const int64_t run1 = min(end, run0 + static_cast<int64_t>(p.tiles) * BEAM_TILE);
+  auto key_of = [&](float x, int64_t e0, int j) -> uint64_t {
+    const int64_t e = e0 + ((j / VEC) * BEAM_THREADS + threadIdx.x) * VEC + j % VEC;
+    return x > -INFINITY ? beam_key(x, static_cast<uint32_t>(e - off)) : 0;
+  };
+  if (threadIdx.x == 0) s.count = s.listed = 0;
+  float m = -INFINITY, sum = 0.f, least = -INFINITY;
+  float x[BEAM_PER];
+  beam_load_tile(from, run0, off, end, x);
+  for (int64_t e0 = run0; e0 < run1; e0 += BEAM_TILE) {
+    float next[BEAM_PER];
+    if (e0 + BEAM_TILE < run1) beam_load_tile(from, e0 + BEAM_TILE, off, end, next);
     float top = x[0];
 #pragma unroll
     for (int j = 1; j < BEAM_PER; ++j) top = fmaxf(top, x[j]);
+    if (e0 == run0) {
+      // the bound that every candidate has to reach, from the run's first tile
+      const uint32_t bound = beam_bound(s, p.K, top > -INFINITY ? order_key(top + 0.f) : 0u);
+      least = bound == 0 ? -INFINITY : beam_key_value(static_cast<uint64_t>(bound) << 32);
+    }
+    if (top >= least && top > -INFINITY) {
+#pragma unroll
+      for (int j = 0; j < BEAM_PER; ++j)
+        if (x[j] >= least && x[j] > -INFINITY) {
+          const int i = atomicAdd(&s.count, 1);
+          if (i < BEAM_ROOM) s.buf[i] = key_of(x[j], e0, j);
+        }
+    }
     if (top > m) {
       sum *= fast_exp2((m - top) * LOG2E);
       m = top;
     }
+    // a NaN score makes the sum NaN, and so does +inf (inf - inf)
+    const float shift = m == -INFINITY ? 0.f : m;
+    float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < BEAM_PER; ++j) {
-      const float d = x[j] - m;  // NaN for a NaN score, and for +inf
-      bad = bad || isnan(x[j]) || x[j] == INFINITY;
-      if (x[j] > -INFINITY) sum += fast_exp2(d * LOG2E);
-    }
-    const float worst = s.listed == p.K ? beam_key_value(s.list[p.K - 1]) : -INFINITY;
-    if (__syncthreads_or(top > worst)) {
-      beam_keep_best<BEAM_PER>(s, p.K, [&](int j) -> uint64_t {
-        const int64_t e = e0 + ((j / VEC) * BEAM_THREADS + threadIdx.x) * VEC + j % VEC;
-        return x[j] > -INFINITY ? beam_key(x[j], static_cast<uint32_t>(e - off)) : 0;
-      });
-    }
+    for (int j = 0; j < BEAM_PER; ++j) part[j & 3] += fast_exp2((x[j] - shift) * LOG2E);
+    sum += (part[0] + part[1]) + (part[2] + part[3]);
+#pragma unroll
+    for (int j = 0; j < BEAM_PER; ++j) x[j] = next[j];
   }
-  // (m, sum) over the block; a NaN or +inf score makes the sum NaN
-  if (bad) sum = NAN;
+  griddep_launch();
+  // (m, sum) over the block
   float mm = m;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
@@ -197,7 +226,8 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_scan_kernel(const BeamParam
   mm = s_m[0];
 #pragma unroll
   for (int i = 1; i < BEAM_THREADS / 32; ++i) mm = fmaxf(mm, s_m[i]);
-  sum = m > -INFINITY || bad ? sum * fast_exp2((m - mm) * LOG2E) : 0.f;
+  // a thread that met nothing above -inf holds 0, or NaN
+  if (m > -INFINITY) sum *= fast_exp2((m - mm) * LOG2E);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) s_s[warp] = sum;
@@ -208,6 +238,21 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_scan_kernel(const BeamParam
 #pragma unroll
     for (int i = 0; i < BEAM_THREADS / 32; ++i) t += s_s[i];
     p.stats[run] = make_float2(mm, t);
+  }
+  if (s.count <= BEAM_ROOM) {
+    beam_rank(s, p.K, s.count);
+  } else {
+    // more scores reached the first tile's bound than there is room for
+    // (scores that rise along the vocabulary, or many equal ones): once more
+    // over the run, keeping the best after every tile
+    for (int64_t e0 = run0; e0 < run1; e0 += BEAM_TILE) {
+      beam_load_tile(from, e0, off, end, x);
+      float top = x[0];
+#pragma unroll
+      for (int j = 1; j < BEAM_PER; ++j) top = fmaxf(top, x[j]);
+      const float worst = s.listed == p.K ? beam_key_value(s.list[p.K - 1]) : -INFINITY;
+      if (__syncthreads_or(top > worst)) beam_keep_best<BEAM_PER>(s, p.K, [&](int j) { return key_of(x[j], e0, j); });
+    }
   }
   if (threadIdx.x < p.K) p.cand[run * p.K + threadIdx.x] = threadIdx.x < s.listed ? s.list[threadIdx.x] : 0;
 }

@@ -44,6 +44,78 @@ __device__ __forceinline__ int2 weights_range(int64_t pos, const int64_t* floor,
 // query without rows has lse -inf; it adds nothing.
 __device__ __forceinline__ float weights_offset(float lse) { return lse == -INFINITY ? -INFINITY : -lse * LOG2E; }
 
+// 2^x for a pair of floats on the FMA pipe, for the terms whose turn it is not
+// on the exponential unit. 2^x = 2^r 2^f with r = round(x), found by adding
+// 1.5 * 2^23, and f = x - r in [-1/2, 1/2]: 2^f is a polynomial of degree 5
+// fitted for this library by iterated weighted least squares (relative error
+// 1.5e-7, a rounding of the sum it goes into); r is added to its exponent. x
+// is clamped at -126: a smaller term counts as 2^-126.
+__device__ __forceinline__ uint64_t weights_exp2_poly(uint64_t x) {
+  constexpr float MAGIC = 12582912.0f;
+  float x0, x1;
+  f2_unpack(x, x0, x1);
+  x = f2_pack(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
+  const uint64_t t = f2_add(x, f2_pack(MAGIC, MAGIC));
+  const uint64_t r = f2_add(t, f2_pack(-MAGIC, -MAGIC));
+  const uint64_t f = f2_fma(r, f2_pack(-1.f, -1.f), x);
+  uint64_t q = f2_fma(f2_pack(0.0013264717999845743f, 0.0013264717999845743f), f, f2_pack(0.009671512991189957f, 0.009671512991189957f));
+  q = f2_fma(q, f, f2_pack(0.05550733953714371f, 0.05550733953714371f));
+  q = f2_fma(q, f, f2_pack(0.24022242426872253f, 0.24022242426872253f));
+  q = f2_fma(q, f, f2_pack(0.6931470036506653f, 0.6931470036506653f));
+  q = f2_fma(q, f, f2_pack(1.f, 1.f));
+  float q0, q1, t0, t1;
+  f2_unpack(q, q0, q1);
+  f2_unpack(t, t0, t1);
+  return f2_pack(__int_as_float(__float_as_int(q0) + (__float_as_int(t0) << 23)),
+                 __int_as_float(__float_as_int(q1) + (__float_as_int(t1) << 23)));
+}
+
+// Adds exp2(x scale + cols[0][c]) over 2 * PAIRS columns c to the four partial
+// sums, POLY of every 8 pairs on the FMA pipe; MASK: of those with cols[1][c] <= n <=
+// cols[2][c] (whole numbers). cols: rows of 128 columns in shared memory,
+// 16-byte aligned.
+template <int PAIRS, int POLY, bool MASK>
+__device__ __forceinline__ void weights_terms(uint64_t (&sum)[2], const uint32_t* x, float scale, const float* cols,
+                                              int n) {
+  const uint64_t scale2 = f2_pack(scale, scale);
+#pragma unroll
+  for (int i = 0; i < PAIRS; i += 2) {
+    const float4 o = *reinterpret_cast<const float4*>(cols + 2 * i);
+    uint64_t a[2];
+    a[0] = f2_fma(f2_pack(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), scale2, f2_pack(o.x, o.y));
+    a[1] = f2_fma(f2_pack(__uint_as_float(x[2 * i + 2]), __uint_as_float(x[2 * i + 3])), scale2, f2_pack(o.z, o.w));
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if constexpr (!MASK) {
+        if (((i + h) * POLY) % 8 < POLY) {
+          sum[h] = f2_add(sum[h], weights_exp2_poly(a[h]));
+          continue;
+        }
+      }
+      float a0, a1;
+      f2_unpack(a[h], a0, a1);
+      a0 = fast_exp2(a0);
+      a1 = fast_exp2(a1);
+      if constexpr (MASK) {
+        const int2 lo = *reinterpret_cast<const int2*>(cols + 128 + 2 * (i + h));
+        const int2 hi = *reinterpret_cast<const int2*>(cols + 256 + 2 * (i + h));
+        a0 = n >= lo.x && n <= hi.x ? a0 : 0.f;
+        a1 = n >= lo.y && n <= hi.y ? a1 : 0.f;
+      }
+      sum[h] = f2_add(sum[h], f2_pack(a0, a1));
+    }
+  }
+}
+
+// D = A B^T over KK + 1 steps of 16 columns, A 128 rows and B `cols` rows in
+// 64-column chunks of 128-byte-swizzled rows; issued by one lane of the warp.
+template <int KK, int COLS>
+__device__ __forceinline__ void weights_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
+  if constexpr (KK > 0) weights_mma<KK - 1, COLS>(d, a, b, idesc);
+  constexpr uint32_t OFF_A = ((KK / 4) * 128 * 128 + (KK % 4) * 32) / 16, OFF_B = ((KK / 4) * COLS * 128 + (KK % 4) * 32) / 16;
+  mma_ss_off_warp<OFF_A, OFF_B>(d, a, b, idesc, KK > 0 ? 1u : 0u);
+}
+
 // ------------------------------------------------------------- key stream
 
 constexpr int WEIGHTS_BAL_ROWS = 1024;  // most batch rows whose tiles are laid end to end
@@ -355,26 +427,30 @@ __global__ void __launch_bounds__(WEIGHTS_STREAM_THREADS, 1)
 
 // ------------------------------------------------------------ query stream
 
-constexpr int WEIGHTS_TILE_THREADS = 320;  // warps 0-7 epilogue, 8 MMA, 9 loader
-constexpr int WEIGHTS_TILE_KEYS = 256;
+constexpr int WEIGHTS_TILE_THREADS = 576;  // warps 0-15 epilogue, 16 MMA, 17 loader
+constexpr int WEIGHTS_TILE_GROUPS = 4;     // key tiles of 128 an item, one for each epilogue warpgroup
 constexpr int WEIGHTS_TILE_COLS = 128;
+constexpr int WEIGHTS_Q_STAGES = 2, WEIGHTS_C_STAGES = 4;
+// Pairs in every 8 whose exponentials take the FMA pipe. 8 x 4,096 places of 16
+// heads, causal: 0 take 388 us, 1 373, 2 371, 3 390.
+constexpr int WEIGHTS_POLY8 = 2;
 
 struct WeightsTileParams {
   float* weights;      // (B, N), row stride weights_ld
   int64_t weights_ld;
   const int4* meta;    // (B, tiles): lowest and highest row any column reads, then that all of them read
-  const float* offset; // (B, tiles, 128): each column's exponent constant
-  const int2* range;   // (B, tiles, 128): each column's rows
+  const float* cols;   // (B, tiles, 3, 128): each column's exponent constant, then its lowest and highest row (int)
   float* partial;      // (chunks, B, N) when chunks > 1
   unsigned* ticket;
   unsigned* status;
   int B, N, tiles, key_blocks, chunks, chunk_tiles, items;
+  int groups;  // key tiles an item has, up to WEIGHTS_TILE_GROUPS
   float scale_log2;
 };
 
 // One CTA a column tile: its columns' constants and rows, and the tile's.
 __global__ void __launch_bounds__(WEIGHTS_TILE_COLS)
-    weights_prep_kernel(const WeightsParams p, int tiles, int4* meta, float* offset, int2* range, unsigned* ticket) {
+    weights_prep_kernel(const WeightsParams p, int tiles, int4* meta, float* cols, unsigned* ticket) {
   __shared__ int s_red[4][4];
   const int b = blockIdx.x / tiles, tile = blockIdx.x - b * tiles;
   griddep_wait();
@@ -390,9 +466,10 @@ __global__ void __launch_bounds__(WEIGHTS_TILE_COLS)
     off = weights_offset(p.lse[at * p.H + (c - static_cast<int64_t>(t) * p.H)]);
     m = make_int4(r.x, r.y, r.x, r.y);
   }
-  const int64_t to = (static_cast<int64_t>(b) * tiles + tile) * WEIGHTS_TILE_COLS + threadIdx.x;
-  offset[to] = off;
-  range[to] = r;
+  float* to = cols + (static_cast<int64_t>(b) * tiles + tile) * (3 * WEIGHTS_TILE_COLS) + threadIdx.x;
+  to[0] = off;
+  to[WEIGHTS_TILE_COLS] = __int_as_float(r.x);
+  to[2 * WEIGHTS_TILE_COLS] = __int_as_float(r.y);
   m.x = __reduce_min_sync(0xffffffffu, m.x);
   m.y = __reduce_max_sync(0xffffffffu, m.y);
   m.z = __reduce_max_sync(0xffffffffu, m.z);
@@ -416,33 +493,33 @@ __global__ void __launch_bounds__(WEIGHTS_TILE_COLS)
   }
 }
 
-template <int C, int STAGES>
+template <int C>
 struct WeightsTileLayout {
-  static constexpr int K_BYTES = WEIGHTS_TILE_KEYS * C * 2;
-  static constexpr int Q_BYTES = WEIGHTS_TILE_COLS * C * 2, OFF_BYTES = WEIGHTS_TILE_COLS * 4;
+  static constexpr int K_BYTES = 128 * C * 2;  // a key tile
+  static constexpr int Q_BYTES = WEIGHTS_TILE_COLS * C * 2, COL_BYTES = WEIGHTS_TILE_COLS * 12;
   static constexpr int OFF_K = 0;
-  static constexpr int OFF_Q = K_BYTES;
-  static constexpr int OFF_COL = OFF_Q + STAGES * Q_BYTES;
-  static constexpr int OFF_BAR = OFF_COL + STAGES * OFF_BYTES;
-  // k_full, k_empty, item_full[2], item_empty[2], s_full[2][2], s_free[2][2], drained, q_full[STAGES],
-  // q_empty[STAGES]
-  static constexpr int NBAR = 15 + 2 * STAGES;
+  static constexpr int OFF_Q = WEIGHTS_TILE_GROUPS * K_BYTES;
+  static constexpr int OFF_COL = OFF_Q + WEIGHTS_Q_STAGES * Q_BYTES;
+  static constexpr int OFF_BAR = OFF_COL + WEIGHTS_C_STAGES * COL_BYTES;
+  // k_full, k_empty, drained, item_full[2], item_empty[2], s_full[4], s_free[4], then q and c full, empty
+  static constexpr int NBAR = 15 + 2 * WEIGHTS_Q_STAGES + 2 * WEIGHTS_C_STAGES;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
   static constexpr int BYTES = OFF_MISC + 32 + 1024;
 };
 
-// The column tiles of an item that read any of its keys, found 32 at a time
-// by the warp: step() gives the next one, or -1.
+// A walk over the column tiles of an item that read any of its keys, found 32
+// at a time by the warp: step() gives the next one, or -1.
 struct WeightsTiles {
   const int4* meta;
-  int at, end, n0, n1;
+  int at, end, lo, hi;
   unsigned mask;
-  __device__ __forceinline__ void start(const int4* m, int first, int last, int lo, int hi) {
+  int4 mine;  // of the tile at + lane
+  __device__ __forceinline__ void start(const int4* m, int first, int last, int n0, int n1) {
     meta = m;
     at = first - 32;
     end = last;
-    n0 = lo;
-    n1 = hi;
+    lo = n0;
+    hi = n1;
     mask = 0;
   }
   __device__ __forceinline__ int step() {
@@ -450,37 +527,43 @@ struct WeightsTiles {
       at += 32;
       if (at >= end) return -1;
       const int i = at + (threadIdx.x & 31);
-      bool live = false;
-      if (i < end) {
-        const int4 m = meta[i];
-        live = m.x <= n1 && m.y >= n0;
-      }
-      mask = __ballot_sync(0xffffffffu, live);
+      mine = i < end ? meta[i] : make_int4(INT_MAX, -1, INT_MAX, -1);
+      mask = __ballot_sync(0xffffffffu, mine.x <= hi && mine.y >= lo);
     }
     const int i = __ffs(mask) - 1;
     mask &= mask - 1;
     return at + i;
   }
+  // Of the tiles at .. at + 31: which have a column that reads one of rows n .. n + 127, and whose columns all read them all.
+  __device__ __forceinline__ unsigned any(int n) const {
+    return __ballot_sync(0xffffffffu, mine.x <= n + 127 && mine.y >= n);
+  }
+  __device__ __forceinline__ unsigned all(int n) const {
+    return __ballot_sync(0xffffffffu, mine.z <= n && mine.w >= n + 127);
+  }
 };
 
-template <int C, int STAGES>
+template <int C>
 __global__ void __launch_bounds__(WEIGHTS_TILE_THREADS, 1)
     weights_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                         const WeightsTileParams p) {
-  using L = WeightsTileLayout<C, STAGES>;
-  constexpr int KEYS = WEIGHTS_TILE_KEYS, COLS = WEIGHTS_TILE_COLS;
+  using L = WeightsTileLayout<C>;
+  constexpr int COLS = WEIGHTS_TILE_COLS, GROUPS = WEIGHTS_TILE_GROUPS;
+  constexpr int QS = WEIGHTS_Q_STAGES, CS = WEIGHTS_C_STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
   uint64_t* k_full = bars;
   uint64_t* k_empty = bars + 1;
-  uint64_t* item_full = bars + 2;
-  uint64_t* item_empty = bars + 4;
-  uint64_t* s_full = bars + 6;   // [buffer][key tile]
-  uint64_t* s_free = bars + 10;  // [buffer][key tile]
-  uint64_t* drained = bars + 14;
+  uint64_t* drained = bars + 2;
+  uint64_t* item_full = bars + 3;
+  uint64_t* item_empty = bars + 5;
+  uint64_t* s_full = bars + 7;   // a key tile's scores are in TMEM
+  uint64_t* s_free = bars + 11;  // and have been read
   uint64_t* q_full = bars + 15;
-  uint64_t* q_empty = q_full + STAGES;
+  uint64_t* q_empty = q_full + QS;
+  uint64_t* c_full = q_empty + QS;
+  uint64_t* c_empty = c_full + CS;
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC);
   volatile int* s_item = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 8);  // two slots
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -491,23 +574,27 @@ __global__ void __launch_bounds__(WEIGHTS_TILE_THREADS, 1)
     mbar_init(drained, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(item_full + i, 1);
-      mbar_init(item_empty + i, 9);  // the MMA warp and the eight epilogue warps
+      mbar_init(item_empty + i, 17);  // the MMA warp and the 16 epilogue warps
     }
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < GROUPS; ++i) {
       mbar_init(s_full + i, 1);
       mbar_init(s_free + i, 4);
     }
-    for (int s = 0; s < STAGES; ++s) {
+    for (int s = 0; s < QS; ++s) {
       mbar_init(q_full + s, 1);
-      mbar_init(q_empty + s, 9);  // the products and the epilogue warps' reads of the constants
+      mbar_init(q_empty + s, 1);
+    }
+    for (int s = 0; s < CS; ++s) {
+      mbar_init(c_full + s, 1);
+      mbar_init(c_empty + s, 16);
     }
     fence_mbar_init();
   }
-  if (warp == 8) {
+  if (warp == 16) {
     tmem_alloc(s_tmem, 512);
     tmem_relinquish();
   }
-  if (warp == 9 && lane == 0) {
+  if (warp == 17 && lane == 0) {
     tma_prefetch(&tm_q);
     tma_prefetch(&tm_k);
   }
@@ -517,7 +604,7 @@ __global__ void __launch_bounds__(WEIGHTS_TILE_THREADS, 1)
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
 
-  // an item: keys [n0, n0 + 256) of row b against column tiles [c0, c1)
+  // an item: keys [n0, n0 + 128 groups) of row b against a run of column tiles
   struct Item {
     int b, n0, chunk;
     WeightsTiles tiles;
@@ -527,14 +614,14 @@ __global__ void __launch_bounds__(WEIGHTS_TILE_THREADS, 1)
     it.chunk = p.chunks - 1 - item / per;  // a causal pass's last columns read the most keys: first
     const int rest = item % per;
     it.b = rest % p.B;
-    it.n0 = rest / p.B * KEYS;
+    it.n0 = rest / p.B * (128 * p.groups);
     const int c0 = it.chunk * p.chunk_tiles;
     it.tiles.start(p.meta + static_cast<int64_t>(it.b) * p.tiles, c0, min(p.tiles, c0 + p.chunk_tiles), it.n0,
-                   it.n0 + KEYS - 1);
+                   it.n0 + 128 * p.groups - 1);
   };
   auto wait = [&](uint64_t* bar, int parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status)); };
 
-  if (warp == 9) {
+  if (warp == 17) {
     // ------------------------------------------------------------ loader
     bool ok = true;
     int u = 0, k_uses = 0;
@@ -558,24 +645,30 @@ __global__ void __launch_bounds__(WEIGHTS_TILE_THREADS, 1)
           if (k_uses > 0 && !(ok = wait(k_empty, (k_uses - 1) & 1))) break;
           ++k_uses;
           if (lane == 0) {
-            mbar_expect_tx(k_full, L::K_BYTES);
-#pragma unroll
-            for (int g = 0; g < 2; ++g)
+            mbar_expect_tx(k_full, p.groups * L::K_BYTES);
+            for (int g = 0; g < p.groups; ++g)
 #pragma unroll
               for (int c = 0; c < C / 64; ++c)
-                tma_load_3d(smem + L::OFF_K + (g * (C / 64) + c) * 128 * 128, &tm_k, k_full, c * 64, it.n0 + g * 128,
+                tma_load_3d(smem + L::OFF_K + g * L::K_BYTES + c * 128 * 128, &tm_k, k_full, c * 64, it.n0 + g * 128,
                             it.b);
           }
         }
-        const int st = u % STAGES;
-        if (u >= STAGES && !(ok = wait(q_empty + st, ((u / STAGES) & 1) ^ 1))) break;
+        const int qs = u % QS, cs = u % CS;
+        if (u >= QS && !(ok = wait(q_empty + qs, ((u / QS) & 1) ^ 1))) break;
         if (lane == 0) {
-          mbar_expect_tx(q_full + st, L::Q_BYTES + L::OFF_BYTES);
+          mbar_expect_tx(q_full + qs, L::Q_BYTES);
 #pragma unroll
           for (int c = 0; c < C / 64; ++c)
-            tma_load_3d(smem + L::OFF_Q + st * L::Q_BYTES + c * COLS * 128, &tm_q, q_full + st, c * 64, ct * COLS, it.b);
-          bulk_load(smem + L::OFF_COL + st * L::OFF_BYTES,
-                    p.offset + (static_cast<int64_t>(it.b) * p.tiles + ct) * COLS, L::OFF_BYTES, q_full + st);
+            tma_load_3d(smem + L::OFF_Q + qs * L::Q_BYTES + c * COLS * 128, &tm_q, q_full + qs, c * 64, ct * COLS, it.b);
+        }
+        if (u >= CS && !(ok = wait(c_empty + cs, ((u / CS) & 1) ^ 1))) {
+          ++u;  // its queries are on their way
+          break;
+        }
+        if (lane == 0) {
+          mbar_expect_tx(c_full + cs, L::COL_BYTES);
+          bulk_load(smem + L::OFF_COL + cs * L::COL_BYTES,
+                    p.cols + (static_cast<int64_t>(it.b) * p.tiles + ct) * (3 * COLS), L::COL_BYTES, c_full + cs);
         }
         __syncwarp();
       }
@@ -583,14 +676,16 @@ __global__ void __launch_bounds__(WEIGHTS_TILE_THREADS, 1)
     // after a wait that ran out: the copies in flight land before the block leaves
     if (!ok) {
       if (k_uses > 0) mbar_wait(k_full, (k_uses - 1) & 1, p.status);
-      for (int st = 0; st < STAGES && st < u; ++st) mbar_wait(q_full + st, ((u - 1 - st) / STAGES) & 1, p.status);
+      for (int st = 0; st < QS && st < u; ++st) mbar_wait(q_full + st, ((u - 1 - st) / QS) & 1, p.status);
+      for (int st = 0; st < CS && st < u; ++st) mbar_wait(c_full + st, ((u - 1 - st) / CS) & 1, p.status);
     }
-  } else if (warp == 8) {
+  } else if (warp == 16) {
     // ------------------------------------------------------- MMA issuer
     constexpr uint32_t IDESC = idesc_bf16(128, COLS, 0, 0);
     const uint32_t k_addr = smem_u32(smem + L::OFF_K);
     bool ok = true;
     int u = 0, k_uses = 0;
+    unsigned uses = 0;  // parity of each key tile's uses (bits 0-3), and whether it had one (bits 4-7)
     for (int i = 0; ok; ++i) {
       if (!(ok = wait(item_full + (i & 1), (i >> 1) & 1))) break;
       const int item = s_item[i & 1];
@@ -599,46 +694,48 @@ __global__ void __launch_bounds__(WEIGHTS_TILE_THREADS, 1)
       if (item < 0) break;
       Item it;
       open(item, it);
-      bool any = false;
+      bool first = true;
+      unsigned any[GROUPS];
+      int from = -1;
       for (int ct = it.tiles.step(); ok && ct >= 0; ct = it.tiles.step(), ++u) {
-        if (!any) {
-          any = true;
+        if (it.tiles.at != from) {
+          from = it.tiles.at;
+#pragma unroll
+          for (int g = 0; g < GROUPS; ++g) any[g] = g < p.groups ? it.tiles.any(it.n0 + g * 128) : 0u;
+        }
+        if (first) {
+          first = false;
           if (!(ok = wait(k_full, k_uses & 1))) break;
           ++k_uses;
         }
-        const int st = u % STAGES, buf = u & 1;
-        if (!(ok = wait(q_full + st, (u / STAGES) & 1))) break;
-        const uint32_t q_addr = smem_u32(smem + L::OFF_Q + st * L::Q_BYTES);
-        for (int g = 0; g < 2; ++g) {
-          if (u >= 2 && !(ok = wait(s_free + buf * 2 + g, ((u >> 1) & 1) ^ 1))) break;
-          tc_fence_after();
-          if (lane == 0) {
+        const int qs = u % QS;
+        if (!(ok = wait(q_full + qs, (u / QS) & 1))) break;
+        const uint64_t q_desc = sdesc_sw128(smem_u32(smem + L::OFF_Q + qs * L::Q_BYTES), 16, 1024);
 #pragma unroll
-            for (int kk = 0; kk < C / 16; ++kk)
-              mma_ss(tmem + (buf * 2 + g) * COLS,
-                     sdesc_sw128(k_addr + (g * (C / 64) + (kk >> 2)) * (128 * 128) + (kk & 3) * 32, 16, 1024),
-                     sdesc_sw128(q_addr + (kk >> 2) * (COLS * 128) + (kk & 3) * 32, 16, 1024), IDESC,
-                     kk > 0 ? 1u : 0u);
-            mma_commit(s_full + buf * 2 + g);
-            if (g == 1) mma_commit(q_empty + st);
-          }
-          __syncwarp();
+        for (int g = 0; g < GROUPS; ++g) {
+          if (!ok || !((any[g] >> (ct - from)) & 1u)) continue;
+          if ((uses >> (4 + g)) & 1u) ok = wait(s_free + g, ((uses >> g) & 1u) ^ 1u);
+          if (!ok) continue;
+          uses = (uses ^ (1u << g)) | (16u << g);
+          tc_fence_after();
+          weights_mma<C / 16 - 1, COLS>(tmem + g * COLS, sdesc_sw128(k_addr + g * L::K_BYTES, 16, 1024), q_desc, IDESC);
+          mma_commit_warp(s_full + g);
         }
+        if (ok) mma_commit_warp(q_empty + qs);
       }
-      if (ok && any && lane == 0) mma_commit(k_empty);
-      __syncwarp();
+      if (ok && !first) mma_commit_warp(k_empty);
     }
-    if (lane == 0) {  // TMEM is freed with no product in flight
-      mma_commit(drained);
-      mbar_wait(drained, 0, p.status);
-    }
-    __syncwarp();
+    mma_commit_warp(drained);  // TMEM is freed with no product in flight
+    wait(drained, 0);
   } else {
     // ----------------------------------------------------------- epilogue
-    const int g = warp >> 2, r = threadIdx.x & 127;
-    const uint32_t lane_addr = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + g * COLS;
+    // A warpgroup takes one of the item's key tiles, a thread one key, in runs
+    // of 16 columns. The next run's scores are on their way from TMEM while a
+    // run is added up; while a warpgroup waits, the others compute.
+    const int g = warp >> 2;
+    const uint32_t from = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + g * COLS;
     bool ok = true;
-    int u = 0;
+    int u = 0, used = 0;
     for (int i = 0; ok; ++i) {
       if (!(ok = wait(item_full + (i & 1), (i >> 1) & 1))) break;
       const int item = s_item[i & 1];
@@ -647,57 +744,54 @@ __global__ void __launch_bounds__(WEIGHTS_TILE_THREADS, 1)
       if (item < 0) break;
       Item it;
       open(item, it);
-      const int n0 = it.n0 + g * 128, n = n0 + r;
-      float sum = 0.f;
+      const int n0 = it.n0 + g * 128, n = n0 + (threadIdx.x & 127);
+      uint64_t sum[2] = {0, 0};
+      unsigned any = 0, all = 0;
+      int first = -1;
       for (int ct = it.tiles.step(); ok && ct >= 0; ct = it.tiles.step(), ++u) {
-        const int st = u % STAGES, buf = u & 1;
-        const int4 m = it.tiles.meta[ct];
-        const bool none = m.x > n0 + 127 || m.y < n0;  // the item's other 128 keys are read, these are not
-        const bool whole = n0 >= m.z && n0 + 127 <= m.w;
-        const int2* range = p.range + (static_cast<int64_t>(it.b) * p.tiles + ct) * COLS;
-        const float* off = reinterpret_cast<const float*>(smem + L::OFF_COL + st * L::OFF_BYTES);
-        if (!(ok = wait(s_full + buf * 2 + g, (u >> 1) & 1))) break;
-        // the constants came by a copy that the products do not order for this thread
-        if (!(ok = wait(q_full + st, (u / STAGES) & 1))) break;
-        tc_fence_after();
-        float part[4] = {0.f, 0.f, 0.f, 0.f};
-        if (!none) {
-#pragma unroll 1
-          for (int c0 = 0; c0 < COLS; c0 += 32) {
+        if (it.tiles.at != first) {
+          first = it.tiles.at;
+          any = g < p.groups ? it.tiles.any(n0) : 0u;
+          all = it.tiles.all(n0);
+        }
+        const int cs = u % CS;
+        if (!(ok = wait(c_full + cs, (u / CS) & 1))) break;
+        if ((any >> (ct - first)) & 1u) {
+          const float* off = reinterpret_cast<const float*>(smem + L::OFF_COL + cs * L::COL_BYTES);
+          if (!(ok = wait(s_full + g, used & 1))) break;
+          ++used;
+          tc_fence_after();
+          const bool whole = (all >> (ct - first)) & 1u;
+#pragma unroll
+          for (int run = 0; run < COLS / 32; ++run) {
             uint32_t x[32];
-            tmem_ld32(lane_addr + buf * 2 * COLS + c0, x);
-            if (whole) {
-#pragma unroll
-              for (int c = 0; c < 32; ++c)
-                part[c & 3] += fast_exp2(fmaf(__uint_as_float(x[c]), p.scale_log2, off[c0 + c]));
-            } else {
-#pragma unroll
-              for (int c = 0; c < 32; ++c) {
-                const float e = fast_exp2(fmaf(__uint_as_float(x[c]), p.scale_log2, off[c0 + c]));
-                const int2 rows = __ldg(range + c0 + c);
-                part[c & 3] += n >= rows.x && n <= rows.y ? e : 0.f;
-              }
+            tmem_ld32(from + run * 32, x);
+            if (run == COLS / 32 - 1) {  // the scores are in registers
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(s_free + g);
             }
+            if (whole)
+              weights_terms<16, WEIGHTS_POLY8, false>(sum, x, p.scale_log2, off + run * 32, n);
+            else
+              weights_terms<16, 0, true>(sum, x, p.scale_log2, off + run * 32, n);
           }
         }
-        sum += (part[0] + part[1]) + (part[2] + part[3]);
-        tc_fence_before();
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(s_free + buf * 2 + g);
-          mbar_arrive(q_empty + st);
-        }
+        if (lane == 0) mbar_arrive(c_empty + cs);
       }
-      if (!ok || n >= p.N) continue;
+      if (!ok || g >= p.groups || n >= p.N) continue;
+      float s0, s1;
+      f2_unpack(f2_add(sum[0], sum[1]), s0, s1);
       if (p.chunks > 1)
-        p.partial[(static_cast<int64_t>(it.chunk) * p.B + it.b) * p.N + n] = sum;
+        p.partial[(static_cast<int64_t>(it.chunk) * p.B + it.b) * p.N + n] = s0 + s1;
       else
-        p.weights[static_cast<int64_t>(it.b) * p.weights_ld + n] += sum;
+        p.weights[static_cast<int64_t>(it.b) * p.weights_ld + n] += s0 + s1;
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == 16) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }

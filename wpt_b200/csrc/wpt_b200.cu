@@ -1344,28 +1344,35 @@ int launch_dependent(const char* what, Kernel kernel, int64_t grid, int threads,
   return WPT_OK;
 }
 
-// Scratch of the query-stream form, in bytes from its start.
+// The query-stream form's cut, and its scratch in bytes from its start.
 struct WeightsPlan {
-  int tiles, key_blocks, chunks, chunk_tiles;
-  int64_t meta, offset, range, partial, ticket, bytes;
+  int tiles, groups, key_blocks, chunks, chunk_tiles;
+  int64_t meta, cols, partial, ticket, bytes;
 };
 
 WeightsPlan weights_plan(int64_t B, int64_t T, int64_t H, int64_t N) {
   WeightsPlan w = {};
-  const int64_t cols = T * H;
+  const int64_t cols = T * H, sms = 148;
   if (cols <= 256) return w;  // the key-stream form needs none
   w.tiles = static_cast<int>((cols + wpt::WEIGHTS_TILE_COLS - 1) / wpt::WEIGHTS_TILE_COLS);
-  w.key_blocks = static_cast<int>((N + wpt::WEIGHTS_TILE_KEYS - 1) / wpt::WEIGHTS_TILE_KEYS);
-  // runs of at most 32 column tiles, shorter ones (not under 4) while that gives every SM work
-  int64_t per = 32;
-  while (per > 4 && B * w.key_blocks * ((w.tiles + per - 1) / per) < 4 * 148) per /= 2;
+  // Items of 1 or 2 key tiles where one wave of them (of 4 column tiles each)
+  // covers the call: 5 rows of 6,007 keys of width 64 and 444 columns take 13.3
+  // us with 2, 19.1 with 1 (two waves), 16.0 with 4 (60 SMs). Else 4, so that
+  // four warpgroups share the exponential unit: 2,000 keys of 32 rows and 1,024
+  // columns take 34.6 us with 4, 38.7 with 2, 53.5 with 1.
+  auto blocks = [&](int64_t groups) { return (N + 128 * groups - 1) / (128 * groups); };
+  w.groups = 1;
+  while (w.groups < wpt::WEIGHTS_TILE_GROUPS && B * blocks(w.groups) * ((w.tiles + 3) / 4) > sms) w.groups *= 2;
+  w.key_blocks = static_cast<int>(blocks(w.groups));
+  // runs of at most 16 column tiles, shorter ones (not under 4) to four items an SM
+  int64_t per = 16;
+  while (per > 4 && B * w.key_blocks * ((w.tiles + per - 1) / per) < 4 * sms) per /= 2;
   w.chunk_tiles = static_cast<int>(per < w.tiles ? per : w.tiles);
   w.chunks = (w.tiles + w.chunk_tiles - 1) / w.chunk_tiles;
   int64_t at = 0;
   const int64_t n = B * w.tiles;
   w.meta = at, at += n * 16;
-  w.offset = at, at += n * wpt::WEIGHTS_TILE_COLS * 4;
-  w.range = at, at += n * wpt::WEIGHTS_TILE_COLS * 8;
+  w.cols = at, at += n * wpt::WEIGHTS_TILE_COLS * 12;
   w.partial = at, at += w.chunks > 1 ? (w.chunks * B * N * 4 + 15) / 16 * 16 : 0;
   w.ticket = at, at += 16;
   w.bytes = at;
@@ -1404,24 +1411,22 @@ int weights_call(const void* q, const CUtensorMap& tk, const wpt::WeightsParams&
     }
   }
   const WeightsPlan w = weights_plan(p.B, p.T, p.H, p.N);
-  constexpr int STAGES = C == 128 ? 4 : 8;
-  using L = wpt::WeightsTileLayout<C, STAGES>;
+  using L = wpt::WeightsTileLayout<C>;
   static_assert(L::BYTES <= 232448, "attention-weight kernel shared memory exceeds 227 KB");
   wpt::WeightsTileParams t;
   t.weights = p.weights;
   t.weights_ld = p.weights_ld;
   int4* meta = reinterpret_cast<int4*>(scratch + w.meta);
-  float* offset = reinterpret_cast<float*>(scratch + w.offset);
-  int2* range = reinterpret_cast<int2*>(scratch + w.range);
+  float* columns = reinterpret_cast<float*>(scratch + w.cols);
   t.meta = meta;
-  t.offset = offset;
-  t.range = range;
+  t.cols = columns;
   t.partial = reinterpret_cast<float*>(scratch + w.partial);
   t.ticket = reinterpret_cast<unsigned*>(scratch + w.ticket);
   t.status = p.status;
   t.B = p.B;
   t.N = p.N;
   t.tiles = w.tiles;
+  t.groups = w.groups;
   t.key_blocks = w.key_blocks;
   t.chunks = w.chunks;
   t.chunk_tiles = w.chunk_tiles;
@@ -1431,13 +1436,12 @@ int weights_call(const void* q, const CUtensorMap& tk, const wpt::WeightsParams&
   t.items = static_cast<int>(items);
   if (int rc = launch_dependent("weights_prep_kernel launch", wpt::weights_prep_kernel,
                                 static_cast<int64_t>(p.B) * w.tiles, wpt::WEIGHTS_TILE_COLS, 0, 1, stream, p, w.tiles,
-                                meta, offset, range, t.ticket))
+                                meta, columns, t.ticket))
     return rc;
   int sms = 148;
   current_device(&sms);
-  if (int rc = launch_dependent("weights_tile_kernel launch", wpt::weights_tile_kernel<C, STAGES>,
-                                std::min<int64_t>(items, sms), wpt::WEIGHTS_TILE_THREADS, L::BYTES, 1, stream, tq, tk,
-                                t))
+  if (int rc = launch_dependent("weights_tile_kernel launch", wpt::weights_tile_kernel<C>, std::min<int64_t>(items, sms),
+                                wpt::WEIGHTS_TILE_THREADS, L::BYTES, 1, stream, tq, tk, t))
     return rc;
   if (w.chunks == 1) return WPT_OK;
   return launch_dependent("weights_reduce_kernel launch", wpt::weights_reduce_kernel,
@@ -1626,8 +1630,7 @@ int launch_reorder(const wpt::ReorderParams& p, int tables, cudaStream_t stream)
 }
 }  // namespace
 
-extern "C" int wpt_cache_reorder(void* const* tables, const int64_t* stride_b, const int64_t* stride_n,
-                                 const int* row_bytes, const int64_t* capacity, int count, const int64_t* parents,
+extern "C" int wpt_cache_reorder(const wpt_cache_table* tables, int count, const int64_t* parents,
                                  const int64_t* lengths, const int64_t* first, int R, int W, void* stream) {
   if (count < 0 || R < 0 || W < 1) return fail(WPT_ERR_INVALID, "bad reorder shape");
   if (W > wpt::BEAM_MAX)
@@ -1635,16 +1638,15 @@ extern "C" int wpt_cache_reorder(void* const* tables, const int64_t* stride_b, c
   if (count > wpt::REORDER_TABLES)
     return fail(WPT_ERR_UNSUPPORTED, "%d tables: a call takes up to %d", count, wpt::REORDER_TABLES);
   if (count == 0 || R == 0) return WPT_OK;
-  if (!tables || !stride_b || !stride_n || !row_bytes || !capacity || !parents || !lengths)
-    return fail(WPT_ERR_INVALID, "a required pointer is NULL");
+  if (!tables || !parents || !lengths) return fail(WPT_ERR_INVALID, "a required pointer is NULL");
   wpt::ReorderParams p;
-  uintptr_t all = 0;
+  int64_t all = 0;
   for (int i = 0; i < count; ++i) {
-    if (row_bytes[i] < 0 || capacity[i] < 0 || capacity[i] > INT_MAX)
+    const wpt_cache_table& t = tables[i];
+    if (t.row_bytes < 0 || t.row_bytes > INT_MAX || t.capacity < 0 || t.capacity > INT_MAX)
       return fail(WPT_ERR_INVALID, "bad table %d", i);
-    if (row_bytes[i] > 0 && capacity[i] > 0 && !tables[i]) return fail(WPT_ERR_INVALID, "table %d is NULL", i);
-    all |= reinterpret_cast<uintptr_t>(tables[i]) | static_cast<uintptr_t>(stride_b[i]) |
-           static_cast<uintptr_t>(stride_n[i]) | static_cast<uintptr_t>(row_bytes[i]);
+    if (t.row_bytes > 0 && t.capacity > 0 && !t.address) return fail(WPT_ERR_INVALID, "table %d is NULL", i);
+    all |= t.address | t.stride_b | t.stride_n | t.row_bytes;
   }
   if (all % 4)
     return fail(WPT_ERR_UNSUPPORTED, "the reordering kernel moves units of 4 bytes: tables, strides and rows must be "
@@ -1655,12 +1657,13 @@ extern "C" int wpt_cache_reorder(void* const* tables, const int64_t* stride_b, c
   const bool wide = all % 16 == 0 && W <= 32;
   int64_t most = 0;
   for (int i = 0; i < count; ++i) {
-    p.table[i].base = static_cast<uint8_t*>(tables[i]);
-    p.table[i].stride_b = stride_b[i];
-    p.table[i].stride_n = stride_n[i];
-    p.table[i].units = row_bytes[i] / (wide ? 16 : 4);
-    p.table[i].capacity = static_cast<int>(capacity[i]);
-    most = std::max(most, capacity[i] * p.table[i].units);
+    const wpt_cache_table& t = tables[i];
+    p.table[i].base = reinterpret_cast<uint8_t*>(t.address);
+    p.table[i].stride_b = t.stride_b;
+    p.table[i].stride_n = t.stride_n;
+    p.table[i].units = static_cast<int>(t.row_bytes / (wide ? 16 : 4));
+    p.table[i].capacity = static_cast<int>(t.capacity);
+    most = std::max(most, t.capacity * p.table[i].units);
   }
   p.parents = parents;
   p.lengths = lengths;

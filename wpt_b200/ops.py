@@ -541,39 +541,35 @@ def accept(scores, drafted, q, uniforms, resample, temperature=1.0, top_k=None, 
 
 # ------------------------------------------- the cache between two decode steps
 
-def _one_device(*tensors):
-    """The CUDA device that all the tensors (None aside) are on."""
-    _need_cuda(*tensors)
-    device = tensors[0].device
+def _on(device, *tensors):
+    """Refuses tensors (None aside) that are not on the CUDA device `device`."""
     for t in tensors:
         if t is not None and t.device != device:
             raise ValueError(f"tensors on {device} and {t.device}: a call takes one device")
-    return device
-
-
-def _here(device):
-    """A context with `device` current, as the launchers need (none when it
-    already is)."""
-    return None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    if device.type != "cuda":
+        raise ValueError(f"wpt_b200 computes on a CUDA device only; got a tensor on {device}")
 
 
 def _call(device, fn, *args):
     """A C-ABI call on `device`'s current stream, whichever device is current."""
-    guard = _here(device)
-    if guard is None:
-        _lib.check(fn(*args, _lib.stream(device)))
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, _lib.stream(device))
     else:
-        with guard:
-            _lib.check(fn(*args, _lib.stream(device)))
+        with torch.cuda.device(device):
+            rc = fn(*args, _lib.stream(device))
+    if rc:
+        _lib.check(rc)
 
 
 def _row_bytes(x):
     """Bytes of one (b, n) entry of a table (B, N, ...) whose entries are contiguous, or None."""
-    size = x.element_size()
-    for length, stride in zip(reversed(x.shape[2:]), reversed(x.stride()[2:])):
-        if length > 1 and stride * x.element_size() != size:
+    es = x.element_size()
+    size = es
+    shape, stride = x.shape, x.stride()
+    for i in range(len(shape) - 1, 1, -1):
+        if shape[i] > 1 and stride[i] * es != size:
             return None
-        size *= length
+        size *= shape[i]
     return size
 
 
@@ -585,32 +581,37 @@ def attention_weights(q, k, positions, lse, scale, weights, window=0, floor=None
     columns T * H the keys stream past the queries (one launch), above that
     the queries past the keys (two, or three where a key's columns are summed
     in several runs)."""
-    device = _one_device(q, k, positions, lse, weights, floor)
-    q = _bf16(q).contiguous()
-    k = _table(k)
+    device = q.device
+    _on(device, k, positions, lse, weights, floor)
     B, T, H, C = q.shape
     N = k.shape[1]
     if k.shape != (B, N, C):
         raise ValueError(f"keys {tuple(k.shape)} against queries {tuple(q.shape)}")
     if lse.shape != (B, T, H) or positions.shape != (B, T) or (floor is not None and floor.shape != (B, T)):
         raise ValueError(f"queries {tuple(q.shape)} need lse {(B, T, H)} and positions {(B, T)}")
-    if weights.dtype != torch.float32 or weights.shape != (B, N) or (N > 1 and weights.stride(1) != 1) or \
-            (B > 1 and weights.stride(0) < N):
+    ld, step = weights.stride() if weights.dim() == 2 else (0, 0)
+    if weights.dtype != torch.float32 or weights.shape != (B, N) or (N > 1 and step != 1) or (B > 1 and ld < N):
         raise ValueError(f"weights must be float32 {(B, N)} with contiguous rows: they are added to in place")
+    _bf16(q)
+    if not q.is_contiguous() or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
+    k = _table(k)
     positions = _rows(positions)
-    floor = None if floor is None else _rows(floor)
-    lse = lse.float().contiguous()
-    if q.numel() == 0 or N == 0:
+    if floor is not None:
+        floor = _rows(floor)
+    if lse.dtype != torch.float32 or not lse.is_contiguous():
+        lse = lse.float().contiguous()
+    if B * T * N == 0:
         return weights
     lib = _lib.lib()
-    scratch, cols = None, T * H
-    if cols > 256:
-        nbytes = lib.wpt_attn_weights_scratch_bytes(B, T, H, N)
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    _call(device, lib.wpt_attn_weights, q.data_ptr(), k.data_ptr(), k.stride(0), k.stride(1), positions.data_ptr(),
-          _lib.ptr(floor), lse.data_ptr(), weights.data_ptr(), weights.stride(0), _lib.ptr(scratch), B, T, H, C, N,
-          int(window), float(scale))
-    LAUNCHES[0] += 1 if cols <= 256 else 2
+    scratch = None
+    if T * H > 256:
+        scratch = torch.empty(lib.wpt_attn_weights_scratch_bytes(B, T, H, N), dtype=torch.uint8, device=device)
+    sb, sn, _ = k.stride()
+    _call(device, lib.wpt_attn_weights, q.data_ptr(), k.data_ptr(), sb, sn, positions.data_ptr(),
+          None if floor is None else floor.data_ptr(), lse.data_ptr(), weights.data_ptr(), ld,
+          None if scratch is None else scratch.data_ptr(), B, T, H, C, N, window, scale)
+    LAUNCHES[0] += 1 if scratch is None else 2
     return weights
 
 
@@ -621,9 +622,10 @@ def cache_evict(held, weights, lengths, keep, recent=0, first=0, capacity=None):
     their order, as new tables of `capacity` rows (default `keep`), zeros
     after them. Returns (held (B, capacity, ...), weights (B, capacity), rows
     (B, keep) int64, -1 padded: the old places, counts (B,) int64)."""
-    device = _one_device(held, weights, lengths)
-    keep, recent, first = int(keep), int(recent), int(first)
-    capacity = keep if capacity is None else int(capacity)
+    device = held.device
+    _on(device, weights, lengths)
+    if capacity is None:
+        capacity = keep
     B, N = held.shape[:2]
     if weights.shape != (B, N) or weights.dtype != torch.float32 or lengths.shape != (B,):
         raise ValueError(f"a table of {B} rows of {N} needs float32 weights {(B, N)} and lengths {(B,)}")
@@ -634,18 +636,21 @@ def cache_evict(held, weights, lengths, keep, recent=0, first=0, capacity=None):
     if row_bytes is None:
         held = held.contiguous()
         row_bytes = _row_bytes(held)
-    if N > 1 and weights.stride(1) != 1 or B > 1 and weights.stride(0) < N:
+    ld, step = weights.stride()
+    if N > 1 and step != 1 or B > 1 and ld < N:
         weights = weights.contiguous()
+        ld = N
     lengths = _rows(lengths)
-    out = torch.empty((B, capacity) + tuple(held.shape[2:]), dtype=held.dtype, device=device)
-    out_weights = torch.empty((B, capacity), dtype=torch.float32, device=device)
-    rows = torch.empty((B, keep), dtype=torch.int64, device=device)
-    counts = torch.empty(B, dtype=torch.int64, device=device)
+    out = torch.empty(B, capacity, *held.shape[2:], dtype=held.dtype, device=device)
+    out_weights = torch.empty(B, capacity, dtype=torch.float32, device=device)
+    rows = torch.empty(B, keep, dtype=torch.int64, device=device)
+    counts = torch.empty_like(lengths)
     es = held.element_size()
-    _call(device, _lib.lib().wpt_cache_evict, held.data_ptr(), held.stride(0) * es, held.stride(1) * es,
-          weights.data_ptr(), weights.stride(0), lengths.data_ptr(), out.data_ptr(), out_weights.data_ptr(),
-          rows.data_ptr(), counts.data_ptr(), B, N, row_bytes, keep, recent, first, capacity)
-    LAUNCHES[0] += 1 + (out.numel() > 0)
+    stride = held.stride()
+    _call(device, _lib.lib().wpt_cache_evict, held.data_ptr(), stride[0] * es, stride[1] * es, weights.data_ptr(), ld,
+          lengths.data_ptr(), out.data_ptr(), out_weights.data_ptr(), rows.data_ptr(), counts.data_ptr(), B, N,
+          row_bytes, keep, recent, first, capacity)
+    LAUNCHES[0] += 2
     return out, out_weights, rows, counts
 
 
@@ -657,29 +662,33 @@ def beam_select(scores, totals, beams, done=None, end=None):
     with the token `end`. Returns (totals (R, beams) fp32, best first, parents
     and tokens (R, beams) int64); -inf, -1 and -1 where there are too few
     candidates."""
-    device = _one_device(scores, totals, done)
-    if scores.dtype not in (torch.float32, torch.bfloat16):
+    device = scores.device
+    _on(device, totals, done)
+    bf16 = scores.dtype == torch.bfloat16
+    if not bf16 and scores.dtype != torch.float32:
         raise NotImplementedError(f"the selection kernels take float32 or bfloat16 scores; got {scores.dtype}")
     R, W, V = scores.shape
-    K = int(beams)
-    if totals.shape != (R, W) or (done is not None and done.shape != (R, W)):
-        raise ValueError(f"scores {tuple(scores.shape)} need totals (and done) {(R, W)}")
-    if done is not None and end is None:
-        raise ValueError("ended beams need the token `end`")
-    if V > 1 and scores.stride(2) != 1:
+    if beams < 1 or totals.shape != (R, W) or (done is not None and done.shape != (R, W)):
+        raise ValueError(f"scores {tuple(scores.shape)} need totals (and done) {(R, W)}, and {beams} beams to pick")
+    if done is not None:
+        if end is None:
+            raise ValueError("ended beams need the token `end`")
+        if done.dtype != torch.bool or not done.is_contiguous():
+            done = done.to(torch.bool).contiguous()
+    sr, sw, sv = scores.stride()
+    if sv != 1 and V > 1:
         scores = scores.contiguous()
+        sr, sw = W * V, V
     if totals.dtype != torch.float32 or not totals.is_contiguous():
         totals = totals.float().contiguous()
-    if done is not None:
-        done = done.to(torch.bool).contiguous()
-    out = torch.empty((R, max(K, 0)), dtype=torch.float32, device=device)
-    picks = torch.empty((2, R, max(K, 0)), dtype=torch.int64, device=device)
-    parents, tokens = picks[0], picks[1]
+    out = torch.empty_like(totals) if beams == W else torch.empty(R, beams, dtype=torch.float32, device=device)
+    parents = torch.empty(R, beams, dtype=torch.int64, device=device)
+    tokens = torch.empty_like(parents)
     lib = _lib.lib()
-    scratch = torch.empty(lib.wpt_beam_scratch_bytes(R, W, V, K), dtype=torch.uint8, device=device)
-    _call(device, lib.wpt_beam_select, scores.data_ptr(), 1 if scores.dtype == torch.bfloat16 else 0,
-          scores.stride(0), scores.stride(1), totals.data_ptr(), _lib.ptr(done), 0 if end is None else int(end),
-          scratch.data_ptr(), out.data_ptr(), parents.data_ptr(), tokens.data_ptr(), R, W, V, K)
+    scratch = torch.empty(lib.wpt_beam_scratch_bytes(R, W, V, beams), dtype=torch.uint8, device=device)
+    _call(device, lib.wpt_beam_select, scores.data_ptr(), bf16, sr, sw, totals.data_ptr(),
+          None if done is None else done.data_ptr(), 0 if end is None else end, scratch.data_ptr(), out.data_ptr(),
+          parents.data_ptr(), tokens.data_ptr(), R, W, V, beams)
     LAUNCHES[0] += 2
     return out, parents, tokens
 
@@ -693,32 +702,30 @@ def cache_reorder(tables, parents, lengths, first=None):
     first[r] (default 0) .. lengths[r * W + p] - 1 of beam p = parents[r, w]
     (-1: it keeps its own). Returns `tables`. A launch for every 32 tables,
     whatever their shapes."""
-    every = [tables] if isinstance(tables, torch.Tensor) else list(tables)
-    if not every:
-        return tables
-    device = _one_device(parents, lengths, first, *every)
+    every = [tables] if isinstance(tables, torch.Tensor) else tables
+    device = parents.device
+    _on(device, lengths, first, *every)
     R, W = parents.shape
     if lengths.shape != (R * W,) or (first is not None and first.shape != (R,)):
         raise ValueError(f"parents {(R, W)} need lengths {(R * W,)} (and first {(R,)})")
     parents, lengths = _rows(parents), _rows(lengths)
-    first = None if first is None else _rows(first)
+    if first is not None:
+        first = _rows(first)
     fields = []
     for t in every:
-        if t.dim() < 2 or t.shape[0] != R * W:
-            raise ValueError(f"a table of {tuple(t.shape)} for {R} texts of {W} beams")
-        size = _row_bytes(t)
-        stride_b, stride_n = t.stride(0) * t.element_size(), t.stride(1) * t.element_size()
-        if size is None or (t.numel() and ((R * W > 1 and stride_b < size) or (t.shape[1] > 1 and stride_n < size))):
+        shape = t.shape
+        if len(shape) < 2 or shape[0] != R * W:
+            raise ValueError(f"a table of {tuple(shape)} for {R} texts of {W} beams")
+        size, es, stride = _row_bytes(t), t.element_size(), t.stride()
+        sb, sn = stride[0] * es, stride[1] * es
+        if size is None or (t.numel() and ((R * W > 1 and sb < size) or (shape[1] > 1 and sn < size))):
             raise ValueError("a reordered table's entries must be contiguous and its places must not overlap: it is "
                              "changed in place")
-        fields.append((t.data_ptr(), stride_b, stride_n, size, t.shape[1]))
+        fields += (t.data_ptr(), sb, sn, size, shape[1])
     lib = _lib.lib()
-    for i in range(0, len(fields), REORDER_TABLES):
-        part = fields[i:i + REORDER_TABLES]
-        n = len(part)
-        base, stride_b, stride_n, size, capacity = zip(*part)
-        _call(device, lib.wpt_cache_reorder, (ctypes.c_void_p * n)(*base), (ctypes.c_int64 * n)(*stride_b),
-              (ctypes.c_int64 * n)(*stride_n), (ctypes.c_int * n)(*size), (ctypes.c_int64 * n)(*capacity), n,
-              parents.data_ptr(), lengths.data_ptr(), _lib.ptr(first), R, W)
+    for i in range(0, len(fields), 5 * REORDER_TABLES):
+        part = fields[i:i + 5 * REORDER_TABLES]
+        _call(device, lib.wpt_cache_reorder, (ctypes.c_int64 * len(part))(*part), len(part) // 5, parents.data_ptr(),
+              lengths.data_ptr(), None if first is None else first.data_ptr(), R, W)
         LAUNCHES[0] += 1
     return tables
