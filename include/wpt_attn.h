@@ -412,7 +412,7 @@ int wpt_cache_evict(const void* held, int64_t held_stride_b, int64_t held_stride
  *   scores   fp32, or bf16 when bf16 is 1; (R, W, V), last dimension
  *            contiguous, the others at strides in elements (any alignment)
  *   totals   fp32 (R, W);  done  bytes (R, W) or NULL
- *   scratch  wpt_beam_scratch_bytes(R, W, V, K) bytes, 8-byte aligned
+ *   scratch  wpt_beam_scratch_bytes(R, W, V, K, bf16) bytes, 8-byte aligned
  *   out_totals fp32, parents and tokens int64: (R, K)
  * W and K up to 64, W * V under 2^32.
  */
@@ -421,7 +421,7 @@ int wpt_beam_select(const void* scores, int bf16, int64_t stride_r, int64_t stri
                     int R, int W, int V, int K, void* stream);
 
 /* Bytes of scratch wpt_beam_select needs (0 for a bad shape). */
-size_t wpt_beam_scratch_bytes(int R, int W, int V, int K);
+size_t wpt_beam_scratch_bytes(int R, int W, int V, int K, int bf16);
 
 /* A cache table: the address on the device, then bytes (capacity in rows). */
 typedef struct {

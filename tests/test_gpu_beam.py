@@ -258,3 +258,16 @@ def test_cache_reorder_refusals(wb):
         wb.cache_reorder(torch.zeros(65, 10, 8, device="cuda"), torch.zeros(1, 65, dtype=torch.int64, device="cuda"),
                          torch.full((65,), 10, device="cuda"))
     assert wb.cache_reorder([], parents, lengths) == []
+
+
+@pytest.mark.parametrize("value", [torch.finfo(torch.float32).min, torch.finfo(torch.float32).max, -2e30, 3e30])
+def test_scores_of_one_far_value(wb, value):
+    """A beam whose scores are all the type's lowest (or highest) value is uniform; one other score above it is all."""
+    V = 9001
+    scores = torch.full((2, 2, V), value)
+    scores[0, 1, 40:] = -float("inf")
+    scores[1, 0, 8500] = 0.0 if value < 0 else value
+    scores[1, 1, 3] = -5.0
+    totals = torch.tensor([[0.0, -9.0], [0.0, -1.0]])
+    x = scores.cuda()
+    _check(wb, wb.beam_select(x, totals.cuda(), 5), x, totals, 5)

@@ -49,7 +49,7 @@ SIGNATURES = {
     "wpt_attn_weights_scratch_bytes": [_I, _I, _I, _I],
     "wpt_cache_evict": [_P, _I64, _I64, _P, _I64, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P],
     "wpt_beam_select": [_P, _I, _I64, _I64, _P, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _P],
-    "wpt_beam_scratch_bytes": [_I, _I, _I, _I],
+    "wpt_beam_scratch_bytes": [_I, _I, _I, _I, _I],
     "wpt_cache_reorder": [_P, _I, _P, _P, _P, _I, _I, _P],
     "wpt_attn_exchange": [_P, _P, _I, _I64, _I, _I, _P, ctypes.POINTER(_P), _I, _I, _P, _P, _P],
 }

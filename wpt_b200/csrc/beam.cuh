@@ -7,17 +7,23 @@
 // the `beams` largest win (ties: the lowest w * V + v). Within a beam the
 // value grows with x, so a beam's best candidates are its largest scores and
 // one pass over the scores finds both them and (m, s). beam_scan_kernel: each
-// CTA takes a run of one beam's scores, keeps a running (m, s) a thread and
-// the run's best candidates in shared memory; a tile of scores is looked at
-// again only when one of them beats the worst of the best so far.
-// beam_merge_kernel: one CTA a text joins the runs' (m, s), turns the
-// candidates into values and ranks them. Bound: HBM, the scores read once.
+// CTA takes a run of one beam's scores. Its first tile gives a bound that the
+// K best of the run reach; scores that do go to shared memory, and after 1, 2,
+// 4, ... tiles those are ranked and the bound becomes the K-th best so far, so
+// that a run of n tiles looks at about K (2 + log2 n) scores twice.
+// beam_merge_kernel: one CTA a text joins the runs' sums, turns the candidates
+// into values and ranks them. Bound: HBM, the scores read once.
+//
+// The sums are kept in base 2 with a whole number in place of the maximum:
+// sum 2^(x L - M), L = log2(e) in fp32, M = round(m L). Moving to a larger M
+// is then exact, and the product's one rounding is that of the difference.
 //
 // Reordering, in place. Every thread owns one unit of bytes of a table place
 // across all of a text's beams: it loads that unit of each beam that another
 // one takes, and only then stores, so no copy of the table is needed.
 #pragma once
 
+#include <cfloat>
 #include <cstdint>
 
 #include "common.cuh"
@@ -27,10 +33,9 @@ namespace wpt {
 
 constexpr int BEAM_MAX = 64;  // beams in and out
 constexpr int BEAM_THREADS = 256;
-constexpr int BEAM_PER = 16;  // scores a thread holds at once
-constexpr int BEAM_TILE = BEAM_THREADS * BEAM_PER;
-constexpr int BEAM_ROOM = 1024;  // candidates of a run above its bound, before they are ranked
-constexpr int BEAM_GROUPS = 64;  // groups of threads whose maxima give the gather's bound
+constexpr int BEAM_PER = 16;    // scores a thread holds at once
+constexpr int BEAM_STAGES = 3;  // tiles of 64 bytes a thread on their way to a block
+constexpr int BEAM_ROOM = 512;  // candidates of a run above its bound, before they are ranked
 
 struct BeamParams {
   const void* scores;  // (R, W, V)
@@ -43,7 +48,7 @@ struct BeamParams {
   int64_t* parents;            // (R, K)
   int64_t* tokens;             // (R, K)
   int R, W, V, K, splits;
-  int tiles;  // tiles of BEAM_TILE scores a run
+  int tiles;  // tiles of 64 bytes a thread a run
   int end;
 };
 
@@ -75,45 +80,58 @@ __device__ __forceinline__ void beam_load16(const __nv_bfloat16* p, float (&x)[8
   }
 }
 
-// The K best keys of BEAM_THREADS * PER offered ones and of the list of the
-// best so far, by all BEAM_THREADS threads. key(j): this thread's j-th key (0
-// for none). s_buf holds the list in its first *count entries and has room
-// for BEAM_MAX + BEAM_THREADS * PER. Keys are unique, so ranks are.
+// The upper half of an ended beam's key: that of a NaN, which no candidate has.
+constexpr uint64_t BEAM_ENDED = 0xFFFFFFFFull << 32;
+
+// A block's list of the best keys so far, and what it is made from (buf: room for
+// the list and the keys offered at once). Keys are unique, so ranks are.
 struct BeamShared {
-  uint64_t list[BEAM_MAX];                 // the best so far, best first
-  uint64_t buf[BEAM_MAX + BEAM_TILE];      // gathered keys
-  uint32_t group[BEAM_GROUPS];
+  uint64_t list[BEAM_MAX];  // best first
+  uint64_t* buf;            // gathered keys
+  alignas(16) uint32_t group[BEAM_THREADS];
   uint32_t bound;
   int count, listed;
 };
 
 // A bound that the K best of the threads' keys reach: the K-th largest of the
-// maxima of BEAM_GROUPS groups of threads (top: a thread's largest key's
-// upper half, 0 for none). Ends after a barrier.
-__device__ __forceinline__ uint32_t beam_bound(BeamShared& s, int K, uint32_t top) {
-  top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-  top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-  if ((threadIdx.x & 3) == 0) s.group[threadIdx.x >> 2] = top;
+// maxima of GROUPS >= K groups of threads (top: a thread's largest key's upper
+// half, 0 for none). Ends after a barrier.
+template <int GROUPS>
+__device__ __forceinline__ void beam_bound_of(BeamShared& s, int K, uint32_t top) {
+#pragma unroll
+  for (int o = 1; o < BEAM_THREADS / GROUPS; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (threadIdx.x % (BEAM_THREADS / GROUPS) == 0) s.group[threadIdx.x / (BEAM_THREADS / GROUPS)] = top;
   __syncthreads();
-  if (threadIdx.x < 32) {
-    const uint32_t a = s.group[threadIdx.x], b = s.group[threadIdx.x + 32];
-    uint32_t bound = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t mid = bound | (1u << bit);
-      const int at_least = __popc(__ballot_sync(0xffffffffu, a >= mid)) + __popc(__ballot_sync(0xffffffffu, b >= mid));
-      if (at_least >= K) bound = mid;
+  if (threadIdx.x < GROUPS) {
+    const int me = threadIdx.x;
+    const uint32_t mine = s.group[me];
+    int rank = 0;
+#pragma unroll 8
+    for (int i = 0; i < GROUPS; i += 4) {
+      const uint4 v = *reinterpret_cast<const uint4*>(s.group + i);
+      rank += (v.x > mine || (v.x == mine && i < me)) + (v.y > mine || (v.y == mine && i + 1 < me)) +
+              (v.z > mine || (v.z == mine && i + 2 < me)) + (v.w > mine || (v.w == mine && i + 3 < me));
     }
-    if (threadIdx.x == 0) s.bound = bound;
+    if (rank == K - 1) s.bound = mine;
   }
   __syncthreads();
+}
+// The more groups, the fewer keys reach the bound (K = 16 of 64: about 18 a
+// tile; K = 64 of 256: 74), and the longer it takes to rank them.
+__device__ __forceinline__ uint32_t beam_bound(BeamShared& s, int K, uint32_t top) {
+  if (K <= 16)
+    beam_bound_of<64>(s, K, top);
+  else
+    beam_bound_of<BEAM_THREADS>(s, K, top);
   return s.bound;
 }
 
-// s.list = the K best of the n unique keys in s.buf, best first.
+// s.list = the K best of the n keys in s.buf, best first.
 __device__ __forceinline__ void beam_rank(BeamShared& s, int K, int n) {
   for (int i = threadIdx.x; i < n; i += BEAM_THREADS) {
     const uint64_t mine = s.buf[i];
     int rank = 0;
+#pragma unroll 8
     for (int j = 0; j < n; ++j) rank += s.buf[j] > mine;
     if (rank < K) s.list[rank] = mine;
   }
@@ -121,6 +139,8 @@ __device__ __forceinline__ void beam_rank(BeamShared& s, int K, int n) {
   __syncthreads();
 }
 
+// The list's K best after BEAM_THREADS * PER more keys (key(j): this thread's
+// j-th, 0 for none).
 template <int PER, class Key>
 __device__ __forceinline__ void beam_keep_best(BeamShared& s, int K, Key key) {
   uint32_t top = 0;
@@ -139,180 +159,289 @@ __device__ __forceinline__ void beam_keep_best(BeamShared& s, int K, Key key) {
   beam_rank(s, K, s.count);
 }
 
-// A thread's BEAM_PER scores of the tile at e0 (positions are counted from the
-// 16-byte boundary at or before the row; off: the row's first): -inf outside it.
-template <typename T>
-__device__ __forceinline__ void beam_load_tile(const T* from, int64_t e0, int off, int64_t end, float (&x)[BEAM_PER]) {
-  constexpr int VEC = 16 / sizeof(T);
-#pragma unroll
-  for (int l = 0; l < BEAM_PER / VEC; ++l) {
-    const int64_t e = e0 + (l * BEAM_THREADS + threadIdx.x) * VEC;
-    float f[VEC];
-    if (e >= off && e + VEC <= end) {
-      beam_load16(from + e, f);
-    } else {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) f[i] = e + i >= off && e + i < end ? beam_load(from + e + i) : -INFINITY;
-    }
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) x[l * VEC + i] = f[i];
-  }
+// Scores past this are so far apart that a sum holds only those equal to the
+// maximum; where the maximum is past it, they are counted in a pass of their own
+// and the running sums stay 0 (masks of the type's lowest value alone in a row).
+constexpr float BEAM_FAR = 1e30f;
+
+// M for a maximum m: -M has to take every score to 0 or less.
+__device__ __forceinline__ float beam_shift(float m) {
+  return m < -BEAM_FAR ? 0.f : m > BEAM_FAR ? INFINITY : rintf(m * LOG2E);
+}
+// 2^(from - to) for whole numbers from <= to (0 under 2^-126; to may be infinite).
+__device__ __forceinline__ float beam_rescale(float from, float to) {
+  return __int_as_float((127 + static_cast<int>(fmaxf(from - to, -127.f))) << 23);
 }
 
+// A scan block's shared memory: its tiles, which the second pass of a run with
+// too many candidates uses for their keys.
+constexpr int BEAM_TILES_BYTES = BEAM_STAGES * BEAM_THREADS * 64;
+static_assert(BEAM_TILES_BYTES >= (BEAM_MAX + BEAM_THREADS * BEAM_PER) * 8, "room for a tile's keys");
 template <typename T>
-__global__ void __launch_bounds__(BEAM_THREADS, 4) beam_scan_kernel(const BeamParams p) {
+constexpr int BEAM_TILE = BEAM_THREADS * 64 / static_cast<int>(sizeof(T));
+
+// Sends for the 64 bytes of scores that this thread takes of the tile at e0
+// (positions are counted from the 16-byte boundary at or before the row; off:
+// the row's first, end: past its last), 16 at a time, into its own part of the
+// stage; -inf outside the row. Only the thread itself reads them.
+template <typename T>
+__device__ __forceinline__ void beam_send(uint8_t* stage, const T* from, int64_t e0, int off, int64_t end) {
   constexpr int VEC = 16 / sizeof(T);
-  __shared__ BeamShared s;
-  __shared__ float s_m[BEAM_THREADS / 32], s_s[BEAM_THREADS / 32];
-  const int split = blockIdx.x % p.splits;
-  const int64_t rw = blockIdx.x / p.splits;
+  if (e0 >= off && e0 + BEAM_TILE<T> <= end) {
+#pragma unroll
+    for (int l = 0; l < 4; ++l)
+      cp_async_16(smem_u32(stage) + (l * BEAM_THREADS + threadIdx.x) * 16,
+                  from + e0 + (l * BEAM_THREADS + threadIdx.x) * VEC, true);
+  } else if (e0 < end) {
+    for (int l = 0; l < 4; ++l) {
+      const int64_t e = e0 + (l * BEAM_THREADS + threadIdx.x) * VEC;
+      T* to = reinterpret_cast<T*>(stage) + (l * BEAM_THREADS + threadIdx.x) * VEC;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i)
+        to[i] = e + i >= off && e + i < end ? from[e + i] : static_cast<T>(-INFINITY);
+    }
+  }
+  cp_async_commit();
+}
+
+struct BeamScanShared {
+  BeamShared s;
+  uint64_t room[BEAM_ROOM];
+  float m[BEAM_THREADS / 32], sum[BEAM_THREADS / 32];
+};
+
+// One run: `tiles` tiles of beam rw's scores from tile split * tiles on. Returns
+// its maximum and sum (in every thread; a NaN or +inf score makes the sum NaN),
+// its best candidates' (score, token) keys in sh.s.list[0 .. sh.s.listed).
+template <typename T>
+__device__ __forceinline__ float2 beam_scan_run(const BeamParams& p, BeamScanShared& sh, uint8_t* s_tiles, int64_t rw,
+                                                int split) {
+  constexpr int VEC = 16 / sizeof(T), HALVES = 4 / sizeof(T), TILE = BEAM_TILE<T>;
+  BeamShared& s = sh.s;
   const int64_t r = rw / p.W, w = rw - r * p.W;
-  griddep_wait();
-  if (p.done != nullptr && p.done[rw]) return;  // an ended beam's scores are not read
   const T* row = static_cast<const T*>(p.scores) + r * p.stride_r + w * p.stride_w;
   const int off = static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
   const int64_t end = static_cast<int64_t>(off) + p.V;
   const T* from = row - off;
-  const int64_t run0 = static_cast<int64_t>(split) * p.tiles * BEAM_TILE;
-  const int64_t run1 = min(end, run0 + static_cast<int64_t>(p.tiles) * BEAM_TILE);
-  auto key_of = [&](float x, int64_t e0, int j) -> uint64_t {
-    const int64_t e = e0 + ((j / VEC) * BEAM_THREADS + threadIdx.x) * VEC + j % VEC;
-    return x > -INFINITY ? beam_key(x, static_cast<uint32_t>(e - off)) : 0;
-  };
-  if (threadIdx.x == 0) s.count = s.listed = 0;
-  float m = -INFINITY, sum = 0.f, least = -INFINITY;
-  float x[BEAM_PER];
-  beam_load_tile(from, run0, off, end, x);
-  for (int64_t e0 = run0; e0 < run1; e0 += BEAM_TILE) {
-    float next[BEAM_PER];
-    if (e0 + BEAM_TILE < run1) beam_load_tile(from, e0 + BEAM_TILE, off, end, next);
-    float top = x[0];
-#pragma unroll
-    for (int j = 1; j < BEAM_PER; ++j) top = fmaxf(top, x[j]);
-    if (e0 == run0) {
-      // the bound that every candidate has to reach, from the run's first tile
-      const uint32_t bound = beam_bound(s, p.K, top > -INFINITY ? order_key(top + 0.f) : 0u);
-      least = bound == 0 ? -INFINITY : beam_key_value(static_cast<uint64_t>(bound) << 32);
-    }
-    if (top >= least && top > -INFINITY) {
-#pragma unroll
-      for (int j = 0; j < BEAM_PER; ++j)
-        if (x[j] >= least && x[j] > -INFINITY) {
-          const int i = atomicAdd(&s.count, 1);
-          if (i < BEAM_ROOM) s.buf[i] = key_of(x[j], e0, j);
-        }
-    }
-    if (top > m) {
-      sum *= fast_exp2((m - top) * LOG2E);
-      m = top;
-    }
-    // a NaN score makes the sum NaN, and so does +inf (inf - inf)
-    const float shift = m == -INFINITY ? 0.f : m;
-    float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int j = 0; j < BEAM_PER; ++j) part[j & 3] += fast_exp2((x[j] - shift) * LOG2E);
-    sum += (part[0] + part[1]) + (part[2] + part[3]);
-#pragma unroll
-    for (int j = 0; j < BEAM_PER; ++j) x[j] = next[j];
+  const int64_t run0 = static_cast<int64_t>(split) * p.tiles * TILE;
+  const int64_t run1 = min(end, run0 + static_cast<int64_t>(p.tiles) * TILE);
+  // thread t's j-th score of the h-th 16 of its 64 bytes
+  auto place = [&](int h, int j) { return ((h * (BEAM_PER / VEC) + j / VEC) * BEAM_THREADS + threadIdx.x) * VEC + j % VEC; };
+  if (threadIdx.x == 0) {
+    s.count = s.listed = 0;
+    s.buf = sh.room;
   }
-  griddep_launch();
+  int at_stage = 0;
+#pragma unroll
+  for (int i = 0; i < BEAM_STAGES - 1; ++i)
+    beam_send(s_tiles + i * BEAM_THREADS * 64, from, run0 + i * TILE, off, run1);
+  float m = -INFINITY, least = -FLT_MAX, shift = 0.f;  // -inf is no candidate
+  uint64_t sums[2] = {0, 0};
+  int tile = 0;
+  for (int64_t e0 = run0; e0 < run1; e0 += TILE, ++tile) {
+    cp_async_wait<BEAM_STAGES - 2>();
+    const uint8_t* stage = s_tiles + at_stage * BEAM_THREADS * 64;
+    float x[BEAM_PER];
+#pragma unroll 1
+    for (int h = 0; h < HALVES; ++h) {
+#pragma unroll
+      for (int l = 0; l < BEAM_PER / VEC; ++l)
+        beam_load16(reinterpret_cast<const T*>(stage) + ((h * (BEAM_PER / VEC) + l) * BEAM_THREADS + threadIdx.x) * VEC,
+                    *reinterpret_cast<float(*)[VEC]>(x + l * VEC));
+      if (h == HALVES - 1) {
+        // the next tile, into the stage read one tile ago, by this thread
+        const int to = at_stage == 0 ? BEAM_STAGES - 1 : at_stage - 1;
+        beam_send(s_tiles + to * BEAM_THREADS * 64, from, e0 + (BEAM_STAGES - 1) * TILE, off, run1);
+      }
+      float top = x[0];
+#pragma unroll
+      for (int j = 1; j < BEAM_PER; ++j) top = fmaxf(top, x[j]);
+      if (e0 == run0 && h == 0) {
+        // the bound that every candidate has to reach, from the run's first scores
+        const uint32_t bound = beam_bound(s, p.K, top > -INFINITY ? order_key(top + 0.f) : 0u);
+        if (bound != 0) least = beam_key_value(static_cast<uint64_t>(bound) << 32);
+      }
+      if (top >= least) {
+        unsigned found = 0;
+#pragma unroll
+        for (int j = 0; j < BEAM_PER; ++j) found |= (x[j] >= least ? 1u : 0u) << j;
+        int i = atomicAdd(&s.count, __popc(found));
+        for (; found && i < BEAM_ROOM; found &= found - 1, ++i) {
+          const int at = __ffs(found) - 1;
+          float value = x[0];
+#pragma unroll
+          for (int j = 1; j < BEAM_PER; ++j) value = at == j ? x[j] : value;
+          sh.room[i] = beam_key(value, static_cast<uint32_t>(e0 + place(h, at) - off));
+        }
+      }
+      if (top > m) {
+        m = top;
+        const float was = shift;
+        shift = beam_shift(m);
+        const float f = sums[0] == 0 && sums[1] == 0 ? 1.f : beam_rescale(was, shift);
+        sums[0] = f2_mul(sums[0], f2_pack(f, f));
+        sums[1] = f2_mul(sums[1], f2_pack(f, f));
+      }
+      // a NaN score makes the sum NaN, and so does +inf (inf - inf)
+      const uint64_t l2 = f2_pack(LOG2E, LOG2E), s2 = f2_pack(-shift, -shift);
+#pragma unroll
+      for (int j = 0; j < BEAM_PER; j += 2) {
+        float a, b;
+        f2_unpack(f2_fma(f2_pack(x[j], x[j + 1]), l2, s2), a, b);
+        sums[(j / 2) & 1] = f2_add(sums[(j / 2) & 1], f2_pack(fast_exp2(a), fast_exp2(b)));
+      }
+    }
+    at_stage = at_stage == BEAM_STAGES - 1 ? 0 : at_stage + 1;
+    if ((tile & (tile + 1)) == 0 && e0 + TILE < run1) {
+      // after 1, 2, 4, ... tiles: the K best so far give a better bound
+      __syncthreads();
+      const int n = s.count;
+      __syncthreads();
+      if (n <= BEAM_ROOM) {
+        beam_rank(s, p.K, n);
+        if (threadIdx.x < s.listed) sh.room[threadIdx.x] = s.list[threadIdx.x];
+        if (threadIdx.x == 0) s.count = s.listed;
+        if (s.listed == p.K) least = fmaxf(least, beam_key_value(s.list[p.K - 1]));
+        __syncthreads();
+      }
+    }
+  }
   // (m, sum) over the block
+  float sum, other;
+  f2_unpack(f2_add(sums[0], sums[1]), sum, other);
+  sum += other;
   float mm = m;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (lane == 0) s_m[warp] = mm;
+  if (lane == 0) sh.m[warp] = mm;
   __syncthreads();
-  mm = s_m[0];
+  mm = sh.m[0];
 #pragma unroll
-  for (int i = 1; i < BEAM_THREADS / 32; ++i) mm = fmaxf(mm, s_m[i]);
-  // a thread that met nothing above -inf holds 0, or NaN
-  if (m > -INFINITY) sum *= fast_exp2((m - mm) * LOG2E);
+  for (int i = 1; i < BEAM_THREADS / 32; ++i) mm = fmaxf(mm, sh.m[i]);
+  if (sum != 0.f) sum *= beam_rescale(shift, beam_shift(mm));
+  if (fabsf(mm) > BEAM_FAR && fabsf(mm) < INFINITY)
+    for (int64_t e = max(run0, static_cast<int64_t>(off)) + threadIdx.x; e < run1; e += BEAM_THREADS)
+      sum += beam_load(from + e) == mm ? 1.f : 0.f;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0) s_s[warp] = sum;
+  if (lane == 0) sh.sum[warp] = sum;
   __syncthreads();
-  const int64_t run = rw * p.splits + split;
-  if (threadIdx.x == 0) {
-    float t = 0.f;
+  sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < BEAM_THREADS / 32; ++i) t += s_s[i];
-    p.stats[run] = make_float2(mm, t);
-  }
+  for (int i = 0; i < BEAM_THREADS / 32; ++i) sum += sh.sum[i];
   if (s.count <= BEAM_ROOM) {
     beam_rank(s, p.K, s.count);
   } else {
-    // more scores reached the first tile's bound than there is room for
-    // (scores that rise along the vocabulary, or many equal ones): once more
-    // over the run, keeping the best after every tile
-    for (int64_t e0 = run0; e0 < run1; e0 += BEAM_TILE) {
-      beam_load_tile(from, e0, off, end, x);
-      float top = x[0];
+    // more scores reached the bound than there is room for (scores that rise
+    // along the vocabulary, or many equal ones): once more over the run,
+    // keeping the best after every 16 scores a thread
+    cp_async_wait<0>();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      s.buf = reinterpret_cast<uint64_t*>(s_tiles);
+      s.listed = 0;
+    }
+    __syncthreads();
+    for (int64_t e0 = run0; e0 < run1; e0 += TILE) {
+      for (int h = 0; h < HALVES; ++h) {
+        float x[BEAM_PER], top = -INFINITY;
 #pragma unroll
-      for (int j = 1; j < BEAM_PER; ++j) top = fmaxf(top, x[j]);
-      const float worst = s.listed == p.K ? beam_key_value(s.list[p.K - 1]) : -INFINITY;
-      if (__syncthreads_or(top > worst)) beam_keep_best<BEAM_PER>(s, p.K, [&](int j) { return key_of(x[j], e0, j); });
+        for (int j = 0; j < BEAM_PER; ++j) {
+          const int64_t e = e0 + place(h, j);
+          x[j] = e >= off && e < run1 ? beam_load(from + e) : -INFINITY;
+          top = fmaxf(top, x[j]);
+        }
+        const float worst = s.listed == p.K ? beam_key_value(s.list[p.K - 1]) : -INFINITY;
+        if (__syncthreads_or(top > worst))
+          beam_keep_best<BEAM_PER>(s, p.K, [&](int j) -> uint64_t {
+            return x[j] > -INFINITY ? beam_key(x[j], static_cast<uint32_t>(e0 + place(h, j) - off)) : 0;
+          });
+      }
     }
   }
-  if (threadIdx.x < p.K) p.cand[run * p.K + threadIdx.x] = threadIdx.x < s.listed ? s.list[threadIdx.x] : 0;
+  return make_float2(mm, sum);
 }
 
-__global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const BeamParams p) {
+struct BeamMergeShared {
+  BeamShared s;
+  uint64_t keys[BEAM_MAX + BEAM_THREADS * 4];
+  float m[BEAM_MAX], log[BEAM_MAX];
+};
+
+// Text r's choice from its runs: stat(w, i) the maximum and sum of beam w's i-th
+// of `splits` runs, cand(w, i, k) its k-th candidate, 0 for none (neither is
+// asked of an ended beam).
+template <class Stat, class Cand>
+__device__ __forceinline__ void beam_merge(const BeamParams& p, BeamMergeShared& sh, int64_t r, Stat stat, Cand cand) {
   constexpr int PER = 4;
-  __shared__ BeamShared s;
-  __shared__ float s_m[BEAM_MAX], s_log[BEAM_MAX];
-  const int64_t r = blockIdx.x;
+  BeamShared& s = sh.s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  griddep_wait();
+  const int per_beam = p.splits * p.K;
+  const int total = p.W * per_beam;
+  // a thread's candidates of the tile at c0: (score, token) keys (an ended
+  // beam's first place: its end token), and their beams' totals
+  uint64_t found[PER];
+  float before[PER];
+  auto load = [&](int c0) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int c = c0 + j * BEAM_THREADS + threadIdx.x;
+      found[j] = 0;
+      if (c >= total) continue;
+      const int w = c / per_beam, i = c - w * per_beam;
+      before[j] = p.totals[r * p.W + w];
+      if (p.done == nullptr || !p.done[r * p.W + w])
+        found[j] = cand(w, i / p.K, i % p.K);
+      else if (i == 0)
+        found[j] = BEAM_ENDED | (0xFFFFFFFFu - static_cast<uint32_t>(p.end));
+    }
+  };
+  load(0);
   for (int w = warp; w < p.W; w += BEAM_THREADS / 32) {
     if (p.done != nullptr && p.done[r * p.W + w]) continue;
-    const float2* st = p.stats + (r * p.W + w) * p.splits;
     float m = -INFINITY;
-    for (int i = lane; i < p.splits; i += 32) m = fmaxf(m, st[i].x);
+    for (int i = lane; i < p.splits; i += 32) m = fmaxf(m, stat(w, i).x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float shift = beam_shift(m);
     float sum = 0.f;
     for (int i = lane; i < p.splits; i += 32) {
-      const float2 v = st[i];
-      // a run of -inf scores only adds nothing; a NaN sum stays NaN
-      sum += v.x > -INFINITY || isnan(v.y) ? v.y * expf(v.x - m) : 0.f;
+      const float2 v = stat(w, i);
+      // a NaN stays one whatever its weight
+      const float weight = fabsf(m) > BEAM_FAR ? (v.x == m ? 1.f : 0.f)
+                           : v.x < -BEAM_FAR   ? 0.f
+                                               : beam_rescale(beam_shift(v.x), shift);
+      sum += v.y * weight;
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) {
-      s_m[w] = m;
-      s_log[w] = logf(sum);
+      // log sum exp(x - m) from sum 2^(x L - M), where 2^L = e^(L ln 2)
+      sh.m[w] = m;
+      const double moved =
+          fabsf(m) > BEAM_FAR ? 0. : (static_cast<double>(shift) - static_cast<double>(m) * LOG2E) * 0.69314718055994531;
+      sh.log[w] = static_cast<float>(moved + log(static_cast<double>(sum)));
     }
   }
-  if (threadIdx.x == 0) s.listed = 0;
+  if (threadIdx.x == 0) {
+    s.listed = 0;
+    s.buf = sh.keys;
+  }
   __syncthreads();
-  const int per_beam = p.splits * p.K;
-  const int total = p.W * per_beam;
   for (int c0 = 0; c0 < total; c0 += BEAM_THREADS * PER) {
-    uint64_t keys[PER];
+    if (c0 > 0) load(c0);
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      const int c = c0 + j * BEAM_THREADS + threadIdx.x;
-      uint64_t key = 0;
-      if (c < total) {
-        const int w = c / per_beam;
-        const float t = p.totals[r * p.W + w];
-        float value = -INFINITY;
-        uint32_t token = 0;
-        if (p.done != nullptr && p.done[r * p.W + w]) {
-          if (c == w * per_beam) value = t, token = p.end;
-        } else {
-          const uint64_t k = p.cand[(r * p.W + w) * per_beam + (c - w * per_beam)];
-          if (k) {
-            value = t + ((beam_key_value(k) - s_m[w]) - s_log[w]);
-            token = 0xFFFFFFFFu - static_cast<uint32_t>(k);
-          }
-        }
-        if (value > -INFINITY) key = beam_key(value, static_cast<uint32_t>(w) * p.V + token);
-      }
-      keys[j] = key;
+      if (found[j] == 0) continue;
+      const int w = (c0 + j * BEAM_THREADS + static_cast<int>(threadIdx.x)) / per_beam;
+      const uint32_t token = 0xFFFFFFFFu - static_cast<uint32_t>(found[j]);
+      const float value = (found[j] >> 32) == (BEAM_ENDED >> 32)
+                              ? before[j]
+                              : before[j] + ((beam_key_value(found[j]) - sh.m[w]) - sh.log[w]);
+      found[j] = value > -INFINITY ? beam_key(value, static_cast<uint32_t>(w) * p.V + token) : 0;
     }
-    beam_keep_best<PER>(s, p.K, [&](int j) { return keys[j]; });
+    beam_keep_best<PER>(s, p.K, [&](int j) { return found[j]; });
   }
   if (threadIdx.x < p.K) {
     const int64_t o = r * p.K + threadIdx.x;
@@ -323,6 +452,30 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const BeamPara
     p.parents[o] = some ? static_cast<int64_t>(flat / static_cast<uint32_t>(p.V)) : -1;
     p.tokens[o] = some ? static_cast<int64_t>(flat % static_cast<uint32_t>(p.V)) : -1;
   }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(BEAM_THREADS, 4) beam_scan_kernel(const BeamParams p) {
+  extern __shared__ __align__(16) uint8_t s_tiles[];
+  __shared__ BeamScanShared sh;
+  const int split = blockIdx.x % p.splits;
+  const int64_t rw = blockIdx.x / p.splits;
+  griddep_wait();
+  if (p.done != nullptr && p.done[rw]) return;  // an ended beam's scores are not read
+  const float2 stat = beam_scan_run<T>(p, sh, s_tiles, rw, split);
+  const int64_t run = rw * p.splits + split;
+  griddep_launch();
+  if (threadIdx.x == 0) p.stats[run] = stat;
+  if (threadIdx.x < p.K) p.cand[run * p.K + threadIdx.x] = threadIdx.x < sh.s.listed ? sh.s.list[threadIdx.x] : 0;
+}
+
+__global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const BeamParams p) {
+  __shared__ BeamMergeShared sh;
+  const int64_t r = blockIdx.x;
+  griddep_wait();
+  beam_merge(
+      p, sh, r, [&](int w, int i) { return p.stats[(r * p.W + w) * p.splits + i]; },
+      [&](int w, int i, int k) { return p.cand[((r * p.W + w) * p.splits + i) * p.K + k]; });
 }
 
 // --------------------------------------------------------------- reordering

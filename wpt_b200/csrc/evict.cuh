@@ -4,11 +4,13 @@
 // weights (ties: the lowest row), `keep` in all, in their order, at the
 // front of new tables.
 //
-// evict_rows_kernel finds them: a radix select of the keep-th largest key
-// (three digits of 11, 11 and 10 bits; a thread-block cluster of `slices`
-// CTAs a row, each with a contiguous slice of the row's keys in shared
-// memory, the digit histograms summed over distributed shared memory), then
-// a count of the kept rows before each warp's run of keys gives their places.
+// evict_rows_kernel finds them: a cluster of `slices` CTAs a row, each with a
+// contiguous slice of the row's keys in shared memory. The threshold key is
+// found by histograms over equal ranges, first of all keys (lowest to highest:
+// a float's bits grow like its logarithm, so skewed weights spread over the
+// bins), then of the one bin that holds it, until a bin's keys are all kept or
+// all equal; the slices' histograms are summed over distributed shared memory.
+// A count of the kept rows before each warp's run of keys gives their places.
 // evict_gather_kernel copies the kept entries. Two kernels rather than one:
 // the selection wants few CTAs a row, the copy wants every SM.
 #pragma once
@@ -22,6 +24,7 @@ namespace wpt {
 
 constexpr int EVICT_THREADS = TOPK_THREADS;  // block_exclusive_scan's block
 constexpr int EVICT_BINS = 2048;
+constexpr int EVICT_COPY_THREADS = 256;
 
 struct EvictParams {
   const float* weights;  // (B, N), row stride weights_ld
@@ -51,17 +54,20 @@ __global__ void __launch_bounds__(EVICT_THREADS) evict_rows_kernel(const EvictPa
   extern __shared__ uint32_t s_keys[];  // cache_cap keys
   __shared__ uint32_t s_hist[2][EVICT_BINS];
   __shared__ int s_warp[EVICT_THREADS / 32];
+  __shared__ uint32_t s_red[EVICT_THREADS / 16];
   __shared__ int s_gt[EVICT_THREADS / 32], s_eq[EVICT_THREADS / 32];
   __shared__ int s_tot[2];
-  __shared__ uint32_t s_digit;
-  __shared__ int s_above, s_in;
+  __shared__ uint32_t s_mm[2];
+  __shared__ int s_bin, s_above, s_in;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.x / p.slices;
   const uint32_t rank = p.slices > 1 ? cluster_rank() : 0u;
+  for (int i = threadIdx.x; i < 2 * EVICT_BINS; i += EVICT_THREADS) (&s_hist[0][0])[i] = 0;
   griddep_wait();
   const int64_t raw = p.lengths[b];
   const int len = raw < 0 ? 0 : raw > p.N ? p.N : static_cast<int>(raw);
   const int count = len < p.keep ? len : p.keep;
+  const bool cut = len > p.keep;
   const float* src = p.weights + static_cast<int64_t>(b) * p.weights_ld;
 
   // this CTA's slice [base, base + n), cut into one run of `run` keys a warp
@@ -72,69 +78,110 @@ __global__ void __launch_bounds__(EVICT_THREADS) evict_rows_kernel(const EvictPa
   const int run = slice / (EVICT_THREADS / 32);
   const bool cached = n <= p.cache_cap;
   const int kept_from = len - p.recent;  // rows from here on, and those before `first`, are always kept
+  constexpr uint32_t ALWAYS = 0xFFFFFFFFu;  // their key; the others' are at most +inf's, 0xFF800000
   auto make_key = [&](int i) -> uint32_t {  // i: index in the slice
     const int row = base + i;
-    return row < p.first || row >= kept_from ? 0xFFFFFFFFu : evict_key(src[row]);
+    return row < p.first || row >= kept_from ? ALWAYS : evict_key(src[row]);
   };
-  auto key_at = [&](int i) { return cached ? s_keys[i] : make_key(i); };
+  // (nothing competes, and nothing is cached, when the always kept rows fill the budget)
+  auto key_at = [&](int i) { return cached && p.keep > p.first + p.recent ? s_keys[i] : make_key(i); };
+  auto meet = [&] {
+    if (p.slices > 1)
+      cluster_sync();
+    else
+      __syncthreads();
+  };
 
   // the threshold: keys above it are kept, and the first `ties` of those equal to it
-  uint32_t threshold = p.keep > 0 ? 0u : 0xFFFFFFFFu;
-  int ties = 0;
-  if (len > p.keep) {
-    if (cached)
-      for (int i = threadIdx.x; i < n; i += EVICT_THREADS) s_keys[i] = make_key(i);
-    uint32_t prefix = 0;
-    int need = p.keep, shift = 32;
-    for (int pass = 0; pass < 3 && need > 0; ++pass) {
-      const int bits = pass < 2 ? 11 : 10;
-      const int high = shift;  // the digit is bits [shift - bits, shift)
-      shift -= bits;
-      uint32_t* hist = s_hist[pass & 1];
-      for (int i = threadIdx.x; i < EVICT_BINS; i += EVICT_THREADS) hist[i] = 0;
-      __syncthreads();
+  uint32_t threshold = ALWAYS - 1;
+  int ties = 0, need = p.keep - p.first - p.recent;
+  if (cut && need > 0) {
+    uint32_t lo = ALWAYS, hi = 0;  // of the keys that compete
+    if (cached) {
+#pragma unroll 4
       for (int i = threadIdx.x; i < n; i += EVICT_THREADS) {
-        const uint32_t key = key_at(i);
-        if (high == 32 || (key >> high) == prefix) atomicAdd(&hist[(key >> shift) & ((1u << bits) - 1)], 1u);
+        const uint32_t key = make_key(i);
+        s_keys[i] = key;
+        if (key != ALWAYS) {
+          lo = min(lo, key);
+          hi = max(hi, key);
+        }
       }
-      // The bins from the top, two a thread. The other histogram is cleared in
-      // the next pass only, which every CTA reaches after this pass's barrier,
-      // so a slower CTA still finds this one whole.
-      if (p.slices > 1)
-        cluster_sync();
-      else
-        __syncthreads();
-      const int hi_bin = EVICT_BINS - 1 - 2 * threadIdx.x;
+    } else {
+      for (int i = threadIdx.x; i < n; i += EVICT_THREADS) {
+        const uint32_t key = make_key(i);
+        if (key != ALWAYS) {
+          lo = min(lo, key);
+          hi = max(hi, key);
+        }
+      }
+    }
+    block_minmax(lo, hi, s_red);
+    if (p.slices > 1) {
+      if (threadIdx.x == 0) {
+        s_mm[0] = lo;
+        s_mm[1] = hi;
+      }
+      cluster_sync();
+      for (int r = 0; r < p.slices; ++r) {
+        lo = min(lo, dsmem_ld_u32(dsmem_map(smem_u32(s_mm), r)));
+        hi = max(hi, dsmem_ld_u32(dsmem_map(smem_u32(s_mm + 1), r)));
+      }
+    }
+    for (int pass = 0;; ++pass) {
+      // keys in [lo, hi], in bins of 2^shift
+      const uint32_t range = hi - lo;
+      const int shift = range < EVICT_BINS ? 0 : 32 - __clz(range) - 11;
+      uint32_t* hist = s_hist[pass & 1];
+#pragma unroll 4
+      for (int i = threadIdx.x; i < n; i += EVICT_THREADS) {
+        const uint32_t d = key_at(i) - lo;  // ALWAYS is above hi
+        if (d <= range) atomicAdd(&hist[d >> shift], 1u);
+      }
+      meet();
+      // The bins from the top, two a thread.
+      const int top_bin = EVICT_BINS - 1 - 2 * threadIdx.x;
       uint32_t c0 = 0, c1 = 0;
       if (p.slices > 1) {
         for (int r = 0; r < p.slices; ++r) {
-          c0 += dsmem_ld_u32(dsmem_map(smem_u32(hist + hi_bin), r));
-          c1 += dsmem_ld_u32(dsmem_map(smem_u32(hist + hi_bin - 1), r));
+          c0 += dsmem_ld_u32(dsmem_map(smem_u32(hist + top_bin), r));
+          c1 += dsmem_ld_u32(dsmem_map(smem_u32(hist + top_bin - 1), r));
         }
       } else {
-        c0 = hist[hi_bin];
-        c1 = hist[hi_bin - 1];
+        c0 = hist[top_bin];
+        c1 = hist[top_bin - 1];
       }
       int total;
       const int above = block_exclusive_scan(static_cast<int>(c0 + c1), s_warp, &total);
       if (above < need && need <= above + static_cast<int>(c0)) {
-        s_digit = hi_bin;
+        s_bin = top_bin;
         s_above = above;
         s_in = c0;
       } else if (above + static_cast<int>(c0) < need && need <= above + static_cast<int>(c0 + c1)) {
-        s_digit = hi_bin - 1;
+        s_bin = top_bin - 1;
         s_above = above + c0;
         s_in = c1;
       }
       __syncthreads();
-      prefix = (prefix << bits) | s_digit;
+      const uint32_t bin_lo = lo + (static_cast<uint32_t>(s_bin) << shift);
       need -= s_above;
-      if (s_in == need) {  // the whole bin is kept: no need to look inside it
-        threshold = (prefix << shift) - 1u;  // keys are at least -inf's, 0x007FFFFF: no wrap
-        need = 0;
-      } else if (pass == 2) {
-        threshold = prefix;
+      if (s_in == need) {  // the whole bin is kept
+        threshold = bin_lo - 1;  // keys are at least -inf's, 0x007FFFFF: no wrap
+        break;
+      }
+      if (shift == 0) {  // one key's bin
+        threshold = bin_lo;
         ties = need;
+        break;
+      }
+      lo = bin_lo;
+      hi = min(hi, bin_lo + ((1u << shift) - 1u));
+      // The two histograms take turns. The next one was last read in the pass
+      // before this one, by CTAs that have all come to this pass's meeting.
+      if (pass > 0) {
+        uint32_t* next = s_hist[(pass + 1) & 1];
+        for (int i = threadIdx.x; i < EVICT_BINS; i += EVICT_THREADS) next[i] = 0;
+        __syncthreads();
       }
     }
   }
@@ -142,7 +189,7 @@ __global__ void __launch_bounds__(EVICT_THREADS) evict_rows_kernel(const EvictPa
   // kept rows of each warp's run of keys, then of the warps and slices before it
   const int run0 = min(n, warp * run), run1 = min(n, run0 + run);
   int gt = 0, eq = 0;
-  if (len > p.keep) {
+  if (cut) {
     for (int i0 = run0; i0 < run1; i0 += 32) {
       const int i = i0 + lane;
       const uint32_t key = i < run1 ? key_at(i) : 0u;
@@ -157,22 +204,25 @@ __global__ void __launch_bounds__(EVICT_THREADS) evict_rows_kernel(const EvictPa
     s_eq[warp] = eq;
   }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    int g = 0, e = 0;
-    for (int w = 0; w < EVICT_THREADS / 32; ++w) {
-      const int g1 = s_gt[w], e1 = s_eq[w];
-      s_gt[w] = g;
-      s_eq[w] = e;
-      g += g1;
-      e += e1;
+  if (warp == 0) {
+    int g = s_gt[lane], e = s_eq[lane];
+    const int g1 = g, e1 = e;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int gy = __shfl_up_sync(0xffffffffu, g, o), ey = __shfl_up_sync(0xffffffffu, e, o);
+      if (lane >= o) {
+        g += gy;
+        e += ey;
+      }
     }
-    s_tot[0] = g;
-    s_tot[1] = e;
+    s_gt[lane] = g - g1;
+    s_eq[lane] = e - e1;
+    if (lane == 31) {
+      s_tot[0] = g;
+      s_tot[1] = e;
+    }
   }
-  if (p.slices > 1)
-    cluster_sync();
-  else
-    __syncthreads();
+  meet();
   gt = s_gt[warp];
   eq = s_eq[warp];
   for (uint32_t r = 0; r < rank; ++r) {
@@ -184,7 +234,7 @@ __global__ void __launch_bounds__(EVICT_THREADS) evict_rows_kernel(const EvictPa
   for (int i0 = run0; i0 < run1; i0 += 32) {
     const int i = i0 + lane;
     bool above = i < run1, equal = false;
-    if (len > p.keep) {
+    if (cut) {
       const uint32_t key = i < run1 ? key_at(i) : 0u;
       above = above && key > threshold;
       equal = i < run1 && ties > 0 && key == threshold;
@@ -222,20 +272,36 @@ struct GatherParams {
 // product over a whole tile of the new table multiplies its unread rows by
 // zero weights, which must not meet a NaN).
 template <typename Unit>
-__global__ void __launch_bounds__(256) evict_gather_kernel(const GatherParams p) {
+__global__ void __launch_bounds__(EVICT_COPY_THREADS) evict_gather_kernel(const GatherParams p) {
+  constexpr int ROWS = 4;  // places a thread has in flight
   const int b = blockIdx.x / p.chunks, chunk = blockIdx.x - b * p.chunks;
   const uint8_t* src = p.src + b * p.src_sb;
   Unit* dst = reinterpret_cast<Unit*>(p.dst) + static_cast<int64_t>(b) * p.capacity * p.units;
   const int64_t* rows = p.rows + static_cast<int64_t>(b) * p.keep;
-  const int64_t total = static_cast<int64_t>(p.capacity) * p.units;
+  // a group of threads a place, a unit each (long rows: several)
+  const int group = min(p.units, EVICT_COPY_THREADS), groups = EVICT_COPY_THREADS / group;
+  const int mine = threadIdx.x / group, unit = threadIdx.x - mine * group;
   griddep_wait();
-  for (int64_t u = static_cast<int64_t>(chunk) * 256 + threadIdx.x; u < total;
-       u += static_cast<int64_t>(p.chunks) * 256) {
-    const int i = static_cast<int>(u / p.units), c = static_cast<int>(u - static_cast<int64_t>(i) * p.units);
-    const int64_t row = i < p.keep ? rows[i] : -1;
-    Unit v{};
-    if (row >= 0) v = *(reinterpret_cast<const Unit*>(src + row * p.src_sn) + c);
-    dst[u] = v;
+  if (mine >= groups) return;
+  const int step = p.chunks * groups;
+  for (int64_t i0 = chunk * groups + mine; i0 < p.capacity; i0 += static_cast<int64_t>(ROWS) * step) {
+    const Unit* from[ROWS];
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+      const int64_t i = i0 + static_cast<int64_t>(k) * step;
+      const int64_t row = i < p.keep ? rows[i] : -1;
+      from[k] = row >= 0 ? reinterpret_cast<const Unit*>(src + row * p.src_sn) : nullptr;
+    }
+    for (int c = unit; c < p.units; c += group) {
+      Unit v[ROWS];
+#pragma unroll
+      for (int k = 0; k < ROWS; ++k) v[k] = from[k] != nullptr ? from[k][c] : Unit{};
+#pragma unroll
+      for (int k = 0; k < ROWS; ++k) {
+        const int64_t i = i0 + static_cast<int64_t>(k) * step;
+        if (i < p.capacity) dst[i * p.units + c] = v[k];
+      }
+    }
   }
 }
 

@@ -1533,7 +1533,7 @@ extern "C" int wpt_cache_evict(const void* held, int64_t held_stride_b, int64_t 
   p.first = first;
   p.capacity = capacity;
   p.slices = 1;
-  while (p.slices < 8 && N > 8192 * p.slices && static_cast<int64_t>(B) * p.slices * 2 <= sms) p.slices *= 2;
+  while (p.slices < 8 && N > 16384 * p.slices && static_cast<int64_t>(B) * p.slices * 2 <= sms) p.slices *= 2;
   const int slice = (N / p.slices + 1024) / 1024 * 1024;
   p.cache_cap = slice < 49152 ? slice : 49152;
   if (int rc = launch_dependent("evict_rows_kernel launch", wpt::evict_rows_kernel, static_cast<int64_t>(B) * p.slices,
@@ -1550,32 +1550,43 @@ extern "C" int wpt_cache_evict(const void* held, int64_t held_stride_b, int64_t 
   g.capacity = capacity;
   const bool wide = at % 16 == 0;
   g.units = row_bytes / (wide ? 16 : 4);
-  const int64_t blocks = (static_cast<int64_t>(capacity) * g.units + 255) / 256;
+  // eight CTAs an SM, no more than have a place for every group of threads
+  const int groups = wpt::EVICT_COPY_THREADS / std::min(std::max(g.units, 1), wpt::EVICT_COPY_THREADS);
+  const int64_t blocks = (static_cast<int64_t>(capacity) + groups - 1) / groups;
   g.chunks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(blocks, (int64_t(8) * sms + B - 1) / B)));
   if (wide)
     return launch_dependent("evict_gather_kernel launch", wpt::evict_gather_kernel<uint4>,
-                            static_cast<int64_t>(B) * g.chunks, 256, 0, 1, s, g);
+                            static_cast<int64_t>(B) * g.chunks, wpt::EVICT_COPY_THREADS, 0, 1, s, g);
   return launch_dependent("evict_gather_kernel launch", wpt::evict_gather_kernel<uint32_t>,
-                          static_cast<int64_t>(B) * g.chunks, 256, 0, 1, s, g);
+                          static_cast<int64_t>(B) * g.chunks, wpt::EVICT_COPY_THREADS, 0, 1, s, g);
 }
 
 namespace {
-// Runs a beam's scores are cut into, and tiles a run.
-void beam_plan(int64_t R, int64_t W, int64_t V, int sms, int* splits, int* tiles) {
-  const int64_t all = (V + 8 + wpt::BEAM_TILE - 1) / wpt::BEAM_TILE;  // a row may start 7 scores into its first tile
-  int64_t want = (4 * static_cast<int64_t>(sms) + R * W - 1) / (R * W);
+// Runs a beam's scores are cut into, and tiles a run: enough runs for two an SM
+// (64 texts of 8 beams: whole beams 29.8 us, halves 30.6, quarters 32.0).
+void beam_plan(int64_t R, int64_t W, int64_t V, bool bf16, int sms, int* splits, int* tiles) {
+  const int es = bf16 ? 2 : 4;
+  const int64_t tile = wpt::BEAM_THREADS * 64 / es;
+  const int64_t all = (V + 16 / es - 1 + tile - 1) / tile;  // a row may start off a 16-byte boundary
+  int64_t want = (2 * static_cast<int64_t>(sms) + R * W - 1) / (R * W);
   if (want > all) want = all;
   if (want < 1) want = 1;
   *tiles = static_cast<int>((all + want - 1) / want);
   *splits = static_cast<int>((all + *tiles - 1) / *tiles);
 }
+
+template <typename T>
+int launch_beam_scan(const wpt::BeamParams& p, cudaStream_t stream) {
+  return launch_dependent("beam_scan_kernel launch", wpt::beam_scan_kernel<T>, static_cast<int64_t>(p.R) * p.W * p.splits,
+                          wpt::BEAM_THREADS, wpt::BEAM_TILES_BYTES, 1, stream, p);
+}
 }  // namespace
 
-extern "C" size_t wpt_beam_scratch_bytes(int R, int W, int V, int K) {
+extern "C" size_t wpt_beam_scratch_bytes(int R, int W, int V, int K, int bf16) {
   if (R < 1 || W < 1 || V < 1 || K < 1) return 0;
   int sms = 148, splits, tiles;
   current_device(&sms);
-  beam_plan(R, W, V, sms, &splits, &tiles);
+  beam_plan(R, W, V, bf16 != 0, sms, &splits, &tiles);
   return static_cast<size_t>(R) * W * splits * (8 + 8 * static_cast<size_t>(K));
 }
 
@@ -1590,13 +1601,13 @@ extern "C" int wpt_beam_select(const void* scores, int bf16, int64_t stride_r, i
   if (R == 0) return WPT_OK;
   if (!scores || !totals || !scratch || !out_totals || !parents || !tokens)
     return fail(WPT_ERR_INVALID, "a required pointer is NULL");
-  if (done && (end < 0 || end >= V)) return fail(WPT_ERR_INVALID, "end token %d of a vocabulary of %d", end, V);
   if (reinterpret_cast<uintptr_t>(scratch) & 7) return fail(WPT_ERR_INVALID, "scratch must be 8-byte aligned");
+  if (done && (end < 0 || end >= V)) return fail(WPT_ERR_INVALID, "end token %d of a vocabulary of %d", end, V);
   if (reinterpret_cast<uintptr_t>(scores) & (bf16 ? 1 : 3)) return fail(WPT_ERR_INVALID, "scores are misaligned");
   int sms = 148;
   current_device(&sms);
   wpt::BeamParams p;
-  beam_plan(R, W, V, sms, &p.splits, &p.tiles);
+  beam_plan(R, W, V, bf16 != 0, sms, &p.splits, &p.tiles);
   p.scores = scores;
   p.stride_r = stride_r;
   p.stride_w = stride_w;
@@ -1613,12 +1624,7 @@ extern "C" int wpt_beam_select(const void* scores, int bf16, int64_t stride_r, i
   p.K = K;
   p.end = end;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int64_t runs = static_cast<int64_t>(R) * W * p.splits;
-  const int rc = bf16 ? launch_dependent("beam_scan_kernel launch", wpt::beam_scan_kernel<__nv_bfloat16>, runs,
-                                         wpt::BEAM_THREADS, 0, 1, s, p)
-                      : launch_dependent("beam_scan_kernel launch", wpt::beam_scan_kernel<float>, runs,
-                                         wpt::BEAM_THREADS, 0, 1, s, p);
-  if (rc) return rc;
+  if (int rc = bf16 ? launch_beam_scan<__nv_bfloat16>(p, s) : launch_beam_scan<float>(p, s)) return rc;
   return launch_dependent("beam_merge_kernel launch", wpt::beam_merge_kernel, R, wpt::BEAM_THREADS, 0, 1, s, p);
 }
 

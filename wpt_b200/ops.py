@@ -685,7 +685,7 @@ def beam_select(scores, totals, beams, done=None, end=None):
     parents = torch.empty(R, beams, dtype=torch.int64, device=device)
     tokens = torch.empty_like(parents)
     lib = _lib.lib()
-    scratch = torch.empty(lib.wpt_beam_scratch_bytes(R, W, V, beams), dtype=torch.uint8, device=device)
+    scratch = torch.empty(lib.wpt_beam_scratch_bytes(R, W, V, beams, bf16), dtype=torch.uint8, device=device)
     _call(device, lib.wpt_beam_select, scores.data_ptr(), bf16, sr, sw, totals.data_ptr(),
           None if done is None else done.data_ptr(), 0 if end is None else end, scratch.data_ptr(), out.data_ptr(),
           parents.data_ptr(), tokens.data_ptr(), R, W, V, beams)
