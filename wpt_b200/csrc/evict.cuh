@@ -10,7 +10,7 @@
 // a float's bits grow like its logarithm, so skewed weights spread over the
 // bins), then of the one bin that holds it, until a bin's keys are all kept or
 // all equal; the slices' histograms are summed over distributed shared memory.
-// A count of the kept rows before each warp's run of keys gives their places.
+// A count of the kept rows before each thread's run of keys gives their places.
 // evict_gather_kernel copies the kept entries. Two kernels rather than one:
 // the selection wants few CTAs a row, the copy wants every SM.
 #pragma once
@@ -24,7 +24,8 @@ namespace wpt {
 
 constexpr int EVICT_THREADS = TOPK_THREADS;  // block_exclusive_scan's block
 constexpr int EVICT_BINS = 2048;
-constexpr int EVICT_COPY_THREADS = 256;
+constexpr int EVICT_QUADS = 4 * EVICT_THREADS;  // a slice is a multiple of this: whole quads a thread
+constexpr int EVICT_COPY_THREADS = 256, EVICT_COPY_CTAS = 5;  // CTAs an SM
 
 struct EvictParams {
   const float* weights;  // (B, N), row stride weights_ld
@@ -51,7 +52,7 @@ __device__ __forceinline__ uint32_t dsmem_ld_u32(uint32_t addr) {
 }
 
 __global__ void __launch_bounds__(EVICT_THREADS) evict_rows_kernel(const EvictParams p) {
-  extern __shared__ uint32_t s_keys[];  // cache_cap keys
+  extern __shared__ __align__(16) uint32_t s_keys[];  // cache_cap keys
   __shared__ uint32_t s_hist[2][EVICT_BINS];
   __shared__ int s_warp[EVICT_THREADS / 32];
   __shared__ uint32_t s_red[EVICT_THREADS / 16];
@@ -62,29 +63,64 @@ __global__ void __launch_bounds__(EVICT_THREADS) evict_rows_kernel(const EvictPa
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.x / p.slices;
   const uint32_t rank = p.slices > 1 ? cluster_rank() : 0u;
-  for (int i = threadIdx.x; i < 2 * EVICT_BINS; i += EVICT_THREADS) (&s_hist[0][0])[i] = 0;
+  reinterpret_cast<uint4*>(s_hist)[threadIdx.x] = make_uint4(0, 0, 0, 0);
+  static_assert(sizeof(s_hist) == EVICT_THREADS * 16, "a quad a thread");
   griddep_wait();
   const int64_t raw = p.lengths[b];
   const int len = raw < 0 ? 0 : raw > p.N ? p.N : static_cast<int>(raw);
   const int count = len < p.keep ? len : p.keep;
-  const bool cut = len > p.keep;
   const float* src = p.weights + static_cast<int64_t>(b) * p.weights_ld;
+  int64_t* rows = p.rows + static_cast<int64_t>(b) * p.keep;
+  float* kept = p.weights_out + static_cast<int64_t>(b) * p.capacity;
+  if (rank == 0) {
+    for (int i = count + threadIdx.x; i < p.keep; i += EVICT_THREADS) rows[i] = -1;
+    for (int i = count + threadIdx.x; i < p.capacity; i += EVICT_THREADS) kept[i] = 0.f;
+    if (threadIdx.x == 0) p.counts[b] = count;
+  }
+  if (len <= p.keep) {  // everything is kept (the same decision on all CTAs of the cluster)
+    for (int i = rank * EVICT_THREADS + threadIdx.x; i < len; i += p.slices * EVICT_THREADS) {
+      rows[i] = i;
+      kept[i] = src[i];
+    }
+    return;
+  }
 
-  // this CTA's slice [base, base + n), cut into one run of `run` keys a warp
-  const int slice = ((len + p.slices - 1) / p.slices + EVICT_THREADS - 1) / EVICT_THREADS * EVICT_THREADS;
+  // this CTA's slice [base, base + n), in quads; `quads` of them a thread
+  const int quads = ((len + p.slices - 1) / p.slices + EVICT_QUADS - 1) / EVICT_QUADS, slice = quads * EVICT_QUADS;
   const int64_t base64 = static_cast<int64_t>(rank) * slice;
   const int base = base64 < len ? static_cast<int>(base64) : len;
   const int n = min(slice, len - base);
-  const int run = slice / (EVICT_THREADS / 32);
-  const bool cached = n <= p.cache_cap;
-  const int kept_from = len - p.recent;  // rows from here on, and those before `first`, are always kept
-  constexpr uint32_t ALWAYS = 0xFFFFFFFFu;  // their key; the others' are at most +inf's, 0xFF800000
-  auto make_key = [&](int i) -> uint32_t {  // i: index in the slice
-    const int row = base + i;
-    return row < p.first || row >= kept_from ? ALWAYS : evict_key(src[row]);
+  const bool cached = slice <= p.cache_cap;
+  const int kept_from = len - p.recent - base;  // slice indices from here on, and under kept_to, are always kept
+  const int kept_to = p.first - base;
+  constexpr uint32_t ALWAYS = 0xFFFFFFFFu;  // their key; the others' are from 0x007FFFFF (-inf) to 0xFF800000; none: 0
+  const bool aligned = (reinterpret_cast<uintptr_t>(src + base) & 15) == 0;
+  // the weights' keys of quad c, whether always kept or not
+  auto load4 = [&](int c) {
+    const int i = 4 * c;
+    if (aligned && i + 4 <= n) {
+      const float4 f = *reinterpret_cast<const float4*>(src + base + i);
+      return make_uint4(evict_key(f.x), evict_key(f.y), evict_key(f.z), evict_key(f.w));
+    }
+    uint4 k = make_uint4(0, 0, 0, 0);
+    if (i < n) k.x = evict_key(src[base + i]);
+    if (i + 1 < n) k.y = evict_key(src[base + i + 1]);
+    if (i + 2 < n) k.z = evict_key(src[base + i + 2]);
+    if (i + 3 < n) k.w = evict_key(src[base + i + 3]);
+    return k;
   };
-  // (nothing competes, and nothing is cached, when the always kept rows fill the budget)
-  auto key_at = [&](int i) { return cached && p.keep > p.first + p.recent ? s_keys[i] : make_key(i); };
+  auto keys4 = [&](int c) {
+    if (cached) return reinterpret_cast<const uint4*>(s_keys)[c];
+    uint4 k = load4(c);
+    const int i = 4 * c;
+    if (i < kept_to || i + 3 >= kept_from) {
+      if (i < n && (i < kept_to || i >= kept_from)) k.x = ALWAYS;
+      if (i + 1 < n && (i + 1 < kept_to || i + 1 >= kept_from)) k.y = ALWAYS;
+      if (i + 2 < n && (i + 2 < kept_to || i + 2 >= kept_from)) k.z = ALWAYS;
+      if (i + 3 < n && (i + 3 < kept_to || i + 3 >= kept_from)) k.w = ALWAYS;
+    }
+    return k;
+  };
   auto meet = [&] {
     if (p.slices > 1)
       cluster_sync();
@@ -92,168 +128,181 @@ __global__ void __launch_bounds__(EVICT_THREADS) evict_rows_kernel(const EvictPa
       __syncthreads();
   };
 
+  // bounds of the keys, and the keys into shared memory
+  uint32_t lo = ALWAYS, hi = 0;
+  for (int c0 = 0; c0 < quads * EVICT_THREADS; c0 += 2 * EVICT_THREADS) {
+    uint4 k[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int c = c0 + h * EVICT_THREADS + threadIdx.x;
+      k[h] = c < quads * EVICT_THREADS ? load4(c) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int c = c0 + h * EVICT_THREADS + threadIdx.x;
+      if (cached && c < quads * EVICT_THREADS) reinterpret_cast<uint4*>(s_keys)[c] = k[h];
+      hi = max(max(hi, max(k[h].x, k[h].y)), max(k[h].z, k[h].w));
+      // 0, past the slice's end, wraps to the largest
+      lo = min(min(lo, min(k[h].x - 1, k[h].y - 1)), min(k[h].z - 1, k[h].w - 1));
+    }
+  }
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  if (lane == 0) {
+    s_red[warp] = lo;
+    s_red[32 + warp] = hi;
+  }
+  __syncthreads();
+  if (cached) {  // the always kept rows' keys
+    for (int i = threadIdx.x; i < min(kept_to, n); i += EVICT_THREADS) s_keys[i] = ALWAYS;
+    for (int i = max(kept_from, 0) + threadIdx.x; i < n; i += EVICT_THREADS) s_keys[i] = ALWAYS;
+  }
+  lo = __reduce_min_sync(0xffffffffu, s_red[lane]);
+  hi = __reduce_max_sync(0xffffffffu, s_red[32 + lane]);
+  if (p.slices > 1) {
+    if (threadIdx.x == 0) {
+      s_mm[0] = lo;
+      s_mm[1] = hi;
+    }
+    cluster_sync();
+    for (int r = 0; r < p.slices; ++r) {
+      lo = min(lo, dsmem_ld_u32(dsmem_map(smem_u32(s_mm), r)));
+      hi = max(hi, dsmem_ld_u32(dsmem_map(smem_u32(s_mm + 1), r)));
+    }
+  } else {
+    __syncthreads();
+  }
+  lo += 1;
+
   // the threshold: keys above it are kept, and the first `ties` of those equal to it
   uint32_t threshold = ALWAYS - 1;
   int ties = 0, need = p.keep - p.first - p.recent;
-  if (cut && need > 0) {
-    uint32_t lo = ALWAYS, hi = 0;  // of the keys that compete
-    if (cached) {
-#pragma unroll 4
-      for (int i = threadIdx.x; i < n; i += EVICT_THREADS) {
-        const uint32_t key = make_key(i);
-        s_keys[i] = key;
-        if (key != ALWAYS) {
-          lo = min(lo, key);
-          hi = max(hi, key);
-        }
+  for (int pass = 0; need > 0; ++pass) {
+    // keys in [lo, hi], in bins of 2^shift
+    const uint32_t range = hi - lo;
+    const int shift = range < EVICT_BINS ? 0 : 32 - __clz(range) - 11;
+    uint32_t* hist = s_hist[pass & 1];
+    auto tally = [&](uint32_t key) {  // 0 and ALWAYS are out of the range
+      const uint32_t d = key - lo;
+      if (d <= range) atomicAdd(&hist[d >> shift], 1u);
+    };
+    for (int c = threadIdx.x; c < quads * EVICT_THREADS; c += EVICT_THREADS) {
+      const uint4 k = keys4(c);
+      tally(k.x);
+      tally(k.y);
+      tally(k.z);
+      tally(k.w);
+    }
+    meet();
+    // The bins from the top, two a thread: each warp's sum, the warps above
+    // it, and the bin where the count reaches `need`.
+    const int top_bin = EVICT_BINS - 1 - 2 * threadIdx.x;
+    int c0 = 0, c1 = 0;
+    if (p.slices > 1) {
+      for (int r = 0; r < p.slices; ++r) {
+        c0 += dsmem_ld_u32(dsmem_map(smem_u32(hist + top_bin), r));
+        c1 += dsmem_ld_u32(dsmem_map(smem_u32(hist + top_bin - 1), r));
       }
     } else {
-      for (int i = threadIdx.x; i < n; i += EVICT_THREADS) {
-        const uint32_t key = make_key(i);
-        if (key != ALWAYS) {
-          lo = min(lo, key);
-          hi = max(hi, key);
-        }
-      }
+      c0 = hist[top_bin];
+      c1 = hist[top_bin - 1];
     }
-    block_minmax(lo, hi, s_red);
-    if (p.slices > 1) {
-      if (threadIdx.x == 0) {
-        s_mm[0] = lo;
-        s_mm[1] = hi;
+    const int sum = __reduce_add_sync(0xffffffffu, c0 + c1);
+    if (lane == 0) s_warp[warp] = sum;
+    __syncthreads();
+    int before = __reduce_add_sync(0xffffffffu, lane < warp ? s_warp[lane] : 0);
+    if (before < need && need <= before + sum) {
+      int incl = c0 + c1;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
       }
-      cluster_sync();
-      for (int r = 0; r < p.slices; ++r) {
-        lo = min(lo, dsmem_ld_u32(dsmem_map(smem_u32(s_mm), r)));
-        hi = max(hi, dsmem_ld_u32(dsmem_map(smem_u32(s_mm + 1), r)));
-      }
-    }
-    for (int pass = 0;; ++pass) {
-      // keys in [lo, hi], in bins of 2^shift
-      const uint32_t range = hi - lo;
-      const int shift = range < EVICT_BINS ? 0 : 32 - __clz(range) - 11;
-      uint32_t* hist = s_hist[pass & 1];
-#pragma unroll 4
-      for (int i = threadIdx.x; i < n; i += EVICT_THREADS) {
-        const uint32_t d = key_at(i) - lo;  // ALWAYS is above hi
-        if (d <= range) atomicAdd(&hist[d >> shift], 1u);
-      }
-      meet();
-      // The bins from the top, two a thread.
-      const int top_bin = EVICT_BINS - 1 - 2 * threadIdx.x;
-      uint32_t c0 = 0, c1 = 0;
-      if (p.slices > 1) {
-        for (int r = 0; r < p.slices; ++r) {
-          c0 += dsmem_ld_u32(dsmem_map(smem_u32(hist + top_bin), r));
-          c1 += dsmem_ld_u32(dsmem_map(smem_u32(hist + top_bin - 1), r));
-        }
-      } else {
-        c0 = hist[top_bin];
-        c1 = hist[top_bin - 1];
-      }
-      int total;
-      const int above = block_exclusive_scan(static_cast<int>(c0 + c1), s_warp, &total);
-      if (above < need && need <= above + static_cast<int>(c0)) {
+      before += incl - c0 - c1;
+      if (before < need && need <= before + c0) {
         s_bin = top_bin;
-        s_above = above;
+        s_above = before;
         s_in = c0;
-      } else if (above + static_cast<int>(c0) < need && need <= above + static_cast<int>(c0 + c1)) {
+      } else if (before + c0 < need && need <= before + c0 + c1) {
         s_bin = top_bin - 1;
-        s_above = above + c0;
+        s_above = before + c0;
         s_in = c1;
       }
+    }
+    __syncthreads();
+    const uint32_t bin_lo = lo + (static_cast<uint32_t>(s_bin) << shift);
+    need -= s_above;
+    if (s_in == need) {  // the whole bin is kept
+      threshold = bin_lo - 1;
+      break;
+    }
+    if (shift == 0) {  // one key's bin
+      threshold = bin_lo;
+      ties = need;
+      break;
+    }
+    lo = bin_lo;
+    hi = min(hi, bin_lo + ((1u << shift) - 1u));
+    // The two histograms take turns. The next one was last read in the pass
+    // before this one, by CTAs that have all come to this pass's meeting.
+    if (pass > 0) {
+      uint32_t* next = s_hist[(pass + 1) & 1];
+      for (int i = threadIdx.x; i < EVICT_BINS; i += EVICT_THREADS) next[i] = 0;
       __syncthreads();
-      const uint32_t bin_lo = lo + (static_cast<uint32_t>(s_bin) << shift);
-      need -= s_above;
-      if (s_in == need) {  // the whole bin is kept
-        threshold = bin_lo - 1;  // keys are at least -inf's, 0x007FFFFF: no wrap
-        break;
-      }
-      if (shift == 0) {  // one key's bin
-        threshold = bin_lo;
-        ties = need;
-        break;
-      }
-      lo = bin_lo;
-      hi = min(hi, bin_lo + ((1u << shift) - 1u));
-      // The two histograms take turns. The next one was last read in the pass
-      // before this one, by CTAs that have all come to this pass's meeting.
-      if (pass > 0) {
-        uint32_t* next = s_hist[(pass + 1) & 1];
-        for (int i = threadIdx.x; i < EVICT_BINS; i += EVICT_THREADS) next[i] = 0;
-        __syncthreads();
-      }
     }
   }
 
-  // kept rows of each warp's run of keys, then of the warps and slices before it
-  const int run0 = min(n, warp * run), run1 = min(n, run0 + run);
+  // kept rows of each thread's run of quads, then of the threads, warps and slices before it
   int gt = 0, eq = 0;
-  if (cut) {
-    for (int i0 = run0; i0 < run1; i0 += 32) {
-      const int i = i0 + lane;
-      const uint32_t key = i < run1 ? key_at(i) : 0u;
-      gt += __popc(__ballot_sync(0xffffffffu, i < run1 && key > threshold));
-      eq += __popc(__ballot_sync(0xffffffffu, i < run1 && ties > 0 && key == threshold));
-    }
-  } else {
-    gt = run1 - run0;
+  const int run0 = threadIdx.x * quads;
+  for (int c = run0; c < run0 + quads; ++c) {
+    const uint4 k = keys4(c);
+    gt += (k.x > threshold) + (k.y > threshold) + (k.z > threshold) + (k.w > threshold);
+    eq += (k.x == threshold) + (k.y == threshold) + (k.z == threshold) + (k.w == threshold);
   }
-  if (lane == 0) {
+  const int my_gt = gt, my_eq = eq;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int gy = __shfl_up_sync(0xffffffffu, gt, o), ey = __shfl_up_sync(0xffffffffu, eq, o);
+    if (lane >= o) {
+      gt += gy;
+      eq += ey;
+    }
+  }
+  if (lane == 31) {
     s_gt[warp] = gt;
     s_eq[warp] = eq;
   }
   __syncthreads();
-  if (warp == 0) {
-    int g = s_gt[lane], e = s_eq[lane];
-    const int g1 = g, e1 = e;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int gy = __shfl_up_sync(0xffffffffu, g, o), ey = __shfl_up_sync(0xffffffffu, e, o);
-      if (lane >= o) {
-        g += gy;
-        e += ey;
-      }
+  gt += __reduce_add_sync(0xffffffffu, lane < warp ? s_gt[lane] : 0) - my_gt;
+  eq += __reduce_add_sync(0xffffffffu, lane < warp ? s_eq[lane] : 0) - my_eq;
+  if (p.slices > 1) {
+    if (threadIdx.x == EVICT_THREADS - 1) {
+      s_tot[0] = gt + my_gt;
+      s_tot[1] = eq + my_eq;
     }
-    s_gt[lane] = g - g1;
-    s_eq[lane] = e - e1;
-    if (lane == 31) {
-      s_tot[0] = g;
-      s_tot[1] = e;
+    cluster_sync();
+    for (uint32_t r = 0; r < rank; ++r) {
+      gt += dsmem_ld_u32(dsmem_map(smem_u32(s_tot), r));
+      eq += dsmem_ld_u32(dsmem_map(smem_u32(s_tot + 1), r));
     }
   }
-  meet();
-  gt = s_gt[warp];
-  eq = s_eq[warp];
-  for (uint32_t r = 0; r < rank; ++r) {
-    gt += dsmem_ld_u32(dsmem_map(smem_u32(s_tot), r));
-    eq += dsmem_ld_u32(dsmem_map(smem_u32(s_tot + 1), r));
-  }
-  int64_t* rows = p.rows + static_cast<int64_t>(b) * p.keep;
-  float* kept = p.weights_out + static_cast<int64_t>(b) * p.capacity;
-  for (int i0 = run0; i0 < run1; i0 += 32) {
-    const int i = i0 + lane;
-    bool above = i < run1, equal = false;
-    if (cut) {
-      const uint32_t key = i < run1 ? key_at(i) : 0u;
-      above = above && key > threshold;
-      equal = i < run1 && ties > 0 && key == threshold;
-    }
-    const unsigned ga = __ballot_sync(0xffffffffu, above), ea = __ballot_sync(0xffffffffu, equal);
-    const unsigned before = (1u << lane) - 1u;
-    const int g = gt + __popc(ga & before), e = eq + __popc(ea & before);
-    if (above || (equal && e < ties)) {
-      const int place = g + min(e, ties);
+  auto put = [&](uint32_t key, int i) {  // i: index in the slice
+    const bool above = key > threshold, equal = key == threshold;
+    if (above || (equal && eq < ties)) {
+      const int place = gt + min(eq, ties);
       rows[place] = base + i;
       kept[place] = src[base + i];
     }
-    gt += __popc(ga);
-    eq += __popc(ea);
-  }
-  if (rank == 0) {
-    for (int i = count + threadIdx.x; i < p.keep; i += EVICT_THREADS) rows[i] = -1;
-    for (int i = count + threadIdx.x; i < p.capacity; i += EVICT_THREADS) kept[i] = 0.f;
-    if (threadIdx.x == 0) p.counts[b] = count;
+    gt += above;
+    eq += equal;
+  };
+  for (int c = run0; c < run0 + quads; ++c) {
+    const uint4 k = keys4(c);
+    put(k.x, 4 * c);
+    put(k.y, 4 * c + 1);
+    put(k.z, 4 * c + 2);
+    put(k.w, 4 * c + 3);
   }
   if (p.slices > 1) cluster_sync();  // a CTA's totals stay readable until every CTA has read them
 }
@@ -272,7 +321,7 @@ struct GatherParams {
 // product over a whole tile of the new table multiplies its unread rows by
 // zero weights, which must not meet a NaN).
 template <typename Unit>
-__global__ void __launch_bounds__(EVICT_COPY_THREADS) evict_gather_kernel(const GatherParams p) {
+__global__ void __launch_bounds__(EVICT_COPY_THREADS, EVICT_COPY_CTAS) evict_gather_kernel(const GatherParams p) {
   constexpr int ROWS = 4;  // places a thread has in flight
   const int b = blockIdx.x / p.chunks, chunk = blockIdx.x - b * p.chunks;
   const uint8_t* src = p.src + b * p.src_sb;

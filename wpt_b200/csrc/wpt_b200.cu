@@ -1534,7 +1534,7 @@ extern "C" int wpt_cache_evict(const void* held, int64_t held_stride_b, int64_t 
   p.capacity = capacity;
   p.slices = 1;
   while (p.slices < 8 && N > 16384 * p.slices && static_cast<int64_t>(B) * p.slices * 2 <= sms) p.slices *= 2;
-  const int slice = (N / p.slices + 1024) / 1024 * 1024;
+  const int slice = (N / p.slices + wpt::EVICT_QUADS) / wpt::EVICT_QUADS * wpt::EVICT_QUADS;
   p.cache_cap = slice < 49152 ? slice : 49152;
   if (int rc = launch_dependent("evict_rows_kernel launch", wpt::evict_rows_kernel, static_cast<int64_t>(B) * p.slices,
                                 wpt::EVICT_THREADS, p.cache_cap * 4, p.slices, s, p))
@@ -1550,10 +1550,10 @@ extern "C" int wpt_cache_evict(const void* held, int64_t held_stride_b, int64_t 
   g.capacity = capacity;
   const bool wide = at % 16 == 0;
   g.units = row_bytes / (wide ? 16 : 4);
-  // eight CTAs an SM, no more than have a place for every group of threads
+  // one wave of CTAs, no more than have a place for every group of threads
   const int groups = wpt::EVICT_COPY_THREADS / std::min(std::max(g.units, 1), wpt::EVICT_COPY_THREADS);
   const int64_t blocks = (static_cast<int64_t>(capacity) + groups - 1) / groups;
-  g.chunks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(blocks, (int64_t(8) * sms + B - 1) / B)));
+  g.chunks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(blocks, int64_t(wpt::EVICT_COPY_CTAS) * sms / B)));
   if (wide)
     return launch_dependent("evict_gather_kernel launch", wpt::evict_gather_kernel<uint4>,
                             static_cast<int64_t>(B) * g.chunks, wpt::EVICT_COPY_THREADS, 0, 1, s, g);
