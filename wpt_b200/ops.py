@@ -541,18 +541,19 @@ def accept(scores, drafted, q, uniforms, resample, temperature=1.0, top_k=None, 
 
 # ------------------------------------------- the cache between two decode steps
 
-def _on(device, *tensors):
-    """Refuses tensors (None aside) that are not on the CUDA device `device`."""
-    for t in tensors:
-        if t is not None and t.device != device:
-            raise ValueError(f"tensors on {device} and {t.device}: a call takes one device")
-    if device.type != "cuda":
-        raise ValueError(f"wpt_b200 computes on a CUDA device only; got a tensor on {device}")
+_current = torch._C._cuda_getDevice
 
 
-def _call(device, fn, *args):
-    """A C-ABI call on `device`'s current stream, whichever device is current."""
-    if device.index == torch.cuda.current_device():
+def _one_device(*tensors):
+    """Raises for tensors (None aside) that are not all on one CUDA device."""
+    _need_cuda(*tensors)
+    on = {t.device for t in tensors if t is not None}
+    raise ValueError(f"tensors on {', '.join(map(str, on))}: a call takes one device")
+
+
+def _call(device, fn, args):
+    """fn(*args, stream) on `device`'s current stream, whichever device is current."""
+    if device.index == _current():
         rc = fn(*args, _lib.stream(device))
     else:
         with torch.cuda.device(device):
@@ -563,9 +564,11 @@ def _call(device, fn, *args):
 
 def _row_bytes(x):
     """Bytes of one (b, n) entry of a table (B, N, ...) whose entries are contiguous, or None."""
-    es = x.element_size()
-    size = es
-    shape, stride = x.shape, x.stride()
+    size = es = x.element_size()
+    shape = x.shape
+    if len(shape) == 3:
+        return es * shape[2] if x.stride(2) == 1 or shape[2] <= 1 else None
+    stride = x.stride()
     for i in range(len(shape) - 1, 1, -1):
         if shape[i] > 1 and stride[i] * es != size:
             return None
@@ -582,18 +585,21 @@ def attention_weights(q, k, positions, lse, scale, weights, window=0, floor=None
     the queries past the keys (two, or three where a key's columns are summed
     in several runs)."""
     device = q.device
-    _on(device, k, positions, lse, weights, floor)
+    if not (q.is_cuda and k.device == device and positions.device == device and lse.device == device and
+            weights.device == device and (floor is None or floor.device == device)):
+        _one_device(q, k, positions, lse, weights, floor)
     B, T, H, C = q.shape
     N = k.shape[1]
-    if k.shape != (B, N, C):
-        raise ValueError(f"keys {tuple(k.shape)} against queries {tuple(q.shape)}")
-    if lse.shape != (B, T, H) or positions.shape != (B, T) or (floor is not None and floor.shape != (B, T)):
-        raise ValueError(f"queries {tuple(q.shape)} need lse {(B, T, H)} and positions {(B, T)}")
-    ld, step = weights.stride() if weights.dim() == 2 else (0, 0)
-    if weights.dtype != torch.float32 or weights.shape != (B, N) or (N > 1 and step != 1) or (B > 1 and ld < N):
-        raise ValueError(f"weights must be float32 {(B, N)} with contiguous rows: they are added to in place")
-    _bf16(q)
-    if not q.is_contiguous() or q.data_ptr() % 16:
+    if k.shape != (B, N, C) or lse.shape != (B, T, H) or positions.shape != (B, T) or \
+            (floor is not None and floor.shape != (B, T)):
+        raise ValueError(f"queries {tuple(q.shape)} with keys {tuple(k.shape)}, lse {tuple(lse.shape)}, positions "
+                         f"{tuple(positions.shape)}")
+    if weights.dtype != torch.float32 or weights.shape != (B, N):
+        raise ValueError(f"weights must be float32 {(B, N)}")
+    ld, step = weights.stride()
+    if (step != 1 and N > 1) or (ld < N and B > 1):
+        raise ValueError("weights must have contiguous rows: they are added to in place")
+    if _bf16(q).data_ptr() % 16 or not q.is_contiguous():
         q = q.clone(memory_format=torch.contiguous_format)
     k = _table(k)
     positions = _rows(positions)
@@ -608,9 +614,10 @@ def attention_weights(q, k, positions, lse, scale, weights, window=0, floor=None
     if T * H > 256:
         scratch = torch.empty(lib.wpt_attn_weights_scratch_bytes(B, T, H, N), dtype=torch.uint8, device=device)
     sb, sn, _ = k.stride()
-    _call(device, lib.wpt_attn_weights, q.data_ptr(), k.data_ptr(), sb, sn, positions.data_ptr(),
-          None if floor is None else floor.data_ptr(), lse.data_ptr(), weights.data_ptr(), ld,
-          None if scratch is None else scratch.data_ptr(), B, T, H, C, N, window, scale)
+    _call(device, lib.wpt_attn_weights,
+          (q.data_ptr(), k.data_ptr(), sb, sn, positions.data_ptr(), None if floor is None else floor.data_ptr(),
+           lse.data_ptr(), weights.data_ptr(), ld, None if scratch is None else scratch.data_ptr(), B, T, H, C, N, window,
+           scale))
     LAUNCHES[0] += 1 if scratch is None else 2
     return weights
 
@@ -623,12 +630,15 @@ def cache_evict(held, weights, lengths, keep, recent=0, first=0, capacity=None):
     after them. Returns (held (B, capacity, ...), weights (B, capacity), rows
     (B, keep) int64, -1 padded: the old places, counts (B,) int64)."""
     device = held.device
-    _on(device, weights, lengths)
+    if not (held.is_cuda and weights.device == device and lengths.device == device):
+        _one_device(held, weights, lengths)
     if capacity is None:
         capacity = keep
-    B, N = held.shape[:2]
+    shape = held.shape
+    B, N = shape[0], shape[1]
     if weights.shape != (B, N) or weights.dtype != torch.float32 or lengths.shape != (B,):
-        raise ValueError(f"a table of {B} rows of {N} needs float32 weights {(B, N)} and lengths {(B,)}")
+        raise ValueError(f"a table of {B} rows of {N} needs float32 weights {(B, N)} and lengths {(B,)}; got "
+                         f"{weights.dtype} {tuple(weights.shape)} and {tuple(lengths.shape)}")
     if keep < 0 or recent < 0 or first < 0 or recent + first > keep or capacity < keep:
         raise ValueError(f"keep={keep} rows cannot hold first={first} and recent={recent}, or capacity={capacity} "
                          "cannot hold them")
@@ -637,19 +647,19 @@ def cache_evict(held, weights, lengths, keep, recent=0, first=0, capacity=None):
         held = held.contiguous()
         row_bytes = _row_bytes(held)
     ld, step = weights.stride()
-    if N > 1 and step != 1 or B > 1 and ld < N:
+    if step != 1 and N > 1 or ld < N and B > 1:
         weights = weights.contiguous()
         ld = N
     lengths = _rows(lengths)
-    out = torch.empty(B, capacity, *held.shape[2:], dtype=held.dtype, device=device)
-    out_weights = torch.empty(B, capacity, dtype=torch.float32, device=device)
-    rows = torch.empty(B, keep, dtype=torch.int64, device=device)
+    out = held.new_empty(B, capacity, *shape[2:])
+    out_weights = weights.new_empty(B, capacity)
+    rows = lengths.new_empty(B, keep)
     counts = torch.empty_like(lengths)
     es = held.element_size()
     stride = held.stride()
-    _call(device, _lib.lib().wpt_cache_evict, held.data_ptr(), stride[0] * es, stride[1] * es, weights.data_ptr(), ld,
-          lengths.data_ptr(), out.data_ptr(), out_weights.data_ptr(), rows.data_ptr(), counts.data_ptr(), B, N,
-          row_bytes, keep, recent, first, capacity)
+    _call(device, _lib.lib().wpt_cache_evict,
+          (held.data_ptr(), stride[0] * es, stride[1] * es, weights.data_ptr(), ld, lengths.data_ptr(), out.data_ptr(),
+           out_weights.data_ptr(), rows.data_ptr(), counts.data_ptr(), B, N, row_bytes, keep, recent, first, capacity))
     LAUNCHES[0] += 2
     return out, out_weights, rows, counts
 
@@ -663,7 +673,8 @@ def beam_select(scores, totals, beams, done=None, end=None):
     and tokens (R, beams) int64); -inf, -1 and -1 where there are too few
     candidates."""
     device = scores.device
-    _on(device, totals, done)
+    if not (scores.is_cuda and totals.device == device and (done is None or done.device == device)):
+        _one_device(scores, totals, done)
     bf16 = scores.dtype == torch.bfloat16
     if not bf16 and scores.dtype != torch.float32:
         raise NotImplementedError(f"the selection kernels take float32 or bfloat16 scores; got {scores.dtype}")
@@ -681,14 +692,15 @@ def beam_select(scores, totals, beams, done=None, end=None):
         sr, sw = W * V, V
     if totals.dtype != torch.float32 or not totals.is_contiguous():
         totals = totals.float().contiguous()
-    out = torch.empty_like(totals) if beams == W else torch.empty(R, beams, dtype=torch.float32, device=device)
-    parents = torch.empty(R, beams, dtype=torch.int64, device=device)
+    out = torch.empty_like(totals) if beams == W else totals.new_empty(R, beams)
+    parents = totals.new_empty(R, beams, dtype=torch.int64)
     tokens = torch.empty_like(parents)
     lib = _lib.lib()
-    scratch = torch.empty(lib.wpt_beam_scratch_bytes(R, W, V, beams, bf16), dtype=torch.uint8, device=device)
-    _call(device, lib.wpt_beam_select, scores.data_ptr(), bf16, sr, sw, totals.data_ptr(),
-          None if done is None else done.data_ptr(), 0 if end is None else end, scratch.data_ptr(), out.data_ptr(),
-          parents.data_ptr(), tokens.data_ptr(), R, W, V, beams)
+    scratch = parents.new_empty(lib.wpt_beam_scratch_bytes(R, W, V, beams, bf16) // 8)
+    _call(device, lib.wpt_beam_select,
+          (scores.data_ptr(), bf16, sr, sw, totals.data_ptr(), None if done is None else done.data_ptr(),
+           0 if end is None else end, scratch.data_ptr(), out.data_ptr(), parents.data_ptr(), tokens.data_ptr(), R, W, V,
+           beams))
     LAUNCHES[0] += 2
     return out, parents, tokens
 
@@ -704,7 +716,8 @@ def cache_reorder(tables, parents, lengths, first=None):
     whatever their shapes."""
     every = [tables] if isinstance(tables, torch.Tensor) else tables
     device = parents.device
-    _on(device, lengths, first, *every)
+    if not (parents.is_cuda and lengths.device == device and (first is None or first.device == device)):
+        _one_device(parents, lengths, first)
     R, W = parents.shape
     if lengths.shape != (R * W,) or (first is not None and first.shape != (R,)):
         raise ValueError(f"parents {(R, W)} need lengths {(R * W,)} (and first {(R,)})")
@@ -714,18 +727,21 @@ def cache_reorder(tables, parents, lengths, first=None):
     fields = []
     for t in every:
         shape = t.shape
+        if t.device != device:
+            _one_device(t, parents)
         if len(shape) < 2 or shape[0] != R * W:
             raise ValueError(f"a table of {tuple(shape)} for {R} texts of {W} beams")
         size, es, stride = _row_bytes(t), t.element_size(), t.stride()
         sb, sn = stride[0] * es, stride[1] * es
-        if size is None or (t.numel() and ((R * W > 1 and sb < size) or (shape[1] > 1 and sn < size))):
+        if size is None or sb < size and R * W > 1 and t.numel() or sn < size and shape[1] > 1 and t.numel():
             raise ValueError("a reordered table's entries must be contiguous and its places must not overlap: it is "
                              "changed in place")
         fields += (t.data_ptr(), sb, sn, size, shape[1])
     lib = _lib.lib()
     for i in range(0, len(fields), 5 * REORDER_TABLES):
         part = fields[i:i + 5 * REORDER_TABLES]
-        _call(device, lib.wpt_cache_reorder, (ctypes.c_int64 * len(part))(*part), len(part) // 5, parents.data_ptr(),
-              lengths.data_ptr(), None if first is None else first.data_ptr(), R, W)
+        _call(device, lib.wpt_cache_reorder,
+              ((ctypes.c_int64 * len(part))(*part), len(part) // 5, parents.data_ptr(), lengths.data_ptr(),
+               None if first is None else first.data_ptr(), R, W))
         LAUNCHES[0] += 1
     return tables
