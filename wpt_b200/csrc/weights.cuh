@@ -72,9 +72,9 @@ __device__ __forceinline__ uint64_t weights_exp2_poly(uint64_t x) {
 
 // Adds exp2(x scale + cols[0][c]) over 2 * PAIRS columns c to the four partial
 // sums, POLY of every 8 pairs on the FMA pipe; MASK: of those with cols[1][c] <= n <=
-// cols[2][c] (whole numbers). cols: rows of 128 columns in shared memory,
+// cols[2][c] (whole numbers). cols: rows of STRIDE columns in shared memory,
 // 16-byte aligned.
-template <int PAIRS, int POLY, bool MASK>
+template <int PAIRS, int POLY, bool MASK, int STRIDE>
 __device__ __forceinline__ void weights_terms(uint64_t (&sum)[2], const uint32_t* x, float scale, const float* cols,
                                               int n) {
   const uint64_t scale2 = f2_pack(scale, scale);
@@ -97,8 +97,8 @@ __device__ __forceinline__ void weights_terms(uint64_t (&sum)[2], const uint32_t
       a0 = fast_exp2(a0);
       a1 = fast_exp2(a1);
       if constexpr (MASK) {
-        const int2 lo = *reinterpret_cast<const int2*>(cols + 128 + 2 * (i + h));
-        const int2 hi = *reinterpret_cast<const int2*>(cols + 256 + 2 * (i + h));
+        const int2 lo = *reinterpret_cast<const int2*>(cols + STRIDE + 2 * (i + h));
+        const int2 hi = *reinterpret_cast<const int2*>(cols + 2 * STRIDE + 2 * (i + h));
         a0 = n >= lo.x && n <= hi.x ? a0 : 0.f;
         a1 = n >= lo.y && n <= hi.y ? a1 : 0.f;
       }
@@ -137,15 +137,17 @@ struct WeightsStreamLayout {
   static constexpr int Q_BYTES = NCOL * C * 2, K_BYTES = 128 * C * 2;
   static constexpr int OFF_Q = 0;  // two buffers
   static constexpr int OFF_K = 2 * Q_BYTES;
-  static constexpr int OFF_COL = OFF_K + STAGES * K_BYTES;  // float offset, int lo, int hi of each column
+  static constexpr int OFF_COL = OFF_K + STAGES * K_BYTES;  // each column's constant (float), then its lowest and highest row
   static constexpr int OFF_PRE = OFF_COL + NCOL * 12;
   static constexpr int OFF_FIRST = OFF_PRE + (WEIGHTS_BAL_ROWS + 2) * 4;
   static constexpr int OFF_BAR = OFF_FIRST + WEIGHTS_BAL_ROWS * 4;
-  // q_full[2], q_empty[2], s_full[2], s_free[2], drained, k_full[STAGES], k_empty[STAGES]
-  static constexpr int NBAR = 9 + 2 * STAGES;
+  // TMEM buffers: enough tiles for the epilogue's change of rows
+  static constexpr int BUFS = NCOL <= 64 ? 8 : 512 / NCOL;
+  // q_full[2], q_empty[2], drained, s_full[BUFS], s_free[BUFS], k_full[STAGES], k_empty[STAGES]
+  static constexpr int NBAR = 5 + 2 * BUFS + 2 * STAGES;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
   static constexpr int BYTES = OFF_MISC + 64 + 1024;
-  static constexpr int TMEM_COLS = 2 * NCOL <= 32 ? 32 : 2 * NCOL;
+  static constexpr int TMEM_COLS = BUFS * NCOL;
 };
 
 // The key tiles [first, first + n) that batch row b's queries read.
@@ -229,10 +231,10 @@ __global__ void __launch_bounds__(WEIGHTS_STREAM_THREADS, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
   uint64_t* q_full = bars;
   uint64_t* q_empty = bars + 2;
-  uint64_t* s_full = bars + 4;
-  uint64_t* s_free = bars + 6;
-  uint64_t* drained = bars + 8;
-  uint64_t* k_full = bars + 9;
+  uint64_t* drained = bars + 4;
+  uint64_t* s_full = bars + 5;
+  uint64_t* s_free = s_full + L::BUFS;
+  uint64_t* k_full = s_free + L::BUFS;
   uint64_t* k_empty = k_full + STAGES;
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC);
   int* s_scan = reinterpret_cast<int*>(smem + L::OFF_MISC + 16);  // 6 warp totals
@@ -243,6 +245,8 @@ __global__ void __launch_bounds__(WEIGHTS_STREAM_THREADS, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(q_full + i, 1);
       mbar_init(q_empty + i, 1);
+    }
+    for (int i = 0; i < L::BUFS; ++i) {
       mbar_init(s_full + i, 1);
       mbar_init(s_free + i, 4);
     }
@@ -322,32 +326,27 @@ __global__ void __launch_bounds__(WEIGHTS_STREAM_THREADS, 1)
     }
     __syncwarp();
   } else if (warp == 4) {
-    if (lane == 0) {
-      constexpr uint32_t IDESC = idesc_bf16(128, NCOL, 0, 0);
-      bool ok = true;
-      int j = 0;
-      for (int seg = 0; ok && walk.step(p); ++seg) {
-        const uint32_t q_addr = smem_u32(smem + L::OFF_Q + (seg & 1) * L::Q_BYTES);
-        if (!(ok = mbar_wait(q_full + (seg & 1), (seg >> 1) & 1, p.status))) break;
-        for (int jj = 0; jj < walk.ntiles; ++jj, ++j) {
-          const int st = j % STAGES, buf = j & 1;
-          if (!(ok = mbar_wait(k_full + st, (j / STAGES) & 1, p.status))) break;
-          if (j >= 2 && !(ok = mbar_wait(s_free + buf, ((j >> 1) & 1) ^ 1, p.status))) break;
-          tc_fence_after();
-          const uint32_t k_addr = smem_u32(smem + L::OFF_K + st * L::K_BYTES);
-#pragma unroll
-          for (int kk = 0; kk < C / 16; ++kk)
-            mma_ss(tmem + buf * NCOL, sdesc_sw128(k_addr + (kk >> 2) * (128 * 128) + (kk & 3) * 32, 16, 1024),
-                   sdesc_sw128(q_addr + (kk >> 2) * (NCOL * 128) + (kk & 3) * 32, 16, 1024), IDESC, kk > 0 ? 1u : 0u);
-          mma_commit(k_empty + st);
-          mma_commit(s_full + buf);
-        }
-        if (ok) mma_commit(q_empty + (seg & 1));
+    constexpr uint32_t IDESC = idesc_bf16(128, NCOL, 0, 0);
+    auto wait = [&](uint64_t* bar, int parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status)); };
+    bool ok = true;
+    int j = 0;
+    for (int seg = 0; ok && walk.step(p); ++seg) {
+      const uint64_t q_desc = sdesc_sw128(smem_u32(smem + L::OFF_Q + (seg & 1) * L::Q_BYTES), 16, 1024);
+      if (!(ok = wait(q_full + (seg & 1), (seg >> 1) & 1))) break;
+      for (int jj = 0; jj < walk.ntiles; ++jj, ++j) {
+        const int st = j % STAGES, buf = j % L::BUFS;
+        if (!(ok = wait(k_full + st, (j / STAGES) & 1))) break;
+        if (j >= L::BUFS && !(ok = wait(s_free + buf, ((j / L::BUFS) & 1) ^ 1))) break;
+        tc_fence_after();
+        weights_mma<C / 16 - 1, NCOL>(tmem + buf * NCOL, sdesc_sw128(smem_u32(smem + L::OFF_K + st * L::K_BYTES), 16, 1024),
+                                      q_desc, IDESC);
+        mma_commit_warp(k_empty + st);
+        mma_commit_warp(s_full + buf);
       }
-      mma_commit(drained);  // TMEM is freed with no product in flight
-      mbar_wait(drained, 0, p.status);
+      if (ok) mma_commit_warp(q_empty + (seg & 1));
     }
-    __syncwarp();
+    mma_commit_warp(drained);  // TMEM is freed with no product in flight
+    wait(drained, 0);
   } else {
     const int r = threadIdx.x;
     const uint32_t lane_addr = tmem + (static_cast<uint32_t>(warp * 32) << 16);
@@ -380,40 +379,36 @@ __global__ void __launch_bounds__(WEIGHTS_STREAM_THREADS, 1)
         any_hi = max(any_hi, s_hi[c]);
       }
       for (int jj = 0; jj < walk.ntiles; ++jj, ++j) {
-        const int n0 = (walk.tile0 + jj) * 128, n = n0 + r, buf = j & 1;
+        const int n0 = (walk.tile0 + jj) * 128, n = n0 + r, buf = j % L::BUFS;
         const bool mine = n >= any_lo && n <= any_hi;
-        float* to = p.weights + static_cast<int64_t>(b) * p.weights_ld + n;
-        const float before = mine ? *to : 0.f;
-        if (!(ok = __all_sync(0xffffffffu, mbar_wait(s_full + buf, (j >> 1) & 1, p.status)))) break;
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(s_full + buf, (j / L::BUFS) & 1, p.status)))) break;
         tc_fence_after();
         const bool whole = n0 >= all_lo && n0 + 127 <= all_hi;
-        float sum = 0.f;
-#pragma unroll
-        for (int c0 = 0; c0 < NCOL; c0 += 32) {
-          constexpr int W = NCOL < 32 ? NCOL : 32;
+        uint64_t sums[2] = {0, 0};
+        constexpr int W = NCOL < 32 ? NCOL : 32;
+#pragma unroll 2
+        for (int c0 = 0; c0 < NCOL; c0 += W) {
           uint32_t x[W];
           if constexpr (W == 32)
             tmem_ld32(lane_addr + buf * NCOL + c0, x);
           else
             tmem_ld16(lane_addr + buf * NCOL + c0, x);
-          float part[4] = {0.f, 0.f, 0.f, 0.f};
-          if (whole) {
-#pragma unroll
-            for (int c = 0; c < W; ++c)
-              part[c & 3] += fast_exp2(fmaf(__uint_as_float(x[c]), p.scale_log2, s_off[c0 + c]));
-          } else {
-#pragma unroll
-            for (int c = 0; c < W; ++c) {
-              const float e = fast_exp2(fmaf(__uint_as_float(x[c]), p.scale_log2, s_off[c0 + c]));
-              part[c & 3] += n >= s_lo[c0 + c] && n <= s_hi[c0 + c] ? e : 0.f;
-            }
+          if (c0 + W == NCOL) {  // the scores are in registers
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(s_free + buf);
           }
-          sum += (part[0] + part[1]) + (part[2] + part[3]);
+          if (whole)
+            weights_terms<W / 2, 0, false, NCOL>(sums, x, p.scale_log2, s_off + c0, n);
+          else
+            weights_terms<W / 2, 0, true, NCOL>(sums, x, p.scale_log2, s_off + c0, n);
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(s_free + buf);
-        if (mine) *to = before + sum;
+        float s0, s1;
+        f2_unpack(f2_add(sums[0], sums[1]), s0, s1);
+        // A reduction in L2 instead of a load, which each tile would wait for: 64
+        // rows of 1,024 to 32,768 keys take 50 us with it, 58 without. A key has one
+        // such addition a call, so their order cannot matter.
+        if (mine) atomicAdd(p.weights + static_cast<int64_t>(b) * p.weights_ld + n, s0 + s1);
       }
     }
   }
@@ -772,9 +767,9 @@ __global__ void __launch_bounds__(WEIGHTS_TILE_THREADS, 1)
               if (lane == 0) mbar_arrive(s_free + g);
             }
             if (whole)
-              weights_terms<16, WEIGHTS_POLY8, false>(sum, x, p.scale_log2, off + run * 32, n);
+              weights_terms<16, WEIGHTS_POLY8, false, COLS>(sum, x, p.scale_log2, off + run * 32, n);
             else
-              weights_terms<16, 0, true>(sum, x, p.scale_log2, off + run * 32, n);
+              weights_terms<16, 0, true, COLS>(sum, x, p.scale_log2, off + run * 32, n);
           }
         }
         __syncwarp();
