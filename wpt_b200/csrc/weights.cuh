@@ -448,6 +448,9 @@ __global__ void __launch_bounds__(WEIGHTS_TILE_COLS)
     weights_prep_kernel(const WeightsParams p, int tiles, int4* meta, float* cols, unsigned* ticket) {
   __shared__ int s_red[4][4];
   const int b = blockIdx.x / tiles, tile = blockIdx.x - b * tiles;
+  // A small grid lets the next kernel set itself up meanwhile; a large one
+  // would share its SMs with it.
+  if (gridDim.x <= 256) griddep_launch();
   griddep_wait();
   if (blockIdx.x == 0 && threadIdx.x == 0) *ticket = 0;
   const int64_t c = static_cast<int64_t>(tile) * WEIGHTS_TILE_COLS + threadIdx.x;
