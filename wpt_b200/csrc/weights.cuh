@@ -15,13 +15,22 @@
 // live key tiles are laid end to end and cut into one equal range a CTA, so
 // rows of any lengths keep the SMs equally busy. Bound: HBM (2 C bytes a key).
 //
-// weights_tile_kernel (more columns, a prompt): 256 keys stay in shared
-// memory and the queries stream past them, 128 columns at a time, S^T
-// double-buffered in TMEM for each 128 keys. Items of (256 keys, a run of
-// column tiles) are handed out by an atomic ticket; where a key's columns
-// are cut into several runs, their sums go to scratch and
-// weights_reduce_kernel adds them in order. Bound: the exponentials (16 a
-// clock an SM against 32 columns' products of 128 terms).
+// 64 rows of 1,024 to 32,768 keys, 32 heads: 54 us for 308 MB (5.7 TB/s).
+//
+// weights_tile_kernel (more columns, a prompt): up to four tiles of 128 keys
+// stay in shared memory and the queries stream past them, 128 columns at a
+// time. A warpgroup a key tile adds up the exponentials of its scores from its
+// quarter of TMEM while the others' products run. Items of (key tiles, a run
+// of column tiles) are handed out by an atomic ticket; where a key's columns
+// are cut into several runs, their sums go to scratch and weights_reduce_kernel
+// adds them in order. weights_prep_kernel lays out each column's constant and
+// rows, and each column tile's extremes, by which tiles that no query reads are
+// skipped and tiles read whole need no mask. Bound: the exponentials (16 a clock
+// an SM: 1,024 clocks for 128 keys x 128 columns, whose products take 512), so
+// a quarter of them take the FMA pipe. 8 x 4,096 places of 16 heads, causal, width 128: 371
+// us, 741 TFLOP/s (0.46 of the measured bf16 peak; a unit's warpgroups wait about
+// a third of the time for their next scores, each having one buffer: two
+// smaller ones, or a spare in turn, measured slower).
 #pragma once
 
 #include <climits>
@@ -150,16 +159,17 @@ struct WeightsStreamLayout {
   static constexpr int TMEM_COLS = BUFS * NCOL;
 };
 
-// The key tiles [first, first + n) that batch row b's queries read.
-__device__ __forceinline__ int2 weights_row_tiles(const WeightsParams& p, int b) {
+// The lowest and highest row that batch row b's queries from `first` on, `step`
+// apart, read; (INT_MAX, -1) for none.
+__device__ __forceinline__ int2 weights_row_range(const WeightsParams& p, int b, int first, int step) {
   int lo = INT_MAX, hi = -1;
-  for (int t = 0; t < p.T; ++t) {
+  for (int t = first; t < p.T; t += step) {
     const int64_t at = static_cast<int64_t>(b) * p.T + t;
     const int2 r = weights_range(p.positions[at], p.floor, at, p.window, p.N);
     lo = min(lo, r.x);
     hi = max(hi, r.y);
   }
-  return hi < lo ? make_int2(0, 0) : make_int2(lo / 128, hi / 128 - lo / 128 + 1);
+  return make_int2(lo, hi);
 }
 
 // A role's walk over its CTA's work: segments of (batch row, key tiles).
@@ -203,11 +213,11 @@ struct WeightsWalk {
       return true;
     }
     for (; next < p.B; next += gridDim.x) {
-      const int2 t = weights_row_tiles(p, next);
-      if (t.y > 0) {
+      const int2 rows = weights_row_range(p, next, 0, 1);
+      if (rows.y >= rows.x) {
         b = next;
-        tile0 = t.x;
-        ntiles = t.y;
+        tile0 = rows.x / 128;
+        ntiles = rows.y / 128 - tile0 + 1;
         next += gridDim.x;
         return true;
       }
@@ -266,16 +276,28 @@ __global__ void __launch_bounds__(WEIGHTS_STREAM_THREADS, 1)
   }
   griddep_wait();
   if (p.B <= WEIGHTS_BAL_ROWS) {
+    // each row's first live tile and their number: a thread a row, or with
+    // many queries a row, a warp
+    auto put = [&](int b, int2 rows) {
+      s_first[b] = rows.y < rows.x ? 0 : rows.x / 128;
+      s_pre[b + 1] = rows.y < rows.x ? 0 : rows.y / 128 - rows.x / 128 + 1;
+    };
+    if (p.T <= 8) {
+      for (int b = threadIdx.x; b < p.B; b += WEIGHTS_STREAM_THREADS) put(b, weights_row_range(p, b, 0, 1));
+    } else {
+      for (int b = warp; b < p.B; b += WEIGHTS_STREAM_THREADS / 32) {
+        int2 rows = weights_row_range(p, b, lane, 32);
+        rows.x = __reduce_min_sync(0xffffffffu, rows.x);
+        rows.y = __reduce_max_sync(0xffffffffu, rows.y);
+        if (lane == 0) put(b, rows);
+      }
+    }
+    __syncthreads();
     // live tiles of the rows before each row
     const int per = (p.B + WEIGHTS_STREAM_THREADS - 1) / WEIGHTS_STREAM_THREADS;
     const int b0 = min(p.B, static_cast<int>(threadIdx.x) * per), b1 = min(p.B, b0 + per);
     int sum = 0;
-    for (int b = b0; b < b1; ++b) {
-      const int2 tiles = weights_row_tiles(p, b);
-      s_first[b] = tiles.x;
-      s_pre[b + 1] = tiles.y;
-      sum += tiles.y;
-    }
+    for (int b = b0; b < b1; ++b) sum += s_pre[b + 1];
     int incl = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -406,7 +428,7 @@ __global__ void __launch_bounds__(WEIGHTS_STREAM_THREADS, 1)
         float s0, s1;
         f2_unpack(f2_add(sums[0], sums[1]), s0, s1);
         // A reduction in L2 instead of a load, which each tile would wait for: 64
-        // rows of 1,024 to 32,768 keys take 50 us with it, 58 without. A key has one
+        // rows of 1,024 to 32,768 keys take 54 us with it, 58 without. A key has one
         // such addition a call, so their order cannot matter.
         if (mine) atomicAdd(p.weights + static_cast<int64_t>(b) * p.weights_ld + n, s0 + s1);
       }

@@ -1564,11 +1564,12 @@ extern "C" int wpt_cache_evict(const void* held, int64_t held_stride_b, int64_t 
 namespace {
 // Runs a beam's scores are cut into, and tiles a run: enough runs for two an SM
 // (64 texts of 8 beams: whole beams 29.8 us, halves 30.6, quarters 32.0).
-void beam_plan(int64_t R, int64_t W, int64_t V, bool bf16, int sms, int* splits, int* tiles) {
+void beam_plan(int64_t R, int64_t W, int64_t V, bool bf16, int* splits, int* tiles) {
+  constexpr int64_t sms = 148;  // whichever device the scratch is asked for on
   const int es = bf16 ? 2 : 4;
   const int64_t tile = wpt::BEAM_THREADS * 64 / es;
   const int64_t all = (V + 16 / es - 1 + tile - 1) / tile;  // a row may start off a 16-byte boundary
-  int64_t want = (2 * static_cast<int64_t>(sms) + R * W - 1) / (R * W);
+  int64_t want = (2 * sms + R * W - 1) / (R * W);
   if (want > all) want = all;
   if (want < 1) want = 1;
   *tiles = static_cast<int>((all + want - 1) / want);
@@ -1584,9 +1585,8 @@ int launch_beam_scan(const wpt::BeamParams& p, cudaStream_t stream) {
 
 extern "C" size_t wpt_beam_scratch_bytes(int R, int W, int V, int K, int bf16) {
   if (R < 1 || W < 1 || V < 1 || K < 1) return 0;
-  int sms = 148, splits, tiles;
-  current_device(&sms);
-  beam_plan(R, W, V, bf16 != 0, sms, &splits, &tiles);
+  int splits, tiles;
+  beam_plan(R, W, V, bf16 != 0, &splits, &tiles);
   return static_cast<size_t>(R) * W * splits * (8 + 8 * static_cast<size_t>(K));
 }
 
@@ -1604,10 +1604,8 @@ extern "C" int wpt_beam_select(const void* scores, int bf16, int64_t stride_r, i
   if (reinterpret_cast<uintptr_t>(scratch) & 7) return fail(WPT_ERR_INVALID, "scratch must be 8-byte aligned");
   if (done && (end < 0 || end >= V)) return fail(WPT_ERR_INVALID, "end token %d of a vocabulary of %d", end, V);
   if (reinterpret_cast<uintptr_t>(scores) & (bf16 ? 1 : 3)) return fail(WPT_ERR_INVALID, "scores are misaligned");
-  int sms = 148;
-  current_device(&sms);
   wpt::BeamParams p;
-  beam_plan(R, W, V, bf16 != 0, sms, &p.splits, &p.tiles);
+  beam_plan(R, W, V, bf16 != 0, &p.splits, &p.tiles);
   p.scores = scores;
   p.stride_r = stride_r;
   p.stride_w = stride_w;
