@@ -10,7 +10,7 @@
 // a float's bits grow like its logarithm, so skewed weights spread over the
 // bins), then of the one bin that holds it, until a bin's keys are all kept or
 // all equal; the slices' histograms are summed over distributed shared memory.
-// A count of the kept rows before each thread's run of keys gives their places.
+// A count of the kept rows before each warp's run of keys gives their places.
 // evict_gather_kernel copies the kept entries. Two kernels rather than one:
 // the selection wants few CTAs a row, the copy wants every SM.
 #pragma once
@@ -252,57 +252,67 @@ __global__ void __launch_bounds__(EVICT_THREADS) evict_rows_kernel(const EvictPa
     }
   }
 
-  // kept rows of each thread's run of quads, then of the threads, warps and slices before it
+  // kept rows of each warp's run of quads, and of the warps and slices before it
   int gt = 0, eq = 0;
-  const int run0 = threadIdx.x * quads;
-  for (int c = run0; c < run0 + quads; ++c) {
-    const uint4 k = keys4(c);
+  const int run0 = warp * 32 * quads + lane;
+  for (int q = 0; q < quads; ++q) {
+    const uint4 k = keys4(run0 + 32 * q);
     gt += (k.x > threshold) + (k.y > threshold) + (k.z > threshold) + (k.w > threshold);
     eq += (k.x == threshold) + (k.y == threshold) + (k.z == threshold) + (k.w == threshold);
   }
-  const int my_gt = gt, my_eq = eq;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int gy = __shfl_up_sync(0xffffffffu, gt, o), ey = __shfl_up_sync(0xffffffffu, eq, o);
-    if (lane >= o) {
-      gt += gy;
-      eq += ey;
-    }
-  }
-  if (lane == 31) {
+  gt = __reduce_add_sync(0xffffffffu, gt);
+  eq = __reduce_add_sync(0xffffffffu, eq);
+  if (lane == 0) {
     s_gt[warp] = gt;
     s_eq[warp] = eq;
   }
   __syncthreads();
-  gt += __reduce_add_sync(0xffffffffu, lane < warp ? s_gt[lane] : 0) - my_gt;
-  eq += __reduce_add_sync(0xffffffffu, lane < warp ? s_eq[lane] : 0) - my_eq;
   if (p.slices > 1) {
-    if (threadIdx.x == EVICT_THREADS - 1) {
-      s_tot[0] = gt + my_gt;
-      s_tot[1] = eq + my_eq;
+    if (warp == 0) {
+      gt = __reduce_add_sync(0xffffffffu, s_gt[lane]);
+      eq = __reduce_add_sync(0xffffffffu, s_eq[lane]);
+      if (lane == 0) {
+        s_tot[0] = gt;
+        s_tot[1] = eq;
+      }
     }
     cluster_sync();
-    for (uint32_t r = 0; r < rank; ++r) {
-      gt += dsmem_ld_u32(dsmem_map(smem_u32(s_tot), r));
-      eq += dsmem_ld_u32(dsmem_map(smem_u32(s_tot + 1), r));
-    }
   }
-  auto put = [&](uint32_t key, int i) {  // i: index in the slice
-    const bool above = key > threshold, equal = key == threshold;
-    if (above || (equal && eq < ties)) {
-      const int place = gt + min(eq, ties);
-      rows[place] = base + i;
-      kept[place] = src[base + i];
-    }
-    gt += above;
-    eq += equal;
-  };
-  for (int c = run0; c < run0 + quads; ++c) {
+  gt = __reduce_add_sync(0xffffffffu, lane < warp ? s_gt[lane] : 0);
+  eq = __reduce_add_sync(0xffffffffu, lane < warp ? s_eq[lane] : 0);
+  for (uint32_t r = 0; r < rank; ++r) {
+    gt += dsmem_ld_u32(dsmem_map(smem_u32(s_tot), r));
+    eq += dsmem_ld_u32(dsmem_map(smem_u32(s_tot + 1), r));
+  }
+  // their places: lanes hold consecutive quads, so that a warp's stores are next to each other
+  for (int q = 0; q < quads; ++q) {
+    const int c = run0 + 32 * q;
     const uint4 k = keys4(c);
-    put(k.x, 4 * c);
-    put(k.y, 4 * c + 1);
-    put(k.z, 4 * c + 2);
-    put(k.w, 4 * c + 3);
+    const uint32_t key[4] = {k.x, k.y, k.z, k.w};
+    int mine = 0;  // above the threshold, and 2^16 times equal to it
+#pragma unroll
+    for (int h = 0; h < 4; ++h) mine += key[h] > threshold ? 1 : key[h] == threshold ? 1 << 16 : 0;
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
+    }
+    const int all = __shfl_sync(0xffffffffu, incl, 31);
+    int g = gt + ((incl - mine) & 0xFFFF), e = eq + ((incl - mine) >> 16);
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      const bool above = key[h] > threshold, equal = key[h] == threshold;
+      if (above || (equal && e < ties)) {
+        const int place = g + min(e, ties);
+        rows[place] = base + 4 * c + h;
+        kept[place] = src[base + 4 * c + h];
+      }
+      g += above;
+      e += equal;
+    }
+    gt += all & 0xFFFF;
+    eq += all >> 16;
   }
   if (p.slices > 1) cluster_sync();  // a CTA's totals stay readable until every CTA has read them
 }
