@@ -24,6 +24,7 @@ namespace wpt {
 
 constexpr int EVICT_THREADS = TOPK_THREADS;  // block_exclusive_scan's block
 constexpr int EVICT_BINS = 2048;
+constexpr int EVICT_SLICES = 8;  // most CTAs a row (a portable cluster)
 constexpr int EVICT_QUADS = 4 * EVICT_THREADS;  // a slice is a multiple of this: whole quads a thread
 constexpr int EVICT_COPY_THREADS = 256, EVICT_COPY_CTAS = 5;  // CTAs an SM
 
@@ -51,9 +52,15 @@ __device__ __forceinline__ uint32_t dsmem_ld_u32(uint32_t addr) {
   return v;
 }
 
+__device__ __forceinline__ uint2 dsmem_ld_u32x2(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+
 __global__ void __launch_bounds__(EVICT_THREADS) evict_rows_kernel(const EvictParams p) {
   extern __shared__ __align__(16) uint32_t s_keys[];  // cache_cap keys
-  __shared__ uint32_t s_hist[2][EVICT_BINS];
+  __shared__ __align__(16) uint32_t s_hist[2][EVICT_BINS];
   __shared__ int s_warp[EVICT_THREADS / 32];
   __shared__ uint32_t s_red[EVICT_THREADS / 16];
   __shared__ int s_gt[EVICT_THREADS / 32], s_eq[EVICT_THREADS / 32];
@@ -130,17 +137,16 @@ __global__ void __launch_bounds__(EVICT_THREADS) evict_rows_kernel(const EvictPa
 
   // bounds of the keys, and the keys into shared memory
   uint32_t lo = ALWAYS, hi = 0;
-  for (int c0 = 0; c0 < quads * EVICT_THREADS; c0 += 2 * EVICT_THREADS) {
-    uint4 k[2];
+  for (int c0 = 0; c0 < quads * EVICT_THREADS; c0 += 4 * EVICT_THREADS) {
+    uint4 k[4];
+    const int in = min(4, quads - c0 / EVICT_THREADS);  // quads a thread takes now
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int c = c0 + h * EVICT_THREADS + threadIdx.x;
-      k[h] = c < quads * EVICT_THREADS ? load4(c) : make_uint4(0, 0, 0, 0);
-    }
+    for (int h = 0; h < 4; ++h)
+      if (h < in) k[h] = load4(c0 + h * EVICT_THREADS + threadIdx.x);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int c = c0 + h * EVICT_THREADS + threadIdx.x;
-      if (cached && c < quads * EVICT_THREADS) reinterpret_cast<uint4*>(s_keys)[c] = k[h];
+    for (int h = 0; h < 4; ++h) {
+      if (h >= in) break;
+      if (cached) reinterpret_cast<uint4*>(s_keys)[c0 + h * EVICT_THREADS + threadIdx.x] = k[h];
       hi = max(max(hi, max(k[h].x, k[h].y)), max(k[h].z, k[h].w));
       // 0, past the slice's end, wraps to the largest
       lo = min(min(lo, min(k[h].x - 1, k[h].y - 1)), min(k[h].z - 1, k[h].w - 1));
@@ -199,9 +205,14 @@ __global__ void __launch_bounds__(EVICT_THREADS) evict_rows_kernel(const EvictPa
     const int top_bin = EVICT_BINS - 1 - 2 * threadIdx.x;
     int c0 = 0, c1 = 0;
     if (p.slices > 1) {
-      for (int r = 0; r < p.slices; ++r) {
-        c0 += dsmem_ld_u32(dsmem_map(smem_u32(hist + top_bin), r));
-        c1 += dsmem_ld_u32(dsmem_map(smem_u32(hist + top_bin - 1), r));
+      uint2 c[EVICT_SLICES];  // all slices' loads in flight at once
+#pragma unroll
+      for (int r = 0; r < EVICT_SLICES; ++r)
+        c[r] = r < p.slices ? dsmem_ld_u32x2(dsmem_map(smem_u32(hist + top_bin - 1), r)) : make_uint2(0, 0);
+#pragma unroll
+      for (int r = 0; r < EVICT_SLICES; ++r) {
+        c0 += c[r].y;
+        c1 += c[r].x;
       }
     } else {
       c0 = hist[top_bin];
@@ -306,7 +317,11 @@ __global__ void __launch_bounds__(EVICT_THREADS) evict_rows_kernel(const EvictPa
       if (above || (equal && e < ties)) {
         const int place = g + min(e, ties);
         rows[place] = base + 4 * c + h;
-        kept[place] = src[base + 4 * c + h];
+        // the key gives the weight back, but for -0, -inf and NaN and always kept rows
+        const uint32_t x = key[h];
+        kept[place] = x > 0x80000000u && x < ALWAYS       ? __uint_as_float(x & 0x7FFFFFFFu)
+                      : x > 0x007FFFFFu && x < 0x80000000u ? __uint_as_float(~x)
+                                                           : src[base + 4 * c + h];
       }
       g += above;
       e += equal;
