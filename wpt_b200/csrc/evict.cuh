@@ -358,14 +358,18 @@ __global__ void __launch_bounds__(EVICT_COPY_THREADS, EVICT_COPY_CTAS) evict_gat
   griddep_wait();
   if (mine >= groups) return;
   const int step = p.chunks * groups;
-  for (int64_t i0 = chunk * groups + mine; i0 < p.capacity; i0 += static_cast<int64_t>(ROWS) * step) {
+  auto row_of = [&](int64_t i) { return i < p.keep ? static_cast<int>(rows[i]) : -1; };
+  int next[ROWS];  // the rows of the places after these, read while these are copied
+  const int64_t begin = static_cast<int64_t>(chunk) * groups + mine;
+#pragma unroll
+  for (int k = 0; k < ROWS; ++k) next[k] = row_of(begin + static_cast<int64_t>(k) * step);
+  for (int64_t i0 = begin; i0 < p.capacity; i0 += static_cast<int64_t>(ROWS) * step) {
     const Unit* from[ROWS];
 #pragma unroll
-    for (int k = 0; k < ROWS; ++k) {
-      const int64_t i = i0 + static_cast<int64_t>(k) * step;
-      const int64_t row = i < p.keep ? rows[i] : -1;
-      from[k] = row >= 0 ? reinterpret_cast<const Unit*>(src + row * p.src_sn) : nullptr;
-    }
+    for (int k = 0; k < ROWS; ++k)
+      from[k] = next[k] >= 0 ? reinterpret_cast<const Unit*>(src + next[k] * p.src_sn) : nullptr;
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) next[k] = row_of(i0 + static_cast<int64_t>(ROWS + k) * step);
     for (int c = unit; c < p.units; c += group) {
       Unit v[ROWS];
 #pragma unroll
