@@ -11,8 +11,10 @@
 // bins), then of the one bin that holds it, until a bin's keys are all kept or
 // all equal; the slices' histograms are summed over distributed shared memory.
 // A count of the kept rows before each warp's run of keys gives their places.
-// evict_gather_kernel copies the kept entries. Two kernels rather than one:
-// the selection wants few CTAs a row, the copy wants every SM.
+// evict_gather_kernel copies the kept entries: the selection wants few CTAs a
+// row, the copy every SM. A few of them the selection's own CTAs copy. 64 rows of
+// 8,192 keys to 2,048 entries of 512 bytes: 31 us, of them 22 for the copy's 134
+// MB (6.1 TB/s).
 #pragma once
 
 #include <cstdint>
@@ -28,6 +30,62 @@ constexpr int EVICT_SLICES = 8;  // most CTAs a row (a portable cluster)
 constexpr int EVICT_QUADS = 4 * EVICT_THREADS;  // a slice is a multiple of this: whole quads a thread
 constexpr int EVICT_COPY_THREADS = 256, EVICT_COPY_CTAS = 5;  // CTAs an SM
 
+struct GatherParams {
+  const uint8_t* src;
+  int64_t src_sb, src_sn;  // bytes
+  uint8_t* dst;            // (B, capacity, row_bytes), contiguous
+  const int64_t* rows;     // (B, keep)
+  int keep, capacity, units;  // units of a row (row_bytes / sizeof(Unit))
+  int chunks;                 // CTAs a cache row
+};
+
+// Copies row rows[b, i] to place i of the new table, for the places of chunk
+// `chunk`, and writes zeros where there is none (rows[b, i] = -1, and the places
+// from keep to capacity: a product over a whole tile of the new table
+// multiplies its unread rows by zero weights, which must not meet a NaN).
+template <typename Unit, int THREADS>
+__device__ __forceinline__ void evict_copy(const GatherParams& p, int b, int chunk) {
+  constexpr int ROWS = 4;  // places a thread has in flight
+  const uint8_t* src = p.src + b * p.src_sb;
+  Unit* dst = reinterpret_cast<Unit*>(p.dst) + static_cast<int64_t>(b) * p.capacity * p.units;
+  const int64_t* rows = p.rows + static_cast<int64_t>(b) * p.keep;
+  // a group of threads a place, a unit each (long rows: several)
+  const int group = min(p.units, THREADS), groups = THREADS / group;
+  const int mine = threadIdx.x / group, unit = threadIdx.x - mine * group;
+  if (mine >= groups) return;
+  const int step = p.chunks * groups;
+  auto row_of = [&](int64_t i) { return i < p.keep ? static_cast<int>(__ldcg(rows + i)) : -1; };
+  int next[ROWS];  // the rows of the places after these, read while these are copied
+  const int64_t begin = static_cast<int64_t>(chunk) * groups + mine;
+#pragma unroll
+  for (int k = 0; k < ROWS; ++k) next[k] = row_of(begin + static_cast<int64_t>(k) * step);
+  for (int64_t i0 = begin; i0 < p.capacity; i0 += static_cast<int64_t>(ROWS) * step) {
+    const Unit* from[ROWS];
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k)
+      from[k] = next[k] >= 0 ? reinterpret_cast<const Unit*>(src + next[k] * p.src_sn) : nullptr;
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) next[k] = row_of(i0 + static_cast<int64_t>(ROWS + k) * step);
+    for (int c = unit; c < p.units; c += group) {
+      Unit v[ROWS];
+#pragma unroll
+      for (int k = 0; k < ROWS; ++k) v[k] = from[k] != nullptr ? from[k][c] : Unit{};
+#pragma unroll
+      for (int k = 0; k < ROWS; ++k) {
+        const int64_t i = i0 + static_cast<int64_t>(k) * step;
+        if (i < p.capacity) dst[i * p.units + c] = v[k];
+      }
+    }
+  }
+}
+
+template <typename Unit>
+__global__ void __launch_bounds__(EVICT_COPY_THREADS, EVICT_COPY_CTAS) evict_gather_kernel(const GatherParams p) {
+  griddep_wait();
+  const int b = blockIdx.x / p.chunks;
+  evict_copy<Unit, EVICT_COPY_THREADS>(p, b, blockIdx.x - b * p.chunks);
+}
+
 struct EvictParams {
   const float* weights;  // (B, N), row stride weights_ld
   int64_t weights_ld;
@@ -38,6 +96,8 @@ struct EvictParams {
   int N, keep, recent, first, capacity;
   int slices;     // CTAs (one cluster) a row
   int cache_cap;  // keys of a slice that shared memory holds
+  int copy;       // 16 or 4: this kernel copies the entries too, in units of so many bytes; 0: another does
+  GatherParams gather;
 };
 
 // The key that orders weights: larger weights, larger keys; -0 as +0; NaN as
@@ -56,6 +116,19 @@ __device__ __forceinline__ uint2 dsmem_ld_u32x2(uint32_t addr) {
   uint2 v;
   asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
   return v;
+}
+
+// The copy by the row's own CTAs, once all of them have written their rows.
+__device__ __forceinline__ void evict_copy_here(const EvictParams& p, int b, int rank) {
+  if (p.copy == 0) return;
+  if (p.slices > 1)
+    cluster_sync();
+  else
+    __syncthreads();
+  if (p.copy == 16)
+    evict_copy<uint4, EVICT_THREADS>(p.gather, b, rank);
+  else
+    evict_copy<uint32_t, EVICT_THREADS>(p.gather, b, rank);
 }
 
 __global__ void __launch_bounds__(EVICT_THREADS) evict_rows_kernel(const EvictParams p) {
@@ -89,6 +162,7 @@ __global__ void __launch_bounds__(EVICT_THREADS) evict_rows_kernel(const EvictPa
       rows[i] = i;
       kept[i] = src[i];
     }
+    evict_copy_here(p, b, rank);
     return;
   }
 
@@ -329,58 +403,11 @@ __global__ void __launch_bounds__(EVICT_THREADS) evict_rows_kernel(const EvictPa
     gt += all & 0xFFFF;
     eq += all >> 16;
   }
-  if (p.slices > 1) cluster_sync();  // a CTA's totals stay readable until every CTA has read them
-}
-
-struct GatherParams {
-  const uint8_t* src;
-  int64_t src_sb, src_sn;  // bytes
-  uint8_t* dst;            // (B, capacity, row_bytes), contiguous
-  const int64_t* rows;     // (B, keep)
-  int keep, capacity, units;  // units of a row (row_bytes / sizeof(Unit))
-  int chunks;                 // CTAs a cache row
-};
-
-// Copies row rows[b, i] to place i of the new table, and writes zeros where
-// there is none (rows[b, i] = -1, and the places from keep to capacity: a
-// product over a whole tile of the new table multiplies its unread rows by
-// zero weights, which must not meet a NaN).
-template <typename Unit>
-__global__ void __launch_bounds__(EVICT_COPY_THREADS, EVICT_COPY_CTAS) evict_gather_kernel(const GatherParams p) {
-  constexpr int ROWS = 4;  // places a thread has in flight
-  const int b = blockIdx.x / p.chunks, chunk = blockIdx.x - b * p.chunks;
-  const uint8_t* src = p.src + b * p.src_sb;
-  Unit* dst = reinterpret_cast<Unit*>(p.dst) + static_cast<int64_t>(b) * p.capacity * p.units;
-  const int64_t* rows = p.rows + static_cast<int64_t>(b) * p.keep;
-  // a group of threads a place, a unit each (long rows: several)
-  const int group = min(p.units, EVICT_COPY_THREADS), groups = EVICT_COPY_THREADS / group;
-  const int mine = threadIdx.x / group, unit = threadIdx.x - mine * group;
-  griddep_wait();
-  if (mine >= groups) return;
-  const int step = p.chunks * groups;
-  auto row_of = [&](int64_t i) { return i < p.keep ? static_cast<int>(rows[i]) : -1; };
-  int next[ROWS];  // the rows of the places after these, read while these are copied
-  const int64_t begin = static_cast<int64_t>(chunk) * groups + mine;
-#pragma unroll
-  for (int k = 0; k < ROWS; ++k) next[k] = row_of(begin + static_cast<int64_t>(k) * step);
-  for (int64_t i0 = begin; i0 < p.capacity; i0 += static_cast<int64_t>(ROWS) * step) {
-    const Unit* from[ROWS];
-#pragma unroll
-    for (int k = 0; k < ROWS; ++k)
-      from[k] = next[k] >= 0 ? reinterpret_cast<const Unit*>(src + next[k] * p.src_sn) : nullptr;
-#pragma unroll
-    for (int k = 0; k < ROWS; ++k) next[k] = row_of(i0 + static_cast<int64_t>(ROWS + k) * step);
-    for (int c = unit; c < p.units; c += group) {
-      Unit v[ROWS];
-#pragma unroll
-      for (int k = 0; k < ROWS; ++k) v[k] = from[k] != nullptr ? from[k][c] : Unit{};
-#pragma unroll
-      for (int k = 0; k < ROWS; ++k) {
-        const int64_t i = i0 + static_cast<int64_t>(k) * step;
-        if (i < p.capacity) dst[i * p.units + c] = v[k];
-      }
-    }
-  }
+  // a CTA's totals stay readable until every CTA has read them
+  if (p.copy != 0)
+    evict_copy_here(p, b, rank);
+  else if (p.slices > 1)
+    cluster_sync();
 }
 
 }  // namespace wpt
