@@ -302,3 +302,22 @@ def test_cache_evict_refusals(wb):
     assert out.shape == (0, 4, 8) and rows.shape == (0, 4)
     out, out_weights, rows, counts = wb.cache_evict(held[:, :0], w[:, :0], n, 4)
     assert not out.any() and not out_weights.any() and (rows == -1).all() and not counts.any()
+
+
+def test_positions_of_one_pass_serve_every_row(wb):
+    q, entries, positions, _, start, lse, scale = _weights_case(3, 2, 16, 128, 50, 0, False, False)
+    args = (q.cuda(), entries.cuda()[..., :128])
+    each = wb.attention_weights(*args, positions.cuda(), lse.cuda(), scale, start.cuda())
+    one = wb.attention_weights(*args, positions[0].cuda(), lse.cuda(), scale, start.cuda())
+    assert torch.equal(each, one)
+    assert torch.equal(wb.attention_weights(*args, positions.cuda(), lse.cuda(), scale) > 0,
+                       torch.ones(3, 50, dtype=torch.bool, device="cuda"))
+
+
+def test_a_small_weight_comes_back_exactly(wb):
+    """Weights under 2^-126 and zeros of both signs are kept as they are."""
+    w = torch.tensor([[1e-42, -0.0, 0.0, -1e-42, 1.0, 2e-42, -2.0, 3.0]]).cuda()
+    held = torch.arange(8.0).view(1, 8, 1).cuda()
+    out, kept, rows, _ = wb.cache_evict(held, w, torch.tensor([8]).cuda(), 5)
+    assert rows.tolist() == [[0, 1, 4, 5, 7]]
+    assert torch.equal(kept.view(torch.int32), w[:, [0, 1, 4, 5, 7]].view(torch.int32))

@@ -306,10 +306,11 @@ def attention_weights(q, k, positions, lse, scale, weights=None, window=0, floor
     (B, N, c) the cache's keys, lse (B, T, H) as forward_with_lse returns it
     for the same rows (a sink's share is then in lse and goes to no row);
     window and floor as there. Returns weights. Not differentiable."""
-    _bf16_only(q, k)
     if weights is None:
         weights = torch.zeros(q.shape[0], k.shape[1], dtype=torch.float32, device=q.device)
-    return ops.attention_weights(q, k, _positions(positions, q.shape[0]), lse, scale, weights, window, floor)
+    if positions.dim() != 2:
+        positions = _positions(positions, q.shape[0])
+    return ops.attention_weights(q, k, positions, lse, scale, weights, window, floor)
 
 
 def cache_evict(held, weights, lengths, keep, recent=0, first=0, capacity=None):
