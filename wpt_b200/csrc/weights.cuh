@@ -27,10 +27,12 @@
 // rows, and each column tile's extremes, by which tiles that no query reads are
 // skipped and tiles read whole need no mask. Bound: the exponentials (16 a clock
 // an SM: 1,024 clocks for 128 keys x 128 columns, whose products take 512), so
-// a quarter of them take the FMA pipe. 8 x 4,096 places of 16 heads, causal, width 128: 371
-// us, 741 TFLOP/s (0.46 of the measured bf16 peak; a unit's warpgroups wait about
-// a third of the time for their next scores, each having one buffer: two
-// smaller ones, or a spare in turn, measured slower).
+// a quarter of them take the FMA pipe. 8 x 4,096 places of 16 heads, causal, width
+// 128: 371 us, 741 TFLOP/s (0.46 of the measured bf16 peak, at 1.54 GHz under the
+// power limit). A run of 32 columns takes a warp 880 clocks, of which the four
+// warps of a scheduler keep its exponential unit busy for 768 and its issue slots
+// for 644; loads from TMEM and waits make up the rest, 0.62 of the unit's rate in
+// all.
 #pragma once
 
 #include <climits>
