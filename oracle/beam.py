@@ -1,6 +1,6 @@
 """CPU restatement of beam search's step, in numpy (float64).
 
-TEST INFRASTRUCTURE ONLY (the checker): only `tests/` may import it; the
+TEST INFRASTRUCTURE ONLY: only `tests/` may import it; the
 product package never does.
 """
 

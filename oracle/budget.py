@@ -1,6 +1,6 @@
 """CPU restatement of eviction by accumulated attention weight, in numpy.
 
-TEST INFRASTRUCTURE ONLY (the checker): only `tests/` may import it; the
+TEST INFRASTRUCTURE ONLY: only `tests/` may import it; the
 product package never does.
 
 attention_weights: what each row of the keys collects from a pass of queries,
