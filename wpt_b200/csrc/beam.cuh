@@ -159,12 +159,14 @@ __device__ __forceinline__ void beam_keep_best(BeamShared& s, int K, Key key) {
   beam_rank(s, K, s.count);
 }
 
-// Scores past this are so far apart that a sum holds only those equal to the
-// maximum; where the maximum is past it, they are counted in a pass of their own
-// and the running sums stay 0 (masks of the type's lowest value alone in a row).
-constexpr float BEAM_FAR = 1e30f;
+// Scores past this, 2^29, are at least 32 apart, so that a sum holds only those
+// equal to the maximum (e^-32 for the next); where the maximum is past it, they
+// are counted in a pass of their own and the running sums stay 0 (masks of a large
+// finite value alone in a row, or in all that a thread reads). Up to it M, a rounded
+// product, is within 32 of m L, so that no term is out of fp32's range.
+constexpr float BEAM_FAR = 536870912.f;
 
-// M for a maximum m: -M has to take every score to 0 or less.
+// M for a maximum m: -M has to take every score to 0 or, by its rounding, little more.
 __device__ __forceinline__ float beam_shift(float m) {
   return m < -BEAM_FAR ? 0.f : m > BEAM_FAR ? INFINITY : rintf(m * LOG2E);
 }
