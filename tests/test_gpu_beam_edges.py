@@ -2,6 +2,8 @@
 values, values that tie only after rounding, refusals that change nothing,
 replay in a graph and other streams. Values against oracle/beam.py."""
 
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -72,3 +74,76 @@ def test_masks_of_large_finite_values(wb, mask, dtype):
         _check_values(wb, wb.beam_select(x, totals.cuda(), beams), x, totals, beams)
     got = wb.beam_select(x[:, 1:], totals[:, 1:].cuda(), 3)  # one beam in: many runs
     _check_values(wb, got, x[:, 1:], totals[:, 1:], 3)
+
+
+# --------------------------------------------- values that tie after rounding
+
+def _live(step, spread):
+    """A number of live tokens whose log sum is, with values within `spread` of
+    the largest, under a fifth of `step` from a multiple of it: at totals that
+    are multiples of `step`, in the range where fp32 numbers are that far
+    apart, all values round to one, whatever the last digits of the sum."""
+    for n in range(4000, 40000):
+        low = math.log(n) / step
+        if abs(low - round(low)) + spread / step < 0.2:
+            return n
+    raise AssertionError
+
+
+# A value is off its float64 one by TOL before its last rounding: a fifth of a
+# step and TOL are less than the half that would change the rounding.
+@pytest.mark.parametrize("total, step, dtype, spread", [
+    (-4096.0, 2.0 ** -11, torch.float32, 100 * 2.0 ** -21),
+    (-2.0 ** 20, 0.125, torch.float32, None),             # scores that rise with the token
+    (-2.0 ** 22, 0.5, torch.bfloat16, 3 * 2.0 ** -5),
+])
+@pytest.mark.parametrize("beams", [1, 4, 17, 64])
+def test_values_that_tie_after_rounding(wb, total, step, dtype, spread, beams):
+    """Equal values go to the lowest beam and token, also where their scores differ."""
+    if spread is None:
+        n = next(n for n in range(28300, 28200, -1) if abs(math.log(n) / step - round(math.log(n) / step)) < 0.05)
+        x = 5 + torch.arange(n) * 2.0 ** -21
+        assert TOL / step + 0.05 + n * 2.0 ** -21 / step < 0.45
+    else:
+        n = _live(step, spread)
+        assert 0.2 + TOL / step < 0.45
+        levels = round(spread * (2 ** 21 if dtype == torch.float32 else 32))
+        g = torch.Generator().manual_seed(1)
+        x = 5 + torch.randint(0, levels, (n,), generator=g) * (spread / levels)
+    for W in (1, 3):
+        V = n + 11
+        scores = torch.full((2, W, V), -math.inf)
+        scores[:, :, 3:3 + n] = x
+        scores = scores.to(dtype).cuda()
+        assert torch.equal(scores[0, 0, 3:3 + n].float().cpu(), x.float())
+        totals = torch.full((2, W), total)
+        totals[1, W - 1] += step  # the last beam of the second text is better
+        out, parents, tokens = wb.beam_select(scores, totals.cuda(), beams)
+        assert (parents[0] == 0).all() and (parents[1] == W - 1).all()
+        want = torch.arange(3, 3 + beams)
+        assert torch.equal(tokens[0].cpu(), want) and torch.equal(tokens[1].cpu(), want)
+        assert (out == out[:, :1]).all()
+        ref = ob.select(scores.float().cpu().numpy(), totals.numpy(), beams)[0]
+        assert np.abs(out.cpu().numpy() - ref).max() <= step
+    assert wb.device_status() == 0
+
+
+def test_ties_join_other_candidates(wb):
+    """A beam's larger values stay first, then the tie's lowest tokens, whichever run they are in; an ended beam among them."""
+    step, total, V = 2.0 ** -11, -4096.0, 60000
+    n = _live(step, 4 * 2.0 ** -21)
+    scores = torch.full((1, 2, V), -math.inf)
+    at = torch.arange(n)
+    scores[0, 0, 1000 + at] = 5 + (at % 5) * 2.0 ** -21
+    scores[0, 1, :2] = 0.0
+    # beam 1 offers two values above the tie, ln 2 under its total
+    totals = torch.tensor([[total, total - 2.0]])
+    out, parents, tokens = wb.beam_select(scores.cuda(), totals.cuda(), 5)
+    assert parents.tolist() == [[1, 1, 0, 0, 0]] and tokens.tolist() == [[0, 1, 1000, 1001, 1002]]
+    done = torch.tensor([[False, True]])
+    tie = round((total - math.log(n)) / step) * step
+    out, parents, tokens = wb.beam_select(scores.cuda(), torch.tensor([[total, tie]]).cuda(), 4, done=done.cuda(), end=7)
+    assert parents.tolist() == [[0, 0, 0, 0]] and tokens.tolist() == [[1000, 1001, 1002, 1003]] and (out == tie).all()
+    out, parents, tokens = wb.beam_select(scores.flip(1).contiguous().cuda(), torch.tensor([[tie, total]]).cuda(), 4,
+                                          done=done.flip(1).cuda(), end=7)
+    assert parents.tolist() == [[0, 1, 1, 1]] and tokens.tolist() == [[7, 1000, 1001, 1002]] and (out == tie).all()

@@ -14,6 +14,12 @@
 // beam_merge_kernel: one CTA a text joins the runs' sums, turns the candidates
 // into values and ranks them. Bound: HBM, the scores read once.
 //
+// Different scores can round to one value, of which the lowest index wins, while
+// a run keeps its largest scores. So a run ranks one candidate more and hands over
+// its score, which no token that it left out passes. Where that score's value is
+// the last chosen one's (scores a rounding of the total apart), the merge reads the
+// run again for tokens of this value.
+//
 // The sums are kept in base 2 with a whole number in place of the maximum:
 // sum 2^(x L - M), L = log2(e) in fp32, M = round(m L). Moving to a larger M
 // is then exact, and the product's one rounding is that of the difference.
@@ -43,7 +49,7 @@ struct BeamParams {
   const float* totals;         // (R, W)
   const uint8_t* done;         // (R, W) or NULL
   float2* stats;               // (R, W, splits): maximum, sum of exp(x - maximum)
-  uint64_t* cand;              // (R, W, splits, K): (score, token) keys, best first, 0 for none
+  uint64_t* cand;              // (R, W, splits, K + 1): (score, token) keys, best first, 0 for none; the last without token
   float* out_totals;           // (R, K)
   int64_t* parents;            // (R, K)
   int64_t* tokens;             // (R, K)
@@ -86,7 +92,7 @@ constexpr uint64_t BEAM_ENDED = 0xFFFFFFFFull << 32;
 // A block's list of the best keys so far, and what it is made from (buf: room for
 // the list and the keys offered at once). Keys are unique, so ranks are.
 struct BeamShared {
-  uint64_t list[BEAM_MAX];  // best first
+  uint64_t list[BEAM_MAX + 1];  // best first
   uint64_t* buf;            // gathered keys
   alignas(16) uint32_t group[BEAM_THREADS];
   uint32_t bound;
@@ -119,7 +125,7 @@ __device__ __forceinline__ void beam_bound_of(BeamShared& s, int K, uint32_t top
 // The more groups, the fewer keys reach the bound (K = 16 of 64: about 18 a
 // tile; K = 64 of 256: 74), and the longer it takes to rank them.
 __device__ __forceinline__ uint32_t beam_bound(BeamShared& s, int K, uint32_t top) {
-  if (K <= 16)
+  if (K <= 17)
     beam_bound_of<64>(s, K, top);
   else
     beam_bound_of<BEAM_THREADS>(s, K, top);
@@ -178,7 +184,7 @@ __device__ __forceinline__ float beam_rescale(float from, float to) {
 // A scan block's shared memory: its tiles, which the second pass of a run with
 // too many candidates uses for their keys.
 constexpr int BEAM_TILES_BYTES = BEAM_STAGES * BEAM_THREADS * 64;
-static_assert(BEAM_TILES_BYTES >= (BEAM_MAX + BEAM_THREADS * BEAM_PER) * 8, "room for a tile's keys");
+static_assert(BEAM_TILES_BYTES >= (BEAM_MAX + 1 + BEAM_THREADS * BEAM_PER) * 8, "room for a tile's keys");
 template <typename T>
 constexpr int BEAM_TILE = BEAM_THREADS * 64 / static_cast<int>(sizeof(T));
 
@@ -214,10 +220,10 @@ struct BeamScanShared {
 
 // One run: `tiles` tiles of beam rw's scores from tile split * tiles on. Returns
 // its maximum and sum (in every thread; a NaN or +inf score makes the sum NaN),
-// its best candidates' (score, token) keys in sh.s.list[0 .. sh.s.listed).
+// its K best candidates' (score, token) keys in sh.s.list[0 .. sh.s.listed).
 template <typename T>
-__device__ __forceinline__ float2 beam_scan_run(const BeamParams& p, BeamScanShared& sh, uint8_t* s_tiles, int64_t rw,
-                                                int split) {
+__device__ __forceinline__ float2 beam_scan_run(const BeamParams& p, int K, BeamScanShared& sh, uint8_t* s_tiles,
+                                                int64_t rw, int split) {
   constexpr int VEC = 16 / sizeof(T), HALVES = 4 / sizeof(T), TILE = BEAM_TILE<T>;
   BeamShared& s = sh.s;
   const int64_t r = rw / p.W, w = rw - r * p.W;
@@ -260,7 +266,7 @@ __device__ __forceinline__ float2 beam_scan_run(const BeamParams& p, BeamScanSha
       for (int j = 1; j < BEAM_PER; ++j) top = fmaxf(top, x[j]);
       if (e0 == run0 && h == 0) {
         // the bound that every candidate has to reach, from the run's first scores
-        const uint32_t bound = beam_bound(s, p.K, top > -INFINITY ? order_key(top + 0.f) : 0u);
+        const uint32_t bound = beam_bound(s, K, top > -INFINITY ? order_key(top + 0.f) : 0u);
         if (bound != 0) least = beam_key_value(static_cast<uint64_t>(bound) << 32);
       }
       if (top >= least) {
@@ -300,10 +306,10 @@ __device__ __forceinline__ float2 beam_scan_run(const BeamParams& p, BeamScanSha
       const int n = s.count;
       __syncthreads();
       if (n <= BEAM_ROOM) {
-        beam_rank(s, p.K, n);
+        beam_rank(s, K, n);
         if (threadIdx.x < s.listed) sh.room[threadIdx.x] = s.list[threadIdx.x];
         if (threadIdx.x == 0) s.count = s.listed;
-        if (s.listed == p.K) least = fmaxf(least, beam_key_value(s.list[p.K - 1]));
+        if (s.listed == K) least = fmaxf(least, beam_key_value(s.list[K - 1]));
         __syncthreads();
       }
     }
@@ -333,7 +339,7 @@ __device__ __forceinline__ float2 beam_scan_run(const BeamParams& p, BeamScanSha
 #pragma unroll
   for (int i = 0; i < BEAM_THREADS / 32; ++i) sum += sh.sum[i];
   if (s.count <= BEAM_ROOM) {
-    beam_rank(s, p.K, s.count);
+    beam_rank(s, K, s.count);
   } else {
     // more scores reached the bound than there is room for (scores that rise
     // along the vocabulary, or many equal ones): once more over the run,
@@ -354,9 +360,9 @@ __device__ __forceinline__ float2 beam_scan_run(const BeamParams& p, BeamScanSha
           x[j] = e >= off && e < run1 ? beam_load(from + e) : -INFINITY;
           top = fmaxf(top, x[j]);
         }
-        const float worst = s.listed == p.K ? beam_key_value(s.list[p.K - 1]) : -INFINITY;
+        const float worst = s.listed == K ? beam_key_value(s.list[K - 1]) : -INFINITY;
         if (__syncthreads_or(top > worst))
-          beam_keep_best<BEAM_PER>(s, p.K, [&](int j) -> uint64_t {
+          beam_keep_best<BEAM_PER>(s, K, [&](int j) -> uint64_t {
             return x[j] > -INFINITY ? beam_key(x[j], static_cast<uint32_t>(e0 + place(h, j) - off)) : 0;
           });
       }
@@ -369,17 +375,76 @@ struct BeamMergeShared {
   BeamShared s;
   uint64_t keys[BEAM_MAX + BEAM_THREADS * 4];
   float m[BEAM_MAX], log[BEAM_MAX];
+  uint8_t again[BEAM_THREADS];
 };
 
+// The value of a candidate with the score x: it does not fall where x grows.
+__device__ __forceinline__ float beam_value(float total, float x, float m, float log) { return total + ((x - m) - log); }
+
+// Offers the tokens that their run left out and whose value is the last chosen one's.
+template <typename T, class Cand>
+__device__ __noinline__ void beam_read_again(const BeamParams& p, BeamMergeShared& sh, int64_t r, Cand cand) {
+  constexpr int TILE = BEAM_TILE<T>, GROUPS = 4, PER = 4;
+  constexpr uint64_t STEP = (sizeof(T) == 2 ? 0x10000ull : 1ull) << 32;  // between the keys of T's neighbouring numbers
+  BeamShared& s = sh.s;
+  const float tie = beam_key_value(s.list[p.K - 1]);
+  const int runs = p.W * p.splits;
+  for (int c0 = 0; c0 < runs; c0 += BEAM_THREADS) {
+    bool again = false;
+    if (c0 + static_cast<int>(threadIdx.x) < runs) {
+      const int w = (c0 + threadIdx.x) / p.splits, i = (c0 + threadIdx.x) - w * p.splits;
+      if (p.done == nullptr || !p.done[r * p.W + w]) {
+        const uint64_t key = cand(w, i, p.K);
+        const float total = p.totals[r * p.W + w];
+        auto value = [&](uint64_t k) { return beam_value(total, beam_key_value(k), sh.m[w], sh.log[w]); };
+        // where no other score has this value, what was left out has higher tokens than what was kept
+        again = key != 0 && value(key) == tie && !(value(key + STEP) > tie && value(key - STEP) < tie);
+      }
+    }
+    sh.again[threadIdx.x] = again;
+    __syncthreads();
+    for (int t = 0; t < BEAM_THREADS && c0 + t < runs; ++t) {
+      if (!sh.again[t]) continue;
+      const int w = (c0 + t) / p.splits, i = (c0 + t) - w * p.splits;
+      const T* row = static_cast<const T*>(p.scores) + r * p.stride_r + w * p.stride_w;
+      const float total = p.totals[r * p.W + w], m = sh.m[w], log = sh.log[w];
+      // the run's scores, as beam_scan_run counts them, without the part before the row
+      const int off = static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+      const int64_t v0 = max(static_cast<int64_t>(0), static_cast<int64_t>(i) * p.tiles * TILE - off);
+      const int64_t v1 = min(static_cast<int64_t>(p.V), static_cast<int64_t>(i + 1) * p.tiles * TILE - off);
+      for (int64_t v = v0 + threadIdx.x; v - threadIdx.x < v1; v += BEAM_THREADS * GROUPS * PER) {
+        uint64_t key[GROUPS * PER];
+        bool any = false;
+#pragma unroll
+        for (int j = 0; j < GROUPS * PER; ++j) {
+          const int64_t at = v + j * BEAM_THREADS;
+          const float value = at < v1 ? beam_value(total, beam_load(row + at), m, log) : -INFINITY;
+          key[j] = value == tie ? beam_key(value, static_cast<uint32_t>(w) * p.V + static_cast<uint32_t>(at)) : 0;
+          if (key[j] <= s.list[p.K - 1]) key[j] = 0;
+          for (int k = 0; key[j] != 0 && k < p.K; ++k)
+            if (s.list[k] == key[j]) key[j] = 0;  // it is chosen already
+          any |= key[j] != 0;
+        }
+        if (!__syncthreads_or(any)) continue;
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g)
+          beam_keep_best<PER>(s, p.K, [&](int j) { return key[g * PER + j]; });
+      }
+    }
+    __syncthreads();
+  }
+}
+
 // Text r's choice from its runs: stat(w, i) the maximum and sum of beam w's i-th
-// of `splits` runs, cand(w, i, k) its k-th candidate, 0 for none (neither is
+// of `splits` runs, cand(w, i, k) its k-th candidate, 0 for none, and for k = K
+// the score that no other of its tokens passes, without a token (neither is
 // asked of an ended beam).
-template <class Stat, class Cand>
+template <typename T, class Stat, class Cand>
 __device__ __forceinline__ void beam_merge(const BeamParams& p, BeamMergeShared& sh, int64_t r, Stat stat, Cand cand) {
   constexpr int PER = 4;
   BeamShared& s = sh.s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int per_beam = p.splits * p.K;
+  const int slots = p.K + 1, per_beam = p.splits * slots;
   const int total = p.W * per_beam;
   // a thread's candidates of the tile at c0: (score, token) keys (an ended
   // beam's first place: its end token), and their beams' totals
@@ -394,7 +459,7 @@ __device__ __forceinline__ void beam_merge(const BeamParams& p, BeamMergeShared&
       const int w = c / per_beam, i = c - w * per_beam;
       before[j] = p.totals[r * p.W + w];
       if (p.done == nullptr || !p.done[r * p.W + w])
-        found[j] = cand(w, i / p.K, i % p.K);
+        found[j] = cand(w, i / slots, i % slots);
       else if (i == 0)
         found[j] = BEAM_ENDED | (0xFFFFFFFFu - static_cast<uint32_t>(p.end));
     }
@@ -431,6 +496,7 @@ __device__ __forceinline__ void beam_merge(const BeamParams& p, BeamMergeShared&
     s.buf = sh.keys;
   }
   __syncthreads();
+  float others = -INFINITY;  // no other token of this thread's runs passes this value
   for (int c0 = 0; c0 < total; c0 += BEAM_THREADS * PER) {
     if (c0 > 0) load(c0);
 #pragma unroll
@@ -440,11 +506,14 @@ __device__ __forceinline__ void beam_merge(const BeamParams& p, BeamMergeShared&
       const uint32_t token = 0xFFFFFFFFu - static_cast<uint32_t>(found[j]);
       const float value = (found[j] >> 32) == (BEAM_ENDED >> 32)
                               ? before[j]
-                              : before[j] + ((beam_key_value(found[j]) - sh.m[w]) - sh.log[w]);
-      found[j] = value > -INFINITY ? beam_key(value, static_cast<uint32_t>(w) * p.V + token) : 0;
+                              : beam_value(before[j], beam_key_value(found[j]), sh.m[w], sh.log[w]);
+      if (token == 0xFFFFFFFFu) others = fmaxf(others, value);
+      found[j] = value > -INFINITY && token != 0xFFFFFFFFu ? beam_key(value, static_cast<uint32_t>(w) * p.V + token) : 0;
     }
     beam_keep_best<PER>(s, p.K, [&](int j) { return found[j]; });
   }
+  if (__syncthreads_or(others > -INFINITY && s.listed == p.K && others >= beam_key_value(s.list[p.K - 1])))
+    beam_read_again<T>(p, sh, r, cand);
   if (threadIdx.x < p.K) {
     const int64_t o = r * p.K + threadIdx.x;
     const bool some = threadIdx.x < s.listed;
@@ -457,27 +526,31 @@ __device__ __forceinline__ void beam_merge(const BeamParams& p, BeamMergeShared&
 }
 
 template <typename T>
-__global__ void __launch_bounds__(BEAM_THREADS, 4) beam_scan_kernel(const BeamParams p) {
+__global__ void __launch_bounds__(BEAM_THREADS, 4) beam_scan_kernel(const __grid_constant__ BeamParams p) {
   extern __shared__ __align__(16) uint8_t s_tiles[];
   __shared__ BeamScanShared sh;
   const int split = blockIdx.x % p.splits;
   const int64_t rw = blockIdx.x / p.splits;
   griddep_wait();
   if (p.done != nullptr && p.done[rw]) return;  // an ended beam's scores are not read
-  const float2 stat = beam_scan_run<T>(p, sh, s_tiles, rw, split);
+  const float2 stat = beam_scan_run<T>(p, p.K + 1, sh, s_tiles, rw, split);
   const int64_t run = rw * p.splits + split;
   griddep_launch();
   if (threadIdx.x == 0) p.stats[run] = stat;
-  if (threadIdx.x < p.K) p.cand[run * p.K + threadIdx.x] = threadIdx.x < sh.s.listed ? sh.s.list[threadIdx.x] : 0;
+  if (threadIdx.x <= p.K) {
+    const uint64_t key = threadIdx.x < sh.s.listed ? sh.s.list[threadIdx.x] : 0;
+    p.cand[run * (p.K + 1) + threadIdx.x] = threadIdx.x < p.K ? key : key >> 32 << 32;
+  }
 }
 
-__global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const BeamParams p) {
+template <typename T>
+__global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const __grid_constant__ BeamParams p) {
   __shared__ BeamMergeShared sh;
   const int64_t r = blockIdx.x;
   griddep_wait();
-  beam_merge(
+  beam_merge<T>(
       p, sh, r, [&](int w, int i) { return p.stats[(r * p.W + w) * p.splits + i]; },
-      [&](int w, int i, int k) { return p.cand[((r * p.W + w) * p.splits + i) * p.K + k]; });
+      [&](int w, int i, int k) { return p.cand[((r * p.W + w) * p.splits + i) * (p.K + 1) + k]; });
 }
 
 // --------------------------------------------------------------- reordering

@@ -1598,7 +1598,7 @@ extern "C" size_t wpt_beam_scratch_bytes(int R, int W, int V, int K, int bf16) {
   if (R < 1 || W < 1 || V < 1 || K < 1) return 0;
   int splits, tiles;
   beam_plan(R, W, V, bf16 != 0, &splits, &tiles);
-  return static_cast<size_t>(R) * W * splits * (8 + 8 * static_cast<size_t>(K));
+  return static_cast<size_t>(R) * W * splits * (8 + 8 * (static_cast<size_t>(K) + 1));
 }
 
 extern "C" int wpt_beam_select(const void* scores, int bf16, int64_t stride_r, int64_t stride_w, const float* totals,
@@ -1634,7 +1634,10 @@ extern "C" int wpt_beam_select(const void* scores, int bf16, int64_t stride_r, i
   p.end = end;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (int rc = bf16 ? launch_beam_scan<__nv_bfloat16>(p, s) : launch_beam_scan<float>(p, s)) return rc;
-  return launch_dependent("beam_merge_kernel launch", wpt::beam_merge_kernel, R, wpt::BEAM_THREADS, 0, 1, s, p);
+  if (bf16)
+    return launch_dependent("beam_merge_kernel launch", wpt::beam_merge_kernel<__nv_bfloat16>, R, wpt::BEAM_THREADS, 0, 1,
+                            s, p);
+  return launch_dependent("beam_merge_kernel launch", wpt::beam_merge_kernel<float>, R, wpt::BEAM_THREADS, 0, 1, s, p);
 }
 
 namespace {
