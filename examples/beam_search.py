@@ -142,8 +142,9 @@ def search(model, prompts, beams, steps, budget=None, end=None, observe=32):
         done = None if end is None else tokens == end
         totals, parents, tokens = wpt_b200.beam_select(model.scores(x[:, 0]).view(R, beams, -1), totals, beams,
                                                        done=done, end=end)
-        moved = [c.table for c in layers] + ([c.weights for c in layers] if budget is not None else [])
-        wpt_b200.cache_reorder(moved, parents, one * rows, first=one[:R] * shared)
+        wpt_b200.cache_reorder([c.table for c in layers], parents, one * rows, first=one[:R] * shared)
+        if budget is not None:  # the shared rows too: their entries are the same in all beams, their weights are not
+            wpt_b200.cache_reorder([c.weights for c in layers], parents, one * rows)
         history = torch.cat([torch.gather(history, 1, parents.clamp_min(0)[..., None].expand_as(history)),
                              tokens[..., None]], 2)
     return history, totals

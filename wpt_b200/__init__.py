@@ -346,8 +346,10 @@ def cache_reorder(tables, parents, lengths, first=None):
     (R * W, N, ...) of the list `tables` (or the one), beam w of text r takes
     the rows first[r] (default 0) .. lengths[r * W + p] - 1 of beam p =
     parents[r, w] (R, W), as beam_select returns them; a parent of -1 leaves
-    the beam as it is. first: the rows before it are the same in all beams of
-    a text (its prompt) and are not moved. Tables of any shape and dtype
+    the beam as it is. first: the rows before it are not moved, for tables
+    where they are the same in all beams of a text (its prompt's entries;
+    not the weights that they have collected, which are each beam's own).
+    Tables of any shape and dtype whose entries are a multiple of 4 bytes
     (accumulated weights (R * W, N) too). Returns `tables`."""
     return ops.cache_reorder(tables, parents, lengths, first)
 

@@ -712,7 +712,8 @@ def cache_reorder(tables, parents, lengths, first=None):
     """Reorders the beams' rows of one table or a list of tables (R * W, N,
     ...) in place: beam w of text r (row r * W + w) takes the table rows
     first[r] (default 0) .. lengths[r * W + p] - 1 of beam p = parents[r, w]
-    (-1: it keeps its own). Returns `tables`. A launch for every 32 tables,
+    (-1: it keeps its own); those before first[r], which have to be the same
+    in all beams of the text, stay. Returns `tables`. A launch for every 32 tables,
     whatever their shapes."""
     every = [tables] if isinstance(tables, torch.Tensor) else tables
     device = parents.device
