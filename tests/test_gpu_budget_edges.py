@@ -1,0 +1,120 @@
+"""Eviction by accumulated attention weight on the GPU where it can go wrong:
+NaN and infinities beside padding columns, broken queries, items that a CTA
+takes one after the other, long runs of columns; the weights' accuracy at
+ordinary inputs; eviction at odd offsets, in a graph and on another stream.
+
+The float64 values of the larger cases are worked out on the GPU with torch."""
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+# A term exp(x), x = scale q.k - lse in fp32, for normalised inputs (scores of
+# standard deviation 1, lse under 10): the product is summed in C / 16 <= 8
+# steps, each of which may drop 2^-23 of a sum of size 1, all in one direction:
+# 9.5e-7 of the term. The other roundings (of lse in base 2 and of the exponent,
+# 2^-24 of at most 16; the exponential, 2^-22; the sums) have independent signs
+# and partly cancel over the at least 12 columns of a key: 3e-7. So a norm of
+# errors is under 1.3e-6 of the norm of what was added. One weight alone, and the
+# largest of the terms that it adds up, may be off by their plain sum with scores
+# up to 6: 6 * 9.5e-7 + 2 * 2^-24 * 16 + 2^-22 = 8e-6.
+NORM, EACH = 1.3e-6, 8e-6
+
+
+@pytest.fixture(scope="module")
+def wb():
+    import wpt_b200
+    from wpt_b200 import build
+    build.build()
+    return wpt_b200
+
+
+def _reference(q, k, positions, scale, start, window=0, floor=None):
+    """(lse fp32, weights float64) of queries on the GPU, in float64."""
+    B, T, H, C = q.shape
+    N = k.shape[1]
+    n = torch.arange(N, device=q.device)
+    lse = torch.empty(B, T, H, device=q.device)
+    out = start.double()
+    step = max(1, 2 ** 25 // (H * N))
+    for b in range(B):
+        keys = k[b].double()
+        for t in range(0, T, step):
+            p = positions[b, t:t + step, None]
+            seen = n <= p
+            if window:
+                seen = seen & (n > p - window)
+            if floor is not None:
+                seen = seen & (n >= floor[b, t:t + step, None])
+            s = torch.matmul(q[b, t:t + step].double().reshape(-1, C), keys.t()).view(-1, H, N) * scale
+            s = s.masked_fill(~seen[:, None], -math.inf)
+            lse[b, t:t + step] = torch.logsumexp(s, -1).float()
+            term = torch.exp(s - lse[b, t:t + step, :, None].double())
+            out[b] += torch.where(seen[:, None], term, 0.0).sum((0, 1))
+    return lse, out
+
+
+def _inputs(B, T, H, C, N, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    q = torch.randn(B, T, H, C, generator=g, device="cuda").bfloat16()
+    k = torch.randn(B, N, C, generator=g, device="cuda").bfloat16()
+    return g, q, k
+
+
+def _check(wb, got, ref, start, norm=NORM):
+    add = ref - start.double()
+    off = (got.double() - ref).abs() - 2.0 ** -23 * ref.abs()  # less the addition to the old weight
+    assert (off <= EACH * add + 1e-30).all(), (off / add.clamp_min(1e-30)).max()
+    assert off.clamp_min(0).norm() <= norm * add.norm() + 1e-30
+    assert wb.device_status() == 0
+
+
+@pytest.mark.parametrize("B, T, H, C, N", [(3, 1, 16, 128, 900), (3, 1, 12, 64, 700), (2, 5, 20, 128, 600),
+                                           (2, 16, 16, 128, 500), (2, 40, 16, 128, 700), (5, 37, 12, 64, 1007)])
+def test_weights_are_within_a_few_roundings(wb, B, T, H, C, N):
+    _, q, k = _inputs(B, T, H, C, N)
+    positions = (N - T + torch.arange(T, device="cuda")).expand(B, T).contiguous()
+    start = torch.zeros(B, N, device="cuda")
+    lse, ref = _reference(q, k, positions, C ** -0.5, start)
+    _check(wb, wb.attention_weights(q, k, positions, lse, C ** -0.5), ref, start)
+
+
+# ------------------------------------------------- NaN, infinities and padding
+
+@pytest.mark.parametrize("T, H", [(2, 6), (2, 12), (2, 33), (3, 70), (2, 150)])
+@pytest.mark.parametrize("floored", [False, True])
+@pytest.mark.parametrize("poison", [math.nan, math.inf, -math.inf])
+def test_rows_between_the_queries_rows_keep_their_weight(wb, T, H, floored, poison):
+    """What rows that no query reads hold reaches no weight, padding columns (T * H is no tile's width) or not."""
+    B, C, N = 2, 128, 400
+    g, q, k = _inputs(B, T, H, C, N)
+    positions = torch.tensor([10, 300, 305][:T], device="cuda").expand(B, T).contiguous()
+    floor = (positions - 7).contiguous() if floored else None
+    window = 0 if floored else 8
+    start = torch.rand(B, N, generator=g, device="cuda")
+    lse, ref = _reference(q, k, positions, C ** -0.5, start, window, floor)
+    read = torch.zeros(N, dtype=torch.bool, device="cuda")
+    for p in positions[0].tolist():
+        read[p - 7:p + 1] = True
+    k[:, ~read] = poison
+    got = wb.attention_weights(q, k, positions, lse, C ** -0.5, start.clone(), window=window, floor=floor)
+    assert torch.equal(got[:, ~read], start[:, ~read])
+    _check(wb, got[:, read], ref[:, read], start[:, read], norm=EACH)
+
+
+@pytest.mark.parametrize("T, H", [(1, 1), (1, 12), (1, 16), (1, 40), (1, 100), (3, 43), (1, 300), (1, 129), (1, 260)])
+def test_a_key_of_minus_infinity_gets_no_weight(wb, T, H):
+    """A row whose scores are all -inf adds exp(-inf) = 0, padding columns or not."""
+    B, C, N = 2, 64, 300
+    g, q, k = _inputs(B, T, H, C, N)
+    q[..., 5] = q[..., 5].abs() + 0.5
+    positions = (N - 1 + torch.arange(T, device="cuda")).expand(B, T).contiguous()  # every row is read by all
+    start = torch.rand(B, N, generator=g, device="cuda")
+    k[:, 7, 5] = k[:, 200, 5] = -math.inf
+    lse, ref = _reference(q, k, positions, C ** -0.5, start)
+    got = wb.attention_weights(q, k, positions, lse, C ** -0.5, start.clone())
+    assert torch.equal(got[:, [7, 200]], start[:, [7, 200]])
+    _check(wb, got, ref, start, norm=EACH)

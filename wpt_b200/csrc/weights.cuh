@@ -374,6 +374,7 @@ __global__ void __launch_bounds__(WEIGHTS_STREAM_THREADS, 1)
   } else {
     const int r = threadIdx.x;
     const uint32_t lane_addr = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+    const int cols = p.T * p.H;
     bool ok = true;
     int j = 0;
     while (walk.step(p)) {
@@ -382,8 +383,8 @@ __global__ void __launch_bounds__(WEIGHTS_STREAM_THREADS, 1)
       if (!named_barrier_and(1, 128, ok)) break;
       for (int c = r; c < NCOL; c += 128) {
         const int t = c / p.H;
-        float off = -INFINITY;  // a padding column adds nothing
-        int2 range = make_int2(0, INT_MAX);
+        float off = -INFINITY;  // a padding column reads nothing
+        int2 range = make_int2(INT_MAX, -1);
         if (t < p.T) {
           const int64_t at = static_cast<int64_t>(b) * p.T + t;
           range = weights_range(p.positions[at], p.floor, at, p.window, p.N);
@@ -396,7 +397,7 @@ __global__ void __launch_bounds__(WEIGHTS_STREAM_THREADS, 1)
       named_barrier(1, 128);
       // rows that every column reads, and that any does
       int all_lo = 0, all_hi = INT_MAX, any_lo = INT_MAX, any_hi = -1;
-      for (int c = 0; c < p.T * p.H; c += p.H) {
+      for (int c = 0; c < cols; c += p.H) {
         all_lo = max(all_lo, s_lo[c]);
         all_hi = min(all_hi, s_hi[c]);
         any_lo = min(any_lo, s_lo[c]);
@@ -422,7 +423,9 @@ __global__ void __launch_bounds__(WEIGHTS_STREAM_THREADS, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(s_free + buf);
           }
-          if (whole)
+          // A padding column's score is 0 times the key, which is NaN where the key is
+          // not finite: its run takes the mask.
+          if (whole && c0 + W <= cols)
             weights_terms<W / 2, 0, false, NCOL>(sums, x, p.scale_log2, s_off + c0, n);
           else
             weights_terms<W / 2, 0, true, NCOL>(sums, x, p.scale_log2, s_off + c0, n);
@@ -481,7 +484,9 @@ __global__ void __launch_bounds__(WEIGHTS_TILE_COLS)
   const int t = static_cast<int>(c / p.H);
   float off = -INFINITY;
   int2 r = make_int2(INT_MAX, -1);
-  int4 m = make_int4(INT_MAX, -1, 0, INT_MAX);  // a column past the last changes nothing
+  // A column past the last reads nothing. Its score is 0 times the key, which is NaN
+  // where the key is not finite, so its tile always takes the mask.
+  int4 m = make_int4(INT_MAX, -1, INT_MAX, -1);
   if (t < p.T) {
     const int64_t at = static_cast<int64_t>(b) * p.T + t;
     r = weights_range(p.positions[at], p.floor, at, p.window, p.N);
