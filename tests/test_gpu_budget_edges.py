@@ -118,3 +118,40 @@ def test_a_key_of_minus_infinity_gets_no_weight(wb, T, H):
     got = wb.attention_weights(q, k, positions, lse, C ** -0.5, start.clone())
     assert torch.equal(got[:, [7, 200]], start[:, [7, 200]])
     _check(wb, got, ref, start, norm=EACH)
+
+
+@pytest.mark.parametrize("T, H", [(1, 16), (1, 24), (9, 8), (40, 16), (37, 12)])
+@pytest.mark.parametrize("broken", ["query", "lse"])
+def test_a_broken_column_shows_in_every_row_that_it_reads(wb, T, H, broken):
+    """A NaN query or lse makes all the weights that it adds to NaN, in whichever column and form; the others stay."""
+    B, C, N = 1, 128, 700
+    _, q, k = _inputs(B, T, H, C, N)
+    positions = torch.full((B, T), N - 1, device="cuda")
+    positions[0, 0] = 300
+    start = torch.zeros(B, N, device="cuda")
+    lse, ref = _reference(q, k, positions, C ** -0.5, start)
+    for h in range(min(H, 16)):
+        bad_q, bad_lse = q.clone(), lse.clone()
+        if broken == "query":
+            bad_q[0, 0, h, 3] = math.nan
+        else:
+            bad_lse[0, 0, h] = math.nan
+        got = wb.attention_weights(bad_q, k, positions, bad_lse, C ** -0.5)
+        assert got[0, :301].isnan().all(), h
+        _check(wb, got[:, 301:], ref[:, 301:], start[:, 301:], norm=EACH)
+
+
+@pytest.mark.parametrize("T, H", [(1, 16), (40, 16)])
+def test_extreme_log_sums(wb, T, H):
+    """lse +inf adds nothing, -inf neither; one far under the scores gives +inf, in every column."""
+    B, C, N = 1, 128, 300
+    _, q, k = _inputs(B, T, H, C, N)
+    positions = torch.full((B, T), N - 1, device="cuda")
+    for value in (math.inf, -math.inf):
+        got = wb.attention_weights(q, k, positions, torch.full((B, T, H), value, device="cuda"), C ** -0.5)
+        assert (got == 0).all()
+    lse, _ = _reference(q, k, positions, C ** -0.5, torch.zeros(B, N, device="cuda"))
+    for h in range(H):
+        low = lse.clone()
+        low[0, 0, h] = -1000.0
+        assert (wb.attention_weights(q, k, positions, low, C ** -0.5) == math.inf).all(), h

@@ -27,8 +27,8 @@
 // rows, and each column tile's extremes, by which tiles that no query reads are
 // skipped and tiles read whole need no mask. Bound: the exponentials (16 a clock
 // an SM: 1,024 clocks for 128 keys x 128 columns, whose products take 512), so
-// a quarter of them take the FMA pipe. 8 x 4,096 places of 16 heads, causal, width
-// 128: 371 us, 741 TFLOP/s (0.46 of the measured bf16 peak, at 1.54 GHz under the
+// an eighth of them take the FMA pipe. 8 x 4,096 places of 16 heads, causal, width
+// 128: 364 us, 755 TFLOP/s (0.47 of the measured bf16 peak, at 1.54 GHz under the
 // power limit). A run of 32 columns takes a warp 880 clocks, of which the four
 // warps of a scheduler keep its exponential unit busy for 768 and its issue slots
 // for 644; loads from TMEM and waits make up the rest, 0.62 of the unit's rate in
@@ -55,17 +55,24 @@ __device__ __forceinline__ int2 weights_range(int64_t pos, const int64_t* floor,
 // query without rows has lse -inf; it adds nothing.
 __device__ __forceinline__ float weights_offset(float lse) { return lse == -INFINITY ? -INFINITY : -lse * LOG2E; }
 
+__device__ __forceinline__ float weights_clamp(float x, float lo, float hi) {  // a NaN stays one
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(lo));
+  asm("min.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(hi));
+  return x;
+}
+
 // 2^x for a pair of floats on the FMA pipe, for the terms whose turn it is not
-// on the exponential unit. 2^x = 2^r 2^f with r = round(x), found by adding
-// 1.5 * 2^23, and f = x - r in [-1/2, 1/2]: 2^f is a polynomial of degree 5
-// fitted for this library by iterated weighted least squares (relative error
-// 1.5e-7, a rounding of the sum it goes into); r is added to its exponent. x
-// is clamped at -126: a smaller term counts as 2^-126.
+// on the exponential unit. 2^x = 2^r 2^f with r = round(x) and f = x - r in
+// [-1/2, 1/2]: 2^f is a polynomial of degree 5 fitted for this library by
+// iterated weighted least squares (relative error 1.5e-7, a rounding of the sum it
+// goes into). Adding 1.5 * 2^23 + 127 rounds x and leaves r + 127 in the low bits,
+// which shifted are 2^r: 0 at r = -127 and +inf at 128, where x is clamped. A
+// product with it, and not an addition to the exponent, keeps a NaN.
 __device__ __forceinline__ uint64_t weights_exp2_poly(uint64_t x) {
-  constexpr float MAGIC = 12582912.0f;
+  constexpr float MAGIC = 12582912.0f + 127.0f;
   float x0, x1;
   f2_unpack(x, x0, x1);
-  x = f2_pack(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
+  x = f2_pack(weights_clamp(x0, -127.f, 128.f), weights_clamp(x1, -127.f, 128.f));
   const uint64_t t = f2_add(x, f2_pack(MAGIC, MAGIC));
   const uint64_t r = f2_add(t, f2_pack(-MAGIC, -MAGIC));
   const uint64_t f = f2_fma(r, f2_pack(-1.f, -1.f), x);
@@ -74,11 +81,9 @@ __device__ __forceinline__ uint64_t weights_exp2_poly(uint64_t x) {
   q = f2_fma(q, f, f2_pack(0.24022242426872253f, 0.24022242426872253f));
   q = f2_fma(q, f, f2_pack(0.6931470036506653f, 0.6931470036506653f));
   q = f2_fma(q, f, f2_pack(1.f, 1.f));
-  float q0, q1, t0, t1;
-  f2_unpack(q, q0, q1);
+  float t0, t1;
   f2_unpack(t, t0, t1);
-  return f2_pack(__int_as_float(__float_as_int(q0) + (__float_as_int(t0) << 23)),
-                 __int_as_float(__float_as_int(q1) + (__float_as_int(t1) << 23)));
+  return f2_mul(q, f2_pack(__int_as_float(__float_as_int(t0) << 23), __int_as_float(__float_as_int(t1) << 23)));
 }
 
 // Adds exp2(x scale + cols[0][c]) over 2 * PAIRS columns c to the four partial
@@ -472,8 +477,8 @@ constexpr int WEIGHTS_TILE_GROUPS = 4;     // key tiles of 128 an item, one for 
 constexpr int WEIGHTS_TILE_COLS = 128;
 constexpr int WEIGHTS_Q_STAGES = 2, WEIGHTS_C_STAGES = 4;
 // Pairs in every 8 whose exponentials take the FMA pipe. 8 x 4,096 places of 16
-// heads, causal: 0 take 388 us, 1 373, 2 371, 3 390.
-constexpr int WEIGHTS_POLY8 = 2;
+// heads, causal: 0 take 389 us, 1 364, 2 368, 3 387.
+constexpr int WEIGHTS_POLY8 = 1;
 
 struct WeightsTileParams {
   float* weights;      // (B, N), row stride weights_ld
