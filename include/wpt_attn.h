@@ -368,7 +368,8 @@ int wpt_cache_append(const void* src, int64_t src_stride_b, int64_t src_stride_n
  *   positions  int64 (B, T);  floor  int64 (B, T) or NULL
  *   lse        fp32 (B, T, H);  weights  fp32 (B, N), row stride weights_ld
  *   scratch    wpt_attn_weights_scratch_bytes(B, T, H, N) bytes, 16-byte
- *              aligned (none is needed, and NULL taken, up to 256 columns T * H)
+ *              aligned (none is needed, and NULL taken, up to 256 columns T * H;
+ *              above that 13 bytes a column, and up to 256 a key or 10 MB in all)
  */
 int wpt_attn_weights(const void* q, const void* k, int64_t k_stride_b, int64_t k_stride_n, const int64_t* positions,
                      const int64_t* floor, const float* lse, float* weights, int64_t weights_ld, void* scratch, int B,

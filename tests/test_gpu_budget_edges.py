@@ -155,3 +155,49 @@ def test_extreme_log_sums(wb, T, H):
         low = lse.clone()
         low[0, 0, h] = -1000.0
         assert (wb.attention_weights(q, k, positions, low, C ** -0.5) == math.inf).all(), h
+
+
+# ------------------------------------------- the query-stream form's machinery
+
+def _runs(wb, B, T, H, N):
+    """Runs that each key's column tiles are summed in: from the scratch's size, which holds a sum a run and key."""
+    from wpt_b200 import _lib
+    size = _lib.lib().wpt_attn_weights_scratch_bytes(B, T, H, N)
+    tiles = -(-T * H // 128)
+    sums = size - 16 - B * tiles * (16 + 128 * 12)
+    return tiles, max(1, sums // (4 * B * N))
+
+
+LONG = [
+    # B, T, H, C, N, window, ragged, floored, column tiles a run
+    (8, 1600, 32, 64, 1501, 0, False, False, 16),   # 400 column tiles: 600 items of 4 key tiles, several a CTA
+    (8, 1600, 32, 128, 1501, 200, True, True, 16),  # items that no query reads among them
+    (5, 1252, 32, 128, 1301, 0, True, False, 8),
+    (3, 900, 24, 64, 2501, 300, True, False, 4),
+    (150, 17, 16, 128, 333, 0, True, True, 3),      # an item a row and CTA, and some over; three column tiles
+    (1, 2200, 64, 128, 17409, 0, False, False, 32),  # runs of more than 16 column tiles
+]
+
+
+@pytest.mark.parametrize("case", LONG, ids=lambda c: "x".join(map(str, c[:6])) + "rf"[:c[6] + c[7]])
+def test_items_one_after_the_other(wb, case):
+    B, T, H, C, N, window, ragged, floored, run = case
+    tiles, runs = _runs(wb, B, T, H, N)
+    assert runs == -(-tiles // run)
+    assert B * -(-N // 512) * runs > 148  # even with four key tiles an item, some CTA takes a second one
+    g, q, k = _inputs(B, T, H, C, N)
+    lengths = torch.randint(0, N + 1, (B,), generator=g, device="cuda") if ragged else torch.full((B,), N, device="cuda")
+    positions = lengths[:, None] - T + torch.arange(T, device="cuda")
+    floor = torch.randint(-3, N + 3, (B, T), generator=g, device="cuda") if floored else None
+    start = torch.rand(B, N, generator=g, device="cuda")
+    lse, ref = _reference(q, k, positions, C ** -0.5, start, window, floor)
+    args = (q, k, positions, lse, C ** -0.5)
+    got = wb.attention_weights(*args, start.clone(), window=window, floor=floor)
+    # the runs' sums and a run's own are of up to thousands of terms, each addition 2^-24 of the running sum, at
+    # random signs: 64 roundings and more, 4e-6 of it
+    assert wb.device_status() == 0
+    add = ref - start.double()
+    off = (got.double() - ref).abs() - 2.0 ** -23 * ref.abs()
+    assert (off <= 2 * EACH * add + 1e-30).all(), (off / add.clamp_min(1e-30)).max()
+    assert off.clamp_min(0).norm() <= 4 * NORM * add.norm()
+    assert torch.equal(got, wb.attention_weights(*args, start.clone(), window=window, floor=floor))

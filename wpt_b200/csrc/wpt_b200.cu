@@ -1364,9 +1364,14 @@ WeightsPlan weights_plan(int64_t B, int64_t T, int64_t H, int64_t N) {
   w.groups = 1;
   while (w.groups < wpt::WEIGHTS_TILE_GROUPS && B * blocks(w.groups) * ((w.tiles + 3) / 4) > sms) w.groups *= 2;
   w.key_blocks = static_cast<int>(blocks(w.groups));
-  // runs of at most 16 column tiles, shorter ones (not under 4) to four items an SM
+  // runs of 16 column tiles, shorter ones (not under 4) to four items an SM
   int64_t per = 16;
   while (per > 4 && B * w.key_blocks * ((w.tiles + per - 1) / per) < 4 * sms) per /= 2;
+  // Longer ones where there are more than 64 a key and eight items an SM are left:
+  // each run leaves a sum a key, B N T H / 512 bytes with runs of 16 (1 GB for a row
+  // of 131,072 places of 32 heads), so at most 256 bytes a key or 5 MB in all. A row
+  // of 32,768 places takes 4.9 to 5.1 ms either way.
+  while ((w.tiles + per - 1) / per > 64 && B * w.key_blocks * ((w.tiles + 2 * per - 1) / (2 * per)) >= 8 * sms) per *= 2;
   w.chunk_tiles = static_cast<int>(per < w.tiles ? per : w.tiles);
   w.chunks = (w.tiles + w.chunk_tiles - 1) / w.chunk_tiles;
   int64_t at = 0;
