@@ -6,6 +6,9 @@ ordinary inputs; eviction at odd offsets, in a graph and on another stream.
 The float64 values of the larger cases are worked out on the GPU with torch."""
 
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -22,6 +25,8 @@ pytestmark = pytest.mark.gpu
 # largest of the terms that it adds up, may be off by their plain sum with scores
 # up to 6: 6 * 9.5e-7 + 2 * 2^-24 * 16 + 2^-22 = 8e-6.
 NORM, EACH = 1.3e-6, 8e-6
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 @pytest.fixture(scope="module")
@@ -201,3 +206,37 @@ def test_items_one_after_the_other(wb, case):
     assert (off <= 2 * EACH * add + 1e-30).all(), (off / add.clamp_min(1e-30)).max()
     assert off.clamp_min(0).norm() <= 4 * NORM * add.norm()
     assert torch.equal(got, wb.attention_weights(*args, start.clone(), window=window, floor=floor))
+
+
+# ------------------------------------------------------------------- eviction
+
+def test_threads_evict_tables_of_all_lengths(wb):
+    """Each thread's calls ask for shared memory of their own size, from the process's first calls on."""
+    code = """
+import threading, torch, wpt_b200
+start, failed = threading.Barrier(8), []
+cases = []
+for n in range(1, 13):
+    cases.append((torch.arange(4096.0 * n).flip(0).view(1, -1).cuda(), torch.tensor([4096 * n]).cuda()))
+def work(t):
+    try:
+        start.wait()
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for i in range(120):
+                w, n = cases[(i * (2 * t + 1) + t) % 12]
+                rows = wpt_b200.cache_evict(w[..., None], w, n, 9)[2]
+                torch.cuda.current_stream().synchronize()
+                if rows.tolist() != [list(range(9))]:
+                    failed.append((t, i, rows.tolist()))
+    except BaseException as e:
+        failed.append((t, repr(e)))
+threads = [threading.Thread(target=work, args=(t,)) for t in range(8)]
+torch.cuda.synchronize()
+[t.start() for t in threads]
+[t.join() for t in threads]
+assert not failed, failed
+print("done")
+"""
+    for _ in range(3):
+        run = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
+        assert run.returncode == 0 and run.stdout.strip() == "done", run.stderr[-2000:]

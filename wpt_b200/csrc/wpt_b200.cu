@@ -207,14 +207,12 @@ int allow_smem(Kernel kernel, int bytes) {
   static std::map<std::pair<const void*, int>, int> done;
   const int dev = current_device();
   const auto key = std::make_pair(reinterpret_cast<const void*>(kernel), dev);
-  {
-    std::lock_guard<std::mutex> lock(mu);
-    auto it = done.find(key);
-    if (it != done.end() && it->second >= bytes) return WPT_OK;
-  }
+  // one lock over the check and the call: the limit never falls under what another thread's launch needs
+  std::lock_guard<std::mutex> lock(mu);
+  auto it = done.find(key);
+  if (it != done.end() && it->second >= bytes) return WPT_OK;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(max dynamic shared memory)");
-  std::lock_guard<std::mutex> lock(mu);
   done[key] = bytes;
   return WPT_OK;
 }
