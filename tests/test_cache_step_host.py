@@ -1,6 +1,12 @@
 """The cache operators' host side without a GPU, where it can go wrong."""
 
+import os
+import subprocess
+import sys
+
 import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 @pytest.fixture(scope="module")
@@ -18,3 +24,19 @@ def test_attn_weights_scratch_is_linear(lib, B, T, H, N):
     columns = -(-T * H // 128) * 128
     size = lib.lib().wpt_attn_weights_scratch_bytes(B, T, H, N)
     assert 0 < size <= 13 * B * columns + max(256 * B * N, 10 << 20)
+
+
+def test_the_package_imports_without_cuda_bindings():
+    """A torch built without CUDA has none of torch._C's CUDA functions: the import works, the first call refuses."""
+    code = """
+import torch
+for name in [n for n in dir(torch._C) if n.startswith("_cuda")]:
+    delattr(torch._C, name)
+import wpt_b200
+try:
+    wpt_b200.cache_evict(torch.zeros(1, 4, 8), torch.zeros(1, 4), torch.zeros(1, dtype=torch.int64), 2)
+except ValueError as e:
+    print(e)
+"""
+    run = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "CUDA device only" in run.stdout, run.stderr[-2000:]

@@ -541,7 +541,7 @@ def accept(scores, drafted, q, uniforms, resample, temperature=1.0, top_k=None, 
 
 # ------------------------------------------- the cache between two decode steps
 
-_current = torch._C._cuda_getDevice
+_current = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)  # the raw query, where there is one
 
 
 def _one_device(*tensors):
