@@ -147,3 +147,14 @@ def test_ties_join_other_candidates(wb):
     out, parents, tokens = wb.beam_select(scores.flip(1).contiguous().cuda(), torch.tensor([[tie, total]]).cuda(), 4,
                                           done=done.flip(1).cuda(), end=7)
     assert parents.tolist() == [[0, 1, 1, 1]] and tokens.tolist() == [[7, 1000, 1001, 1002]] and (out == tie).all()
+
+
+# ------------------------------------------------------------------- refusals
+
+def test_a_refused_reorder_moves_nothing(wb):
+    tables = [torch.arange(2 * 3.0, device="cuda").view(2, 3, 1) for _ in range(40)]
+    was = tables[0].clone()
+    tables[35] = torch.zeros(2, 3, 1, dtype=torch.int16, device="cuda")  # 2-byte entries
+    with pytest.raises(NotImplementedError):
+        wb.cache_reorder(tables, torch.tensor([[1, 0]], device="cuda"), torch.tensor([3, 3], device="cuda"))
+    assert all(torch.equal(t, was) for t in tables[:35])

@@ -706,6 +706,7 @@ def beam_select(scores, totals, beams, done=None, end=None):
 
 
 REORDER_TABLES = 32  # tables wpt_cache_reorder takes in one launch
+BEAM_MAX = 64  # beams in and out
 
 
 def cache_reorder(tables, parents, lengths, first=None):
@@ -725,7 +726,7 @@ def cache_reorder(tables, parents, lengths, first=None):
     parents, lengths = _rows(parents), _rows(lengths)
     if first is not None:
         first = _rows(first)
-    fields = []
+    fields, units = [], 0
     for t in every:
         shape = t.shape
         if t.device != device:
@@ -738,6 +739,10 @@ def cache_reorder(tables, parents, lengths, first=None):
             raise ValueError("a reordered table's entries must be contiguous and its places must not overlap: it is "
                              "changed in place")
         fields += (t.data_ptr(), sb, sn, size, shape[1])
+        units |= t.data_ptr() | sb | sn | size
+    if units % 4 or (fields and W > BEAM_MAX):  # before the first launch: a call that is refused moves nothing
+        raise NotImplementedError("the reordering kernel takes up to 64 beams and moves units of 4 bytes: tables, strides "
+                                  "and entries must be multiples of 4 bytes")
     lib = _lib.lib()
     for i in range(0, len(fields), 5 * REORDER_TABLES):
         part = fields[i:i + 5 * REORDER_TABLES]
