@@ -1,6 +1,7 @@
 """The cache operators' host side without a GPU, where it can go wrong."""
 
 import os
+import random
 import subprocess
 import sys
 
@@ -40,3 +41,28 @@ except ValueError as e:
 """
     run = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert run.returncode == 0 and "CUDA device only" in run.stdout, run.stderr[-2000:]
+
+
+def test_overlapping_places_are_found():
+    """A table's strides, and two tables' of the same strides, against every byte of their places."""
+    from wpt_b200.ops import _places_overlap, _tables_overlap
+    rng = random.Random(0)
+
+    def places(at, rows, sb, sn, size, N):
+        each = [set(range(at + b * sb + n * sn, at + b * sb + n * sn + size)) for b in range(rows) for n in range(N)]
+        every = set().union(*each)
+        return every, len(every) < sum(map(len, each))
+
+    found = 0
+    for _ in range(4000):
+        rows, N, N2 = rng.randint(1, 4), rng.randint(1, 5), rng.randint(1, 5)
+        sb, sn, at = rng.choice([0, *range(40)]), rng.randint(0, 12), rng.randint(0, 60)
+        size, size2 = rng.randint(1, 6), rng.randint(1, 6)
+        one, shared = places(0, rows, sb, sn, size, N)
+        other, shared2 = places(at, rows, sb, sn, size2, N2)
+        assert _places_overlap(rows, sb, sn, size, N) == shared
+        assert _places_overlap(rows, sb, sn, size, N, at, size2, N2) == bool(one & other)
+        if not shared and not shared2:
+            assert _tables_overlap(rows, [at, sb, sn, size2, N2, 0, sb, sn, size, N]) == bool(one & other)
+            found += bool(one & other)
+    assert found > 100

@@ -151,6 +151,30 @@ def test_ties_join_other_candidates(wb):
 
 # ------------------------------------------------------------------- refusals
 
+def test_tables_that_share_memory_are_refused(wb):
+    parents, lengths = torch.tensor([[1, 0, 0]], device="cuda"), torch.full((3,), 10, device="cuda")
+    t = torch.randn(3, 10, 8, device="cuda")
+    flat = torch.randn(1000, device="cuda")
+    was = t.clone()
+    for bad in ([t, t], [t, torch.zeros_like(t), t[:, 5:]], [t, t.transpose(0, 1).contiguous().transpose(0, 1), t[..., 4:]],
+                flat.as_strided((3, 10, 8), (8, 8, 1)), flat.as_strided((3, 10, 8), (40, 8, 1)),
+                flat.as_strided((3, 10, 8), (12, 20, 1))):
+        with pytest.raises(ValueError):
+            wb.cache_reorder(bad, parents, lengths)
+    empty = torch.zeros(3, 0, 8, device="cuda")
+    with pytest.raises(ValueError):
+        wb.cache_reorder([t, empty, t[..., 4:]], parents, lengths)
+    assert torch.equal(t, was)
+    # what shares a range of addresses and no byte is taken: the halves of entries, in either order of places
+    for big in (torch.randn(3, 10, 16, device="cuda"), torch.randn(10, 3, 16, device="cuda").transpose(0, 1)):
+        want = ob.reorder(big.cpu().numpy(), parents.cpu().numpy(), lengths.cpu().numpy())
+        wb.cache_reorder([big[..., 8:], big[..., :8]], parents, lengths)
+        assert np.array_equal(big.cpu().numpy(), want)
+    odd = flat.as_strided((3, 10, 8), (8, 24, 1))
+    want = ob.reorder(odd.cpu().numpy(), parents.cpu().numpy(), lengths.cpu().numpy())
+    assert np.array_equal(wb.cache_reorder(odd, parents, lengths).cpu().numpy(), want)
+
+
 def test_a_refused_reorder_moves_nothing(wb):
     tables = [torch.arange(2 * 3.0, device="cuda").view(2, 3, 1) for _ in range(40)]
     was = tables[0].clone()

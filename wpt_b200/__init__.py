@@ -350,7 +350,8 @@ def cache_reorder(tables, parents, lengths, first=None):
     where they are the same in all beams of a text (its prompt's entries;
     not the weights that they have collected, which are each beam's own).
     Tables of any shape and dtype whose entries are a multiple of 4 bytes
-    (accumulated weights (R * W, N) too). Returns `tables`."""
+    (accumulated weights (R * W, N) too), no two of them sharing memory.
+    Returns `tables`."""
     return ops.cache_reorder(tables, parents, lengths, first)
 
 

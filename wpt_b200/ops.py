@@ -705,6 +705,48 @@ def beam_select(scores, totals, beams, done=None, end=None):
     return out, parents, tokens
 
 
+def _places_overlap(rows, sb, sn, size, N, at=None, size2=0, N2=0):
+    """Whether two of a table's places (b, n), `size` bytes at b * sb + n * sn (b
+    under `rows`, n under N), share a byte; given `at`, whether one does with a place of
+    a table of the same strides (places of size2 bytes, n under N2) that starts there."""
+    same = at is None
+    if same:
+        at, size2, N2 = 0, size, N
+    for b in range(1 - rows, rows):  # n2 * sn - n * sn in (-size2, size) - at - b * sb, over n2 - n
+        low, high = -size2 - at - b * sb, size - at - b * sb
+        if sn == 0:
+            if low < 0 < high and not (same and b == 0 and N == 1):
+                return True
+            continue
+        first, last = max(1 - N, low // sn + 1), min(N2 - 1, -(-high // sn) - 1)
+        if last - first + 1 > (same and b == 0 and first <= 0 <= last):  # a place may share with itself
+            return True
+    return False
+
+
+def _tables_overlap(rows, fields):
+    """Whether tables, five numbers each (first byte, sb, sn, size, N), share memory, as
+    far as that is told by their extents and, where these cross, by equal strides."""
+    tables = sorted(zip(*(fields[i::5] for i in range(5))))
+    tables = [t for t in tables if rows * t[3] * t[4]]
+    for i, (start, sb, sn, size, N) in enumerate(tables):
+        end = start + (rows - 1) * sb + (N - 1) * sn + size
+        for start2, sb2, sn2, size2, N2 in tables[i + 1:]:
+            if start2 >= end:
+                break
+            at = start2 - start
+            if (sb, sn) != (sb2, sn2) and (rows, N, N2) != (1, 1, 1):
+                continue
+            # parts of the same wider entries, as keys and values: no need to look further
+            wide = at + size2
+            if size <= at and (wide <= sn and (rows == 1 or sb >= (max(N, N2) - 1) * sn + wide) or
+                               wide <= sb and sn >= (rows - 1) * sb + wide):
+                continue
+            if _places_overlap(rows, sb, sn, size, N, at, size2, N2):
+                return True
+    return False
+
+
 REORDER_TABLES = 32  # tables wpt_cache_reorder takes in one launch
 BEAM_MAX = 64  # beams in and out
 
@@ -727,6 +769,7 @@ def cache_reorder(tables, parents, lengths, first=None):
     if first is not None:
         first = _rows(first)
     fields, units = [], 0
+    low, high, crossed = 0, 0, False  # the addresses of the tables so far; whether one lies among them
     for t in every:
         shape = t.shape
         if t.device != device:
@@ -735,11 +778,26 @@ def cache_reorder(tables, parents, lengths, first=None):
             raise ValueError(f"a table of {tuple(shape)} for {R} texts of {W} beams")
         size, es, stride = _row_bytes(t), t.element_size(), t.stride()
         sb, sn = stride[0] * es, stride[1] * es
-        if size is None or sb < size and R * W > 1 and t.numel() or sn < size and shape[1] > 1 and t.numel():
+        N = shape[1]
+        if size is None or (t.numel() and not (sn >= size and sb >= (N - 1) * sn + size) and
+                            not (sb >= size and sn >= (R * W - 1) * sb + size) and
+                            _places_overlap(R * W, sb, sn, size, N)):
             raise ValueError("a reordered table's entries must be contiguous and its places must not overlap: it is "
                              "changed in place")
-        fields += (t.data_ptr(), sb, sn, size, shape[1])
-        units |= t.data_ptr() | sb | sn | size
+        at = t.data_ptr()
+        fields += (at, sb, sn, size, N)
+        units |= at | sb | sn | size
+        end = at + (R * W - 1) * sb + (N - 1) * sn + size
+        if not size * N:
+            continue
+        if at >= high:
+            high, low = end, low or at
+        elif end <= low:
+            low = at
+        else:
+            crossed = True
+    if crossed and _tables_overlap(R * W, fields):
+        raise ValueError("two reordered tables share memory: they are changed in place")
     if units % 4 or (fields and W > BEAM_MAX):  # before the first launch: a call that is refused moves nothing
         raise NotImplementedError("the reordering kernel takes up to 64 beams and moves units of 4 bytes: tables, strides "
                                   "and entries must be multiples of 4 bytes")
