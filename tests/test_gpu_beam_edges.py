@@ -151,6 +151,19 @@ def test_ties_join_other_candidates(wb):
 
 # ------------------------------------------------------------------- refusals
 
+def test_numbers_past_32_bits_are_refused(wb):
+    x, t = torch.zeros(2, 3, 10, device="cuda"), torch.zeros(2, 3, device="cuda")
+    done = torch.ones(2, 3, dtype=torch.bool, device="cuda")
+    for end in (2 ** 32 + 1, -2 ** 32 + 1, -1):
+        with pytest.raises(ValueError):
+            wb.beam_select(x, t, 2, done=done, end=end)
+    with pytest.raises(NotImplementedError):
+        wb.beam_select(x, t, 2 ** 32 + 2)
+    wide = torch.zeros(1, 1, 1, device="cuda").expand(1, 1, 2 ** 32 + 10)
+    with pytest.raises(NotImplementedError):
+        wb.beam_select(wide, t[:1, :1], 2)
+
+
 def test_tables_that_share_memory_are_refused(wb):
     parents, lengths = torch.tensor([[1, 0, 0]], device="cuda"), torch.full((3,), 10, device="cuda")
     t = torch.randn(3, 10, 8, device="cuda")

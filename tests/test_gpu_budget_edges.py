@@ -208,7 +208,34 @@ def test_items_one_after_the_other(wb, case):
     assert torch.equal(got, wb.attention_weights(*args, start.clone(), window=window, floor=floor))
 
 
+# ------------------------------------------------------------------ arguments
+
+def test_a_window_past_32_bits_is_no_window(wb):
+    _, q, k = _inputs(2, 1, 16, 128, 300)
+    positions = torch.full((2, 1), 299, device="cuda")
+    _, lse = wb.forward_with_lse(q, k, k, positions, 0.1)
+    every = wb.attention_weights(q, k, positions, lse, 0.1)
+    assert torch.equal(wb.attention_weights(q, k, positions, lse, 0.1, window=2 ** 32 + 5), every)
+    assert torch.equal(wb.attention_weights(q, k, positions, lse, 0.1, window=2 ** 31), every)
+    with pytest.raises(ValueError):
+        wb.attention_weights(q, k, positions, lse, 0.1, window=-2 ** 32 + 5)
+
+
 # ------------------------------------------------------------------- eviction
+
+def test_cache_evict_of_tables_past_32_bits_is_refused(wb):
+    n = torch.ones(1, dtype=torch.int64, device="cuda")
+    long = torch.zeros(1, 1, device="cuda").expand(1, 2 ** 32 + 5)
+    with pytest.raises(NotImplementedError):
+        wb.cache_evict(long[..., None], long, n, 1)
+    held, weights = torch.zeros(1, 4, 8, device="cuda"), torch.zeros(1, 4, device="cuda")
+    with pytest.raises(NotImplementedError):
+        wb.cache_evict(held, weights, n, 1, capacity=2 ** 32 + 5)
+    with pytest.raises(NotImplementedError):
+        wb.cache_evict(held, weights, n, 2 ** 32 + 5)
+    with pytest.raises(NotImplementedError):
+        wb.cache_evict(torch.zeros(1, device="cuda").expand(1, 4, 2 ** 30 + 4), weights, n, 1)
+
 
 def test_threads_evict_tables_of_all_lengths(wb):
     """Each thread's calls ask for shared memory of their own size, from the process's first calls on."""

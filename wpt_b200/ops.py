@@ -541,6 +541,7 @@ def accept(scores, drafted, q, uniforms, resample, temperature=1.0, top_k=None, 
 
 # ------------------------------------------- the cache between two decode steps
 
+BEAM_MAX = 64  # beams in and out of beam_select, and of cache_reorder
 _current = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)  # the raw query, where there is one
 
 
@@ -596,6 +597,9 @@ def attention_weights(q, k, positions, lse, scale, weights, window=0, floor=None
                          f"{tuple(positions.shape)}")
     if weights.dtype != torch.float32 or weights.shape != (B, N):
         raise ValueError(f"weights must be float32 {(B, N)}")
+    if window < 0 or (B | T | H | N) >> 31:  # past the library's 32-bit arguments
+        raise ValueError(f"window={window}, or a shape past 2**31: {tuple(q.shape)}, {N} keys")
+    window = min(window, 2 ** 31 - 1)  # past every table
     ld, step = weights.stride()
     if (step != 1 and N > 1) or (ld < N and B > 1):
         raise ValueError("weights must have contiguous rows: they are added to in place")
@@ -642,10 +646,15 @@ def cache_evict(held, weights, lengths, keep, recent=0, first=0, capacity=None):
     if keep < 0 or recent < 0 or first < 0 or recent + first > keep or capacity < keep:
         raise ValueError(f"keep={keep} rows cannot hold first={first} and recent={recent}, or capacity={capacity} "
                          "cannot hold them")
+    es = held.element_size()
     row_bytes = _row_bytes(held)
-    if row_bytes is None:
+    apart = row_bytes is None
+    if apart:
+        row_bytes = es * math.prod(shape[2:])
+    if (B | N | capacity | row_bytes) >> 31:  # past the library's 32-bit arguments
+        raise NotImplementedError(f"a table of {tuple(shape)} cut to keep={keep}, capacity={capacity}: too large")
+    if apart:
         held = held.contiguous()
-        row_bytes = _row_bytes(held)
     ld, step = weights.stride()
     if step != 1 and N > 1 or ld < N and B > 1:
         weights = weights.contiguous()
@@ -655,7 +664,6 @@ def cache_evict(held, weights, lengths, keep, recent=0, first=0, capacity=None):
     out_weights = weights.new_empty(B, capacity)
     rows = lengths.new_empty(B, keep)
     counts = torch.empty_like(lengths)
-    es = held.element_size()
     stride = held.stride()
     _call(device, _lib.lib().wpt_cache_evict,
           (held.data_ptr(), stride[0] * es, stride[1] * es, weights.data_ptr(), ld, lengths.data_ptr(), out.data_ptr(),
@@ -681,9 +689,14 @@ def beam_select(scores, totals, beams, done=None, end=None):
     R, W, V = scores.shape
     if beams < 1 or totals.shape != (R, W) or (done is not None and done.shape != (R, W)):
         raise ValueError(f"scores {tuple(scores.shape)} need totals (and done) {(R, W)}, and {beams} beams to pick")
-    if done is not None:
-        if end is None:
-            raise ValueError("ended beams need the token `end`")
+    if W > BEAM_MAX or beams > BEAM_MAX or (R | V) >> 31:  # V: past the library's 32-bit arguments
+        raise NotImplementedError(f"{beams} beams of scores {tuple(scores.shape)}: the selection kernels take up to "
+                                  f"{BEAM_MAX} beams in and out, and vocabularies under 2**31")
+    if done is None:
+        end = 0  # not read
+    else:
+        if end is None or not 0 <= end < V:
+            raise ValueError(f"ended beams need the token `end` of the vocabulary; got {end} of {V}")
         if done.dtype != torch.bool or not done.is_contiguous():
             done = done.to(torch.bool).contiguous()
     sr, sw, sv = scores.stride()
@@ -699,7 +712,7 @@ def beam_select(scores, totals, beams, done=None, end=None):
     scratch = parents.new_empty(lib.wpt_beam_scratch_bytes(R, W, V, beams, bf16) // 8)
     _call(device, lib.wpt_beam_select,
           (scores.data_ptr(), bf16, sr, sw, totals.data_ptr(), None if done is None else done.data_ptr(),
-           0 if end is None else end, scratch.data_ptr(), out.data_ptr(), parents.data_ptr(), tokens.data_ptr(), R, W, V,
+           end, scratch.data_ptr(), out.data_ptr(), parents.data_ptr(), tokens.data_ptr(), R, W, V,
            beams))
     LAUNCHES[0] += 2
     return out, parents, tokens
@@ -748,7 +761,6 @@ def _tables_overlap(rows, fields):
 
 
 REORDER_TABLES = 32  # tables wpt_cache_reorder takes in one launch
-BEAM_MAX = 64  # beams in and out
 
 
 def cache_reorder(tables, parents, lengths, first=None):
