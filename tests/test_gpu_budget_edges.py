@@ -10,8 +10,11 @@ import os
 import subprocess
 import sys
 
+import numpy as np
 import pytest
 import torch
+
+from oracle import budget as ob
 
 pytestmark = pytest.mark.gpu
 
@@ -222,6 +225,28 @@ def test_a_window_past_32_bits_is_no_window(wb):
 
 
 # ------------------------------------------------------------------- eviction
+
+def _evict_case(B, N, width, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    held = torch.randn(B, N, width, generator=g).bfloat16()
+    weights = torch.rand(B, N, generator=g)
+    lengths = torch.randint(N // 2, N + 1, (B,), generator=g)
+    return held, weights, lengths
+
+
+def _same(got, ref):
+    return np.array_equal(got[0].cpu().view(torch.int16).numpy(), ref[0]) and all(
+        np.array_equal(a.cpu().numpy(), b) for a, b in zip(got[1:], ref[1:]))
+
+
+def test_cache_evict_at_offsets_of_two_bytes(wb):
+    held, weights, lengths = _evict_case(3, 200, 24)
+    ref = ob.evict(held.view(torch.int16).numpy(), weights.numpy(), lengths.numpy(), 50, 7, 3)
+    for width, at in ((25, 1), (26, 1), (25, 0)):  # odd strides, an odd offset
+        big = torch.zeros(3, 200, width, dtype=torch.bfloat16, device="cuda")
+        big[..., at:at + 24] = held.cuda()
+        assert _same(wb.cache_evict(big[..., at:at + 24], weights.cuda(), lengths.cuda(), 50, 7, 3), ref)
+
 
 def test_cache_evict_of_tables_past_32_bits_is_refused(wb):
     n = torch.ones(1, dtype=torch.int64, device="cuda")

@@ -651,6 +651,8 @@ def cache_evict(held, weights, lengths, keep, recent=0, first=0, capacity=None):
     apart = row_bytes is None
     if apart:
         row_bytes = es * math.prod(shape[2:])
+    elif es < 4:  # the kernels copy units of 4 bytes
+        apart = (held.data_ptr() | es * held.stride(0) | es * held.stride(1)) % 4 != 0
     if (B | N | capacity | row_bytes) >> 31:  # past the library's 32-bit arguments
         raise NotImplementedError(f"a table of {tuple(shape)} cut to keep={keep}, capacity={capacity}: too large")
     if apart:
