@@ -213,6 +213,16 @@ def test_items_one_after_the_other(wb, case):
 
 # ------------------------------------------------------------------ arguments
 
+def test_positions_of_one_row_serve_every_row(wb):
+    _, q, k = _inputs(3, 2, 16, 128, 50)
+    one = torch.tensor([[30, 31]], device="cuda")
+    _, lse = wb.forward_with_lse(q, k, k, one, 0.1)
+    assert torch.equal(wb.attention_weights(q, k, one, lse, 0.1),
+                       wb.attention_weights(q, k, one.expand(3, 2).contiguous(), lse, 0.1))
+    with pytest.raises(ValueError):
+        wb.attention_weights(q, k, one.expand(2, 2), lse, 0.1)
+
+
 def test_a_window_past_32_bits_is_no_window(wb):
     _, q, k = _inputs(2, 1, 16, 128, 300)
     positions = torch.full((2, 1), 299, device="cuda")

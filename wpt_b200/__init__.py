@@ -308,7 +308,7 @@ def attention_weights(q, k, positions, lse, scale, weights=None, window=0, floor
     window and floor as there. Returns weights. Not differentiable."""
     if weights is None:
         weights = torch.zeros(q.shape[0], k.shape[1], dtype=torch.float32, device=q.device)
-    if positions.dim() != 2:
+    if positions.dim() == 1 or positions.shape[0] == 1:
         positions = _positions(positions, q.shape[0])
     return ops.attention_weights(q, k, positions, lse, scale, weights, window, floor)
 
