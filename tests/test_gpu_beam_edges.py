@@ -195,3 +195,44 @@ def test_a_refused_reorder_moves_nothing(wb):
     with pytest.raises(NotImplementedError):
         wb.cache_reorder(tables, torch.tensor([[1, 0]], device="cuda"), torch.tensor([3, 3], device="cuda"))
     assert all(torch.equal(t, was) for t in tables[:35])
+
+
+# ----------------------------------------------------------- graphs, streams
+
+def test_reorder_replays_in_a_graph_and_on_another_stream(wb):
+    R, W, N = 3, 4, 50
+    g = torch.Generator().manual_seed(2)
+    start = [torch.randn(R * W, N, 16, generator=g), torch.randn(R * W, N, generator=g)]
+    parents = torch.randint(0, W, (R, W), generator=g)
+    lengths = torch.randint(1, N + 1, (R * W,), generator=g)
+    want = [ob.reorder(t.numpy(), parents.numpy(), lengths.numpy()) for t in start]
+    tables = [t.cuda() for t in start]
+    on_gpu = parents.cuda(), lengths.cuda()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        wb.cache_reorder(tables, *on_gpu)
+    stream.synchronize()
+    assert all(np.array_equal(t.cpu().numpy(), w) for t, w in zip(tables, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        wb.cache_reorder(tables, *on_gpu)
+    for t, s in zip(tables, start):
+        t.copy_(s)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(np.array_equal(t.cpu().numpy(), w) for t, w in zip(tables, want))
+
+
+def test_select_replays_in_a_graph(wb):
+    x = torch.randn(3, 4, 5003, generator=torch.Generator().manual_seed(5)).cuda()
+    totals = torch.zeros(3, 4, device="cuda")
+    want = wb.beam_select(x, totals, 6)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = wb.beam_select(x, totals, 6)
+    for t in got:
+        t.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

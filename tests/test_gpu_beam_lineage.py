@@ -1,6 +1,6 @@
-"""What belongs to a beam follows it: the accumulated weights that
-examples/beam_search.py holds, against a replay of each beam's own
-lineage."""
+"""What belongs to a beam follows it: the accumulated weights and the totals
+that examples/beam_search.py holds, against a replay of each beam's own
+lineage, and ended beams' totals."""
 
 import importlib.util
 import os
@@ -70,3 +70,49 @@ def test_weights_follow_their_beam(example, monkeypatch):
     assert tokens.shape == (R, W, steps) and calls[0] == layers * (steps - 1)
     assert moved[0] > W  # beams took others' places
     assert wpt_b200.device_status() == 0
+
+
+def test_an_ended_beams_total_stays(example, monkeypatch):
+    """Once a continuation has ended, every later step carries its total on to the bit."""
+    import wpt_b200
+    model = example.Decoder(vocab=50, model=256)
+    prompts = _prompts(model, 3, 20)
+    free, _ = example.search(model, prompts, 4, 3)
+    end = int(free[0, 0, 0])
+    seen, kept = [], [0]
+    select = wpt_b200.beam_select
+
+    def watched(scores, totals, beams, done=None, end=None):
+        out, parents, tokens = select(scores, totals, beams, done=done, end=end)
+        if done is not None:
+            before = torch.gather(totals, 1, parents)
+            ended = torch.gather(done, 1, parents)
+            assert (tokens[ended] == end).all()
+            assert torch.equal(out[ended], before[ended])
+            assert (out[~ended] < before[~ended]).all()  # a live token's probability is under 1
+            kept[0] += int(ended.sum())
+        seen.append(out)
+        return out, parents, tokens
+
+    monkeypatch.setattr(wpt_b200, "beam_select", watched)
+    tokens, totals = example.search(model, prompts, 4, 12, end=end)
+    assert kept[0] > 0 and torch.equal(totals, seen[-1])
+    ended = (tokens[..., -1] == end)
+    assert ended.any()
+
+
+def test_a_wider_search_holds_a_narrow_ones_choices(example):
+    """As many beams as there are continuations of two tokens find the best one; a narrow search finds no better."""
+    model = example.Decoder(vocab=7, model=256)
+    prompts = _prompts(model, 3, 30)
+    every, totals = example.search(model, prompts, 49, 2)
+    # 49 different continuations of 7 x 7; the first step offers 7, the rest are empty
+    assert (totals > -float("inf")).all() and (every >= 0).all()
+    for r in range(3):
+        assert len({tuple(t) for t in every[r].tolist()}) == 49
+    # the probabilities of all continuations sum to one
+    assert (totals.double().exp().sum(1) - 1).abs().max() < 1e-3
+    for beams in (1, 2, 7):
+        best = example.search(model, prompts, beams, 2)[1][:, 0]
+        assert (best <= totals[:, 0] + 0.2).all()  # the same numbers but for the bf16 roundings of another batch
+    assert torch.equal(example.search(model, prompts, 7, 2)[0][:, 0], every[:, 0])

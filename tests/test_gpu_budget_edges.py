@@ -258,6 +258,27 @@ def test_cache_evict_at_offsets_of_two_bytes(wb):
         assert _same(wb.cache_evict(big[..., at:at + 24], weights.cuda(), lengths.cuda(), 50, 7, 3), ref)
 
 
+@pytest.mark.parametrize("B, N, keep", [(3, 500, 100), (2, 30000, 9000)])
+def test_cache_evict_replays_in_a_graph_and_on_another_stream(wb, B, N, keep):
+    held, weights, lengths = _evict_case(B, N, 64)
+    ref = ob.evict(held.view(torch.int16).numpy(), weights.numpy(), lengths.numpy(), keep, 7, 3)
+    args = held.cuda(), weights.cuda(), lengths.cuda(), keep, 7, 3
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        got = wb.cache_evict(*args)
+    stream.synchronize()
+    assert _same(got, ref)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = wb.cache_evict(*args)
+    for t in got:
+        t.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert _same(got, ref)
+
+
 def test_cache_evict_of_tables_past_32_bits_is_refused(wb):
     n = torch.ones(1, dtype=torch.int64, device="cuda")
     long = torch.zeros(1, 1, device="cuda").expand(1, 2 ** 32 + 5)
