@@ -405,11 +405,12 @@ int wpt_cache_evict(const void* held, int64_t held_stride_b, int64_t held_stride
  * (beam w, token v) is
  *   totals[r, w] + ((x - m) - log(sum over v of exp(x - m))),  m the beam's
  *   largest score,
- * and the K largest win (equal values: the lowest w * V + v), best first. An
- * ended beam (done) offers one candidate: itself, its total unchanged, with
- * the token `end`; its scores are not read. A value that is -inf or NaN is
- * no candidate (so a score of NaN or +inf takes its whole beam out); places
- * without a candidate get total -inf, parent and token -1.
+ * in fp32, and the K largest win (equal values, of equal scores or not: the
+ * lowest w * V + v), best first. An ended beam (done) offers one candidate:
+ * itself, its total unchanged, with the token `end`; its scores are not read.
+ * A value that is -inf or NaN is no candidate (so a score of NaN or +inf takes
+ * its whole beam out); places without a candidate get total -inf, parent and
+ * token -1.
  *   scores   fp32, or bf16 when bf16 is 1; (R, W, V), last dimension
  *            contiguous, the others at strides in elements (any alignment)
  *   totals   fp32 (R, W);  done  bytes (R, W) or NULL

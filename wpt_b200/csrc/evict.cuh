@@ -20,11 +20,11 @@
 #include <cstdint>
 
 #include "common.cuh"
-#include "select.cuh"  // order_key, block_exclusive_scan
+#include "select.cuh"  // order_key
 
 namespace wpt {
 
-constexpr int EVICT_THREADS = TOPK_THREADS;  // block_exclusive_scan's block
+constexpr int EVICT_THREADS = 1024;  // a whole block a row, or slice: the selection is a chain of block steps
 constexpr int EVICT_BINS = 2048;
 constexpr int EVICT_SLICES = 8;  // most CTAs a row (a portable cluster)
 constexpr int EVICT_QUADS = 4 * EVICT_THREADS;  // a slice is a multiple of this: whole quads a thread

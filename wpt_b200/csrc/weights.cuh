@@ -28,11 +28,11 @@
 // skipped and tiles read whole need no mask. Bound: the exponentials (16 a clock
 // an SM: 1,024 clocks for 128 keys x 128 columns, whose products take 512), so
 // an eighth of them take the FMA pipe. 8 x 4,096 places of 16 heads, causal, width
-// 128: 364 us, 755 TFLOP/s (0.47 of the measured bf16 peak, at 1.54 GHz under the
-// power limit). A run of 32 columns takes a warp 880 clocks, of which the four
-// warps of a scheduler keep its exponential unit busy for 768 and its issue slots
-// for 644; loads from TMEM and waits make up the rest, 0.62 of the unit's rate in
-// all.
+// 128: 364 us, 755 TFLOP/s (0.47 of the measured bf16 peak, at 1.53 GHz under the
+// power limit). A run of 32 columns keeps a scheduler's exponential unit busy for
+// 896 clocks (28 exponentials a thread, four warps). Over the whole kernel the unit
+// is busy 71% of the time and the issue slots 46%; loads from TMEM and waits make up
+// the rest.
 #pragma once
 
 #include <climits>
@@ -780,8 +780,9 @@ __global__ void __launch_bounds__(WEIGHTS_TILE_THREADS, 1)
   } else {
     // ----------------------------------------------------------- epilogue
     // A warpgroup takes one of the item's key tiles, a thread one key, in runs
-    // of 16 columns. The next run's scores are on their way from TMEM while a
-    // run is added up; while a warpgroup waits, the others compute.
+    // of 32 columns. It waits for each run's scores from TMEM and then adds them up;
+    // while a warpgroup waits, the others compute (the next run's load under way
+    // meanwhile took as long or longer).
     const int g = warp >> 2;
     const uint32_t from = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + g * COLS;
     bool ok = true;
