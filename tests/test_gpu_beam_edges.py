@@ -236,3 +236,36 @@ def test_select_replays_in_a_graph(wb):
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("kind", ["masked", "equal"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_equal_scores_cost_no_more_than_a_few_passes(wb, kind, dtype):
+    """Most tokens at a finite mask, or all scores equal: within ten times the time of scores that differ (a run's
+    scores are then read a few times over, not ranked against each other), and the right choice."""
+    R, W, V, beams = 16, 8, 50001, 8
+    g = torch.Generator(device="cuda").manual_seed(9)
+    plain = torch.randn(R, W, V, generator=g, device="cuda")
+    hidden = torch.rand(R, W, V, generator=g, device="cuda") < 0.9999
+    scores = dict(masked=plain.masked_fill(hidden, -1e9), equal=torch.zeros_like(plain))[kind].to(dtype)
+    plain = plain.to(dtype)
+    totals = -torch.rand(R, W, generator=g, device="cuda")
+
+    def time(x):
+        wb.beam_select(x, totals, beams)
+        best = math.inf
+        for _ in range(5):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            for _ in range(10):
+                wb.beam_select(x, totals, beams)
+            b.record()
+            b.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return best
+
+    assert time(scores) < 10 * time(plain)
+    _check_values(wb, wb.beam_select(scores, totals, beams), scores, totals, beams)
+    if kind == "equal":
+        _, parents, tokens = wb.beam_select(scores, totals, beams)
+        assert (parents == totals.argmax(1, keepdim=True)).all() and (tokens == torch.arange(beams, device="cuda")).all()

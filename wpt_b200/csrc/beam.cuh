@@ -10,7 +10,8 @@
 // CTA takes a run of one beam's scores. Its first tile gives a bound that the
 // K best of the run reach; scores that do go to shared memory, and after 1, 2,
 // 4, ... tiles those are ranked and the bound becomes the K-th best so far, so
-// that a run of n tiles looks at about K (2 + log2 n) scores twice.
+// that a run of n tiles looks at about K (2 + log2 n) scores twice. Scores equal to
+// the bound count only in tokens up to its own.
 // beam_merge_kernel: one CTA a text joins the runs' sums, turns the candidates
 // into values and ranks them. Bound: HBM, the scores read once.
 //
@@ -67,6 +68,9 @@ __device__ __forceinline__ float beam_key_value(uint64_t key) {
   return __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k);
 }
 
+// The next number above a key's.
+__device__ __forceinline__ float beam_above(uint64_t key) { return beam_key_value(key + (1ull << 32)); }
+
 __device__ __forceinline__ float beam_load(const float* p) { return *p; }
 __device__ __forceinline__ float beam_load(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 __device__ __forceinline__ void beam_load16(const float* p, float (&x)[4]) {
@@ -94,29 +98,38 @@ constexpr uint64_t BEAM_ENDED = 0xFFFFFFFFull << 32;
 struct BeamShared {
   uint64_t list[BEAM_MAX + 1];  // best first
   uint64_t* buf;            // gathered keys
-  alignas(16) uint32_t group[BEAM_THREADS];
-  uint32_t bound;
+  alignas(16) uint64_t group[BEAM_THREADS];
+  uint64_t bound;
   int count, listed;
 };
 
 // A bound that the K best of the threads' keys reach: the K-th largest of the
-// maxima of GROUPS >= K groups of threads (top: a thread's largest key's upper
-// half, 0 for none). Ends after a barrier.
-template <int GROUPS>
-__device__ __forceinline__ void beam_bound_of(BeamShared& s, int K, uint32_t top) {
+// maxima of GROUPS >= K groups of threads (top: a thread's largest, 0 for none), 0
+// where fewer have one. Of whole keys, or of their upper halves, which is quicker,
+// but equal scores then all reach it. Ends after a barrier.
+template <int GROUPS, typename Key>
+__device__ __forceinline__ void beam_bound_of(BeamShared& s, int K, Key top) {
+  constexpr int VEC = 16 / sizeof(Key);
+  Key* group = reinterpret_cast<Key*>(s.group);
 #pragma unroll
   for (int o = 1; o < BEAM_THREADS / GROUPS; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (threadIdx.x % (BEAM_THREADS / GROUPS) == 0) s.group[threadIdx.x / (BEAM_THREADS / GROUPS)] = top;
+  if (threadIdx.x % (BEAM_THREADS / GROUPS) == 0) group[threadIdx.x / (BEAM_THREADS / GROUPS)] = top;
   __syncthreads();
   if (threadIdx.x < GROUPS) {
     const int me = threadIdx.x;
-    const uint32_t mine = s.group[me];
+    const Key mine = group[me];
     int rank = 0;
 #pragma unroll 8
-    for (int i = 0; i < GROUPS; i += 4) {
-      const uint4 v = *reinterpret_cast<const uint4*>(s.group + i);
-      rank += (v.x > mine || (v.x == mine && i < me)) + (v.y > mine || (v.y == mine && i + 1 < me)) +
-              (v.z > mine || (v.z == mine && i + 2 < me)) + (v.w > mine || (v.w == mine && i + 3 < me));
+    for (int i = 0; i < GROUPS; i += VEC) {
+      const uint4 raw = *reinterpret_cast<const uint4*>(group + i);
+      Key v[VEC];
+      if constexpr (VEC == 4) {
+        v[0] = raw.x, v[1] = raw.y, v[2] = raw.z, v[3] = raw.w;
+      } else {
+        v[0] = static_cast<uint64_t>(raw.y) << 32 | raw.x, v[1] = static_cast<uint64_t>(raw.w) << 32 | raw.z;
+      }
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) rank += v[j] > mine || (v[j] == mine && i + j < me);
     }
     if (rank == K - 1) s.bound = mine;
   }
@@ -124,12 +137,13 @@ __device__ __forceinline__ void beam_bound_of(BeamShared& s, int K, uint32_t top
 }
 // The more groups, the fewer keys reach the bound (K = 16 of 64: about 18 a
 // tile; K = 64 of 256: 74), and the longer it takes to rank them.
-__device__ __forceinline__ uint32_t beam_bound(BeamShared& s, int K, uint32_t top) {
+template <typename Key>
+__device__ __forceinline__ Key beam_bound(BeamShared& s, int K, Key top) {
   if (K <= 17)
     beam_bound_of<64>(s, K, top);
   else
     beam_bound_of<BEAM_THREADS>(s, K, top);
-  return s.bound;
+  return static_cast<Key>(s.bound);
 }
 
 // s.list = the K best of the n keys in s.buf, best first.
@@ -146,20 +160,21 @@ __device__ __forceinline__ void beam_rank(BeamShared& s, int K, int n) {
 }
 
 // The list's K best after BEAM_THREADS * PER more keys (key(j): this thread's
-// j-th, 0 for none).
-template <int PER, class Key>
+// j-th, 0 for none). Bound: whole keys (uint64_t) or upper halves.
+template <int PER, typename Bound, class Key>
 __device__ __forceinline__ void beam_keep_best(BeamShared& s, int K, Key key) {
-  uint32_t top = 0;
+  constexpr int SHIFT = 64 - 8 * static_cast<int>(sizeof(Bound));
+  Bound top = 0;
 #pragma unroll
-  for (int j = 0; j < PER; ++j) top = max(top, static_cast<uint32_t>(key(j) >> 32));
+  for (int j = 0; j < PER; ++j) top = max(top, static_cast<Bound>(key(j) >> SHIFT));
   if (threadIdx.x < s.listed) s.buf[threadIdx.x] = s.list[threadIdx.x];
   if (threadIdx.x == 0) s.count = s.listed;
-  const uint32_t bound = beam_bound(s, K, top);
+  const Bound bound = beam_bound(s, K, top);
   const uint64_t worst = s.listed == K ? s.list[K - 1] : 0;
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
     const uint64_t k = key(j);
-    if (k > worst && static_cast<uint32_t>(k >> 32) >= bound) s.buf[atomicAdd(&s.count, 1)] = k;
+    if (k > worst && static_cast<Bound>(k >> SHIFT) >= bound) s.buf[atomicAdd(&s.count, 1)] = k;
   }
   __syncthreads();
   beam_rank(s, K, s.count);
@@ -210,6 +225,35 @@ __device__ __forceinline__ void beam_send(uint8_t* stage, const T* from, int64_t
     }
   }
   cp_async_commit();
+}
+
+// After a first tile with more scores equal to the bound than there is room for (a
+// finite mask over most tokens, equal scores): its candidates again, of equal
+// scores those of the lowest tokens. Returns the bound from here on. stage: the
+// tile, from token `token0` on. (64 texts of 8 beams with all but
+// 65 tokens a beam at -1e9: 36 us, 2,300 without.)
+template <typename T>
+__device__ __noinline__ float beam_gather_keys(BeamShared& s, uint64_t* room, int K, const uint8_t* stage, int64_t token0) {
+  constexpr int PER = 64 / sizeof(T), VEC = 16 / sizeof(T);
+  auto key = [&](int j) -> uint64_t {
+    const int at = (j / VEC * BEAM_THREADS + threadIdx.x) * VEC + j % VEC;
+    const float x = beam_load(reinterpret_cast<const T*>(stage) + at);
+    return x > -INFINITY ? beam_key(x, static_cast<uint32_t>(token0 + at)) : 0;
+  };
+  uint64_t top = 0;
+  for (int j = 0; j < PER; ++j) top = max(top, key(j));
+  const uint64_t bound = beam_bound(s, K, top);
+  if (threadIdx.x == 0) s.count = 0;
+  __syncthreads();
+  if (top >= bound)
+    for (int j = 0; j < PER; ++j) {
+      const uint64_t k = key(j);
+      if (k == 0 || k < bound) continue;
+      const int i = atomicAdd(&s.count, 1);
+      if (i < BEAM_ROOM) room[i] = k;
+    }
+  __syncthreads();
+  return bound != 0 ? beam_above(bound) : -FLT_MAX;
 }
 
 struct BeamScanShared {
@@ -309,8 +353,11 @@ __device__ __forceinline__ float2 beam_scan_run(const BeamParams& p, int K, Beam
         beam_rank(s, K, n);
         if (threadIdx.x < s.listed) sh.room[threadIdx.x] = s.list[threadIdx.x];
         if (threadIdx.x == 0) s.count = s.listed;
-        if (s.listed == K) least = fmaxf(least, beam_key_value(s.list[K - 1]));
+        // the tokens from here on are higher: scores equal to the last one do not count
+        if (s.listed == K) least = fmaxf(least, beam_above(s.list[K - 1]));
         __syncthreads();
+      } else if (tile == 0) {
+        least = beam_gather_keys<T>(s, sh.room, K, stage, e0 - off);
       }
     }
   }
@@ -362,7 +409,7 @@ __device__ __forceinline__ float2 beam_scan_run(const BeamParams& p, int K, Beam
         }
         const float worst = s.listed == K ? beam_key_value(s.list[K - 1]) : -INFINITY;
         if (__syncthreads_or(top > worst))
-          beam_keep_best<BEAM_PER>(s, K, [&](int j) -> uint64_t {
+          beam_keep_best<BEAM_PER, uint64_t>(s, K, [&](int j) -> uint64_t {
             return x[j] > -INFINITY ? beam_key(x[j], static_cast<uint32_t>(e0 + place(h, j) - off)) : 0;
           });
       }
@@ -428,7 +475,7 @@ __device__ __noinline__ void beam_read_again(const BeamParams& p, BeamMergeShare
         if (!__syncthreads_or(any)) continue;
 #pragma unroll
         for (int g = 0; g < GROUPS; ++g)
-          beam_keep_best<PER>(s, p.K, [&](int j) { return key[g * PER + j]; });
+          beam_keep_best<PER, uint32_t>(s, p.K, [&](int j) { return key[g * PER + j]; });
       }
     }
     __syncthreads();
@@ -510,7 +557,7 @@ __device__ __forceinline__ void beam_merge(const BeamParams& p, BeamMergeShared&
       if (token == 0xFFFFFFFFu) others = fmaxf(others, value);
       found[j] = value > -INFINITY && token != 0xFFFFFFFFu ? beam_key(value, static_cast<uint32_t>(w) * p.V + token) : 0;
     }
-    beam_keep_best<PER>(s, p.K, [&](int j) { return found[j]; });
+    beam_keep_best<PER, uint32_t>(s, p.K, [&](int j) { return found[j]; });
   }
   if (__syncthreads_or(others > -INFINITY && s.listed == p.K && others >= beam_key_value(s.list[p.K - 1])))
     beam_read_again<T>(p, sh, r, cand);
