@@ -355,6 +355,69 @@ int wpt_cache_append(const void* src, int64_t src_stride_b, int64_t src_stride_n
                      int64_t capacity, void* stream);
 
 /*
+ * Rotary positions (packages/wpt-model/src/wpt_model/attention.py:59): x (B, T,
+ * H, C) bf16, or fp32 with f32, at any strides (elements; the last dim
+ * contiguous) -> y, contiguous, same type. Of each head the channels start ..
+ * start + dims - 1 are turned in pairs (a, b),
+ *   y_a = magnitude * (x_a cos t - x_b sin t), y_b = magnitude * (x_b cos t + x_a sin t),
+ * t = positions[b * positions_stride_b + t] * frequencies[i], pair i being
+ * channels i and i + dims / 2 of them, or with `interleaved` 2 i and 2 i + 1;
+ * the others are copied. inverse: by -t (the gradient of x from that of y).
+ *   frequencies  (dims / 2,) radians a position, fp64 with frequencies_f64,
+ *                else fp32; finite. Angles are taken modulo a turn exactly.
+ */
+int wpt_rotate(const void* x, int64_t x_stride_b, int64_t x_stride_t, int64_t x_stride_h, const int64_t* positions,
+               int64_t positions_stride_b, const void* frequencies, int frequencies_f64, void* y, int f32, int B, int T,
+               int H, int C, int dims, int start, int interleaved, float magnitude, int inverse, void* stream);
+
+/*
+ * The paged generation cache, held in 8 bits: pages (P, S, 2 C) e4m3, an
+ * entry's key then its value (page and entry strides in BYTES, multiples of
+ * 16), S 16, 32, 64 or a multiple of 128; scales (P, S / 16, 2) fp32
+ * (scales_stride: elements from page to page), what the keys and the values of
+ * each block of 16 entries are multiplied by; table (B, M) int32, or int64 with
+ * table_i64: entry n of row b is entry n % S of page table[b, n / S], numbers
+ * outside 0 .. P - 1 being no page.
+ *
+ * wpt_paged_append: row b's new entries src[b, i] (B, n, 2 C; bf16, or fp32
+ * with f32; strides in elements), i < counts[b], become its entries first[b] +
+ * i. dims > 0: the keys' channels start .. are turned as wpt_rotate does, by
+ * positions[b, i] (B, n), or by first[b] + i where positions is NULL. A block's
+ * scales are the least powers of two, 2^-60 at least, that bring its values
+ * within 448; a block with earlier entries of the row (before first[b]) keeps
+ * a larger scale, and where its scale grows the earlier entries are rounded
+ * again. Infinities and values past 448 * 2^60 are held as NaN. Entries
+ * outside the table or on no page are not written and set the status word's
+ * shape bit (bit 1). C a multiple of 16 up to 512.
+ */
+int wpt_paged_append(const void* src, int f32, int64_t src_stride_b, int64_t src_stride_n, void* pages,
+                     int64_t page_stride, int64_t entry_stride, float* scales, int64_t scales_stride, const void* table,
+                     int table_i64, int64_t table_stride_b, const int64_t* first, const int64_t* counts,
+                     const int64_t* positions, const void* frequencies, int frequencies_f64, int B, int n, int C, int M,
+                     int P, int S, int dims, int start, int interleaved, float magnitude, void* stream);
+
+/*
+ * Attention over the 8-bit paged cache for few queries a row (C = 128, up to
+ * 64 heads; any T is computed, 64 / H queries at a time): query t of row b
+ * reads the row's entries max(0, p - window + 1) .. min(p, M S - 1), p =
+ * positions[b, t] (window 0: no window), but for those on no page; q, out, lse
+ * and sink as above. What other entries hold (NaN too) reaches no result.
+ * Value scales are 0, or 2^-60 to 2^60.
+ *   splits, chunk_tiles  each query group's entries go to `splits` CTAs,
+ *              chunk_tiles tiles of 128 each (splits * chunk_tiles tiles must
+ *              cover the rows, or the window and a tile); with splits > 1
+ *              scratch holds wpt_paged_scratch_bytes(B, T, H, splits) bytes,
+ *              16-byte aligned, or is NULL for 2 to 8 splits: then a group's
+ *              splits are one thread-block cluster and need none.
+ */
+size_t wpt_paged_scratch_bytes(int B, int T, int H, int splits);
+int wpt_paged_attention(const void* q, const void* pages, int64_t page_stride, int64_t entry_stride,
+                        const float* scales, int64_t scales_stride, const void* table, int table_i64,
+                        int64_t table_stride_b, const int64_t* positions, const float* sink, void* out, float* lse,
+                        void* scratch, int splits, int chunk_tiles, int B, int T, int H, int C, int M, int P, int S,
+                        int window, float scale, void* stream);
+
+/*
  * The attention weight that each cached row collects from a pass of queries:
  *   weights[b, n] += sum over t, h of exp(scale * q[b, t, h] . k[b, n] - lse[b, t, h])
  * over the queries that read row n: max(0, p - window + 1, floor) <= n <=

@@ -25,6 +25,13 @@ and, for a generation cache between two steps,
     beam_select(scores, totals, beams)
     cache_reorder(tables, parents, lengths)
 
+for the layers around a generation step (rotary positions, and a paged cache
+held in 8 bits with the attention that reads it)
+
+    rotate(x, positions, frequencies)
+    paged_append(pages, scales, table, new, first, counts)
+    paged_attention(q, pages, scales, table, positions, scale) -> (out, lse)
+
 with the reference's argument meanings, dtypes, -1 conventions and errors.
 Forward passes run hand-written CUDA kernels (libwpt_b200.so, C ABI in
 include/wpt_attn.h); there is no CPU path and no other backend: a missing
@@ -355,6 +362,90 @@ def cache_reorder(tables, parents, lengths, first=None):
     return ops.cache_reorder(tables, parents, lengths, first)
 
 
+# ---------------------------------------------------------- rotary positions
+
+def rotary_frequencies(dims, base=10000.0, scaling=None, factor=1.0, original=None, low=1.0, high=32.0, device=None):
+    """(dims / 2,) float64 angles a position for rotate and paged_append: base
+    ** (-2 i / dims), for a context `factor` times as long as the `original`
+    one slowed by `scaling`: None, "linear" (all pairs by the factor), "base"
+    (a larger base: the slowest pair by the factor, the fastest not) or "parts"
+    (pairs of fewer than `low` turns in the original context by the factor,
+    those of more than `high` not, a line between). On `device` (None: the
+    CPU), once; a caller keeps it."""
+    return ops.rotary_frequencies(dims, base, scaling, factor, original, low, high, device)
+
+
+class _Rotate(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, positions, frequencies, start, interleaved, magnitude):
+        ctx.save_for_backward(positions, frequencies)
+        ctx.how = start, interleaved, magnitude
+        return ops.rotate(x, positions, frequencies, start, interleaved, magnitude)
+
+    @staticmethod
+    def backward(ctx, d_out):
+        positions, frequencies = ctx.saved_tensors
+        return ops.rotate(d_out, positions, frequencies, *ctx.how, inverse=True), None, None, None, None, None
+
+
+def rotate(x, positions, frequencies, start=None, interleaved=False, magnitude=1.0):
+    """Rotary positions (attention.py:59, which turns the last 64 channels of a
+    window layer's queries and keys): x (B, T, C) or (B, T, H, C), bf16 or fp32,
+    at positions (T,) or (B, T), with the pairs of the channels start .. start +
+    dims - 1 of each head (default: the last ones; dims = 2 len(frequencies))
+    turned by position * frequencies and multiplied by magnitude, the others
+    copied. A pair is channels i and i + dims / 2 of them, or 2 i and 2 i + 1
+    (interleaved). Angles are exact at far positions. Differentiable in x;
+    returns a new tensor in x's dtype."""
+    if not _needs_grad(x):
+        return ops.rotate(x, positions, frequencies, start, interleaved, magnitude)
+    return _Rotate.apply(x, positions, frequencies, start, interleaved, magnitude)
+
+
+# ---------------------------------------------------- the 8-bit paged cache
+
+def paged_cache(pages, page, width, device=None):
+    """An empty paged generation cache held in 8 bits: (pages (pages, page, 2 *
+    width) float8_e4m3fn, an entry's key then its value; scales (pages, page /
+    16, 2) float32, what the keys and the values of each block of 16 entries
+    are multiplied by). page: 16, 32, 64 or a multiple of 128 entries. Half the
+    bytes of a bf16 table."""
+    return ops.paged_cache(pages, page, width, device)
+
+
+def paged_append(pages, scales, table, new, first, counts, frequencies=None, positions=None, start=None,
+                 interleaved=False, magnitude=1.0):
+    """cache_append for a paged cache (cache.py:110-128), in place: row b's new
+    entries new[b, :counts[b]] ((B, n, 2 C), bf16 or fp32) become its entries
+    first[b] .., entry i being entry i % S of page table[b, i // S] (table
+    (B, M) int32 or int64, -1 for none; the pages written to are the row's own).
+    With frequencies, the keys are turned on the way as rotate turns them, at
+    positions (B, n) or, by default, at their places first[b] + i.
+
+    A block's scales are the least powers of two that bring its values within
+    e4m3's 448 (2^-60 at least); a block that already holds entries of the row
+    before first[b] keeps its scale if that is larger, else its earlier
+    entries are rounded again to the new one. Infinities, and values past 448 *
+    2^60, are held as NaN. Entries outside the table or on no page are not
+    written (device_status's bit 1). One launch, no host synchronisation.
+    Returns (pages, scales). Not differentiable."""
+    return ops.paged_append(pages, scales, table, new, first, counts, frequencies, positions, start, interleaved,
+                            magnitude)
+
+
+def paged_attention(q, pages, scales, table, positions, scale, window=0, sink=None):
+    """forward_with_lse over the 8-bit paged cache: q (B, T, H, 128) bf16, up
+    to 64 heads, at positions (T,) or (B, T); query t of row b reads the row's
+    entries 0 .. position (given a window, the last `window` of them), with
+    sink (H,) in each head's denominator. Entries on no page are not read, and
+    what they and entries past the position hold reaches no result. Made for few
+    queries a row (decode, drafts); any number is computed, 64 / H at a time.
+    Returns (out (B, T, H, 128) bf16, lse (B, T, H) fp32); 0 and -inf (or the
+    sink) for a query without entries. Not differentiable."""
+    _bf16_only(q)
+    return ops.paged_attention(q, pages, scales, table, _positions(positions, q.shape[0]), scale, window, sink)
+
+
 # ------------------------------------------------------------- installation
 
 def install(kernels, attention=None, device=None, check=True):
@@ -385,6 +476,6 @@ def install(kernels, attention=None, device=None, check=True):
 
 
 __all__ = ["install", "drafter_attention", "cache_append", "attention_weights", "cache_evict", "beam_select",
-           "cache_reorder", "sample", "accept", "NAME",
+           "cache_reorder", "rotary_frequencies", "rotate", "paged_cache", "paged_append", "paged_attention", "sample", "accept", "NAME",
            "WINDOW", "chosen_columns", "exact_attention", "sparse_attention", "window_attention", "tree_attention",
            "forward_with_lse", "device_status", "LibraryMissing"]

@@ -51,12 +51,19 @@ SIGNATURES = {
     "wpt_beam_select": [_P, _I, _I64, _I64, _P, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _P],
     "wpt_beam_scratch_bytes": [_I, _I, _I, _I, _I],
     "wpt_cache_reorder": [_P, _I, _P, _P, _P, _I, _I, _P],
+    "wpt_rotate": [_P, _I64, _I64, _I64, _P, _I64, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P],
+    "wpt_paged_append": [_P, _I, _I64, _I64, _P, _I64, _I64, _P, _I64, _P, _I, _I64, _P, _P, _P, _P, _I, _I, _I, _I,
+                         _I, _I, _I, _I, _I, _I, _F, _P],
+    "wpt_paged_scratch_bytes": [_I, _I, _I, _I],
+    "wpt_paged_attention": [_P, _P, _I64, _I64, _P, _I64, _P, _I, _I64, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I,
+                            _I, _I, _I, _F, _P],
     "wpt_attn_exchange": [_P, _P, _I, _I64, _I, _I, _P, ctypes.POINTER(_P), _I, _I, _P, _P, _P],
 }
 
 RESTYPES = {"wpt_last_error": ctypes.c_char_p, "wpt_accept_scratch_bytes": ctypes.c_size_t,
             "wpt_attn_backward_scratch_bytes": ctypes.c_size_t, "wpt_peer_bytes": ctypes.c_size_t,
-            "wpt_attn_weights_scratch_bytes": ctypes.c_size_t, "wpt_beam_scratch_bytes": ctypes.c_size_t}
+            "wpt_attn_weights_scratch_bytes": ctypes.c_size_t, "wpt_beam_scratch_bytes": ctypes.c_size_t,
+            "wpt_paged_scratch_bytes": ctypes.c_size_t}
 
 _lib = None
 

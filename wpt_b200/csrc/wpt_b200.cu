@@ -22,7 +22,9 @@
 #include "exchange.cuh"
 #include "head.cuh"
 #include "merge.cuh"
+#include "paged.cuh"
 #include "prefill.cuh"
+#include "rotary.cuh"
 #include "select.cuh"
 #include "stream.cuh"
 #include "tree.cuh"
@@ -91,7 +93,7 @@ int encoder(EncodeTiled* out) {
   return WPT_OK;
 }
 
-// A bf16 tensor map with 128-byte swizzle and 64-element inner boxes.
+// A tensor map with 128-byte swizzle, of bf16 where nothing else is said.
 // Makes the current device's primary context current on this host thread.
 // Runtime calls bind it lazily, but the driver's tensor-map encoder needs it
 // bound already, and a thread that has made no runtime call on the device
@@ -116,16 +118,17 @@ int bind_context() {
 struct MapKey {
   const void* base;
   int rank, dev;
+  CUtensorMapDataType type;
   cuuint64_t dims[3], strides[2];
   cuuint32_t box[3];
 };
 
 int tensor_map_encode(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims,
-                      const cuuint64_t* strides_bytes, const cuuint32_t* box);
+                      const cuuint64_t* strides_bytes, const cuuint32_t* box, CUtensorMapDataType type);
 int current_device(int* sms = nullptr);
 
 int tensor_map(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides_bytes,
-               const cuuint32_t* box) {
+               const cuuint32_t* box, CUtensorMapDataType type = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16) {
   constexpr int SLOTS = 16;
   static thread_local MapKey keys[SLOTS];
   static thread_local CUtensorMap maps[SLOTS];
@@ -135,6 +138,7 @@ int tensor_map(CUtensorMap* map, const void* base, int rank, const cuuint64_t* d
   key.base = base;
   key.rank = rank;
   key.dev = current_device();
+  key.type = type;
   for (int i = 0; i < rank; ++i) {
     key.dims[i] = dims[i];
     key.box[i] = box[i];
@@ -145,7 +149,7 @@ int tensor_map(CUtensorMap* map, const void* base, int rank, const cuuint64_t* d
       *map = maps[i];
       return WPT_OK;
     }
-  if (int rc = tensor_map_encode(map, base, rank, dims, strides_bytes, box)) return rc;
+  if (int rc = tensor_map_encode(map, base, rank, dims, strides_bytes, box, type)) return rc;
   keys[next] = key;
   maps[next] = *map;
   next = (next + 1) % SLOTS;
@@ -154,12 +158,12 @@ int tensor_map(CUtensorMap* map, const void* base, int rank, const cuuint64_t* d
 }
 
 int tensor_map_encode(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims,
-                      const cuuint64_t* strides_bytes, const cuuint32_t* box) {
+                      const cuuint64_t* strides_bytes, const cuuint32_t* box, CUtensorMapDataType type) {
   EncodeTiled encode;
   if (int rc = encoder(&encode)) return rc;
   if (int rc = bind_context()) return rc;
   cuuint32_t elem[3] = {1, 1, 1};
-  CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, strides_bytes,
+  CUresult r = encode(map, type, rank, const_cast<void*>(base), dims, strides_bytes,
                       box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(WPT_ERR_INVALID, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
@@ -1704,4 +1708,262 @@ extern "C" int wpt_cache_reorder(const wpt_cache_table* tables, int count, const
   }
   if (W <= 16) return launch_reorder<uint32_t, 16>(p, count, s);
   return launch_reorder<uint32_t, 64>(p, count, s);
+}
+
+// --------------------------------------- rotary positions, the 8-bit paged cache
+
+namespace {
+
+// A launch as a programmatic dependent of the kernel before it on the stream
+// (each of these kernels waits on the device before it touches memory).
+template <class... Args>
+cudaError_t launch_dependent(void (*kernel)(Args...), dim3 grid, int threads, int smem, int cluster_y,
+                             cudaStream_t stream, const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 1;
+  attr[1].val.clusterDim.y = cluster_y;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster_y > 1 ? 2 : 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// Whether turned and copied channels are whole vectors of `ve` elements.
+bool rotary_vectors(int ve, int C, int dims, int start, int interleaved) {
+  return C % ve == 0 && start % ve == 0 && (interleaved ? dims : dims / 2) % ve == 0;
+}
+
+int check_rotary(int C, int dims, int start, const void* frequencies) {
+  if (dims < 0 || dims % 2 || start < 0 || static_cast<int64_t>(start) + dims > C)
+    return fail(WPT_ERR_INVALID, "%d turned channels from %d on of %d", dims, start, C);
+  if (dims > 0 && !frequencies) return fail(WPT_ERR_INVALID, "a required pointer is NULL");
+  return WPT_OK;
+}
+
+template <class T, int VE>
+cudaError_t launch_rotate(const wpt::RotateParams& p, int interleaved, int64_t blocks, cudaStream_t s) {
+  return launch_dependent(interleaved ? wpt::rotate_kernel<T, VE, true> : wpt::rotate_kernel<T, VE, false>,
+                          dim3(static_cast<unsigned>(blocks)), 256, 0, 1, s, p);
+}
+
+template <class T, int VE>
+int launch_append(const wpt::AppendParams& p, int interleaved, unsigned blocks, cudaStream_t s) {
+  auto kernel = interleaved ? wpt::paged_append_kernel<T, VE, true> : wpt::paged_append_kernel<T, VE, false>;
+  const int smem = wpt::PAGE_BLOCK * 2 * p.C * 4;
+  if (int rc = allow_smem(kernel, smem)) return rc;
+  cudaError_t e = launch_dependent(kernel, dim3(blocks), 128, smem, 1, s, p);
+  if (e != cudaSuccess) return cuda_fail(e, "paged_append_kernel launch");
+  return WPT_OK;
+}
+
+template <int NCOL>
+int launch_paged(const CUtensorMap& tm, const wpt::PagedParams& p, int groups, cudaStream_t s) {
+  using L = wpt::PagedLayout<NCOL>;
+  static_assert(L::BYTES <= (L::CTAS == 2 ? 115712 : 232448), "paged attention kernel: too much shared memory");
+  auto kernel = wpt::paged_kernel<NCOL>;
+  if (int rc = allow_smem(kernel, L::BYTES)) return rc;
+  cudaError_t e = launch_dependent(kernel, dim3(groups, p.splits), wpt::PAGED_THREADS, L::BYTES, p.cluster, s, tm, p);
+  if (e != cudaSuccess) return cuda_fail(e, "paged_kernel launch");
+  return WPT_OK;
+}
+
+int paged_columns(int T, int H) {
+  const int64_t cols = static_cast<int64_t>(T) * H;
+  return cols <= 16 ? 16 : cols <= 32 ? 32 : 64;
+}
+
+bool page_size_ok(int S) { return S == 16 || S == 32 || S == 64 || (S >= 128 && S % 128 == 0); }
+
+}  // namespace
+
+extern "C" int wpt_rotate(const void* x, int64_t x_stride_b, int64_t x_stride_t, int64_t x_stride_h,
+                          const int64_t* positions, int64_t positions_stride_b, const void* frequencies,
+                          int frequencies_f64, void* y, int f32, int B, int T, int H, int C, int dims, int start,
+                          int interleaved, float magnitude, int inverse, void* stream) {
+  if (B < 0 || T < 0 || H < 0 || C < 1) return fail(WPT_ERR_INVALID, "bad shape B=%d T=%d H=%d C=%d", B, T, H, C);
+  if (int rc = check_rotary(C, dims, start, frequencies)) return rc;
+  if (B == 0 || T == 0 || H == 0) return WPT_OK;
+  if (!x || !y || !positions) return fail(WPT_ERR_INVALID, "a required pointer is NULL");
+  wpt::RotateParams p;
+  p.x = x;
+  p.y = y;
+  p.xsb = x_stride_b;
+  p.xst = x_stride_t;
+  p.xsh = x_stride_h;
+  p.positions = positions;
+  p.psb = positions_stride_b;
+  p.frequencies = frequencies;
+  p.f64 = frequencies_f64;
+  p.T = T;
+  p.H = H;
+  p.C = C;
+  p.dims = dims;
+  p.start = start;
+  p.sign = inverse ? -1.f : 1.f;
+  p.magnitude = magnitude;
+  const int wide = f32 ? 4 : 8;
+  const bool vectors = rotary_vectors(wide, C, dims, start, interleaved) && aligned16(x) && aligned16(y) &&
+                       x_stride_b % wide == 0 && x_stride_t % wide == 0 && x_stride_h % wide == 0;
+  const int ve = vectors ? wide : 1;
+  p.items = dims / 2 / (interleaved && ve > 1 ? ve / 2 : ve) + (C - dims) / ve;
+  // a thread's angles serve up to 8 heads, fewer where that would leave SMs without threads
+  int sms = 148;
+  current_device(&sms);
+  const int64_t tokens = static_cast<int64_t>(B) * T;
+  int heads = 8;
+  while (heads > 1 && tokens * p.items * ((H + heads - 1) / heads) < static_cast<int64_t>(sms) * 1024) heads /= 2;
+  p.lanes = (H + heads - 1) / heads;
+  p.total = tokens * p.items * p.lanes;
+  const int64_t blocks = (p.total + 255) / 256;
+  if (blocks >= (int64_t(1) << 31)) return fail(WPT_ERR_UNSUPPORTED, "too much to rotate in one call");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  if (f32)
+    e = vectors ? launch_rotate<float, 4>(p, interleaved, blocks, s) : launch_rotate<float, 1>(p, interleaved, blocks, s);
+  else
+    e = vectors ? launch_rotate<__nv_bfloat16, 8>(p, interleaved, blocks, s)
+                : launch_rotate<__nv_bfloat16, 1>(p, interleaved, blocks, s);
+  if (e != cudaSuccess) return cuda_fail(e, "rotate_kernel launch");
+  return WPT_OK;
+}
+
+extern "C" int wpt_paged_append(const void* src, int f32, int64_t src_stride_b, int64_t src_stride_n, void* pages,
+                                int64_t page_stride, int64_t entry_stride, float* scales, int64_t scales_stride,
+                                const void* table, int table_i64, int64_t table_stride_b, const int64_t* first,
+                                const int64_t* counts, const int64_t* positions, const void* frequencies,
+                                int frequencies_f64, int B, int n, int C, int M, int P, int S, int dims, int start,
+                                int interleaved, float magnitude, void* stream) {
+  if (B < 0 || n < 0 || M < 0 || P < 0 || C < 1) return fail(WPT_ERR_INVALID, "bad paged_append shape");
+  if (C % 16 || C > 512) return fail(WPT_ERR_UNSUPPORTED, "entries of 2 x %d: the paged cache takes multiples of 16 up to 512", C);
+  if (!page_size_ok(S)) return fail(WPT_ERR_UNSUPPORTED, "pages of %d entries: 16, 32, 64 or a multiple of 128", S);
+  if (int rc = check_rotary(C, dims, start, frequencies)) return rc;
+  if (B == 0 || n == 0 || M == 0 || P == 0) return WPT_OK;
+  if (!src || !pages || !scales || !table || !first || !counts) return fail(WPT_ERR_INVALID, "a required pointer is NULL");
+  if (!aligned16(pages) || page_stride % 16 || entry_stride % 16 || entry_stride < 2 * C)
+    return fail(WPT_ERR_INVALID, "pages and their strides must be multiples of 16 bytes");
+  const int wide = f32 ? 4 : 8;
+  const bool vectors = rotary_vectors(wide, C, dims, start, interleaved) && aligned16(src) &&
+                       src_stride_b % wide == 0 && src_stride_n % wide == 0;
+  wpt::AppendParams p;
+  p.src = src;
+  p.ssb = src_stride_b;
+  p.ssn = src_stride_n;
+  p.pages = static_cast<uint8_t*>(pages);
+  p.psp = page_stride;
+  p.psr = entry_stride;
+  p.scales = scales;
+  p.scp = scales_stride;
+  p.table = table;
+  p.tsb = table_stride_b;
+  p.first = first;
+  p.counts = counts;
+  p.positions = positions;
+  p.frequencies = frequencies;
+  if (int rc = status_word(&p.status)) return rc;
+  p.t64 = table_i64;
+  p.f64 = frequencies_f64;
+  p.B = B;
+  p.n = n;
+  p.C = C;
+  p.M = M;
+  p.P = P;
+  p.S = S;
+  p.dims = dims;
+  p.start = start;
+  p.magnitude = magnitude;
+  p.blocks = (n - 1) / wpt::PAGE_BLOCK + 2;  // n entries reach into that many blocks at most
+  const int64_t blocks = static_cast<int64_t>(B) * p.blocks;
+  if (blocks >= (int64_t(1) << 31)) return fail(WPT_ERR_UNSUPPORTED, "too many entries to append");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const unsigned grid = static_cast<unsigned>(blocks);
+  if (f32) return vectors ? launch_append<float, 4>(p, interleaved, grid, s) : launch_append<float, 1>(p, interleaved, grid, s);
+  return vectors ? launch_append<__nv_bfloat16, 8>(p, interleaved, grid, s)
+                 : launch_append<__nv_bfloat16, 1>(p, interleaved, grid, s);
+}
+
+extern "C" size_t wpt_paged_scratch_bytes(int B, int T, int H, int splits) {
+  if (B < 1 || T < 1 || H < 1 || H > 64 || splits < 1) return 0;
+  const int ncol = paged_columns(T, H), TQ = ncol / H;
+  return static_cast<size_t>(B) * ((T + TQ - 1) / TQ) * splits * ncol * (128 * 4 + 8);
+}
+
+extern "C" int wpt_paged_attention(const void* q, const void* pages, int64_t page_stride, int64_t entry_stride,
+                                   const float* scales, int64_t scales_stride, const void* table, int table_i64,
+                                   int64_t table_stride_b, const int64_t* positions, const float* sink, void* out,
+                                   float* lse, void* scratch, int splits, int chunk_tiles, int B, int T, int H, int C,
+                                   int M, int P, int S, int window, float scale, void* stream) {
+  if (C != 128) return fail(WPT_ERR_UNSUPPORTED, "head width %d: the paged attention kernel takes 128", C);
+  if (H < 1 || H > 64) return fail(WPT_ERR_UNSUPPORTED, "%d heads: the paged attention kernel takes 1 to 64", H);
+  if (!page_size_ok(S)) return fail(WPT_ERR_UNSUPPORTED, "pages of %d entries: 16, 32, 64 or a multiple of 128", S);
+  if (B < 0 || T < 0 || M < 0 || P < 0 || window < 0) return fail(WPT_ERR_INVALID, "bad shape B=%d T=%d M=%d P=%d", B, T, M, P);
+  if (B == 0 || T == 0) return WPT_OK;
+  if (static_cast<int64_t>(M) * S > INT_MAX - 1024) return fail(WPT_ERR_UNSUPPORTED, "a table of %d pages of %d entries", M, S);
+  if (static_cast<int64_t>(B) * T >= (int64_t(1) << 31) / H) return fail(WPT_ERR_UNSUPPORTED, "B*T*H too large");
+  if (splits < 1 || chunk_tiles < 1 || splits > 65535) return fail(WPT_ERR_INVALID, "splits and chunk_tiles must be >= 1");
+  if (!q || !positions || !out || !lse || (M > 0 && P > 0 && (!pages || !scales || !table)))
+    return fail(WPT_ERR_INVALID, "a required pointer is NULL");
+  if (!aligned16(q) || !aligned16(out) || (scratch && !aligned16(scratch)))
+    return fail(WPT_ERR_INVALID, "q, out and scratch must be 16-byte aligned");
+  const bool cluster = splits > 1 && scratch == nullptr;
+  if (cluster && splits > 8) return fail(WPT_ERR_INVALID, "%d splits without scratch: at most 8", splits);
+  CUtensorMap tm;
+  memset(&tm, 0, sizeof(tm));
+  if (M > 0 && P > 0) {
+    if (!aligned16(pages) || page_stride % 16 || entry_stride % 16 || entry_stride < 2 * C)
+      return fail(WPT_ERR_INVALID, "pages and their strides must be multiples of 16 bytes");
+    const cuuint64_t dims[3] = {2 * 128, static_cast<cuuint64_t>(S), static_cast<cuuint64_t>(P)};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(entry_stride),
+                                   static_cast<cuuint64_t>(P > 1 ? page_stride : entry_stride * S)};
+    const cuuint32_t box[3] = {128, static_cast<cuuint32_t>(S < 128 ? S : 128), 1};
+    if (int rc = tensor_map(&tm, pages, 3, dims, strides, box, CU_TENSOR_MAP_DATA_TYPE_UINT8)) return rc;
+  }
+  wpt::PagedParams p;
+  const int ncol = paged_columns(T, H);
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.scales = scales;
+  p.scp = scales_stride;
+  p.table = table;
+  p.tsb = table_stride_b;
+  p.positions = positions;
+  p.sink = sink;
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.lse = lse;
+  p.t64 = table_i64;
+  if (int rc = status_word(&p.status)) return rc;
+  p.B = B;
+  p.T = T;
+  p.H = H;
+  p.M = P > 0 ? M : 0;  // no page: no row
+  p.P = P;
+  p.S = S;
+  p.window = window;
+  p.TQ = ncol / H;
+  p.groups_per_row = (T + p.TQ - 1) / p.TQ;
+  p.splits = splits;
+  p.chunk_tiles = chunk_tiles;
+  p.cluster = cluster ? splits : 1;
+  p.scale_log2 = scale * wpt::LOG2E;
+  const int64_t groups = static_cast<int64_t>(B) * p.groups_per_row;
+  p.part_o = static_cast<float*>(scratch);
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + (scratch ? groups * splits * ncol * 128 : 0));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  int rc;
+  switch (ncol) {
+    case 16: rc = launch_paged<16>(tm, p, static_cast<int>(groups), s); break;
+    case 32: rc = launch_paged<32>(tm, p, static_cast<int>(groups), s); break;
+    default: rc = launch_paged<64>(tm, p, static_cast<int>(groups), s); break;
+  }
+  if (rc || splits == 1 || cluster) return rc;
+  const int64_t rows = static_cast<int64_t>(B) * T * H;
+  cudaError_t e = launch_dependent(wpt::paged_merge_kernel, dim3(static_cast<unsigned>((rows + 7) / 8)), 256, 0, 1, s, p, ncol);
+  if (e != cudaSuccess) return cuda_fail(e, "paged_merge_kernel launch");
+  return WPT_OK;
 }

@@ -823,3 +823,259 @@ def cache_reorder(tables, parents, lengths, first=None):
                None if first is None else first.data_ptr(), R, W))
         LAUNCHES[0] += 1
     return tables
+
+
+# ------------------------------------- rotary positions, the 8-bit paged cache
+
+PAGE_BLOCK = 16  # cached entries that share a scale
+
+
+def rotary_frequencies(dims, base=10000.0, scaling=None, factor=1.0, original=None, low=1.0, high=32.0, device=None):
+    """(dims / 2,) float64 angles a position, base ** (-2 i / dims), for rotate
+    and paged_append. For a context `factor` times as long as the `original` one:
+    scaling "linear" slows every pair by the factor, "base" enlarges the base so
+    that the slowest pair slows by it and the fastest stays, "parts" slows the
+    pairs that turn fewer than `low` times in the original context, leaves those
+    over `high` times as they are and goes linearly between."""
+    if dims < 0 or dims % 2:
+        raise ValueError(f"an even number of channels turns; got {dims}")
+    if scaling not in (None, "linear", "base", "parts"):
+        raise ValueError(f"scaling {scaling!r}: None, 'linear', 'base' or 'parts'")
+    if not base > 0 or not factor > 0 or (scaling == "parts" and (original is None or not high > low)):
+        raise ValueError(f"base={base}, factor={factor}, original={original}, low={low}, high={high}")
+    if scaling == "base":
+        base = base * factor ** (dims / max(1, dims - 2))
+    f = base ** (-torch.arange(0, dims, 2, dtype=torch.float64) / max(1, dims))
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "parts":
+        keep = ((original * f / (2 * math.pi) - low) / (high - low)).clamp(0, 1)
+        f = f * keep + f / factor * (1 - keep)
+    return f.to(device) if device is not None else f
+
+
+def _frequencies(frequencies, C, start):
+    """(contiguous fp32 or fp64 frequencies, dims, the first channel that turns) of heads of C channels."""
+    if frequencies is None:
+        return None, 0, 0
+    if frequencies.dim() != 1 or not frequencies.is_floating_point():
+        raise ValueError(f"frequencies are (dims / 2,) floating-point angles; got {frequencies.dtype} "
+                         f"{tuple(frequencies.shape)}")
+    if frequencies.dtype not in (torch.float64, torch.float32):
+        frequencies = frequencies.float()
+    if not frequencies.is_contiguous():
+        frequencies = frequencies.contiguous()
+    dims = 2 * frequencies.shape[0]
+    if start is None:
+        start = C - dims
+    if start < 0 or start + dims > C:
+        raise ValueError(f"{dims} turned channels from {start} on do not fit in {C}")
+    return frequencies, dims, start
+
+
+def rotate(x, positions, frequencies, start=None, interleaved=False, magnitude=1.0, inverse=False):
+    """x (B, T, C) or (B, T, H, C), bf16 or fp32, with the channels start ..
+    start + dims - 1 of each head (default: the last) turned by their positions
+    (T,) or (B, T) times frequencies (dims / 2,), times magnitude; inverse turns
+    the other way (the gradient). A new contiguous tensor."""
+    device = x.device
+    if not (x.is_cuda and positions.device == device and frequencies.device == device):
+        _one_device(x, positions, frequencies)
+    f32 = x.dtype == torch.float32
+    if not f32 and x.dtype != torch.bfloat16:
+        raise NotImplementedError(f"the rotation kernel takes bfloat16 or float32; got {x.dtype}")
+    shape = x.shape
+    if len(shape) not in (3, 4):
+        raise ValueError(f"x must be (B, T, C) or (B, T, H, C); got {tuple(shape)}")
+    B, T, C = shape[0], shape[1], shape[-1]
+    H = shape[2] if len(shape) == 4 else 1
+    if positions.shape != (T,) and positions.shape != (B, T) and positions.shape != (1, T):
+        raise ValueError(f"positions must be {(T,)} or {(B, T)}; got {tuple(positions.shape)}")
+    if (B | T | H | C) >> 31:
+        raise NotImplementedError(f"x of {tuple(shape)}: past the library's 32-bit arguments")
+    frequencies, dims, start = _frequencies(frequencies, C, start)
+    if positions.dtype != torch.int64 or positions.stride(-1) != 1:
+        positions = positions.to(torch.int64).contiguous()
+    if x.stride(-1) != 1:
+        x = x.contiguous()
+    y = torch.empty(shape, dtype=x.dtype, device=device)
+    if y.numel() == 0:
+        return y
+    stride = x.stride()
+    _call(device, _lib.lib().wpt_rotate,
+          (x.data_ptr(), stride[0], stride[1], stride[2] if len(shape) == 4 else 0, positions.data_ptr(),
+           positions.stride(0) if positions.shape[0] == B and positions.dim() == 2 else 0, frequencies.data_ptr(),
+           frequencies.dtype == torch.float64, y.data_ptr(), f32, B, T, H, C, dims, start, interleaved, magnitude,
+           inverse))
+    LAUNCHES[0] += 1
+    return y
+
+
+def _pages(pages, scales, table, width=None):
+    """Checks a paged cache's tensors; (P, S, C, M)."""
+    if pages.dtype != torch.float8_e4m3fn or scales.dtype != torch.float32:
+        raise NotImplementedError(f"the paged cache holds float8_e4m3fn with float32 scales; got {pages.dtype} and "
+                                  f"{scales.dtype}")
+    if pages.dim() != 3 or pages.shape[2] % 2 or pages.shape[1] % PAGE_BLOCK or \
+            scales.shape != (pages.shape[0], pages.shape[1] // PAGE_BLOCK, 2):
+        raise ValueError(f"pages {tuple(pages.shape)} must be (P, S, 2 C), S a multiple of {PAGE_BLOCK}, with scales "
+                         f"(P, S / {PAGE_BLOCK}, 2); got {tuple(scales.shape)}")
+    P, S, C2 = pages.shape
+    if S not in (16, 32, 64) and S % 128:
+        raise NotImplementedError(f"pages of {S} entries: 16, 32, 64 or a multiple of 128")
+    if table.dim() != 2 or table.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"the page table must be (B, M) int32 or int64; got {table.dtype} {tuple(table.shape)}")
+    ps, ss = pages.stride(), scales.stride()
+    if pages.numel() and (ps[2] != 1 or ps[1] < C2 or (P > 1 and ps[0] < S * ps[1]) or (ps[0] | ps[1]) % 16 or
+                          pages.data_ptr() % 16):
+        raise ValueError("pages must have contiguous entries, 16-byte aligned, and pages that do not overlap")
+    if scales.numel() and (ss[2] != 1 or (ss[1] != 2 and S > PAGE_BLOCK) or (P > 1 and ss[0] < S // PAGE_BLOCK * 2)):
+        raise ValueError("scales must be contiguous within a page")
+    if (P | S | table.shape[1] | table.shape[1] * S) >> 31:
+        raise NotImplementedError(f"{P} pages of {S} entries, {table.shape[1]} a row: past the library's 32-bit arguments")
+    return P, S, C2 // 2, table.shape[1]
+
+
+def _table_rows(table):
+    return table if table.shape[1] < 2 or table.stride(1) == 1 else table.contiguous()
+
+
+def paged_cache(pages, page, width, device=None):
+    """An empty paged cache for entries of `width` channels (a key, then a
+    value, 2 * width): pages (pages, page, 2 * width) float8_e4m3fn and scales
+    (pages, page / 16, 2) float32, zeros."""
+    if page not in (16, 32, 64) and (page < 128 or page % 128):
+        raise NotImplementedError(f"pages of {page} entries: 16, 32, 64 or a multiple of 128")
+    if width < 16 or width % 16 or width > 512:
+        raise NotImplementedError(f"entries of 2 x {width}: the paged cache takes multiples of 16 up to 512")
+    device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
+    return (torch.zeros(pages, page, 2 * width, dtype=torch.float8_e4m3fn, device=device),
+            torch.zeros(pages, page // PAGE_BLOCK, 2, device=device))
+
+
+def paged_append(pages, scales, table, new, first, counts, frequencies=None, positions=None, start=None,
+                 interleaved=False, magnitude=1.0):
+    """Writes new (B, n, 2 C), bf16 or fp32, to the paged cache, in place: row
+    b's entries new[b, :counts[b]] become its entries first[b] .., entry i on
+    page table[b, i // S]. With frequencies, keys are turned on the way, as
+    rotate does, by positions (B, n) (default: their places first[b] + i). A
+    block's scales become the least powers of two that hold its values; where it
+    holds earlier entries of the row, not less than they were, and those are
+    rounded again where a scale grows. Places outside the table or on no page
+    (-1) are not written and set the status word's shape bit."""
+    device = pages.device
+    if not (pages.is_cuda and scales.device == device and table.device == device and new.device == device and
+            first.device == device and counts.device == device and
+            (frequencies is None or frequencies.device == device) and (positions is None or positions.device == device)):
+        _one_device(pages, scales, table, new, first, counts, frequencies, positions)
+    P, S, C, M = _pages(pages, scales, table)
+    f32 = new.dtype == torch.float32
+    if not f32 and new.dtype != torch.bfloat16:
+        raise NotImplementedError(f"the append kernel takes bfloat16 or float32 entries; got {new.dtype}")
+    B = table.shape[0]
+    if new.dim() != 3 or new.shape[0] != B or new.shape[2] != 2 * C or first.shape != (B,) or counts.shape != (B,):
+        raise ValueError(f"entries {tuple(new.shape)} for a table of {B} rows and pages of 2 x {C}, with first "
+                         f"{tuple(first.shape)} and counts {tuple(counts.shape)}")
+    n = new.shape[1]
+    if positions is not None and positions.shape != (B, n):
+        raise ValueError(f"positions must be {(B, n)}; got {tuple(positions.shape)}")
+    if (B | n) >> 31:
+        raise NotImplementedError(f"entries {tuple(new.shape)}: past the library's 32-bit arguments")
+    frequencies, dims, start = _frequencies(frequencies, C, start)
+    first, counts = _rows(first), _rows(counts)
+    positions = None if positions is None else _rows(positions)
+    table = _table_rows(table)
+    if new.stride(2) != 1:
+        new = new.contiguous()
+    if B * n * P * M == 0:
+        return pages, scales
+    _call(device, _lib.lib().wpt_paged_append,
+          (new.data_ptr(), f32, new.stride(0), new.stride(1), pages.data_ptr(), pages.stride(0), pages.stride(1),
+           scales.data_ptr(), scales.stride(0), table.data_ptr(), table.dtype == torch.int64, table.stride(0),
+           first.data_ptr(), counts.data_ptr(), _lib.ptr(positions), _lib.ptr(frequencies),
+           frequencies is not None and frequencies.dtype == torch.float64, B, n, C, M, P, S, dims, start, interleaved,
+           magnitude))
+    LAUNCHES[0] += 1
+    return pages, scales
+
+
+def _paged_plan(B, T, H, N, window, sms):
+    """(splits, chunk_tiles, cluster) of a paged attention call over rows of up
+    to N entries, remembered per shape."""
+    key = ("paged", B, T, H, N, window, sms)
+    plan = _PLAN_CACHE.get(key)
+    if plan is None:
+        if len(_PLAN_CACHE) > 4096:
+            _PLAN_CACHE.clear()
+        plan = _PLAN_CACHE[key] = _paged_plan_for(B, T, H, N, window, sms)
+    return plan
+
+
+def _paged_plan_for(B, T, H, N, window, sms):
+    cols = min(T * H, 64)
+    ncol = 16 if cols <= 16 else 32 if cols <= 32 else 64
+    TQ = ncol // H
+    groups = B * math.ceil(T / TQ)
+    tiles = max(1, math.ceil(N / 128))
+    if window:
+        tiles = min(tiles, (window + TQ - 2) // 128 + 2)
+    slots = sms * (1 if ncol == 64 else 2)  # CTAs at a time
+    chunk = max(1, min(tiles, 16))
+    if groups * math.ceil(tiles / chunk) > 4 * slots:
+        chunk = min(tiles, 16 * math.ceil(tiles * groups / (4 * slots) / 16))
+    elif groups * math.ceil(tiles / chunk) < slots:
+        chunk = max(1, math.ceil(tiles * groups / slots))
+    splits = math.ceil(tiles / chunk)
+    if 1 < splits and groups * min(splits, 8) <= slots and tiles <= 64:  # one wave of clusters
+        splits = min(splits, 8)
+        chunk = math.ceil(tiles / splits)
+        splits = math.ceil(tiles / chunk)
+    return splits, chunk, 1 < splits <= 8 and groups * splits <= slots
+
+
+def paged_attention(q, pages, scales, table, positions, scale, window=0, sink=None):
+    """Attention of q (B, T, H, 128) bf16 over each row's entries 0 ..
+    positions (B, T) of the paged cache (its last `window` ones, given a
+    window), sink (H,) in the denominators: (out (B, T, H, 128) bf16, lse
+    (B, T, H) fp32). Entries on no page (-1) are not read; a query without
+    entries gives 0 and -inf (or its sink)."""
+    device = q.device
+    if not (q.is_cuda and pages.device == device and scales.device == device and table.device == device and
+            positions.device == device and (sink is None or sink.device == device)):
+        _one_device(q, pages, scales, table, positions, sink)
+    P, S, C, M = _pages(pages, scales, table)
+    _bf16(q)
+    if q.dim() != 4 or q.shape[3] != C or table.shape[0] != q.shape[0] or positions.shape != q.shape[:2]:
+        raise ValueError(f"queries {tuple(q.shape)} with pages of 2 x {C}, a table of {table.shape[0]} rows and "
+                         f"positions {tuple(positions.shape)}")
+    B, T, H, _ = q.shape
+    if sink is not None and sink.shape != (H,):
+        raise ValueError(f"sink must be {(H,)}; got {tuple(sink.shape)}")
+    if window < 0 or (B | T) >> 31:
+        raise ValueError(f"window={window}, or a shape past 2**31: {tuple(q.shape)}")
+    if C != 128 or H > 64:
+        raise NotImplementedError(f"{H} heads of width {C}: the paged attention kernel takes head width 128 and up to 64 "
+                                  "heads")
+    window = min(window, 2 ** 31 - 1)  # past every table
+    if not q.is_contiguous() or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
+    positions = _rows(positions)
+    table = _table_rows(table)
+    if sink is not None and (sink.dtype != torch.float32 or not sink.is_contiguous()):
+        sink = sink.float().contiguous()
+    out = torch.empty_like(q)
+    lse = torch.empty((B, T, H), dtype=torch.float32, device=device)
+    if B * T * H == 0:
+        return out, lse
+    splits, chunk, cluster = _paged_plan(B, T, H, M * S, window, sm_count(device))
+    lib = _lib.lib()
+    scratch = None
+    if splits > 1 and not cluster:
+        scratch = torch.empty(lib.wpt_paged_scratch_bytes(B, T, H, splits), dtype=torch.uint8, device=device)
+    ps = pages.stride()
+    _call(device, lib.wpt_paged_attention,
+          (q.data_ptr(), pages.data_ptr(), ps[0], ps[1], scales.data_ptr(), scales.stride(0), table.data_ptr(),
+           table.dtype == torch.int64, table.stride(0), positions.data_ptr(), _lib.ptr(sink), out.data_ptr(),
+           lse.data_ptr(), _lib.ptr(scratch), splits, chunk, B, T, H, C, M, P, S, window, scale))
+    LAUNCHES[0] += 1 + (scratch is not None)
+    return out, lse
