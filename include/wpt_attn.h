@@ -403,18 +403,19 @@ int wpt_paged_append(const void* src, int f32, int64_t src_stride_b, int64_t src
  * positions[b, t] (window 0: no window), but for those on no page; q, out, lse
  * and sink as above. What other entries hold (NaN too) reaches no result.
  * Value scales are 0, or 2^-60 to 2^60.
- *   splits, chunk_tiles  each query group's entries go to `splits` CTAs,
- *              chunk_tiles tiles of 128 each (splits * chunk_tiles tiles must
- *              cover the rows, or the window and a tile); with splits > 1
- *              scratch holds wpt_paged_scratch_bytes(B, T, H, splits) bytes,
- *              16-byte aligned, or is NULL for 2 to 8 splits: then a group's
- *              splits are one thread-block cluster and need none.
+ *   splits     how the work is split. 1 to 8: each query group's entries go to
+ *              that many CTAs in equal runs, a thread-block cluster where more
+ *              than one; ctas and scratch are not used. 0: all groups' entries
+ *              in equal runs over `ctas` CTAs, for up to 256 groups (64 / H
+ *              queries of a row each; 32 / H or 16 / H where T * H is no
+ *              more), with scratch of wpt_paged_scratch_bytes bytes, 16-byte
+ *              aligned.
  */
-size_t wpt_paged_scratch_bytes(int B, int T, int H, int splits);
+size_t wpt_paged_scratch_bytes(int B, int T, int H, int splits, int ctas);
 int wpt_paged_attention(const void* q, const void* pages, int64_t page_stride, int64_t entry_stride,
                         const float* scales, int64_t scales_stride, const void* table, int table_i64,
                         int64_t table_stride_b, const int64_t* positions, const float* sink, void* out, float* lse,
-                        void* scratch, int splits, int chunk_tiles, int B, int T, int H, int C, int M, int P, int S,
+                        void* scratch, int splits, int ctas, int B, int T, int H, int C, int M, int P, int S,
                         int window, float scale, void* stream);
 
 /*

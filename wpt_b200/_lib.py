@@ -54,7 +54,7 @@ SIGNATURES = {
     "wpt_rotate": [_P, _I64, _I64, _I64, _P, _I64, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P],
     "wpt_paged_append": [_P, _I, _I64, _I64, _P, _I64, _I64, _P, _I64, _P, _I, _I64, _P, _P, _P, _P, _I, _I, _I, _I,
                          _I, _I, _I, _I, _I, _I, _F, _P],
-    "wpt_paged_scratch_bytes": [_I, _I, _I, _I],
+    "wpt_paged_scratch_bytes": [_I, _I, _I, _I, _I],
     "wpt_paged_attention": [_P, _P, _I64, _I64, _P, _I64, _P, _I, _I64, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I,
                             _I, _I, _I, _F, _P],
     "wpt_attn_exchange": [_P, _P, _I, _I64, _I, _I, _P, ctypes.POINTER(_P), _I, _I, _P, _P, _P],

@@ -74,8 +74,11 @@ struct AppendParams {
   float magnitude;
 };
 
+__device__ __forceinline__ int64_t page_number(const void* table, int t64, int64_t at) {
+  return t64 ? static_cast<const int64_t*>(table)[at] : static_cast<const int32_t*>(table)[at];
+}
 __device__ __forceinline__ int64_t page_of(const void* table, int t64, int64_t at, int P) {
-  const int64_t id = t64 ? static_cast<const int64_t*>(table)[at] : static_cast<const int32_t*>(table)[at];
+  const int64_t id = page_number(table, t64, at);
   return id >= 0 && id < P ? id : -1;
 }
 
@@ -232,18 +235,27 @@ __global__ void __launch_bounds__(128) paged_append_kernel(const AppendParams p)
 //
 // What e4m3 and e5m2 cannot hold of q and of the weights goes into more
 // columns of the same product, whose M (the streamed side) is read once:
-//   q (bf16, 8 significant bits), by a power of two of its row into 224 ..
-//   448, is hi + lo / 16, both e4m3: exact down to 2^-10 of the row's
-//   largest value and within 2^-22.8 of that below.
+//   q (bf16, 8 significant bits), by a power of two that brings the group's
+//   largest value into 224 .. 448, is hi + lo / 16, both e4m3: exact down to
+//   2^-10 of that value, and within 2^-22.8 of it below.
 //   a weight w = 2^x, as fp16 (11 significant bits) 3 e5m2 numbers, each the
-//   upper byte (e5m2 is fp16's) of what the ones before it leave, rounded:
-//   within 2^-10 w down to 2^-21 of the largest weight (bf16's 2^-8 would
-//   do), and an absolute 2^-30 of it under that, so that a long tail of small
-//   weights keeps its sum.
+//   upper byte (e5m2 is fp16's) of what the ones before it leave, the last one
+//   times 32 and rounded: within 2^-8.6 w (2^-9, and fp16's 2^-11; a bf16
+//   weight's is 2^-8), and 2^-22 where w is small. 1 is what the first tile's
+//   largest weight comes out as, 2^15 the largest that fits: a column is
+//   rescaled when a score passes those of the first tile by 15 (base 2), and a
+//   run of n keys may lose n 2^-22 of its largest weight.
 // Scales. A key's scale multiplies its score. A value's scale 2^lv joins the
 // exponent, w = 2^(s + lv - m), m the running maximum of s + lv, so O needs no
 // scaling; the softmax's sum takes w 2^-lv. Sums, maxima and accumulators are
 // fp32.
+//
+// Work. A group is up to 64 columns (query, head) of a batch row, its tiles
+// those that its queries read. Balanced: every CTA works out the groups' tile
+// counts and takes an equal run of all tiles in a row, a part of one group or
+// of several (segments); a group in several CTAs leaves parts for
+// paged_merge_kernel. Otherwise a group's tiles go in equal runs to a cluster of
+// up to 8 CTAs that merges through distributed shared memory.
 //
 // Warps 0-3 prepare q, then take thread r = key r of a tile of 128 (as the
 // key-stream kernel's do); warp 4 issues products; warp 5 brings K and V by
@@ -258,47 +270,59 @@ struct PagedParams {
   const float* sink;             // (H,) or null
   __nv_bfloat16* out;            // (B, T, H, 128)
   float* lse;                    // (B, T, H)
-  float* part_o;                 // (groups * splits, NCOL, 128), not normalised
-  float2* part_ml;               // (groups * splits, NCOL): exponent of the maximum, sum
+  float* part_o;                 // (parts, NCOL, 128), not normalised
+  float2* part_ml;               // (parts, NCOL): exponent of the maximum, sum
+  int2* info;                    // balanced: each group's first part and its parts
   unsigned* status;
   int t64;
-  int B, T, H, M, P, S, window, TQ, groups_per_row, splits, chunk_tiles;
-  int cluster;                   // > 1: the splits of a group are one cluster
+  unsigned M, S;                 // pages a row, entries a page
+  int B, T, H, P, window, TQ, groups_per_row, groups;
+  int splits;                    // CTAs of a group, a cluster where > 1; 0: balanced, all groups' tiles over the grid
   float scale_log2;
 };
 
-// The exponent unit's weights come out 2^13 times as large: with a lazy
-// maximum at most 2 under the true one they reach 2^15 (fp16 ends at 2^16).
-constexpr float PAGED_UP = 13.f, PAGED_SLACK = 2.f;
+constexpr float PAGED_TOP = 15.f;  // weights up to 2^15 (fp16 ends at 2^16)
+// Minus the base of a column that has read nothing: any score is past it.
+constexpr float PAGED_UNSET = 1e30f;
+
+constexpr int PAGED_GROUPS = 256;  // of a balanced call, at most
+constexpr int PAGED_SEGMENT = 4;   // what a segment costs beside its tiles, in tiles
 
 template <int NCOL>
 struct PagedLayout {
   static constexpr int C = 128, BN = 128;
-  static constexpr int NK = NCOL == 64 ? 4 : 2, NV = NCOL == 64 ? 5 : 3;  // ring stages of keys and of values
+  static constexpr int NK = NCOL == 64 ? 4 : 2, NV = NCOL == 64 ? 4 : 2;  // ring stages of keys and of values
   static constexpr int CTAS = NCOL == 64 ? 1 : 2;                         // a SM
+  static constexpr bool IN_REGS = NCOL <= 32;                             // bases stay in registers
   static constexpr int TILE = BN * C;
   static constexpr int Q_BYTES = 2 * NCOL * C;
   static constexpr int P_BYTES = BN * (NCOL == 64 ? 256 : 128);
   static constexpr int OFF_K = ((Q_BYTES + 1023) / 1024) * 1024;
   static constexpr int OFF_V = OFF_K + NK * TILE;
   static constexpr int OFF_P = OFF_V + NV * TILE;
-  static constexpr int OFF_COL = OFF_P + P_BYTES;            // float4 a column: factor, base, bound, -
-  static constexpr int OFF_RED = OFF_COL + NCOL * 16;        // 4 x NCOL floats
-  static constexpr int OFF_ALPHA = OFF_RED + 4 * NCOL * 4;   // float2 a column: factor, shift
-  static constexpr int OFF_L = OFF_ALPHA + NCOL * 8;
-  static constexpr int OFF_SCALE = OFF_L + NCOL * 4;         // NV x 8 blocks x float4
-  static constexpr int OFF_NAN = OFF_SCALE + NV * 8 * 16;    // 4 words a column
+  static constexpr int OFF_BASE = OFF_P + 2 * P_BYTES;       // minus a column's base, PAGED_UNSET while none is set
+  static constexpr int OFF_RED = OFF_BASE + NCOL * 4;        // 4 x NCOL floats
+  static constexpr int OFF_ALPHA = OFF_RED + 4 * NCOL * 4;   // the factor of a rescaled column, 1 for others
+  static constexpr int OFF_L = OFF_ALPHA + NCOL * 4;
+  static constexpr int OFF_TOP = OFF_L + NCOL * 4;           // a column's largest exponent, where it is to be raised
+  static constexpr int OFF_SCALE = OFF_TOP + NCOL * 4;         // 2 tiles x 8 blocks x float4
+  static constexpr int OFF_NAN = OFF_SCALE + 2 * 8 * 16;     // 4 words a column
   static constexpr int OFF_QLO = OFF_NAN + NCOL * 16;
   static constexpr int OFF_QHI = OFF_QLO + 64 * 4;
-  static constexpr int OFF_BAR = OFF_QHI + 64 * 4;
-  static constexpr int NBAR = 1 + 2 * NK + 3 * NV + 2 + 1 + 1;
+  static constexpr int OFF_TILES = OFF_QHI + 64 * 4;         // groups: tiles before each, and the first tile
+  static constexpr int OFF_BAR = OFF_TILES + (2 * PAGED_GROUPS + 2) * 4;
+  static constexpr int NBAR = 1 + 2 * NK + 2 * NV + 2 + 2 + 1;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
-  static constexpr int BYTES = OFF_MISC + 32 + 1024;
+  static constexpr int BYTES = OFF_MISC + 64 + 1024;
   static constexpr int S_COLS = 2 * NCOL, O_COLS = 3 * NCOL;
   static constexpr int TMEM_COLS = 2 * S_COLS + O_COLS <= 128 ? 128 : 2 * S_COLS + O_COLS <= 256 ? 256 : 512;
 };
 
-constexpr int PAGED_THREADS = 224;
+constexpr int PAGED_THREADS = 256;
+// Registers: the softmax warps hold a column's score, sum, factor and base
+// each, the others little. 128 threads of 192 and 128 of 64 are the 256 of 128
+// that a block of two on an SM is launched with.
+constexpr int PAGED_REGS = 128, PAGED_REGS_SOFTMAX = 200, PAGED_REGS_OTHERS = 56;
 
 // kind::f8f6f4, fp32 accumulators; types 0 e4m3, 1 e5m2
 __host__ __device__ constexpr uint32_t idesc_f8(int M, int N, int a_type, int b_type, int a_mn, int b_mn) {
@@ -333,9 +357,8 @@ __device__ __forceinline__ void paged_pv_steps(uint32_t d, uint64_t dv, uint64_t
   mma_f8_off_warp<off, off>(d, dv, dp, idesc, KK > 0 ? 1u : acc0);
 }
 
-// The rows a query reads: lo .. hi of its batch row (hi < lo: none).
-__device__ __forceinline__ void paged_query_rows(const PagedParams& p, int b, int t, int& lo, int& hi) {
-  const int64_t pos = p.positions[static_cast<int64_t>(b) * p.T + t];
+// The rows that a query at `pos` reads: lo .. hi of its batch row (hi < lo: none).
+__device__ __forceinline__ void paged_rows(const PagedParams& p, int64_t pos, int& lo, int& hi) {
   const int64_t last = static_cast<int64_t>(p.M) * p.S - 1;
   const int64_t top = pos < last ? pos : last;
   int64_t low = 0;
@@ -344,11 +367,27 @@ __device__ __forceinline__ void paged_query_rows(const PagedParams& p, int b, in
   lo = low > INT_MAX ? INT_MAX : static_cast<int>(low);
 }
 
-// fp16 pair -> its rounded upper bytes (kept in place) and what they leave
+// fp16 pair (not negative) -> its upper bytes, cut off, and in h what they leave
 __device__ __forceinline__ uint32_t e5m2_part(uint32_t& h) {
-  const uint32_t part = (h + 0x00800080u) & 0xff00ff00u;
+  const uint32_t part = h & 0xff00ff00u;
   asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(h) : "r"(part));
   return part;
+}
+// floats in the order of their ints (NaN aside), and back
+__device__ __forceinline__ int ordered(float x) {
+  const int i = __float_as_int(x);
+  return i ^ ((i >> 31) & 0x7fffffff);
+}
+__device__ __forceinline__ float unordered(int i) { return __int_as_float(i ^ ((i >> 31) & 0x7fffffff)); }
+__device__ __forceinline__ float warp_max(float x) {  // NaN ignored
+  float r;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t half2_times32(uint32_t h) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(h), "r"(0x50005000u));
+  return r;
 }
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   uint32_t r;
@@ -376,14 +415,14 @@ __device__ __forceinline__ float paged_total(float M, float L, const float* sink
 // Cluster mode: a group's splits, one CTA each, merge through distributed
 // shared memory; CTA k owns columns k, k + S, ... (as stream_cluster_merge).
 template <int NCOL>
-__device__ __forceinline__ void paged_cluster_merge(const PagedParams& p, const float4* s_col, const float* s_l,
+__device__ __forceinline__ void paged_cluster_merge(const PagedParams& p, const float* s_base, const float* s_l,
                                                     const float* s_o, float* s_w, int64_t row0, int ncols) {
   constexpr int C = 128;
   cluster_sync();
-  const int S = p.cluster;
+  const int S = p.splits;
   const int rank = static_cast<int>(cluster_rank());
   const int mine = ncols > rank ? (ncols - rank + S - 1) / S : 0;
-  const uint32_t am = smem_u32(s_col), al = smem_u32(s_l), ao = smem_u32(s_o);
+  const uint32_t am = smem_u32(s_base), al = smem_u32(s_l), ao = smem_u32(s_o);
   if (static_cast<int>(threadIdx.x) < mine) {
     const int cl = threadIdx.x, c = rank + cl * S;
     float mi[8], li[8];
@@ -392,7 +431,7 @@ __device__ __forceinline__ void paged_cluster_merge(const PagedParams& p, const 
       mi[i] = -INFINITY;
       li[i] = 0.f;
       if (i < S) {
-        mi[i] = dsmem_ld(dsmem_map(am + c * 16 + 4, i));
+        mi[i] = -dsmem_ld(dsmem_map(am + c * 4, i));
         li[i] = dsmem_ld(dsmem_map(al + c * 4, i));
       }
     }
@@ -448,10 +487,11 @@ __global__ void __launch_bounds__(PAGED_THREADS, PagedLayout<NCOL>::CTAS)
   uint8_t* sK = smem + L::OFF_K;
   uint8_t* sV = smem + L::OFF_V;
   uint8_t* sP = smem + L::OFF_P;
-  float4* s_col = reinterpret_cast<float4*>(smem + L::OFF_COL);
+  float* s_base = reinterpret_cast<float*>(smem + L::OFF_BASE);
   float* s_red = reinterpret_cast<float*>(smem + L::OFF_RED);
-  float2* s_alpha = reinterpret_cast<float2*>(smem + L::OFF_ALPHA);
+  float* s_alpha = reinterpret_cast<float*>(smem + L::OFF_ALPHA);
   float* s_l = reinterpret_cast<float*>(smem + L::OFF_L);
+  int* s_top = reinterpret_cast<int*>(smem + L::OFF_TOP);
   float4* s_scale = reinterpret_cast<float4*>(smem + L::OFF_SCALE);
   uint32_t* s_nan = reinterpret_cast<uint32_t*>(smem + L::OFF_NAN);
   int* s_qlo = reinterpret_cast<int*>(smem + L::OFF_QLO);
@@ -462,450 +502,643 @@ __global__ void __launch_bounds__(PAGED_THREADS, PagedLayout<NCOL>::CTAS)
   uint64_t* k_empty = k_full + NK;
   uint64_t* v_full = k_empty + NK;
   uint64_t* v_empty = v_full + NV;
-  uint64_t* sc_full = v_empty + NV;
-  uint64_t* s_full = sc_full + NV;
+  uint64_t* s_full = v_empty + NV;  // a tile's scores, and its scales
   uint64_t* p_ready = s_full + 2;
-  uint64_t* o_done = p_ready + 1;
+  uint64_t* o_done = p_ready + 2;
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC);
-  int* s_range = reinterpret_cast<int*>(smem + L::OFF_MISC + 4);  // rows read by some query, rows read by all, any NaN
+  int* s_any_nan = reinterpret_cast<int*>(smem + L::OFF_MISC + 4);
+  int* s_sum = reinterpret_cast<int*>(smem + L::OFF_MISC + 8);  // 8 warps; later the largest |q| of four
+  int* s_before = reinterpret_cast<int*>(smem + L::OFF_TILES);  // [g]: the groups before g, tiles and what is set aside
+  int* s_first = s_before + PAGED_GROUPS + 1;                   // [g]: its first tile
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int group = blockIdx.x, split = blockIdx.y;
-  const int b = group / p.groups_per_row;
-  const int t0 = (group - b * p.groups_per_row) * p.TQ;
-  const int TQg = min(p.TQ, p.T - t0);
-  const int ncols = TQg * p.H;
-  const int64_t row0 = (static_cast<int64_t>(b) * p.T + t0) * p.H;
+  const bool balanced = p.splits == 0;
+  const int gbase = balanced ? 0 : blockIdx.x;  // the group that s_before[0] stands for
+  const int gcount = balanced ? p.groups : 1;
 
-  if (warp == 0) {
-    griddep_wait();
-    int rlo = INT_MAX, rhi = -1, alo = 0, ahi = INT_MAX;
-    for (int tq = lane; tq < TQg; tq += 32) {
-      int lo, hi;
-      paged_query_rows(p, b, t0 + tq, lo, hi);
-      s_qlo[tq] = lo;
-      s_qhi[tq] = hi;
-      if (hi >= lo) {
-        rlo = min(rlo, lo);
-        rhi = max(rhi, hi);
-      }
-      alo = max(alo, lo);
-      ahi = min(ahi, hi);
-    }
-    rlo = __reduce_min_sync(0xffffffffu, rlo);
-    rhi = __reduce_max_sync(0xffffffffu, rhi);
-    alo = __reduce_max_sync(0xffffffffu, alo);
-    ahi = __reduce_min_sync(0xffffffffu, ahi);
-    if (lane == 0) {
-      s_range[0] = rlo;
-      s_range[1] = rhi;
-      s_range[2] = alo;
-      s_range[3] = ahi;
-      s_range[4] = 0;
-    }
-  } else if (warp == 1) {
-    for (int i = lane; i < NCOL; i += 32) {
-      s_col[i] = make_float4(0.f, -PAGED_UP, -INFINITY, 0.f);
-      s_l[i] = 0.f;
-    }
-  } else if (warp == 2) {
+  if (warp == 3) {
     for (int i = lane; i < NCOL * 4; i += 32) s_nan[i] = 0u;
-  } else if (warp == 3 && lane == 0) {
-    mbar_init(q_full, 128);
-    for (int s = 0; s < NK; ++s) {
-      mbar_init(k_full + s, 1);
-      mbar_init(k_empty + s, 1);
+    for (int i = lane; i < NCOL; i += 32) {
+      s_base[i] = PAGED_UNSET;
+      s_l[i] = 0.f;
+      s_top[i] = INT_MIN;
     }
-    for (int s = 0; s < NV; ++s) {
-      mbar_init(v_full + s, 1);
-      mbar_init(v_empty + s, 1);
-      mbar_init(sc_full + s, 1);
+    if (lane == 0) {
+      mbar_init(q_full, 128);
+      for (int s = 0; s < NK; ++s) {
+        mbar_init(k_full + s, 1);
+        mbar_init(k_empty + s, 1);
+      }
+      for (int s = 0; s < NV; ++s) {
+        mbar_init(v_full + s, 1);
+        mbar_init(v_empty + s, 1);
+      }
+      for (int s = 0; s < 2; ++s) {
+        mbar_init(s_full + s, 2);
+        mbar_init(p_ready + s, 128);
+      }
+      mbar_init(o_done, 1);
+      fence_mbar_init();
+      *s_any_nan = 0;
     }
-    mbar_init(s_full, 1);
-    mbar_init(s_full + 1, 1);
-    mbar_init(p_ready, 128);
-    mbar_init(o_done, 1);
-    fence_mbar_init();
   } else if (warp == 4) {
     tmem_alloc(s_tmem, L::TMEM_COLS);
     tmem_relinquish();
   }
   griddep_wait();
+  // the groups' tiles: thread g counts group g's, a scan adds them up
+  int count = 0;
+  if (static_cast<int>(threadIdx.x) < gcount) {
+    const int g = gbase + threadIdx.x, b = g / p.groups_per_row, t0 = (g - b * p.groups_per_row) * p.TQ;
+    int rlo = INT_MAX, rhi = -1;
+    for (int t = t0; t < min(t0 + p.TQ, p.T); ++t) {
+      int lo, hi;
+      paged_rows(p, p.positions[static_cast<int64_t>(b) * p.T + t], lo, hi);
+      if (hi >= lo) {
+        rlo = min(rlo, lo);
+        rhi = max(rhi, hi);
+      }
+    }
+    int first = 0;
+    if (rhi >= 0) {
+      first = rlo / BN;
+      count = rhi / BN - first + 1;
+    }
+    s_first[threadIdx.x] = first;
+  }
+  const int aside = balanced ? PAGED_SEGMENT : 0;
+  if (count > 0) count += aside;
+  int upto = count;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += x;
+  }
+  if (lane == 31) s_sum[warp] = upto;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  // tiles of 128 entries, from the one that holds the first row read
-  const int rlo = s_range[0], rhi = s_range[1];
-  const int tile0 = rhi >= rlo ? rlo / BN + split * p.chunk_tiles : 0;
-  const int ntiles = rhi >= rlo ? max(0, min(p.chunk_tiles, rhi / BN - tile0 + 1)) : 0;
-  const int64_t seg = static_cast<int64_t>(group) * p.splits + split;
+  int all = 0;
+#pragma unroll
+  for (int w = 0; w < PAGED_THREADS / 32; ++w) {
+    if (w < warp) upto += s_sum[w];
+    all += s_sum[w];
+  }
+  s_before[threadIdx.x + 1] = upto;
+  if (threadIdx.x == 0) s_before[0] = 0;
+  // this CTA's run of tiles
+  // no more runs than tiles, so that every CTA from a group's first to its last has a part of it
+  const int parts = balanced ? max(1, min(static_cast<int>(gridDim.x), all)) : p.splits;
+  const int part_of = balanced ? min(static_cast<int>(blockIdx.x), parts) : blockIdx.y;
+  const int begin = static_cast<int>(static_cast<int64_t>(all) * part_of / parts);
+  const int end = part_of < parts ? static_cast<int>(static_cast<int64_t>(all) * (part_of + 1) / parts) : begin;
+  if (balanced && blockIdx.x == 0 && static_cast<int>(threadIdx.x) < gcount) {
+    // parts of group g: from the CTA whose run holds its first tile to the one that holds its last
+    const int before = upto - count + aside;
+    auto holder = [&](int64_t tile) { return static_cast<int>(((tile + 1) * parts + all - 1) / all) - 1; };
+    p.info[threadIdx.x] = count == 0 ? make_int2(0, 0)
+                                     : make_int2(holder(before) + threadIdx.x, holder(upto - 1) - holder(before) + 1);
+  }
+  __syncthreads();
+  const uint32_t tmem = *s_tmem;
+  griddep_launch();
 
-  if (ntiles == 0) {
-    if (p.cluster > 1) {
-      paged_cluster_merge<NCOL>(p, s_col, s_l, reinterpret_cast<const float*>(sK), reinterpret_cast<float*>(sP), row0,
-                                ncols);
-    } else if (p.splits > 1) {
-      if (static_cast<int>(threadIdx.x) < ncols) p.part_ml[seg * NCOL + threadIdx.x] = make_float2(-INFINITY, 0.f);
-    } else {
-      for (int i = threadIdx.x; i < ncols * (C / 2); i += PAGED_THREADS)
-        reinterpret_cast<uint32_t*>(p.out + row0 * C)[i] = 0u;
-      if (static_cast<int>(threadIdx.x) < ncols)
-        p.lse[row0 + threadIdx.x] = p.sink != nullptr ? p.sink[threadIdx.x % p.H] : -INFINITY;
+  // The segments of the run, the same for every warp: next() until false.
+  struct Segments {
+    const int *before, *first;
+    int aside, at, end, g;  // the run's next place; the group (from gbase) of the segment
+    int tile0, n;           // its first tile and its tiles
+    bool whole;             // all of its group's
+    __device__ __forceinline__ bool next() {
+      while (at < end) {
+        while (before[g + 1] <= at) ++g;
+        const int from = before[g] + aside, stop = min(end, before[g + 1]);
+        tile0 = max(at, from);
+        n = stop - tile0;
+        tile0 += first[g] - from;
+        whole = n == before[g + 1] - from;
+        at = stop;
+        if (n > 0) return true;  // else the run ends in what is set aside for the group
+      }
+      return false;
+    }
+  };
+  Segments sg{s_before, s_first, aside, begin, end, 0, 0, 0, false};
+
+  if (begin == end) {  // nothing to read
+    if (!balanced) {
+      const int b = gbase / p.groups_per_row, t0 = (gbase - b * p.groups_per_row) * p.TQ;
+      const int ncols = min(p.TQ, p.T - t0) * p.H;
+      const int64_t row0 = (static_cast<int64_t>(b) * p.T + t0) * p.H;
+      if (p.splits > 1) {
+        paged_cluster_merge<NCOL>(p, s_base, s_l, reinterpret_cast<const float*>(sP), reinterpret_cast<float*>(sK),
+                                  row0, ncols);
+      } else {
+        for (int i = threadIdx.x; i < ncols * (C / 2); i += PAGED_THREADS)
+          reinterpret_cast<uint32_t*>(p.out + row0 * C)[i] = 0u;
+        if (static_cast<int>(threadIdx.x) < ncols)
+          p.lse[row0 + threadIdx.x] = p.sink != nullptr ? p.sink[threadIdx.x % p.H] : -INFINITY;
+      }
     }
     tc_fence_before();
     __syncthreads();
     if (warp == 4) {
       tc_fence_after();
-      tmem_dealloc(*s_tmem, L::TMEM_COLS);
+      tmem_dealloc(tmem, L::TMEM_COLS);
     }
     return;
   }
-  const uint32_t tmem = *s_tmem;
-  griddep_launch();
 
   if (warp == 5) {
+    if constexpr (L::CTAS == 2) setmaxnreg_dec<PAGED_REGS_OTHERS>();
     // ------------------------------------------------ keys and values by TMA
-    const int rows = min(p.S, BN), per = BN / rows;  // entries of a box, boxes of a tile
+    const int rows = min(static_cast<int>(p.S), BN), per = BN / rows;  // entries of a box, boxes of a tile
     const int batch = 32 / per;                      // tiles whose page numbers the warp holds, a lane a box
     const int part = lane % per;
-    auto lookup = [&](int j0) {  // the page of this lane's box in tile j0 + lane / per
-      const int64_t n = static_cast<int64_t>(tile0 + j0 + lane / per) * BN + part * rows;
-      if (j0 + lane / per >= ntiles || n / p.S >= p.M) return -1;
-      return static_cast<int>(page_of(p.table, p.t64, b * p.tsb + n / p.S, p.P));
-    };
-    int mine = lookup(0), next = lookup(batch);
     bool ok = true;
-    for (int j = 0; ok && j < ntiles; ++j) {
-      const int in = j % batch;
-      if (in == 0 && j > 0) {
-        mine = next;
-        next = lookup(j + batch);
+    int j = 0;  // the ring's tile
+    while (ok && sg.next()) {
+      const int b = (gbase + sg.g) / p.groups_per_row;
+      // the number of this lane's page in tile i0 + lane / per: loaded a batch ahead, checked when it is used
+      auto lookup = [&](int i0) {
+        const unsigned at = (static_cast<unsigned>(sg.tile0 + i0 + lane / per) * BN + part * rows) / p.S;
+        const bool there = i0 + lane / per < sg.n && at < p.M;
+        return there ? page_number(p.table, p.t64, b * p.tsb + at) : -1;
+      };
+      int64_t next = lookup(0);
+      int page = -1;
+      for (int i = 0; i < sg.n; ++i, ++j) {
+        const int in = i % batch;
+        if (in == 0) {
+          page = next >= 0 && next < p.P ? static_cast<int>(next) : -1;
+          next = lookup(i + batch);
+        }
+        const int row = static_cast<int>(static_cast<unsigned>(sg.tile0 + i) * BN % p.S);  // 0 for pages within a tile
+        const int sk = j % NK, sv = j % NV;
+        if (j >= NK) ok = __all_sync(0xffffffffu, mbar_wait(k_empty + sk, ((j / NK) & 1) ^ 1, p.status));
+        if (!ok) break;
+        if (lane == 0) mbar_expect_tx(k_full + sk, L::TILE);
+        __syncwarp();
+        if (lane / per == in) tma_load_3d(sK + sk * L::TILE + part * rows * C, &tm, k_full + sk, 0, row, page);
+        if (j >= NV) ok = __all_sync(0xffffffffu, mbar_wait(v_empty + sv, ((j / NV) & 1) ^ 1, p.status));
+        if (!ok) break;
+        if (lane == 0) mbar_expect_tx(v_full + sv, L::TILE);
+        __syncwarp();
+        if (lane / per == in) tma_load_3d(sV + sv * L::TILE + part * rows * C, &tm, v_full + sv, C, row, page);
       }
-      const int row = static_cast<int>((static_cast<int64_t>(tile0 + j) * BN) % p.S);  // 0 for pages within a tile
-      const int sk = j % NK, sv = j % NV;
-      if (j >= NK) ok = __all_sync(0xffffffffu, mbar_wait(k_empty + sk, ((j / NK) & 1) ^ 1, p.status));
-      if (!ok) break;
-      if (lane == 0) mbar_expect_tx(k_full + sk, L::TILE);
-      __syncwarp();
-      if (lane / per == in) tma_load_3d(sK + sk * L::TILE + part * rows * C, &tm, k_full + sk, 0, row, mine);
-      if (j >= NV) ok = __all_sync(0xffffffffu, mbar_wait(v_empty + sv, ((j / NV) & 1) ^ 1, p.status));
-      if (!ok) break;
-      if (lane == 0) mbar_expect_tx(v_full + sv, L::TILE);
-      __syncwarp();
-      if (lane / per == in) tma_load_3d(sV + sv * L::TILE + part * rows * C, &tm, v_full + sv, C, row, mine);
     }
   } else if (warp == 6) {
+    if constexpr (L::CTAS == 2) setmaxnreg_dec<PAGED_REGS_OTHERS>();
     // ------------------------------------- scales: a lane a block, four tiles at a time
-    auto lookup = [&](int j0) {
-      float4 r = make_float4(0.f, 0.f, 0.f, 0.f);  // key scale, log2 of the value scale, its inverse, 1: there
-      const int j = j0 + (lane >> 3);
-      const int64_t n = static_cast<int64_t>(tile0 + j) * BN + (lane & 7) * PAGE_BLOCK;
-      if (j >= ntiles || n / p.S >= p.M) return r;
-      const int64_t page = page_of(p.table, p.t64, b * p.tsb + n / p.S, p.P);
-      if (page < 0) return r;
-      const float* at = p.scales + page * p.scp + (n % p.S) / PAGE_BLOCK * 2;
-      r.x = at[0];
-      // 2^-60 at least: what is scaled by less (0: an empty block) is nothing; over 2^60: NaN
-      const float v = at[1];
-      r.y = v < power_of_two(SCALE_LEAST) && v >= 0.f ? static_cast<float>(SCALE_LEAST)
-            : v <= power_of_two(60)                   ? log2f(v)
-                                                      : __int_as_float(0x7fffffff);
-      r.z = fast_exp2(-r.y);
-      r.w = 1.f;
-      return r;
-    };
-    float4 mine = lookup(0), next = lookup(4);
     bool ok = true;
-    for (int j = 0; ok && j < ntiles; ++j) {
-      if ((j & 3) == 0 && j > 0) {
-        mine = next;
-        next = lookup(j + 4);
+    int j = 0;
+    while (ok && sg.next()) {
+      const int b = (gbase + sg.g) / p.groups_per_row;
+      // page numbers are loaded two batches ahead, scales one
+      auto number = [&](int i0) {
+        const unsigned at = (static_cast<unsigned>(sg.tile0 + i0 + (lane >> 3)) * BN + (lane & 7) * PAGE_BLOCK) / p.S;
+        const bool there = i0 + (lane >> 3) < sg.n && at < p.M;
+        return there ? page_number(p.table, p.t64, b * p.tsb + at) : -1;
+      };
+      auto pair = [&](int i0, int64_t page) {
+        if (page < 0 || page >= p.P) return make_float2(0.f, -1.f);  // no page
+        const unsigned n = static_cast<unsigned>(sg.tile0 + i0 + (lane >> 3)) * BN + (lane & 7) * PAGE_BLOCK;
+        const float* at = p.scales + page * p.scp + n % p.S / PAGE_BLOCK * 2;
+        return make_float2(at[0], at[1]);
+      };
+      int64_t page = number(0);
+      float2 raw = pair(0, page);
+      bool there = page >= 0 && page < p.P;
+      page = number(4);
+      float4 mine;
+      for (int i = 0; i < sg.n; ++i, ++j) {
+        if ((i & 3) == 0) {
+          // key scale; log2 of the value scale, 2^-60 at least (what is scaled by less, as the 0 of an empty
+          // block, is nothing), NaN over 2^60; its inverse; 1: there
+          const float v = raw.y;
+          mine.x = raw.x;
+          mine.y = v < power_of_two(SCALE_LEAST) && v >= 0.f ? static_cast<float>(SCALE_LEAST)
+                   : v <= power_of_two(60)                   ? log2f(v)
+                                                             : __int_as_float(0x7fffffff);
+          mine.z = mine.y == mine.y ? fast_exp2(-mine.y) : 1.f;  // (a NaN is in the exponents that are read)
+          mine.w = 1.f;
+          if (!there) mine = make_float4(0.f, 0.f, 0.f, 0.f);
+          raw = pair(i + 4, page);
+          there = page >= 0 && page < p.P;
+          page = number(i + 8);
+        }
+        // the slot of tile j - 2 is free once its P V is done (its scores' phase, which this arrival must not
+        // fall into, ended before)
+        if (j >= 2)
+          ok = __all_sync(0xffffffffu, mbar_wait(v_empty + (j - 2) % NV, ((j - 2) / NV) & 1, p.status));
+        if (!ok) break;
+        if ((lane >> 3) == (i & 3)) s_scale[(j & 1) * 8 + (lane & 7)] = mine;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(s_full + (j & 1));
       }
-      const int st = j % NV;
-      if (j >= NV) ok = __all_sync(0xffffffffu, mbar_wait(v_empty + st, ((j / NV) & 1) ^ 1, p.status));
-      if (!ok) break;
-      if ((lane >> 3) == (j & 3)) s_scale[st * 8 + (lane & 7)] = mine;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(sc_full + st);
     }
   } else if (warp == 4) {
+    if constexpr (L::CTAS == 2) setmaxnreg_dec<PAGED_REGS_OTHERS>();
     // --------------------------------------------------------- MMA issuer
     constexpr uint32_t IDESC_S = idesc_f8(128, 2 * NCOL, 0, 0, 0, 0);
     constexpr uint32_t IDESC_O = idesc_f8(128, 3 * NCOL, 0, 1, 1, 1);
     const uint32_t tS = tmem, tO = tmem + 2 * L::S_COLS;
     const uint32_t k_addr = smem_u32(sK), v_addr = smem_u32(sV);
     const uint64_t dq = sdesc_sw128(smem_u32(sQ), 16, 1024);
-    const uint64_t dp = sdesc_sw128(smem_u32(sP), BN * 128, 1024);
+    const uint32_t p_addr = smem_u32(sP);
     auto wait = [&](uint64_t* bar, int parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status)); };
-    bool ok = wait(q_full, 0);
-    for (int j = 0; ok && j <= ntiles; ++j) {
-      if (j < ntiles) {
-        const int st = j % NK;
-        if (!(ok = wait(k_full + st, (j / NK) & 1))) break;
-        tc_fence_after();
-        paged_s_steps<3>(tS + (j & 1) * L::S_COLS, sdesc_sw128(k_addr + st * L::TILE, 16, 1024), dq, IDESC_S);
-        mma_commit_warp(s_full + (j & 1));
-        mma_commit_warp(k_empty + st);
-      }
-      if (j > 0) {
-        const int jp = j - 1, st = jp % NV;
-        if (!(ok = wait(v_full + st, (jp / NV) & 1))) break;
-        if (!(ok = wait(p_ready, jp & 1))) break;
-        tc_fence_after();
-        paged_pv_steps<3>(tO, sdesc_sw128(v_addr + st * L::TILE, BN * 128, 1024), dp, IDESC_O, jp > 0 ? 1u : 0u);
-        mma_commit_warp(v_empty + st);
-        mma_commit_warp(o_done);
+    bool ok = true;
+    int j = 0, nseg = 0;
+    while (ok && sg.next()) {
+      ok = wait(q_full, nseg++ & 1);
+      for (int i = 0; ok && i <= sg.n; ++i) {
+        if (i < sg.n) {
+          const int st = j % NK;
+          if (!(ok = wait(k_full + st, (j / NK) & 1))) break;
+          tc_fence_after();
+          paged_s_steps<3>(tS + (j & 1) * L::S_COLS, sdesc_sw128(k_addr + st * L::TILE, 16, 1024), dq, IDESC_S);
+          mma_commit_warp(s_full + (j & 1));
+          mma_commit_warp(k_empty + st);
+          ++j;
+        }
+        if (i > 0) {
+          const int jp = i < sg.n ? j - 2 : j - 1, st = jp % NV;
+          if (!(ok = wait(v_full + st, (jp / NV) & 1))) break;
+          if (!(ok = wait(p_ready + (jp & 1), (jp >> 1) & 1))) break;
+          tc_fence_after();
+          paged_pv_steps<3>(tO, sdesc_sw128(v_addr + st * L::TILE, BN * 128, 1024),
+                            sdesc_sw128(p_addr + (jp & 1) * L::P_BYTES, BN * 128, 1024), IDESC_O, i > 1 ? 1u : 0u);
+          mma_commit_warp(v_empty + st);
+          mma_commit_warp(o_done);
+        }
       }
     }
+  } else if (warp == 7) {
+    if constexpr (L::CTAS == 2) setmaxnreg_dec<PAGED_REGS_OTHERS>();
   } else {
+    if constexpr (L::CTAS == 2) setmaxnreg_inc<PAGED_REGS_SOFTMAX>();
     const int r = threadIdx.x;
-    // ------------------------------------------- q: hi and lo rows, a warp a column
-    for (int col = warp; col < NCOL; col += 4) {
-      uint2 raw = make_uint2(0u, 0u);
-      if (col < ncols) raw = *reinterpret_cast<const uint2*>(p.q + (row0 + col) * C + lane * 4);
-      const float x[4] = {__uint_as_float(raw.x << 16), __uint_as_float(raw.x & 0xffff0000u),
-                          __uint_as_float(raw.y << 16), __uint_as_float(raw.y & 0xffff0000u)};
-      uint32_t top = 0u;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) top = max(top, __float_as_uint(x[k]) & 0x7fffffffu);
-      top = __reduce_max_sync(0xffffffffu, top);
-      const bool finite = top < 0x7f800000u;
-      const int e = finite ? scale_exponent(top, -100) : 0;
-      const float inv = power_of_two(-e);
-      float hi[4], lo[4];
-      uint32_t packed_hi = 0u, packed_lo = 0u;
-      if (finite) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) hi[k] = x[k] * inv;
-        packed_hi = pack_e4m3x4(hi[0], hi[1], hi[2], hi[3]);
-        const uint32_t u = unpack_e4m3x2(packed_hi & 0xffffu), w = unpack_e4m3x2(packed_hi >> 16);
-        lo[0] = (hi[0] - half_lo(u)) * 16.f;
-        lo[1] = (hi[1] - half_hi(u)) * 16.f;
-        lo[2] = (hi[2] - half_lo(w)) * 16.f;
-        lo[3] = (hi[3] - half_hi(w)) * 16.f;
-        packed_lo = pack_e4m3x4(lo[0], lo[1], lo[2], lo[3]);
-      }
-      const uint32_t chunk = lane >> 2, in = (lane & 3) * 4;
-      *reinterpret_cast<uint32_t*>(sQ + sw128_offset(col, chunk) + in) = packed_hi;
-      *reinterpret_cast<uint32_t*>(sQ + sw128_offset(NCOL + col, chunk) + in) = packed_lo;
-      // a query with an infinity or NaN has no result but NaN
-      if (lane == 0)
-        s_col[col].x = finite ? power_of_two(e) * p.scale_log2 : __int_as_float(0x7fffffff);
-    }
-    fence_proxy_async();
-    mbar_arrive(q_full);
-    named_barrier(1, 128);  // s_col
-
-    // --------------------------------------------------- softmax: thread r = key r
     const uint32_t lane_addr = tmem + (static_cast<uint32_t>(warp * 32) << 16);
     const uint32_t tO = lane_addr + 2 * L::S_COLS;
     const uint64_t head_bits = p.H >= 64 ? ~0ull : ((1ull << p.H) - 1);
-    const uint64_t all_cols = ncols >= 64 ? ~0ull : ((1ull << ncols) - 1);
-    const int alo = s_range[2], ahi = s_range[3];
-    float lp[NCOL];
+    // A segment's queries: each warp's columns (warp, warp + 4, ...), four channels a lane, and a lane's
+    // positions, loaded while the segment before ends.
+    uint2 ahead_q[NCOL / 4];
+    int64_t ahead_pos[2];
+    Segments nx = sg;
+    bool more = nx.next();
+    auto load_ahead = [&]() {
+      const int group = gbase + nx.g, b = group / p.groups_per_row, t0 = (group - b * p.groups_per_row) * p.TQ;
+      const int TQg = min(p.TQ, p.T - t0), ncols = TQg * p.H;
+      const int64_t query = static_cast<int64_t>(b) * p.T + t0;
+      const __nv_bfloat16* q = p.q + query * p.H * C + lane * 4;
 #pragma unroll
-    for (int c = 0; c < NCOL; ++c) lp[c] = 0.f;
+      for (int i = 0; i < NCOL / 4; ++i)
+        if (warp + 4 * i < ncols) ahead_q[i] = *reinterpret_cast<const uint2*>(q + (warp + 4 * i) * C);
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        if (lane + 32 * k < TQg) ahead_pos[k] = p.positions[query + lane + 32 * k];
+    };
+    if (more) load_ahead();
     bool ok = true;
-    for (int j = 0; j < ntiles; ++j) {
-      const int st = j % NV;
-      ok = __all_sync(0xffffffffu, mbar_wait(sc_full + st, (j / NV) & 1, p.status));
-      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(s_full + (j & 1), (j >> 1) & 1, p.status));
-      tc_fence_after();
-      const float4 sc = s_scale[st * 8 + (r >> 4)];
-      const int n0 = (tile0 + j) * BN;
-      float s[NCOL];
-      {
-        const uint32_t sa = lane_addr + (j & 1) * L::S_COLS;
-        if constexpr (NCOL == 16) {
-          uint32_t x[32];
-          tmem_ld32(sa, x);
+    int j = 0;
+    while (ok && more) {
+      sg = nx;
+      const int group = gbase + sg.g, b = group / p.groups_per_row, t0 = (group - b * p.groups_per_row) * p.TQ;
+      const int TQg = min(p.TQ, p.T - t0), ncols = TQg * p.H;
+      const int64_t row0 = (static_cast<int64_t>(b) * p.T + t0) * p.H;
+      const uint64_t all_cols = ncols >= 64 ? ~0ull : ((1ull << ncols) - 1);
+      // each query's rows, and those that all of them read
+      int alo = 0, ahi = INT_MAX;
 #pragma unroll
-          for (int c = 0; c < 16; ++c) s[c] = fmaf(__uint_as_float(x[16 + c]), 0.0625f, __uint_as_float(x[c]));
-        } else {
-#pragma unroll
-          for (int c0 = 0; c0 < NCOL; c0 += 32) {
-            uint32_t x[32], y[32];
-            tmem_ld32x2(sa + c0, sa + NCOL + c0, x, y);
-#pragma unroll
-            for (int c = 0; c < 32; ++c) s[c0 + c] = fmaf(__uint_as_float(y[c]), 0.0625f, __uint_as_float(x[c]));
+      for (int k = 0; k < 2; ++k) {
+        const int tq = lane + 32 * k;
+        if (tq < TQg) {
+          int lo, hi;
+          paged_rows(p, ahead_pos[k], lo, hi);
+          if (warp == 0) {
+            s_qlo[tq] = lo;
+            s_qhi[tq] = hi;
           }
+          alo = max(alo, lo);
+          ahi = min(ahi, hi);
         }
       }
-      // exponents relative to the columns' bases; a row that nothing masks keeps padding columns too
-      uint64_t vis = ~0ull;
-      const bool inside = n0 >= alo && n0 + BN - 1 <= ahi;
-      if (!inside) {
-        const int row = n0 + r;
-        vis = 0ull;
-        for (int tq = 0; tq < TQg; ++tq)
-          if (row >= s_qlo[tq] && row <= s_qhi[tq]) vis |= head_bits << (tq * p.H);
-        if (vis == all_cols) vis = ~0ull;
+      alo = __reduce_max_sync(0xffffffffu, alo);
+      ahi = __reduce_min_sync(0xffffffffu, ahi);
+      // q: the group's largest value, then hi and lo rows. A query with an infinity or NaN has no result but NaN.
+      uint32_t top_q = 0u;
+#pragma unroll
+      for (int i = 0; i < NCOL / 4; ++i) {
+        const int col = warp + 4 * i;
+        if (col >= ncols) ahead_q[i] = make_uint2(0u, 0u);
+        const uint2 raw = ahead_q[i];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t bits = (((k & 2) ? raw.y : raw.x) << ((k & 1) ? 0 : 16)) & 0x7fff0000u;
+          top_q = max(top_q, bits < 0x7f800000u ? bits : 0u);
+        }
       }
-      if (sc.w == 0.f) vis = 0ull;
-      bool raise = false;
+      top_q = __reduce_max_sync(0xffffffffu, top_q);
+      if (lane == 0) s_sum[warp] = static_cast<int>(top_q);
+      named_barrier(1, 128);
+      top_q = max(max(s_sum[0], s_sum[1]), max(s_sum[2], s_sum[3]));
+      const int e_q = scale_exponent(top_q, -100);
+      const float inv_q = power_of_two(-e_q), factor = power_of_two(e_q) * p.scale_log2;
 #pragma unroll
-      for (int c = 0; c < NCOL; ++c) {
-        const float4 col = s_col[c];
-        s[c] = fmaf(s[c] * sc.x, col.x, sc.y) - col.y;
-        if (vis != ~0ull && !((vis >> c) & 1ull)) s[c] = -INFINITY;
-        raise |= s[c] > col.z;
+      for (int i = 0; i < NCOL / 4; ++i) {
+        const int col = warp + 4 * i;
+        const uint2 raw = ahead_q[i];
+        float x[4] = {__uint_as_float(raw.x << 16), __uint_as_float(raw.x & 0xffff0000u),
+                      __uint_as_float(raw.y << 16), __uint_as_float(raw.y & 0xffff0000u)};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const bool finite = (__float_as_uint(x[k]) & 0x7fffffffu) < 0x7f800000u;
+          x[k] = finite ? x[k] * inv_q : __int_as_float(0x7fffffff);
+        }
+        const uint32_t hi = pack_e4m3x4(x[0], x[1], x[2], x[3]);
+        const uint32_t u = unpack_e4m3x2(hi & 0xffffu), w = unpack_e4m3x2(hi >> 16);
+        const uint32_t lo = pack_e4m3x4((x[0] - half_lo(u)) * 16.f, (x[1] - half_hi(u)) * 16.f,
+                                        (x[2] - half_lo(w)) * 16.f, (x[3] - half_hi(w)) * 16.f);
+        const uint32_t chunk = lane >> 2, in = (lane & 3) * 4;
+        *reinterpret_cast<uint32_t*>(sQ + sw128_offset(col, chunk) + in) = hi;
+        *reinterpret_cast<uint32_t*>(sQ + sw128_offset(NCOL + col, chunk) + in) = lo;
       }
-      // values that nothing may read hold nothing; one that some columns may read and that holds NaN is taken
-      // out of the product and noted for those columns
-      if (vis != ~0ull) {
-        if (ok) ok = mbar_wait(v_full + st, (j / NV) & 1, p.status);
-        uint8_t* vr = sV + st * L::TILE + r * 128;
-        bool clear = vis == 0ull;
-        if (!clear && ok) {
-          uint32_t bits[4] = {0u, 0u, 0u, 0u};
-          for (int ch = 0; ch < 32; ++ch) {
-            const uint32_t w = *reinterpret_cast<const uint32_t*>(vr + (((ch >> 2) ^ (r & 7)) << 4) + (ch & 3) * 4);
+      fence_proxy_async();
+      mbar_arrive(q_full);
+      named_barrier(1, 128);  // s_qlo, s_qhi; s_sum is read
+
+      // softmax: thread r = key r. Pairs of columns: minus bases (in registers, or shared memory), sums, exponents
+      uint64_t nb[L::IN_REGS ? NCOL / 2 : 1], lp[NCOL / 2], e[NCOL / 2];
+      auto two = [](const float* at, int i) { return reinterpret_cast<const uint64_t*>(at)[i]; };
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if (((w >> (8 * k)) & 0x7fu) == 0x7fu) bits[ch >> 3] |= 1u << ((ch & 7) * 4 + k);
-          }
-          if (bits[0] | bits[1] | bits[2] | bits[3]) {
-            clear = true;
-            s_range[4] = 1;
-            for (int c = 0; c < ncols; ++c)
-              if ((vis >> c) & 1ull)
-                for (int k = 0; k < 4; ++k) atomicOr(s_nan + c * 4 + k, bits[k]);
-          }
+      for (int i = 0; i < NCOL / 2; ++i) lp[i] = 0ull;
+      for (int i = 0; i < sg.n; ++i, ++j) {
+        ok = __all_sync(0xffffffffu, mbar_wait(s_full + (j & 1), (j >> 1) & 1, p.status));
+        tc_fence_after();
+        const float4 sc = s_scale[(j & 1) * 8 + (r >> 4)];
+        const float fk = sc.x * factor;
+        const uint64_t ks = f2_pack(fk, fk), lv = f2_pack(sc.y, sc.y);
+        // which columns read this key; ~0 (padding columns too) where all do
+        const int n0 = (sg.tile0 + i) * BN;
+        uint64_t vis = ~0ull;
+        if (n0 < alo || n0 + BN - 1 > ahi) {
+          const int row = n0 + r;
+          vis = 0ull;
+          for (int tq = 0; tq < TQg; ++tq)
+            if (row >= s_qlo[tq] && row <= s_qhi[tq]) vis |= head_bits << (tq * p.H);
+          if (vis == all_cols) vis = ~0ull;
         }
-        if (clear && ok)
-          for (int ch = 0; ch < 8; ++ch) *reinterpret_cast<uint4*>(vr + ch * 16) = make_uint4(0u, 0u, 0u, 0u);
-      }
-      // the lazy maximum, as in the key-stream kernel: most tiles raise no column's
-      if (named_barrier_or(1, 128, raise || !ok)) {
-#pragma unroll
-        for (int c32 = 0; c32 < (NCOL + 31) / 32; ++c32) {
-          float tmp[32];
-#pragma unroll
-          for (int c = 0; c < 32; ++c) tmp[c] = (c32 * 32 + c < NCOL) ? s[(c32 * 32 + c) % NCOL] : -INFINITY;
-          const float m = transpose_reduce32(tmp, MaxOp());
-          if (c32 * 32 + lane < NCOL) s_red[warp * NCOL + c32 * 32 + lane] = m;
-        }
-        ok = named_barrier_and(1, 128, ok);
-        if (!ok) break;
-        if (r < NCOL) {
-          const float top = fmaxf(fmaxf(s_red[r], s_red[NCOL + r]), fmaxf(s_red[2 * NCOL + r], s_red[3 * NCOL + r]));
-          const float4 col = s_col[r];
-          float2 a = make_float2(1.f, 0.f);
-          if (top > col.z) {
-            a.y = top - PAGED_UP;
-            if (col.z != -INFINITY) a.x = fast_exp2(-a.y);  // else nothing was added up yet
-            s_col[r] = make_float4(col.x, col.y + a.y, PAGED_UP + PAGED_SLACK, 0.f);
-          }
-          s_alpha[r] = a;
-        }
-        named_barrier(1, 128);
-        bool any = false;
-#pragma unroll
-        for (int c = 0; c < NCOL; ++c) {
-          const float2 a = s_alpha[c];
-          s[c] -= a.y;
-          lp[c] *= a.x;
-          any |= a.x != 1.f;
-        }
-        if (any && j > 0) {
-          ok = __all_sync(0xffffffffu, mbar_wait(o_done, (j - 1) & 1, p.status));
-          if (ok) {
-            tc_fence_after();
-#pragma unroll
-            for (int c0 = 0; c0 < L::O_COLS; c0 += 16) {
-              uint32_t x[16];
-              tmem_ld16(tO + c0, x);
-#pragma unroll
-              for (int c = 0; c < 16; ++c)
-                x[c] = __float_as_uint(__uint_as_float(x[c]) * s_alpha[(c0 + c) % NCOL].x);
-              tmem_st16(tO + c0, x);
+        if (sc.w == 0.f) vis = 0ull;
+        // A value that no column may read is 0 in the product; where only some may (drafts that come before it do
+        // not), a NaN in it is taken out of the product and noted for those columns.
+        if (vis != ~0ull) {
+          if (ok) ok = mbar_wait(v_full + j % NV, (j / NV) & 1, p.status);
+          uint8_t* vr = sV + j % NV * L::TILE + r * 128;
+#pragma unroll 1
+          for (int ch = 0; ok && ch < 32; ++ch) {  // four channels each
+            uint32_t* at = reinterpret_cast<uint32_t*>(vr + (((ch >> 2) ^ (r & 7)) << 4) + (ch & 3) * 4);
+            const uint32_t w = *at;
+            const uint32_t nan = __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu);
+            if (vis == 0ull) {
+              *at = 0u;
+            } else if (nan != 0u) {
+              *at = w & ~nan;
+              *s_any_nan = 1;
+              const uint32_t bits = ((nan & 1u) | (nan >> 7 & 2u) | (nan >> 14 & 4u) | (nan >> 21 & 8u)) << (ch & 7) * 4;
+              for (int c = 0; c < ncols; ++c)
+                if ((vis >> c) & 1ull) atomicOr(s_nan + c * 4 + (ch >> 3), bits);
             }
-            tmem_wait_st();
           }
         }
-      }
-      // weights, their sums, and their three parts
+        __syncwarp();
+        // The maximum is lazy, as in the key-stream kernel: a column's base changes only when a score is PAGED_TOP past
+        // it. A segment's first tile sets the bases, each warp a quarter of them, to the maxima of its own 32 keys; a
+        // tile with a score past its column's bound is taken twice, that column's base being its maximum then. What
+        // is run once in a segment is kept short: such code is fetched anew each time. (A wait that failed is
+        // carried to the barriers, where all warps agree to stop.)
+        const uint32_t sa = lane_addr + (j & 1) * L::S_COLS;
+        auto score = [&](uint32_t hi, uint32_t lo) {
+          return fmaf(fmaf(__uint_as_float(lo), 0.0625f, __uint_as_float(hi)), fk, sc.y);
+        };
+        if (i == 0) {
+#pragma unroll 1
+          for (int c = warp * (NCOL / 4); c < (warp + 1) * (NCOL / 4); c += 4) {
+            uint32_t x[4], y[4];
+            tmem_ld4x2(sa + c, sa + NCOL + c, x, y);
+            float m[4];
 #pragma unroll
-      for (int c = 0; c < NCOL; ++c) {
-        s[c] = fast_exp2(s[c]);
-        lp[c] = fmaf(s[c], sc.z, lp[c]);
-      }
-      // a row without a value scale adds nothing (its inverse is 0 too)
-      if (j > 0 && ok) ok = __all_sync(0xffffffffu, mbar_wait(o_done, (j - 1) & 1, p.status));  // P's buffer is free
-      if (ok) {
-#pragma unroll
-        for (int c0 = 0; c0 < NCOL; c0 += 16) {
-          uint32_t part[3][4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            uint32_t x = pack_half2(s[c0 + 4 * k], s[c0 + 4 * k + 1]);
-            uint32_t y = pack_half2(s[c0 + 4 * k + 2], s[c0 + 4 * k + 3]);
-#pragma unroll
-            for (int i = 0; i < 3; ++i) part[i][k] = __byte_perm(e5m2_part(x), e5m2_part(y), 0x7531);
+            for (int k = 0; k < 4; ++k) {
+              m[k] = warp_max((vis >> (c + k)) & 1ull ? score(x[k], y[k]) : -INFINITY);
+              m[k] = m[k] == -INFINITY ? PAGED_UNSET : -m[k];
+            }
+            if (lane == 0) *reinterpret_cast<float4*>(s_base + c) = make_float4(m[0], m[1], m[2], m[3]);
           }
+          if (r == 0) bulk_wait_read();  // the segment before has left P's buffers
+          named_barrier(1, 128);
+        }
+        bool stop = false;
+        for (int pass = 0;; ++pass) {
+          // the exponents s + lv - base
+          if (L::IN_REGS && (pass != 0 || i == 0)) {
 #pragma unroll
-          for (int i = 0; i < 3; ++i) {
-            const int at = i * NCOL + c0;  // the column's byte in the key's row
-            *reinterpret_cast<uint4*>(sP + (at >> 7) * (BN * 128) + sw128_offset(r, (at & 127) >> 4)) =
-                make_uint4(part[i][0], part[i][1], part[i][2], part[i][3]);
+            for (int k = 0; k < NCOL / 2; ++k) nb[L::IN_REGS ? k : 0] = two(s_base, k);
           }
+          const uint64_t low = f2_pack(0.0625f, 0.0625f);
+#pragma unroll
+          for (int c0 = 0; c0 < NCOL; c0 += 16) {
+            uint32_t x[16], y[16];
+            tmem_ld16x2(sa + c0, sa + NCOL + c0, x, y);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const int at = c0 / 2 + k;
+              const uint64_t nbase = L::IN_REGS ? nb[L::IN_REGS ? at : 0] : two(s_base, at);
+              const uint64_t t = f2_fma(f2_pack(__uint_as_float(y[2 * k]), __uint_as_float(y[2 * k + 1])), low,
+                                        f2_pack(__uint_as_float(x[2 * k]), __uint_as_float(x[2 * k + 1])));
+              e[at] = f2_fma(t, ks, f2_add(lv, nbase));
+            }
+          }
+          if (vis != ~0ull) {
+#pragma unroll
+            for (int k = 0; k < NCOL / 2; ++k) {
+              float x, y;
+              f2_unpack(e[k], x, y);
+              e[k] = f2_pack((vis >> (2 * k)) & 1ull ? x : -INFINITY, (vis >> (2 * k + 1)) & 1ull ? y : -INFINITY);
+            }
+          }
+          if (pass == 1) break;
+          float top = -INFINITY;
+#pragma unroll
+          for (int k = 0; k < NCOL / 2; ++k) {
+            float x, y;
+            f2_unpack(e[k], x, y);
+            top = fmaxf(fmaxf(x, y), top);
+          }
+          if (!named_barrier_or(1, 128, top > PAGED_TOP || !ok)) break;
+#pragma unroll 1
+          for (int c = 0; c < NCOL; c += 4) {
+            uint32_t x[4], y[4];
+            tmem_ld4x2(sa + c, sa + NCOL + c, x, y);
+            const float4 base = *reinterpret_cast<const float4*>(s_base + c);
+            const float past[4] = {base.x, base.y, base.z, base.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float v = score(x[k], y[k]);
+              if (((vis >> (c + k)) & 1ull) && v + past[k] > PAGED_TOP) atomicMax(s_top + c + k, ordered(v));
+            }
+          }
+          stop = !named_barrier_and(1, 128, ok);
+          if (stop) break;
+          if (r < NCOL) {
+            float a = 1.f;
+            if (s_top[r] != INT_MIN) {
+              const float base = -unordered(s_top[r]);
+              if (s_base[r] != PAGED_UNSET) a = fast_exp2(base - s_base[r]);  // else nothing was added up
+              s_base[r] = base;
+              s_top[r] = INT_MIN;
+            }
+            s_alpha[r] = a;
+          }
+          named_barrier(1, 128);
+#pragma unroll
+          for (int k = 0; k < NCOL / 2; ++k) lp[k] = f2_mul(lp[k], two(s_alpha, k));
+          if (i > 0) {
+            ok = __all_sync(0xffffffffu, mbar_wait(o_done, (j - 1) & 1, p.status));
+            if (ok) {
+              tc_fence_after();
+#pragma unroll 1
+              for (int c0 = 0; c0 < L::O_COLS; c0 += 16) {
+                const float* alpha = s_alpha + c0 % NCOL;
+                bool some = false;
+#pragma unroll
+                for (int c = 0; c < 16; ++c) some |= alpha[c] != 1.f;
+                if (!some) continue;
+                uint32_t x[16];
+                tmem_ld16(tO + c0, x);
+#pragma unroll
+                for (int c = 0; c < 16; ++c) x[c] = __float_as_uint(__uint_as_float(x[c]) * alpha[c]);
+                tmem_st16(tO + c0, x);
+              }
+              tmem_wait_st();
+            }
+          }
+        }
+        if (stop) {
+          ok = false;
+          break;
+        }
+        // weights, their sums (a key on no page adds 0 times 0), and as fp16 pairs
+        uint32_t h[NCOL / 2];
+        const uint64_t iv = f2_pack(sc.z, sc.z);
+#pragma unroll
+        for (int k = 0; k < NCOL / 2; ++k) {
+          float x, y;
+          f2_unpack(e[k], x, y);
+          x = fast_exp2(x);
+          y = fast_exp2(y);
+          lp[k] = f2_fma(f2_pack(x, y), iv, lp[k]);
+          h[k] = pack_half2(x, y);
+        }
+        // P's buffer is free: the scores came after tile j - 2's P V
+        {
+          uint8_t* pj = sP + (j & 1) * L::P_BYTES;
+#pragma unroll
+          for (int c0 = 0; c0 < NCOL; c0 += 16) {
+            uint32_t part[3][4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              uint32_t x = h[c0 / 2 + 2 * k], y = h[c0 / 2 + 2 * k + 1];
+#pragma unroll
+              for (int n = 0; n < 2; ++n) part[n][k] = __byte_perm(e5m2_part(x), e5m2_part(y), 0x7531);
+              part[2][k] = __byte_perm(half2_times32(x) + 0x00800080u, half2_times32(y) + 0x00800080u, 0x7531);
+            }
+#pragma unroll
+            for (int n = 0; n < 3; ++n) {
+              const int at = n * NCOL + c0;  // the column's byte in the key's row
+              *reinterpret_cast<uint4*>(pj + (at >> 7) * (BN * 128) + sw128_offset(r, (at & 127) >> 4)) =
+                  make_uint4(part[n][0], part[n][1], part[n][2], part[n][3]);
+            }
+          }
+        }
+        tc_fence_before();
+        fence_proxy_async();
+        mbar_arrive(p_ready + (j & 1));
+      }
+      more = nx.next();
+      if (more) load_ahead();
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(o_done, (j - 1) & 1, p.status));
+      tc_fence_after();
+      // per-column sums over the 128 keys
+#pragma unroll
+      for (int c32 = 0; c32 < (NCOL + 31) / 32; ++c32) {
+        float tmp[32];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          tmp[2 * i] = tmp[2 * i + 1] = 0.f;
+          if (c32 * 16 + i < NCOL / 2) f2_unpack(lp[(c32 * 16 + i) % (NCOL / 2)], tmp[2 * i], tmp[2 * i + 1]);
+        }
+        const float sum = transpose_reduce32(tmp, SumOp());
+        if (c32 * 32 + lane < NCOL) s_red[warp * NCOL + c32 * 32 + lane] = sum;
+      }
+      ok = named_barrier_and(1, 128, ok);
+      // a whole group's result is final; else a part
+      const bool final = balanced ? sg.whole : p.splits == 1;
+      const int64_t seg = static_cast<int64_t>(blockIdx.x) + group;
+      if (r < NCOL) {
+        const float l = (s_red[r] + s_red[NCOL + r]) + (s_red[2 * NCOL + r] + s_red[3 * NCOL + r]);
+        if (p.splits > 1) {
+          s_l[r] = ok ? l : 0.f;
+        } else if (r < ncols && final) {
+          float inv;
+          const float lse = paged_total(l != 0.f ? -s_base[r] : -INFINITY, l, p.sink, r % p.H, inv);
+          s_l[r] = inv;
+          if (ok) p.lse[row0 + r] = lse;
+        } else {
+          s_l[r] = 1.f;
+          if (r < ncols) p.part_ml[seg * NCOL + r] = ok ? make_float2(-s_base[r], l) : make_float2(-INFINITY, 0.f);
+        }
+      }
+      named_barrier(1, 128);
+      // thread r: channel r. The result goes through shared memory, in the P buffers that no product reads any more
+      // (a cluster's to be merged from there), and leaves as one bulk copy.
+      const bool any_nan = *s_any_nan != 0, wide = !final || p.splits > 1;
+#pragma unroll 1
+      for (int c = 0; ok && c < NCOL; c += 4) {
+        uint32_t x[4], y[4], z[4];
+        tmem_ld4x3(tO + c, tO + NCOL + c, tO + 2 * NCOL + c, x, y, z);
+        const float4 l4 = *reinterpret_cast<const float4*>(s_l + c);
+        const float f[4] = {l4.x, l4.y, l4.z, l4.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          float o = __uint_as_float(x[k]) + fmaf(__uint_as_float(z[k]), 0.03125f, __uint_as_float(y[k]));
+          if (any_nan && ((s_nan[(c + k) * 4 + (r >> 5)] >> lane) & 1u)) o = __int_as_float(0x7fffffff);
+          if (wide)
+            reinterpret_cast<float*>(sP)[(c + k) * C + r] = o;
+          else
+            reinterpret_cast<__nv_bfloat16*>(sP)[(c + k) * C + r] = __float2bfloat16_rn(o * f[k]);
+        }
+      }
+      if (p.splits <= 1) {
+        fence_proxy_async();
+        named_barrier(1, 128);
+        if (r == 0 && ok) {
+          if (wide)
+            bulk_store(p.part_o + seg * NCOL * C, sP, ncols * C * 4);
+          else
+            bulk_store(p.out + row0 * C, sP, ncols * C * 2);
+          bulk_commit();
         }
       }
       tc_fence_before();
-      fence_proxy_async();
-      mbar_arrive(p_ready);
-    }
-    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(o_done, (ntiles - 1) & 1, p.status));
-    tc_fence_after();
-    // per-column sums over the 128 keys
+      if (any_nan && more) {  // for the next segment
+        if (r < NCOL) {
 #pragma unroll
-    for (int c32 = 0; c32 < (NCOL + 31) / 32; ++c32) {
-      float tmp[32];
-#pragma unroll
-      for (int c = 0; c < 32; ++c) tmp[c] = (c32 * 32 + c < NCOL) ? lp[(c32 * 32 + c) % NCOL] : 0.f;
-      const float sum = transpose_reduce32(tmp, SumOp());
-      if (c32 * 32 + lane < NCOL) s_red[warp * NCOL + c32 * 32 + lane] = sum;
-    }
-    ok = named_barrier_and(1, 128, ok);
-    if (r < ncols) {
-      const float l = (s_red[r] + s_red[NCOL + r]) + (s_red[2 * NCOL + r] + s_red[3 * NCOL + r]);
-      if (p.cluster > 1) {
-        s_l[r] = ok ? l : 0.f;
-      } else if (p.splits == 1) {
-        float inv;
-        const float lse = paged_total(l != 0.f ? s_col[r].y : -INFINITY, l, p.sink, r % p.H, inv);
-        s_l[r] = inv;
-        if (ok) p.lse[row0 + r] = lse;
-      } else {
-        p.part_ml[seg * NCOL + r] = ok ? make_float2(s_col[r].y, l) : make_float2(-INFINITY, 0.f);
-      }
-    }
-    named_barrier(1, 128);
-    const bool any_nan = s_range[4] != 0;
-    if (ok) {
-#pragma unroll
-      for (int c0 = 0; c0 < NCOL; c0 += 16) {  // thread r: channel r
-        uint32_t x[16], y[16], z[16];
-        tmem_ld16(tO + c0, x);
-        tmem_ld16(tO + NCOL + c0, y);
-        tmem_ld16(tO + 2 * NCOL + c0, z);
-#pragma unroll
-        for (int c = 0; c < 16; ++c) {
-          const int col = c0 + c;
-          float o = __uint_as_float(x[c]) + (__uint_as_float(y[c]) + __uint_as_float(z[c]));
-          if (any_nan && ((s_nan[col * 4 + (r >> 5)] >> lane) & 1u)) o = __int_as_float(0x7fffffff);
-          if (p.cluster > 1) {
-            reinterpret_cast<float*>(sK)[col * C + r] = o;  // the rings hold no tile any more
-          } else if (col < ncols) {
-            if (p.splits == 1) {
-              p.out[(row0 + col) * C + r] = __float2bfloat16_rn(o * s_l[col]);
-            } else {
-              p.part_o[(seg * NCOL + col) * C + r] = o;
-            }
-          }
+          for (int k = 0; k < 4; ++k) s_nan[r * 4 + k] = 0u;
         }
+        if (r == 0) *s_any_nan = 0;
       }
     }
+    if (r == 0) bulk_wait_all();
   }
   tc_fence_before();
   __syncthreads();
@@ -913,17 +1146,22 @@ __global__ void __launch_bounds__(PAGED_THREADS, PagedLayout<NCOL>::CTAS)
     tc_fence_after();
     tmem_dealloc(tmem, L::TMEM_COLS);
   }
-  if (p.cluster > 1)
-    paged_cluster_merge<NCOL>(p, s_col, s_l, reinterpret_cast<const float*>(sK), reinterpret_cast<float*>(sP), row0,
-                              ncols);
+  if (p.splits > 1) {
+    const int b = gbase / p.groups_per_row, t0 = (gbase - b * p.groups_per_row) * p.TQ;
+    paged_cluster_merge<NCOL>(p, s_base, s_l, reinterpret_cast<const float*>(sP), reinterpret_cast<float*>(sK),
+                              (static_cast<int64_t>(b) * p.T + t0) * p.H, min(p.TQ, p.T - t0) * p.H);
+  }
 }
 
-// Splits that wrote partials: one warp a row (query, head), four channels a lane.
+// Balanced: groups in several CTAs, or in none. A warp a row (query, head),
+// four channels a lane; with SPREAD a row's parts go over the 8 warps of a CTA
+// and are added up in shared memory (one long row has a part in every CTA).
+template <bool SPREAD>
 __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedParams p, int ncol) {
   griddep_wait();
-  constexpr int C = 128;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
+  constexpr int C = 128, WARPS = 8, STEP = SPREAD ? WARPS : 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t row = SPREAD ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * WARPS + warp;
   if (row >= static_cast<int64_t>(p.B) * p.T * p.H) return;
   const int64_t query = row / p.H;
   const int h = static_cast<int>(row - query * p.H);
@@ -931,24 +1169,16 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedParams p, i
   const int t = static_cast<int>(query - b * p.T);
   const int64_t group = b * p.groups_per_row + t / p.TQ;
   const int col = (t % p.TQ) * p.H + h;
+  const int2 info = p.info[group];
+  if (info.y == 1) return;  // one CTA had all of it
   float M = -INFINITY, L = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s0 = 0; s0 < p.splits; s0 += 8) {
-    float2 ml[8];
-    float4 o[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      ml[k] = make_float2(-INFINITY, 0.f);
-      o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (s0 + k < p.splits) {
-        const int64_t at = (group * p.splits + s0 + k) * ncol + col;
-        ml[k] = p.part_ml[at];
-        o[k] = *reinterpret_cast<const float4*>(p.part_o + at * C + lane * 4);
-      }
-    }
+  // adds parts (exponents and sums ml, outputs o; a sum of 0: nothing was read, nothing was written)
+  constexpr int MOST = SPREAD ? WARPS : 4;
+  auto add = [&](const float2 (&ml)[MOST], const float4 (&o)[MOST]) {
     float top = M;
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
+    for (int k = 0; k < MOST; ++k)
       if (ml[k].y != 0.f) top = fmaxf(top, ml[k].x);
     if (top != M) {
       const float a = M == -INFINITY ? 0.f : fast_exp2(M - top);
@@ -957,8 +1187,8 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedParams p, i
       M = top;
     }
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      if (ml[k].y == 0.f) continue;  // the split read nothing: its output was not written
+    for (int k = 0; k < MOST; ++k) {
+      if (ml[k].y == 0.f) continue;
       const float w = fast_exp2(ml[k].x - M);
       L = fmaf(w, ml[k].y, L);
       acc.x = fmaf(w, o[k].x, acc.x);
@@ -966,6 +1196,40 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedParams p, i
       acc.z = fmaf(w, o[k].z, acc.z);
       acc.w = fmaf(w, o[k].w, acc.w);
     }
+  };
+  for (int s0 = SPREAD ? warp : 0; s0 < info.y; s0 += MOST * STEP) {
+    float2 ml[MOST];
+    float4 o[MOST];
+#pragma unroll
+    for (int k = 0; k < MOST; ++k) {
+      ml[k] = make_float2(-INFINITY, 0.f);
+      o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (s0 + k * STEP < info.y) {
+        const int64_t at = static_cast<int64_t>(info.x + s0 + k * STEP) * ncol + col;
+        ml[k] = p.part_ml[at];
+        o[k] = *reinterpret_cast<const float4*>(p.part_o + at * C + lane * 4);
+      }
+    }
+    add(ml, o);
+  }
+  if constexpr (SPREAD) {
+    __shared__ float4 s_acc[WARPS][32];
+    __shared__ float2 s_ml[WARPS];
+    s_acc[warp][lane] = acc;
+    if (lane == 0) s_ml[warp] = make_float2(M, L);
+    __syncthreads();
+    if (warp > 0) return;
+    M = -INFINITY;
+    L = 0.f;
+    acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float2 ml[WARPS];
+    float4 o[WARPS];
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      ml[w] = s_ml[w];
+      o[w] = s_acc[w][lane];
+    }
+    add(ml, o);
   }
   float inv;
   const float lse = paged_total(M, L, p.sink, h, inv);

@@ -1765,12 +1765,24 @@ int launch_append(const wpt::AppendParams& p, int interleaved, unsigned blocks, 
 }
 
 template <int NCOL>
-int launch_paged(const CUtensorMap& tm, const wpt::PagedParams& p, int groups, cudaStream_t s) {
+int launch_paged(const CUtensorMap& tm, const wpt::PagedParams& p, int ctas, cudaStream_t s) {
   using L = wpt::PagedLayout<NCOL>;
   static_assert(L::BYTES <= (L::CTAS == 2 ? 115712 : 232448), "paged attention kernel: too much shared memory");
   auto kernel = wpt::paged_kernel<NCOL>;
   if (int rc = allow_smem(kernel, L::BYTES)) return rc;
-  cudaError_t e = launch_dependent(kernel, dim3(groups, p.splits), wpt::PAGED_THREADS, L::BYTES, p.cluster, s, tm, p);
+  // its register split draws on what the block was launched with: fewer would leave the increase waiting
+  static std::atomic<int> regs{0};
+  if (L::CTAS == 2 && regs.load(std::memory_order_relaxed) == 0) {
+    cudaFuncAttributes fa;
+    cudaError_t e = cudaFuncGetAttributes(&fa, kernel);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncGetAttributes(paged_kernel)");
+    regs.store(fa.numRegs, std::memory_order_relaxed);
+  }
+  if (L::CTAS == 2 && regs.load(std::memory_order_relaxed) != wpt::PAGED_REGS)
+    return fail(WPT_ERR_CUDA, "paged_kernel built with %d registers a thread, its register split needs %d",
+                regs.load(std::memory_order_relaxed), wpt::PAGED_REGS);
+  const dim3 grid = p.splits == 0 ? dim3(ctas) : dim3(p.groups, p.splits);
+  cudaError_t e = launch_dependent(kernel, grid, wpt::PAGED_THREADS, L::BYTES, p.splits, s, tm, p);
   if (e != cudaSuccess) return cuda_fail(e, "paged_kernel launch");
   return WPT_OK;
 }
@@ -1889,17 +1901,17 @@ extern "C" int wpt_paged_append(const void* src, int f32, int64_t src_stride_b, 
                  : launch_append<__nv_bfloat16, 1>(p, interleaved, grid, s);
 }
 
-extern "C" size_t wpt_paged_scratch_bytes(int B, int T, int H, int splits) {
-  if (B < 1 || T < 1 || H < 1 || H > 64 || splits < 1) return 0;
+extern "C" size_t wpt_paged_scratch_bytes(int B, int T, int H, int splits, int ctas) {
+  if (B < 1 || T < 1 || H < 1 || H > 64 || splits != 0 || ctas < 1) return 0;
   const int ncol = paged_columns(T, H), TQ = ncol / H;
-  return static_cast<size_t>(B) * ((T + TQ - 1) / TQ) * splits * ncol * (128 * 4 + 8);
+  const size_t groups = static_cast<size_t>(B) * ((T + TQ - 1) / TQ);
+  return (groups + ctas) * ncol * (128 * 4 + 8) + groups * 8;
 }
 
 extern "C" int wpt_paged_attention(const void* q, const void* pages, int64_t page_stride, int64_t entry_stride,
                                    const float* scales, int64_t scales_stride, const void* table, int table_i64,
                                    int64_t table_stride_b, const int64_t* positions, const float* sink, void* out,
-                                   float* lse, void* scratch, int splits, int chunk_tiles, int B, int T, int H, int C,
-                                   int M, int P, int S, int window, float scale, void* stream) {
+                                   float* lse, void* scratch, int splits, int ctas, int B, int T, int H, int C, int M, int P, int S, int window, float scale, void* stream) {
   if (C != 128) return fail(WPT_ERR_UNSUPPORTED, "head width %d: the paged attention kernel takes 128", C);
   if (H < 1 || H > 64) return fail(WPT_ERR_UNSUPPORTED, "%d heads: the paged attention kernel takes 1 to 64", H);
   if (!page_size_ok(S)) return fail(WPT_ERR_UNSUPPORTED, "pages of %d entries: 16, 32, 64 or a multiple of 128", S);
@@ -1907,13 +1919,20 @@ extern "C" int wpt_paged_attention(const void* q, const void* pages, int64_t pag
   if (B == 0 || T == 0) return WPT_OK;
   if (static_cast<int64_t>(M) * S > INT_MAX - 1024) return fail(WPT_ERR_UNSUPPORTED, "a table of %d pages of %d entries", M, S);
   if (static_cast<int64_t>(B) * T >= (int64_t(1) << 31) / H) return fail(WPT_ERR_UNSUPPORTED, "B*T*H too large");
-  if (splits < 1 || chunk_tiles < 1 || splits > 65535) return fail(WPT_ERR_INVALID, "splits and chunk_tiles must be >= 1");
+  if (splits < 0 || splits > 8) return fail(WPT_ERR_INVALID, "%d splits: 1 to 8, or 0 for a balanced call", splits);
   if (!q || !positions || !out || !lse || (M > 0 && P > 0 && (!pages || !scales || !table)))
     return fail(WPT_ERR_INVALID, "a required pointer is NULL");
   if (!aligned16(q) || !aligned16(out) || (scratch && !aligned16(scratch)))
     return fail(WPT_ERR_INVALID, "q, out and scratch must be 16-byte aligned");
-  const bool cluster = splits > 1 && scratch == nullptr;
-  if (cluster && splits > 8) return fail(WPT_ERR_INVALID, "%d splits without scratch: at most 8", splits);
+  const int ncol = paged_columns(T, H), TQ = ncol / H;
+  const int64_t groups = static_cast<int64_t>(B) * ((T + TQ - 1) / TQ);
+  if (splits == 0) {
+    if (!scratch || ctas < 1) return fail(WPT_ERR_INVALID, "a balanced call needs scratch and CTAs");
+    if (groups > wpt::PAGED_GROUPS || groups * ((static_cast<int64_t>(M) * S + 127) / 128 + wpt::PAGED_SEGMENT) >= (int64_t(1) << 31) ||
+        ctas > (1 << 20))
+      return fail(WPT_ERR_UNSUPPORTED, "a balanced call takes up to %d query groups (got %lld) and 2^31 tiles",
+                  wpt::PAGED_GROUPS, static_cast<long long>(groups));
+  }
   CUtensorMap tm;
   memset(&tm, 0, sizeof(tm));
   if (M > 0 && P > 0) {
@@ -1926,7 +1945,6 @@ extern "C" int wpt_paged_attention(const void* q, const void* pages, int64_t pag
     if (int rc = tensor_map(&tm, pages, 3, dims, strides, box, CU_TENSOR_MAP_DATA_TYPE_UINT8)) return rc;
   }
   wpt::PagedParams p;
-  const int ncol = paged_columns(T, H);
   p.q = static_cast<const __nv_bfloat16*>(q);
   p.scales = scales;
   p.scp = scales_stride;
@@ -1945,25 +1963,28 @@ extern "C" int wpt_paged_attention(const void* q, const void* pages, int64_t pag
   p.P = P;
   p.S = S;
   p.window = window;
-  p.TQ = ncol / H;
-  p.groups_per_row = (T + p.TQ - 1) / p.TQ;
+  p.TQ = TQ;
+  p.groups_per_row = (T + TQ - 1) / TQ;
+  p.groups = static_cast<int>(groups);
   p.splits = splits;
-  p.chunk_tiles = chunk_tiles;
-  p.cluster = cluster ? splits : 1;
   p.scale_log2 = scale * wpt::LOG2E;
-  const int64_t groups = static_cast<int64_t>(B) * p.groups_per_row;
+  const int64_t parts = splits == 0 ? groups + ctas : 0;
   p.part_o = static_cast<float*>(scratch);
-  p.part_ml = reinterpret_cast<float2*>(p.part_o + (scratch ? groups * splits * ncol * 128 : 0));
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + parts * ncol * 128);
+  p.info = reinterpret_cast<int2*>(p.part_ml + parts * ncol);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   int rc;
   switch (ncol) {
-    case 16: rc = launch_paged<16>(tm, p, static_cast<int>(groups), s); break;
-    case 32: rc = launch_paged<32>(tm, p, static_cast<int>(groups), s); break;
-    default: rc = launch_paged<64>(tm, p, static_cast<int>(groups), s); break;
+    case 16: rc = launch_paged<16>(tm, p, ctas, s); break;
+    case 32: rc = launch_paged<32>(tm, p, ctas, s); break;
+    default: rc = launch_paged<64>(tm, p, ctas, s); break;
   }
-  if (rc || splits == 1 || cluster) return rc;
+  if (rc || splits != 0) return rc;
   const int64_t rows = static_cast<int64_t>(B) * T * H;
-  cudaError_t e = launch_dependent(wpt::paged_merge_kernel, dim3(static_cast<unsigned>((rows + 7) / 8)), 256, 0, 1, s, p, ncol);
+  // parts of a group: about ctas / groups + 1
+  const bool spread = ctas > 7 * groups;
+  cudaError_t e = launch_dependent(spread ? wpt::paged_merge_kernel<true> : wpt::paged_merge_kernel<false>,
+                                   dim3(static_cast<unsigned>(spread ? rows : (rows + 7) / 8)), 256, 0, 1, s, p, ncol);
   if (e != cudaSuccess) return cuda_fail(e, "paged_merge_kernel launch");
   return WPT_OK;
 }

@@ -1000,8 +1000,8 @@ def paged_append(pages, scales, table, new, first, counts, frequencies=None, pos
 
 
 def _paged_plan(B, T, H, N, window, sms):
-    """(splits, chunk_tiles, cluster) of a paged attention call over rows of up
-    to N entries, remembered per shape."""
+    """(splits, ctas) of a paged attention call over rows of up to N entries,
+    remembered per shape."""
     key = ("paged", B, T, H, N, window, sms)
     plan = _PLAN_CACHE.get(key)
     if plan is None:
@@ -1017,20 +1017,16 @@ def _paged_plan_for(B, T, H, N, window, sms):
     TQ = ncol // H
     groups = B * math.ceil(T / TQ)
     tiles = max(1, math.ceil(N / 128))
-    if window:
+    if window:  # what neighbouring queries reach
         tiles = min(tiles, (window + TQ - 2) // 128 + 2)
     slots = sms * (1 if ncol == 64 else 2)  # CTAs at a time
-    chunk = max(1, min(tiles, 16))
-    if groups * math.ceil(tiles / chunk) > 4 * slots:
-        chunk = min(tiles, 16 * math.ceil(tiles * groups / (4 * slots) / 16))
-    elif groups * math.ceil(tiles / chunk) < slots:
-        chunk = max(1, math.ceil(tiles * groups / slots))
-    splits = math.ceil(tiles / chunk)
-    if 1 < splits and groups * min(splits, 8) <= slots and tiles <= 64:  # one wave of clusters
-        splits = min(splits, 8)
-        chunk = math.ceil(tiles / splits)
-        splits = math.ceil(tiles / chunk)
-    return splits, chunk, 1 < splits <= 8 and groups * splits <= slots
+    # few tiles for few groups: one launch, a group's tiles over a cluster
+    splits = min(8, tiles, max(1, slots // groups))
+    if tiles <= 4 * splits:
+        return splits, 1
+    if groups <= 256 and groups * (math.ceil(N / 128) + 8) < 2 ** 31:
+        return 0, min(slots, groups * tiles)
+    return 1, 1  # more groups than CTAs at a time
 
 
 def paged_attention(q, pages, scales, table, positions, scale, window=0, sink=None):
@@ -1067,15 +1063,15 @@ def paged_attention(q, pages, scales, table, positions, scale, window=0, sink=No
     lse = torch.empty((B, T, H), dtype=torch.float32, device=device)
     if B * T * H == 0:
         return out, lse
-    splits, chunk, cluster = _paged_plan(B, T, H, M * S, window, sm_count(device))
+    splits, ctas = _paged_plan(B, T, H, M * S, window, sm_count(device))
     lib = _lib.lib()
     scratch = None
-    if splits > 1 and not cluster:
-        scratch = torch.empty(lib.wpt_paged_scratch_bytes(B, T, H, splits), dtype=torch.uint8, device=device)
+    if splits == 0:
+        scratch = torch.empty(lib.wpt_paged_scratch_bytes(B, T, H, splits, ctas), dtype=torch.uint8, device=device)
     ps = pages.stride()
     _call(device, lib.wpt_paged_attention,
           (q.data_ptr(), pages.data_ptr(), ps[0], ps[1], scales.data_ptr(), scales.stride(0), table.data_ptr(),
            table.dtype == torch.int64, table.stride(0), positions.data_ptr(), _lib.ptr(sink), out.data_ptr(),
-           lse.data_ptr(), _lib.ptr(scratch), splits, chunk, B, T, H, C, M, P, S, window, scale))
+           lse.data_ptr(), _lib.ptr(scratch), splits, ctas, B, T, H, C, M, P, S, window, scale))
     LAUNCHES[0] += 1 + (scratch is not None)
     return out, lse
