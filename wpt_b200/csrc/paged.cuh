@@ -69,8 +69,10 @@ struct AppendParams {
   const void* frequencies;         // (dims / 2,) or null
   unsigned* status;
   int t64, f64;
-  int B, n, C, M, P, S, dims, start;
+  unsigned S;                      // entries a page
+  int B, n, C, M, P, dims, start;
   int blocks;                      // grid blocks a row
+  int turn_rows, turn_pairs;       // APPEND_THREADS / (dims / 2), and the rest
   float magnitude;
 };
 
@@ -82,17 +84,58 @@ __device__ __forceinline__ int64_t page_of(const void* table, int t64, int64_t a
   return id >= 0 && id < P ? id : -1;
 }
 
+// Where an entry's vector v sits among its key's turned channels: whether it is
+// one of them, its first pair, whether it holds the first channels of its pairs
+// (halves), and how many vectors on its pairs' others are.
+template <int VE, bool INTERLEAVED>
+struct TurnedVector {
+  bool turned, front;
+  int pair, partner;
+  __device__ __forceinline__ TurnedVector(int v, int start, int dims) {
+    const int at = v * VE - start, half = dims >> 1;
+    turned = at >= 0 && at < dims;
+    front = INTERLEAVED || at < half;
+    pair = INTERLEAVED ? at / 2 : front ? at : at - half;
+    partner = !turned || INTERLEAVED ? 0 : front ? half / VE : -half / VE;
+  }
+  // u, widened, turned in place; z: its partner vector, widened (halves); sn, cs: of its pairs
+  __device__ __forceinline__ void turn(float (&u)[VE], const float (&z)[VE], const float* sn, const float* cs) const {
+    if constexpr (INTERLEAVED) {
+#pragma unroll
+      for (int k = 0; k < VE / 2; ++k) {
+        float a, b;
+        turn_pair(u[2 * k], u[2 * k + 1], sn[k], cs[k], a, b);
+        u[2 * k] = a;
+        u[2 * k + 1] = b;
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < VE; ++k) {  // x_a cos - x_b sin, or x_b cos + x_a sin
+        const float s = front ? -sn[k] : sn[k];
+        u[k] = __fadd_rn(__fmul_rn(u[k], cs[k]), __fmul_rn(z[k], s));
+      }
+    }
+  }
+};
+
+constexpr int APPEND_THREADS = 128;
+
 // Appending. One CTA a block of 16 entries (and batch row), so a block's scale
-// needs no exchange: the block's new entries are turned, widened to fp32 in
-// shared memory, their largest value gives the scale, and a second pass
-// rounds them. Bound by HBM for prompts; a step of one entry a row is a chain
-// of three loads (first, the page's number, its scale).
-template <class T, int VE, bool INTERLEAVED>
-__global__ void __launch_bounds__(128) paged_append_kernel(const AppendParams p) {
+// needs no exchange: all threads work out the sines and cosines of its entries
+// (a table in shared memory: 16 x dims / 2 pairs, where the lanes that turn
+// would each compute 8 a token while the others wait), the new entries are
+// turned and widened to fp32, their largest value gives the scale, and they are
+// rounded. ROWS: a warp takes an entry, a lane a vector of it (with halves, the
+// other channels of its pairs come from the lane that loaded them), and the
+// entries stay in registers; else they go through shared memory. Bound by HBM for prompts; a step of one entry a row is a chain of
+// three loads (first, the page's number, its scale).
+template <class T, int VE, bool INTERLEAVED, bool ROWS>
+__global__ void __launch_bounds__(APPEND_THREADS, ROWS ? 8 : 1) paged_append_kernel(const AppendParams p) {
   using V = Vec<T, VE>;
   using Raw = typename V::Raw;
-  extern __shared__ float s_val[];  // (16, 2 C)
-  __shared__ uint32_t s_red[4][2];
+  constexpr int WARPS = APPEND_THREADS / 32;
+  extern __shared__ float s_all[];  // sines and cosines (16, dims / 2), then, unless ROWS, values (16, 2 C)
+  __shared__ uint32_t s_red[WARPS][2];
   griddep_wait();
   const int b = blockIdx.x / p.blocks;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -111,12 +154,47 @@ __global__ void __launch_bounds__(128) paged_append_kernel(const AppendParams p)
   const int64_t begun = lo;  // entries before it are earlier ones
   if (lo < n0) lo = n0;
   if (hi > n0 + PAGE_BLOCK) hi = n0 + PAGE_BLOCK;
-  const int64_t page = page_of(p.table, p.t64, b * p.tsb + n0 / p.S, p.P);
+  const unsigned at_entry = static_cast<unsigned>(n0);  // under the table's capacity
+  const int64_t page = page_of(p.table, p.t64, b * p.tsb + at_entry / p.S, p.P);
+  const int live = static_cast<int>(hi - lo);
+  const int slot0 = static_cast<int>(lo - n0);
+  const int64_t row0 = lo - first;  // the first new entry's number
+  const T* src = static_cast<const T*>(p.src) + b * p.ssb + row0 * p.ssn;
+  const int half = p.dims >> 1;
+  constexpr int MINE = PAGE_BLOCK / WARPS;  // ROWS: entries of a warp: warp, warp + WARPS, ...
+  const int ca = lane * VE;             // and the lane's first channel
+  const bool some = ca < 2 * p.C;
+  Raw raw[MINE];
+  if constexpr (ROWS) {
+#pragma unroll
+    for (int q = 0; q < MINE; ++q)
+      if (some && warp + WARPS * q < live) raw[q] = *reinterpret_cast<const Raw*>(src + (warp + WARPS * q) * p.ssn + ca);
+  }
+  float2* s_turn = reinterpret_cast<float2*>(s_all);
+  float* s_val = s_all + PAGE_BLOCK * p.dims;
+  {
+    int i = half > 0 ? tid / half : live, k = tid - i * half, last = -1;
+    uint64_t turn = 0;
+    while (i < live) {
+      if (k != last) turn = rotate_turn(p.frequencies, p.f64, k);
+      last = k;
+      const int64_t pos = p.positions ? p.positions[static_cast<int64_t>(b) * p.n + row0 + i] : lo + i;
+      float sn, cs;
+      turn_sincos(pos, turn, sn, cs);
+      s_turn[i * half + k] = make_float2(sn * p.magnitude, cs * p.magnitude);
+      i += p.turn_rows;
+      k += p.turn_pairs;
+      if (k >= half) {
+        k -= half;
+        ++i;
+      }
+    }
+  }
   if (page < 0) {
     if (tid == 0) atomicOr(p.status, STATUS_BAD_SHAPE);
     return;
   }
-  const int in_page = static_cast<int>(n0 % p.S);
+  const int in_page = static_cast<int>(at_entry % p.S);
   uint8_t* rows = p.pages + page * p.psp + in_page * p.psr;
   float* scale_at = p.scales + page * p.scp + in_page / PAGE_BLOCK * 2;
   const bool older = n0 < begun;  // the block holds earlier entries
@@ -125,96 +203,178 @@ __global__ void __launch_bounds__(128) paged_append_kernel(const AppendParams p)
     old[0] = scale_at[0];
     old[1] = scale_at[1];
   }
+  if (p.dims > 0) __syncthreads();
 
-  // first pass: turn, widen, largest value
-  constexpr int PAIRS = INTERLEAVED && VE > 1 ? VE / 2 : VE;
-  const int half = p.dims >> 1, turned = half / PAIRS;
-  const int items = turned + (2 * p.C - p.dims) / VE;
-  const int live = static_cast<int>(hi - lo);
-  const int slot0 = static_cast<int>(lo - n0);
-  const T* src = static_cast<const T*>(p.src) + b * p.ssb + (lo - first) * p.ssn;
+  // turned and widened values, and the bits of the largest absolute ones (NaN's above all)
   uint32_t amax[2] = {0u, 0u};
-  auto size = [](float v) {  // |v|'s bits, 0 for what counts as infinite
-    const uint32_t bits = __float_as_uint(v) & 0x7fffffffu;
-    return bits <= SCALE_TOP_BITS ? bits : 0u;
-  };
-  for (int at = tid; at < live * items; at += 128) {
-    const int i = at / items, item = at - i * items;
-    const T* x = src + i * p.ssn;
-    float* out_at = s_val + (slot0 + i) * 2 * p.C;
-    if (item >= turned) {
-      int c = (item - turned) * VE;
-      if (c >= p.start) c += p.dims;
-      float v[VE];
-      V::widen(*reinterpret_cast<const Raw*>(x + c), v);
+  auto note = [](float v, uint32_t& m) { m = max(m, __float_as_uint(v) & 0x7fffffffu); };
+  float u[ROWS ? MINE : 1][VE];
+  if constexpr (ROWS) {
+    const TurnedVector<VE, INTERLEAVED> tv(ca < p.C ? lane : -1 - p.dims, p.start, p.dims);
+    uint32_t m = 0u;
 #pragma unroll
-      for (int k = 0; k < VE; ++k) {
-        out_at[c + k] = v[k];
-        const uint32_t bits = size(v[k]);
-        amax[0] = c < p.C ? max(amax[0], bits) : amax[0];
-        amax[1] = c < p.C ? amax[1] : max(amax[1], bits);
+    for (int q = 0; q < MINE; ++q) {
+      if (warp + WARPS * q >= live) break;  // the whole warp
+      Raw z = raw[q];
+      if constexpr (!INTERLEAVED) z = V::from_lane(raw[q], lane + tv.partner);
+      V::widen(raw[q], u[q]);
+      if (tv.turned) {
+        float c[VE], sn[VE], cs[VE];
+        V::widen(z, c);
+        const float4* at = reinterpret_cast<const float4*>(s_turn + (warp + WARPS * q) * half + tv.pair);
+#pragma unroll
+        for (int k = 0; k < (INTERLEAVED ? VE / 2 : VE); k += 2) {
+          const float4 t = at[k / 2];
+          sn[k] = t.x;
+          cs[k] = t.y;
+          sn[k + 1] = t.z;
+          cs[k + 1] = t.w;
+        }
+        tv.turn(u[q], c, sn, cs);
       }
-    } else {
-      const int64_t row = lo - first + i;
-      const int64_t pos = p.positions ? p.positions[static_cast<int64_t>(b) * p.n + row] : lo + i;
-      constexpr bool ONE = INTERLEAVED && VE > 1;
-      const int ca = p.start + (INTERLEAVED ? 2 * PAIRS : PAIRS) * item;
-      const int cb = INTERLEAVED ? ca + 1 : ca + half;
-      float a[VE], z[VE];
-      V::widen(*reinterpret_cast<const Raw*>(x + ca), a);
-      if constexpr (!ONE) V::widen(*reinterpret_cast<const Raw*>(x + cb), z);
+      if (some) {
 #pragma unroll
-      for (int k = 0; k < PAIRS; ++k) {
-        float sn, cs, u, w;
-        turn_sincos(pos, rotate_turn(p.frequencies, p.f64, item * PAIRS + k), sn, cs);
-        turn_pair(ONE ? a[ONE ? 2 * k : 0] : a[k], ONE ? a[ONE ? 2 * k + 1 : 0] : z[k], sn, cs, u, w);
-        u *= p.magnitude;
-        w *= p.magnitude;
-        out_at[ONE ? ca + 2 * k : ca + k] = u;
-        out_at[ONE ? ca + 2 * k + 1 : cb + k] = w;
-        amax[0] = max(amax[0], max(size(u), size(w)));
+        for (int k = 0; k < VE; ++k) note(u[q][k], m);
       }
     }
-  }
+    amax[0] = ca < p.C ? m : 0u;
+    amax[1] = ca < p.C ? 0u : m;
+  } else {
+    // items: pairs (with VE > 1, vectors of them), then the channels that do not turn
+    constexpr bool ONE = INTERLEAVED && VE > 1;  // an item is one vector of whole pairs
+    constexpr int PAIRS = ONE ? VE / 2 : VE;
+    const int turned = half / PAIRS, items = turned + (2 * p.C - p.dims) / VE;
+    for (int at = tid; at < live * items; at += APPEND_THREADS) {
+      const int i = at / items, item = at - i * items;
+      const T* x = src + i * p.ssn;
+      float* to = s_val + (slot0 + i) * 2 * p.C;
+      uint32_t m = 0u;
+      int c = (item - turned) * VE;
+      if (item >= turned) {
+        if (c >= p.start) c += p.dims;
+        V::widen(*reinterpret_cast<const Raw*>(x + c), u[0]);
+      } else {
+        c = p.start + (INTERLEAVED ? 2 * PAIRS : PAIRS) * item;
+        const int cb = INTERLEAVED ? c + 1 : c + half;
+        float w[VE];
+        V::widen(*reinterpret_cast<const Raw*>(x + c), u[0]);
+        if constexpr (!ONE) V::widen(*reinterpret_cast<const Raw*>(x + cb), w);
 #pragma unroll
-  for (int w = 0; w < 2; ++w) {
-    amax[w] = __reduce_max_sync(0xffffffffu, amax[w]);
-    if (lane == 0) s_red[warp][w] = amax[w];
+        for (int k = 0; k < PAIRS; ++k) {
+          const float2 t = s_turn[i * half + item * PAIRS + k];
+          float& a = u[0][ONE ? 2 * k : k];
+          float& z = ONE ? u[0][ONE ? 2 * k + 1 : 0] : w[k];
+          float y0, y1;
+          turn_pair(a, z, t.x, t.y, y0, y1);
+          a = y0;
+          z = y1;
+        }
+        if constexpr (!ONE) {
+#pragma unroll
+          for (int k = 0; k < VE; ++k) {
+            to[cb + k] = w[k];
+            note(w[k], m);
+          }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < VE; ++k) {
+        to[c + k] = u[0][k];
+        note(u[0][k], m);
+      }
+      amax[0] = max(amax[0], c < p.C ? m : 0u);
+      amax[1] = max(amax[1], c < p.C ? 0u : m);
+    }
   }
-  __syncthreads();
+  auto largest = [&]() {  // of the block, in amax
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t m = __reduce_max_sync(0xffffffffu, amax[h]);
+      if (lane == 0) s_red[warp][h] = m;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) amax[h] = __reduce_max_sync(0xffffffffu, s_red[lane % WARPS][h]);
+  };
+  largest();
+  // infinities, NaN and values past 448 * 2^60 do not count (seldom: looked at again without them), and become NaN
+  const bool huge = max(amax[0], amax[1]) > SCALE_TOP_BITS;
+  auto fits = [](float v) { return (__float_as_uint(v) & 0x7fffffffu) <= SCALE_TOP_BITS; };
+  if (huge) {
+    amax[0] = amax[1] = 0u;
+    uint32_t m = 0u;
+    if constexpr (ROWS) {
+#pragma unroll
+      for (int q = 0; q < MINE; ++q)
+        if (some && warp + WARPS * q < live) {
+#pragma unroll
+          for (int k = 0; k < VE; ++k) {
+            if (fits(u[q][k]))
+              note(u[q][k], m);
+            else
+              u[q][k] = __int_as_float(0x7fffffff);
+          }
+        }
+      amax[0] = ca < p.C ? m : 0u;
+      amax[1] = ca < p.C ? 0u : m;
+    } else {
+      for (int at = tid; at < live * 2 * p.C; at += APPEND_THREADS) {
+        float& v = s_val[slot0 * 2 * p.C + at];
+        if (fits(v))
+          note(v, amax[at % (2 * p.C) < p.C ? 0 : 1]);
+        else
+          v = __int_as_float(0x7fffffff);
+      }
+    }
+    __syncthreads();  // s_red has been read
+    largest();
+  }
   float scale[2], inv[2];
   bool grown[2];
 #pragma unroll
-  for (int w = 0; w < 2; ++w) {
-    const uint32_t m = max(max(s_red[0][w], s_red[1][w]), max(s_red[2][w], s_red[3][w]));
-    scale[w] = power_of_two(scale_exponent(m, SCALE_LEAST));
-    grown[w] = old[w] < scale[w];
-    if (!grown[w]) scale[w] = old[w];
-    inv[w] = 1.f / scale[w];
+  for (int h = 0; h < 2; ++h) {
+    scale[h] = power_of_two(scale_exponent(amax[h], SCALE_LEAST));
+    grown[h] = old[h] < scale[h];
+    if (!grown[h]) scale[h] = old[h];
+    inv[h] = 1.f / scale[h];
   }
-  // second pass: round, four channels a thread
-  const int quads = p.C / 2;
-  for (int at = tid; at < live * quads; at += 128) {
-    const int i = slot0 + at / quads, c = 4 * (at % quads);
-    const float4 v = *reinterpret_cast<const float4*>(s_val + i * 2 * p.C + c);
-    const float f = c >= p.C ? inv[1] : inv[0];
-    float q[4] = {v.x, v.y, v.z, v.w};
+  if constexpr (ROWS) {
+    if (some) {
+      const float f = ca >= p.C ? inv[1] : inv[0];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const bool fits = (__float_as_uint(q[k]) & 0x7fffffffu) <= SCALE_TOP_BITS;
-      q[k] = fits ? q[k] * f : __int_as_float(0x7fffffff);  // infinities and what counts as one: NaN
+      for (int q = 0; q < MINE; ++q)
+        if (warp + WARPS * q < live) {
+          uint32_t out4[VE / 4];
+#pragma unroll
+          for (int k = 0; k < VE; k += 4)
+            out4[k / 4] = pack_e4m3x4(u[q][k] * f, u[q][k + 1] * f, u[q][k + 2] * f, u[q][k + 3] * f);
+          uint8_t* to = rows + (slot0 + warp + WARPS * q) * p.psr + ca;
+          if constexpr (VE == 8)
+            *reinterpret_cast<uint2*>(to) = make_uint2(out4[0], out4[VE / 4 - 1]);
+          else
+            *reinterpret_cast<uint32_t*>(to) = out4[0];
+        }
     }
-    *reinterpret_cast<uint32_t*>(rows + i * p.psr + c) = pack_e4m3x4(q[0], q[1], q[2], q[3]);
+  } else {
+    const int quads = p.C / 2;
+    for (int at = tid; at < live * quads; at += APPEND_THREADS) {
+      const int i = slot0 + at / quads, c = 4 * (at % quads);
+      const float4 v = *reinterpret_cast<const float4*>(s_val + i * 2 * p.C + c);
+      const float f = c >= p.C ? inv[1] : inv[0];
+      *reinterpret_cast<uint32_t*>(rows + i * p.psr + c) =
+          pack_e4m3x4(v.x * f, v.y * f, v.z * f, v.w * f);
+    }
   }
-  if (older) {  // a larger scale: the earlier entries are rounded again
+  if (older && (grown[0] || grown[1])) {  // a larger scale: the earlier entries are rounded again
+    const int quads = p.C / 2;
     const float shrink[2] = {old[0] * inv[0], old[1] * inv[1]};
-    for (int at = tid; at < slot0 * quads; at += 128) {
+    for (int at = tid; at < slot0 * quads; at += APPEND_THREADS) {
       const int i = at / quads, c = 4 * (at % quads);
       if (!(c >= p.C ? grown[1] : grown[0])) continue;
       const float f = c >= p.C ? shrink[1] : shrink[0];
       uint32_t* word = reinterpret_cast<uint32_t*>(rows + i * p.psr + c);
-      const uint32_t x = *word, u = unpack_e4m3x2(x & 0xffffu), w = unpack_e4m3x2(x >> 16);
-      *word = pack_e4m3x4(half_lo(u) * f, half_hi(u) * f, half_lo(w) * f, half_hi(w) * f);
+      const uint32_t x = *word, y = unpack_e4m3x2(x & 0xffffu), z = unpack_e4m3x2(x >> 16);
+      *word = pack_e4m3x4(half_lo(y) * f, half_hi(y) * f, half_lo(z) * f, half_hi(z) * f);
     }
   }
   if (tid == 0) {
@@ -222,7 +382,6 @@ __global__ void __launch_bounds__(128) paged_append_kernel(const AppendParams p)
     scale_at[1] = scale[1];
   }
 }
-
 
 // ------------------------------------------------------------- attention
 //

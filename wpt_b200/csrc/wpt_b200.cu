@@ -1748,18 +1748,36 @@ int check_rotary(int C, int dims, int start, const void* frequencies) {
   return WPT_OK;
 }
 
+template <class T, int VE, bool INTERLEAVED>
+auto rotate_kernel_for(int copies) {
+  void (*kernel)(wpt::RotateParams) = wpt::rotate_kernel<T, VE, INTERLEAVED, -1>;
+  if constexpr (VE > 1) {
+    if (copies == 0) kernel = wpt::rotate_kernel<T, VE, INTERLEAVED, 0>;
+    if (copies == 1) kernel = wpt::rotate_kernel<T, VE, INTERLEAVED, 1>;
+    if (copies == 2) kernel = wpt::rotate_kernel<T, VE, INTERLEAVED, 2>;
+  }
+  return kernel;
+}
 template <class T, int VE>
-cudaError_t launch_rotate(const wpt::RotateParams& p, int interleaved, int64_t blocks, cudaStream_t s) {
-  return launch_dependent(interleaved ? wpt::rotate_kernel<T, VE, true> : wpt::rotate_kernel<T, VE, false>,
-                          dim3(static_cast<unsigned>(blocks)), 256, 0, 1, s, p);
+cudaError_t launch_rotate(const wpt::RotateParams& p, int interleaved, int copies, int64_t blocks, cudaStream_t s) {
+  const auto kernel = interleaved ? rotate_kernel_for<T, VE, true>(copies) : rotate_kernel_for<T, VE, false>(copies);
+  const int smem = p.dims / 2 * 8;
+  if (smem > 48 * 1024 && allow_smem(kernel, smem) != WPT_OK) return cudaErrorInvalidValue;
+  return launch_dependent(kernel, dim3(static_cast<unsigned>(blocks)), 256, smem, 1, s, p);
 }
 
 template <class T, int VE>
 int launch_append(const wpt::AppendParams& p, int interleaved, unsigned blocks, cudaStream_t s) {
-  auto kernel = interleaved ? wpt::paged_append_kernel<T, VE, true> : wpt::paged_append_kernel<T, VE, false>;
-  const int smem = wpt::PAGE_BLOCK * 2 * p.C * 4;
+  // a warp's lanes cover an entry's vectors: the entries stay in registers, else in shared memory
+  const bool rows = VE > 1 && 2 * p.C / VE <= 32;
+  void (*kernel)(wpt::AppendParams) = interleaved ? wpt::paged_append_kernel<T, VE, true, false>
+                                                  : wpt::paged_append_kernel<T, VE, false, false>;
+  if constexpr (VE > 1) {
+    if (rows) kernel = interleaved ? wpt::paged_append_kernel<T, VE, true, true> : wpt::paged_append_kernel<T, VE, false, true>;
+  }
+  const int smem = wpt::PAGE_BLOCK * (rows ? 0 : 2 * p.C * 4) + wpt::PAGE_BLOCK * p.dims / 2 * 8;
   if (int rc = allow_smem(kernel, smem)) return rc;
-  cudaError_t e = launch_dependent(kernel, dim3(blocks), 128, smem, 1, s, p);
+  cudaError_t e = launch_dependent(kernel, dim3(blocks), wpt::APPEND_THREADS, smem, 1, s, p);
   if (e != cudaSuccess) return cuda_fail(e, "paged_append_kernel launch");
   return WPT_OK;
 }
@@ -1802,6 +1820,7 @@ extern "C" int wpt_rotate(const void* x, int64_t x_stride_b, int64_t x_stride_t,
                           int interleaved, float magnitude, int inverse, void* stream) {
   if (B < 0 || T < 0 || H < 0 || C < 1) return fail(WPT_ERR_INVALID, "bad shape B=%d T=%d H=%d C=%d", B, T, H, C);
   if (int rc = check_rotary(C, dims, start, frequencies)) return rc;
+  if (dims > 32768) return fail(WPT_ERR_UNSUPPORTED, "%d turned channels: up to 32768", dims);
   if (B == 0 || T == 0 || H == 0) return WPT_OK;
   if (!x || !y || !positions) return fail(WPT_ERR_INVALID, "a required pointer is NULL");
   wpt::RotateParams p;
@@ -1825,7 +1844,9 @@ extern "C" int wpt_rotate(const void* x, int64_t x_stride_b, int64_t x_stride_t,
   const bool vectors = rotary_vectors(wide, C, dims, start, interleaved) && aligned16(x) && aligned16(y) &&
                        x_stride_b % wide == 0 && x_stride_t % wide == 0 && x_stride_h % wide == 0;
   const int ve = vectors ? wide : 1;
-  p.items = dims / 2 / (interleaved && ve > 1 ? ve / 2 : ve) + (C - dims) / ve;
+  const int turned = dims / 2 / (interleaved && ve > 1 ? ve / 2 : ve), rest = (C - dims) / ve;
+  const int copies = vectors && turned > 0 && rest % turned == 0 && rest / turned <= 2 ? rest / turned : -1;
+  p.items = copies < 0 ? turned + rest : turned;
   // a thread's angles serve up to 8 heads, fewer where that would leave SMs without threads
   int sms = 148;
   current_device(&sms);
@@ -1839,10 +1860,11 @@ extern "C" int wpt_rotate(const void* x, int64_t x_stride_b, int64_t x_stride_t,
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (f32)
-    e = vectors ? launch_rotate<float, 4>(p, interleaved, blocks, s) : launch_rotate<float, 1>(p, interleaved, blocks, s);
+    e = vectors ? launch_rotate<float, 4>(p, interleaved, copies, blocks, s)
+                : launch_rotate<float, 1>(p, interleaved, copies, blocks, s);
   else
-    e = vectors ? launch_rotate<__nv_bfloat16, 8>(p, interleaved, blocks, s)
-                : launch_rotate<__nv_bfloat16, 1>(p, interleaved, blocks, s);
+    e = vectors ? launch_rotate<__nv_bfloat16, 8>(p, interleaved, copies, blocks, s)
+                : launch_rotate<__nv_bfloat16, 1>(p, interleaved, copies, blocks, s);
   if (e != cudaSuccess) return cuda_fail(e, "rotate_kernel launch");
   return WPT_OK;
 }
@@ -1859,6 +1881,7 @@ extern "C" int wpt_paged_append(const void* src, int f32, int64_t src_stride_b, 
   if (int rc = check_rotary(C, dims, start, frequencies)) return rc;
   if (B == 0 || n == 0 || M == 0 || P == 0) return WPT_OK;
   if (!src || !pages || !scales || !table || !first || !counts) return fail(WPT_ERR_INVALID, "a required pointer is NULL");
+  if (static_cast<int64_t>(M) * S > INT_MAX - 1024) return fail(WPT_ERR_UNSUPPORTED, "a table of %d pages of %d entries", M, S);
   if (!aligned16(pages) || page_stride % 16 || entry_stride % 16 || entry_stride < 2 * C)
     return fail(WPT_ERR_INVALID, "pages and their strides must be multiples of 16 bytes");
   const int wide = f32 ? 4 : 8;
@@ -1891,6 +1914,8 @@ extern "C" int wpt_paged_append(const void* src, int f32, int64_t src_stride_b, 
   p.dims = dims;
   p.start = start;
   p.magnitude = magnitude;
+  p.turn_rows = dims > 0 ? wpt::APPEND_THREADS / (dims / 2) : 0;
+  p.turn_pairs = dims > 0 ? wpt::APPEND_THREADS % (dims / 2) : 0;
   p.blocks = (n - 1) / wpt::PAGE_BLOCK + 2;  // n entries reach into that many blocks at most
   const int64_t blocks = static_cast<int64_t>(B) * p.blocks;
   if (blocks >= (int64_t(1) << 31)) return fail(WPT_ERR_UNSUPPORTED, "too many entries to append");

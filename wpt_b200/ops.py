@@ -858,14 +858,14 @@ def _frequencies(frequencies, C, start):
     """(contiguous fp32 or fp64 frequencies, dims, the first channel that turns) of heads of C channels."""
     if frequencies is None:
         return None, 0, 0
-    if frequencies.dim() != 1 or not frequencies.is_floating_point():
-        raise ValueError(f"frequencies are (dims / 2,) floating-point angles; got {frequencies.dtype} "
-                         f"{tuple(frequencies.shape)}")
-    if frequencies.dtype not in (torch.float64, torch.float32):
+    shape, dtype = frequencies.shape, frequencies.dtype
+    if len(shape) != 1 or not dtype.is_floating_point:
+        raise ValueError(f"frequencies are (dims / 2,) floating-point angles; got {dtype} {tuple(shape)}")
+    if dtype is not torch.float64 and dtype is not torch.float32:
         frequencies = frequencies.float()
     if not frequencies.is_contiguous():
         frequencies = frequencies.contiguous()
-    dims = 2 * frequencies.shape[0]
+    dims = 2 * shape[0]
     if start is None:
         start = C - dims
     if start < 0 or start + dims > C:
@@ -881,59 +881,78 @@ def rotate(x, positions, frequencies, start=None, interleaved=False, magnitude=1
     device = x.device
     if not (x.is_cuda and positions.device == device and frequencies.device == device):
         _one_device(x, positions, frequencies)
-    f32 = x.dtype == torch.float32
-    if not f32 and x.dtype != torch.bfloat16:
+    f32 = x.dtype is torch.float32
+    if not f32 and x.dtype is not torch.bfloat16:
         raise NotImplementedError(f"the rotation kernel takes bfloat16 or float32; got {x.dtype}")
-    shape = x.shape
-    if len(shape) not in (3, 4):
+    shape, at = x.shape, positions.shape
+    if len(shape) == 4:
+        B, T, H, C = shape
+    elif len(shape) == 3:
+        B, T, C = shape
+        H = 1
+    else:
         raise ValueError(f"x must be (B, T, C) or (B, T, H, C); got {tuple(shape)}")
-    B, T, C = shape[0], shape[1], shape[-1]
-    H = shape[2] if len(shape) == 4 else 1
-    if positions.shape != (T,) and positions.shape != (B, T) and positions.shape != (1, T):
-        raise ValueError(f"positions must be {(T,)} or {(B, T)}; got {tuple(positions.shape)}")
+    each = len(at) == 2 and at[0] == B  # each row has positions of its own
+    if at[-1:] != shape[1:2] or not (each or len(at) == 1 or (len(at) == 2 and at[0] == 1)):
+        raise ValueError(f"positions must be {(T,)} or {(B, T)}; got {tuple(at)}")
     if (B | T | H | C) >> 31:
         raise NotImplementedError(f"x of {tuple(shape)}: past the library's 32-bit arguments")
     frequencies, dims, start = _frequencies(frequencies, C, start)
-    if positions.dtype != torch.int64 or positions.stride(-1) != 1:
+    if positions.dtype is not torch.int64 or positions.stride(-1) != 1:
         positions = positions.to(torch.int64).contiguous()
-    if x.stride(-1) != 1:
-        x = x.contiguous()
-    y = torch.empty(shape, dtype=x.dtype, device=device)
-    if y.numel() == 0:
+    if x.is_contiguous():
+        y = torch.empty_like(x)
+    else:
+        if x.stride(-1) != 1:
+            x = x.contiguous()
+        y = x.new_empty(shape)
+    if B * T * H * C == 0:
         return y
     stride = x.stride()
     _call(device, _lib.lib().wpt_rotate,
           (x.data_ptr(), stride[0], stride[1], stride[2] if len(shape) == 4 else 0, positions.data_ptr(),
-           positions.stride(0) if positions.shape[0] == B and positions.dim() == 2 else 0, frequencies.data_ptr(),
-           frequencies.dtype == torch.float64, y.data_ptr(), f32, B, T, H, C, dims, start, interleaved, magnitude,
-           inverse))
+           positions.stride(0) if each else 0, frequencies.data_ptr(), frequencies.dtype is torch.float64, y.data_ptr(), f32,
+           B, T, H, C, dims, start, interleaved, magnitude, inverse))
     LAUNCHES[0] += 1
     return y
 
 
-def _pages(pages, scales, table, width=None):
+_PAGE_LAYOUTS = {}  # what _pages found for shapes, strides and types that it has seen
+
+
+def _pages(pages, scales, table):
     """Checks a paged cache's tensors; (P, S, C, M)."""
-    if pages.dtype != torch.float8_e4m3fn or scales.dtype != torch.float32:
-        raise NotImplementedError(f"the paged cache holds float8_e4m3fn with float32 scales; got {pages.dtype} and "
-                                  f"{scales.dtype}")
-    if pages.dim() != 3 or pages.shape[2] % 2 or pages.shape[1] % PAGE_BLOCK or \
-            scales.shape != (pages.shape[0], pages.shape[1] // PAGE_BLOCK, 2):
-        raise ValueError(f"pages {tuple(pages.shape)} must be (P, S, 2 C), S a multiple of {PAGE_BLOCK}, with scales "
-                         f"(P, S / {PAGE_BLOCK}, 2); got {tuple(scales.shape)}")
-    P, S, C2 = pages.shape
-    if S not in (16, 32, 64) and S % 128:
+    ps, pt, ss, st, ts = pages.shape, pages.stride(), scales.shape, scales.stride(), table.shape
+    key = ps, pt, ss, st, ts, pages.dtype, scales.dtype, table.dtype
+    found = _PAGE_LAYOUTS.get(key)
+    if found is None:
+        if len(_PAGE_LAYOUTS) > 4096:
+            _PAGE_LAYOUTS.clear()
+        found = _PAGE_LAYOUTS[key] = _page_layout(ps, pt, ss, st, ts, pages.dtype, scales.dtype, table.dtype)
+    if pages.data_ptr() % 16:
+        raise ValueError("pages must be 16-byte aligned")
+    return found
+
+
+def _page_layout(ps, pt, ss, st, ts, pages_dtype, scales_dtype, table_dtype):
+    if pages_dtype != torch.float8_e4m3fn or scales_dtype != torch.float32:
+        raise NotImplementedError(f"the paged cache holds float8_e4m3fn with float32 scales; got {pages_dtype} and "
+                                  f"{scales_dtype}")
+    if len(ps) != 3 or ps[2] % 2 or ps[1] % PAGE_BLOCK or ss != (ps[0], ps[1] // PAGE_BLOCK, 2):
+        raise ValueError(f"pages {tuple(ps)} must be (P, S, 2 C), S a multiple of {PAGE_BLOCK}, with scales (P, S / "
+                         f"{PAGE_BLOCK}, 2); got {tuple(ss)}")
+    P, S, C2 = ps
+    if S not in (16, 32, 64) and (S % 128 or S == 0):
         raise NotImplementedError(f"pages of {S} entries: 16, 32, 64 or a multiple of 128")
-    if table.dim() != 2 or table.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"the page table must be (B, M) int32 or int64; got {table.dtype} {tuple(table.shape)}")
-    ps, ss = pages.stride(), scales.stride()
-    if pages.numel() and (ps[2] != 1 or ps[1] < C2 or (P > 1 and ps[0] < S * ps[1]) or (ps[0] | ps[1]) % 16 or
-                          pages.data_ptr() % 16):
+    if len(ts) != 2 or table_dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"the page table must be (B, M) int32 or int64; got {table_dtype} {tuple(ts)}")
+    if P * C2 and (pt[2] != 1 or pt[1] < C2 or (P > 1 and pt[0] < (S - 1) * pt[1] + C2) or (pt[0] | pt[1]) % 16):
         raise ValueError("pages must have contiguous entries, 16-byte aligned, and pages that do not overlap")
-    if scales.numel() and (ss[2] != 1 or (ss[1] != 2 and S > PAGE_BLOCK) or (P > 1 and ss[0] < S // PAGE_BLOCK * 2)):
+    if P and (st[2] != 1 or (st[1] != 2 and S > PAGE_BLOCK) or (P > 1 and st[0] < S // PAGE_BLOCK * 2)):
         raise ValueError("scales must be contiguous within a page")
-    if (P | S | table.shape[1] | table.shape[1] * S) >> 31:
-        raise NotImplementedError(f"{P} pages of {S} entries, {table.shape[1]} a row: past the library's 32-bit arguments")
-    return P, S, C2 // 2, table.shape[1]
+    if (P | S | ts[1] | ts[1] * S) >> 31:
+        raise NotImplementedError(f"{P} pages of {S} entries, {ts[1]} a row: past the library's 32-bit arguments")
+    return P, S, C2 // 2, ts[1]
 
 
 def _table_rows(table):
@@ -969,14 +988,14 @@ def paged_append(pages, scales, table, new, first, counts, frequencies=None, pos
             (frequencies is None or frequencies.device == device) and (positions is None or positions.device == device)):
         _one_device(pages, scales, table, new, first, counts, frequencies, positions)
     P, S, C, M = _pages(pages, scales, table)
-    f32 = new.dtype == torch.float32
-    if not f32 and new.dtype != torch.bfloat16:
+    f32 = new.dtype is torch.float32
+    if not f32 and new.dtype is not torch.bfloat16:
         raise NotImplementedError(f"the append kernel takes bfloat16 or float32 entries; got {new.dtype}")
-    B = table.shape[0]
-    if new.dim() != 3 or new.shape[0] != B or new.shape[2] != 2 * C or first.shape != (B,) or counts.shape != (B,):
-        raise ValueError(f"entries {tuple(new.shape)} for a table of {B} rows and pages of 2 x {C}, with first "
+    B, shape = table.shape[0], new.shape
+    if len(shape) != 3 or shape[0] != B or shape[2] != 2 * C or first.shape != (B,) or counts.shape != (B,):
+        raise ValueError(f"entries {tuple(shape)} for a table of {B} rows and pages of 2 x {C}, with first "
                          f"{tuple(first.shape)} and counts {tuple(counts.shape)}")
-    n = new.shape[1]
+    n = shape[1]
     if positions is not None and positions.shape != (B, n):
         raise ValueError(f"positions must be {(B, n)}; got {tuple(positions.shape)}")
     if (B | n) >> 31:
@@ -989,11 +1008,12 @@ def paged_append(pages, scales, table, new, first, counts, frequencies=None, pos
         new = new.contiguous()
     if B * n * P * M == 0:
         return pages, scales
+    ns, ps = new.stride(), pages.stride()
     _call(device, _lib.lib().wpt_paged_append,
-          (new.data_ptr(), f32, new.stride(0), new.stride(1), pages.data_ptr(), pages.stride(0), pages.stride(1),
-           scales.data_ptr(), scales.stride(0), table.data_ptr(), table.dtype == torch.int64, table.stride(0),
-           first.data_ptr(), counts.data_ptr(), _lib.ptr(positions), _lib.ptr(frequencies),
-           frequencies is not None and frequencies.dtype == torch.float64, B, n, C, M, P, S, dims, start, interleaved,
+          (new.data_ptr(), f32, ns[0], ns[1], pages.data_ptr(), ps[0], ps[1], scales.data_ptr(), scales.stride(0),
+           table.data_ptr(), table.dtype is torch.int64, table.stride(0), first.data_ptr(), counts.data_ptr(),
+           None if positions is None else positions.data_ptr(), None if frequencies is None else frequencies.data_ptr(),
+           frequencies is not None and frequencies.dtype is torch.float64, B, n, C, M, P, S, dims, start, interleaved,
            magnitude))
     LAUNCHES[0] += 1
     return pages, scales
@@ -1041,10 +1061,11 @@ def paged_attention(q, pages, scales, table, positions, scale, window=0, sink=No
         _one_device(q, pages, scales, table, positions, sink)
     P, S, C, M = _pages(pages, scales, table)
     _bf16(q)
-    if q.dim() != 4 or q.shape[3] != C or table.shape[0] != q.shape[0] or positions.shape != q.shape[:2]:
-        raise ValueError(f"queries {tuple(q.shape)} with pages of 2 x {C}, a table of {table.shape[0]} rows and "
+    shape = q.shape
+    if len(shape) != 4 or shape[3] != C or table.shape[0] != shape[0] or positions.shape != shape[:2]:
+        raise ValueError(f"queries {tuple(shape)} with pages of 2 x {C}, a table of {table.shape[0]} rows and "
                          f"positions {tuple(positions.shape)}")
-    B, T, H, _ = q.shape
+    B, T, H, _ = shape
     if sink is not None and sink.shape != (H,):
         raise ValueError(f"sink must be {(H,)}; got {tuple(sink.shape)}")
     if window < 0 or (B | T) >> 31:
@@ -1057,10 +1078,10 @@ def paged_attention(q, pages, scales, table, positions, scale, window=0, sink=No
         q = q.clone(memory_format=torch.contiguous_format)
     positions = _rows(positions)
     table = _table_rows(table)
-    if sink is not None and (sink.dtype != torch.float32 or not sink.is_contiguous()):
+    if sink is not None and (sink.dtype is not torch.float32 or not sink.is_contiguous()):
         sink = sink.float().contiguous()
     out = torch.empty_like(q)
-    lse = torch.empty((B, T, H), dtype=torch.float32, device=device)
+    lse = q.new_empty((B, T, H), dtype=torch.float32)
     if B * T * H == 0:
         return out, lse
     splits, ctas = _paged_plan(B, T, H, M * S, window, sm_count(device))
@@ -1071,7 +1092,8 @@ def paged_attention(q, pages, scales, table, positions, scale, window=0, sink=No
     ps = pages.stride()
     _call(device, lib.wpt_paged_attention,
           (q.data_ptr(), pages.data_ptr(), ps[0], ps[1], scales.data_ptr(), scales.stride(0), table.data_ptr(),
-           table.dtype == torch.int64, table.stride(0), positions.data_ptr(), _lib.ptr(sink), out.data_ptr(),
-           lse.data_ptr(), _lib.ptr(scratch), splits, ctas, B, T, H, C, M, P, S, window, scale))
+           table.dtype is torch.int64, table.stride(0), positions.data_ptr(), None if sink is None else sink.data_ptr(),
+           out.data_ptr(), lse.data_ptr(), None if scratch is None else scratch.data_ptr(), splits, ctas, B, T, H, C, M, P,
+           S, window, scale))
     LAUNCHES[0] += 1 + (scratch is not None)
     return out, lse
