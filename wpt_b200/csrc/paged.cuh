@@ -400,10 +400,10 @@ __global__ void __launch_bounds__(APPEND_THREADS, ROWS ? 8 : 1) paged_append_ker
 //   a weight w = 2^x, as fp16 (11 significant bits) 3 e5m2 numbers, each the
 //   upper byte (e5m2 is fp16's) of what the ones before it leave, the last one
 //   times 32 and rounded: within 2^-8.6 w (2^-9, and fp16's 2^-11; a bf16
-//   weight's is 2^-8), and 2^-22 where w is small. 1 is what the first tile's
-//   largest weight comes out as, 2^15 the largest that fits: a column is
-//   rescaled when a score passes those of the first tile by 15 (base 2), and a
-//   run of n keys may lose n 2^-22 of its largest weight.
+//   weight's is 2^-8), and 2^-22 where w is small. 1 is the largest weight of
+//   the keys that set a column's base (32 or more of the first tile), 2^15 the
+//   largest that fits: a column is rescaled when a score passes its base by 15
+//   (base 2), and a run of n keys may lose n 2^-22 of its largest weight.
 // Scales. A key's scale multiplies its score. A value's scale 2^lv joins the
 // exponent, w = 2^(s + lv - m), m the running maximum of s + lv, so O needs no
 // scaling; the softmax's sum takes w 2^-lv. Sums, maxima and accumulators are
@@ -418,7 +418,16 @@ __global__ void __launch_bounds__(APPEND_THREADS, ROWS ? 8 : 1) paged_append_ker
 //
 // Warps 0-3 prepare q, then take thread r = key r of a tile of 128 (as the
 // key-stream kernel's do); warp 4 issues products; warp 5 brings K and V by
-// TMA, a box for each page of a tile; warp 6 brings the scales.
+// TMA, a box for each page of a tile; warp 6 brings the scales. Two CTAs share
+// an SM (64 columns: one), so that one's exponents run under the other's loads.
+//
+// What bounds it: at 64 rows of 4,097 to 32,768 keys and 16 columns HBM and the
+// softmax warps' instructions about equally, 60 us for 278 MB (4.6 TB/s), of
+// which 5 are the merge; one row of 131,071 keys and 64 drafts of 10,000 keys are
+// chains of latencies: the groups' tiles, a page's number, its tile, the products,
+// the parts, the merge (26 and 17 us). A segment's fixed cost is code that is
+// fetched anew for it (the kernel is larger than the instruction cache), which is
+// why what runs once a segment is in loops that are not unrolled.
 struct PagedParams {
   const __nv_bfloat16* q;        // (B, T, H, 128) contiguous
   const float* scales;
@@ -489,31 +498,20 @@ __host__ __device__ constexpr uint32_t idesc_f8(int M, int N, int a_type, int b_
          (static_cast<uint32_t>(a_mn) << 15) | (static_cast<uint32_t>(b_mn) << 16) |
          (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
 }
-template <uint32_t OFF_A, uint32_t OFF_B>
-__device__ __forceinline__ void mma_f8_off_warp(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
-                                                uint32_t accumulate) {
+__device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p, e;\n\t.reg .b64 da, db;\n\t"
-      "add.s64 da, %1, %5;\n\tadd.s64 db, %2, %6;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "elect.sync _|e, 0xffffffff;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %3, p;\n\t}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "n"(OFF_A), "n"(OFF_B)
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// S^T = K Q^T, 4 steps of 32 channels; both K-major rows of 128 bytes.
-template <int KK>
-__device__ __forceinline__ void paged_s_steps(uint32_t d, uint64_t dk, uint64_t dq, uint32_t idesc) {
-  if constexpr (KK > 0) paged_s_steps<KK - 1>(d, dk, dq, idesc);
-  constexpr uint32_t off = KK * 32 / 16;
-  mma_f8_off_warp<off, off>(d, dk, dq, idesc, KK > 0 ? 1u : 0u);
-}
-// O^T += V^T P^T, 4 steps of 32 keys; both MN-major, 128 bytes a key.
-template <int KK>
-__device__ __forceinline__ void paged_pv_steps(uint32_t d, uint64_t dv, uint64_t dp, uint32_t idesc, uint32_t acc0) {
-  if constexpr (KK > 0) paged_pv_steps<KK - 1>(d, dv, dp, idesc, acc0);
-  constexpr uint32_t off = KK * 32 * 128 / 16;
-  mma_f8_off_warp<off, off>(d, dv, dp, idesc, KK > 0 ? 1u : acc0);
+// Four steps of 32 along K, `step` 16-byte units on in both operands: S^T = K
+// Q^T (32 channels, rows of 128 bytes: 32 bytes on) or O^T += V^T P^T (32 keys of
+// 128 bytes). One thread issues these and their commits.
+__device__ __forceinline__ void paged_steps(uint32_t d, uint64_t da, uint64_t db, uint32_t step, uint32_t idesc,
+                                            uint32_t accumulate) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) mma_f8(d, da + k * step, db + k * step, idesc, k > 0 ? 1u : accumulate);
 }
 
 // The rows that a query at `pos` reads: lo .. hi of its batch row (hi < lo: none).
@@ -609,6 +607,7 @@ __device__ __forceinline__ void paged_cluster_merge(const PagedParams& p, const 
     for (int i = 0; i < 8; ++i) s_w[cl * 9 + i] = li[i] != 0.f ? w[i] * inv : 0.f;
   }
   __syncthreads();
+#pragma unroll 1
   for (int item = threadIdx.x; item < mine * (C / 4); item += blockDim.x) {
     const int cl = item / (C / 4), quad = item % (C / 4), c = rank + cl * S;
     float4 o[8];
@@ -676,7 +675,9 @@ __global__ void __launch_bounds__(PAGED_THREADS, PagedLayout<NCOL>::CTAS)
   const int gcount = balanced ? p.groups : 1;
 
   if (warp == 3) {
+#pragma unroll 1
     for (int i = lane; i < NCOL * 4; i += 32) s_nan[i] = 0u;
+#pragma unroll 1
     for (int i = lane; i < NCOL; i += 32) {
       s_base[i] = PAGED_UNSET;
       s_l[i] = 0.f;
@@ -710,6 +711,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, PagedLayout<NCOL>::CTAS)
   if (static_cast<int>(threadIdx.x) < gcount) {
     const int g = gbase + threadIdx.x, b = g / p.groups_per_row, t0 = (g - b * p.groups_per_row) * p.TQ;
     int rlo = INT_MAX, rhi = -1;
+#pragma unroll 1
     for (int t = t0; t < min(t0 + p.TQ, p.T); ++t) {
       int lo, hi;
       paged_rows(p, p.positions[static_cast<int64_t>(b) * p.T + t], lo, hi);
@@ -769,7 +771,9 @@ __global__ void __launch_bounds__(PAGED_THREADS, PagedLayout<NCOL>::CTAS)
     int tile0, n;           // its first tile and its tiles
     bool whole;             // all of its group's
     __device__ __forceinline__ bool next() {
+#pragma unroll 1
       while (at < end) {
+#pragma unroll 1
         while (before[g + 1] <= at) ++g;
         const int from = before[g] + aside, stop = min(end, before[g + 1]);
         tile0 = max(at, from);
@@ -784,31 +788,18 @@ __global__ void __launch_bounds__(PAGED_THREADS, PagedLayout<NCOL>::CTAS)
   };
   Segments sg{s_before, s_first, aside, begin, end, 0, 0, 0, false};
 
-  if (begin == end) {  // nothing to read
-    if (!balanced) {
+  if (begin == end) {  // nothing to read (a cluster's share of that is merged below)
+    if (p.splits == 1) {
       const int b = gbase / p.groups_per_row, t0 = (gbase - b * p.groups_per_row) * p.TQ;
       const int ncols = min(p.TQ, p.T - t0) * p.H;
       const int64_t row0 = (static_cast<int64_t>(b) * p.T + t0) * p.H;
-      if (p.splits > 1) {
-        paged_cluster_merge<NCOL>(p, s_base, s_l, reinterpret_cast<const float*>(sP), reinterpret_cast<float*>(sK),
-                                  row0, ncols);
-      } else {
-        for (int i = threadIdx.x; i < ncols * (C / 2); i += PAGED_THREADS)
-          reinterpret_cast<uint32_t*>(p.out + row0 * C)[i] = 0u;
-        if (static_cast<int>(threadIdx.x) < ncols)
-          p.lse[row0 + threadIdx.x] = p.sink != nullptr ? p.sink[threadIdx.x % p.H] : -INFINITY;
-      }
+#pragma unroll 1
+      for (int i = threadIdx.x; i < ncols * (C / 2); i += PAGED_THREADS)
+        reinterpret_cast<uint32_t*>(p.out + row0 * C)[i] = 0u;
+      if (static_cast<int>(threadIdx.x) < ncols)
+        p.lse[row0 + threadIdx.x] = p.sink != nullptr ? p.sink[threadIdx.x % p.H] : -INFINITY;
     }
-    tc_fence_before();
-    __syncthreads();
-    if (warp == 4) {
-      tc_fence_after();
-      tmem_dealloc(tmem, L::TMEM_COLS);
-    }
-    return;
-  }
-
-  if (warp == 5) {
+  } else if (warp == 5) {
     if constexpr (L::CTAS == 2) setmaxnreg_dec<PAGED_REGS_OTHERS>();
     // ------------------------------------------------ keys and values by TMA
     const int rows = min(static_cast<int>(p.S), BN), per = BN / rows;  // entries of a box, boxes of a tile
@@ -816,6 +807,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, PagedLayout<NCOL>::CTAS)
     const int part = lane % per;
     bool ok = true;
     int j = 0;  // the ring's tile
+#pragma unroll 1
     while (ok && sg.next()) {
       const int b = (gbase + sg.g) / p.groups_per_row;
       // the number of this lane's page in tile i0 + lane / per: loaded a batch ahead, checked when it is used
@@ -826,6 +818,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, PagedLayout<NCOL>::CTAS)
       };
       int64_t next = lookup(0);
       int page = -1;
+#pragma unroll 1
       for (int i = 0; i < sg.n; ++i, ++j) {
         const int in = i % batch;
         if (in == 0) {
@@ -851,6 +844,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, PagedLayout<NCOL>::CTAS)
     // ------------------------------------- scales: a lane a block, four tiles at a time
     bool ok = true;
     int j = 0;
+#pragma unroll 1
     while (ok && sg.next()) {
       const int b = (gbase + sg.g) / p.groups_per_row;
       // page numbers are loaded two batches ahead, scales one
@@ -870,6 +864,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, PagedLayout<NCOL>::CTAS)
       bool there = page >= 0 && page < p.P;
       page = number(4);
       float4 mine;
+#pragma unroll 1
       for (int i = 0; i < sg.n; ++i, ++j) {
         if ((i & 3) == 0) {
           // key scale; log2 of the value scale, 2^-60 at least (what is scaled by less, as the 0 of an empty
@@ -908,16 +903,21 @@ __global__ void __launch_bounds__(PAGED_THREADS, PagedLayout<NCOL>::CTAS)
     auto wait = [&](uint64_t* bar, int parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status)); };
     bool ok = true;
     int j = 0, nseg = 0;
+#pragma unroll 1
     while (ok && sg.next()) {
       ok = wait(q_full, nseg++ & 1);
+#pragma unroll 1
       for (int i = 0; ok && i <= sg.n; ++i) {
         if (i < sg.n) {
           const int st = j % NK;
           if (!(ok = wait(k_full + st, (j / NK) & 1))) break;
           tc_fence_after();
-          paged_s_steps<3>(tS + (j & 1) * L::S_COLS, sdesc_sw128(k_addr + st * L::TILE, 16, 1024), dq, IDESC_S);
-          mma_commit_warp(s_full + (j & 1));
-          mma_commit_warp(k_empty + st);
+          if (lane == 0) {
+            paged_steps(tS + (j & 1) * L::S_COLS, sdesc_sw128(k_addr + st * L::TILE, 16, 1024), dq, 32 / 16, IDESC_S, 0u);
+            mma_commit(s_full + (j & 1));
+            mma_commit(k_empty + st);
+          }
+          __syncwarp();
           ++j;
         }
         if (i > 0) {
@@ -925,10 +925,14 @@ __global__ void __launch_bounds__(PAGED_THREADS, PagedLayout<NCOL>::CTAS)
           if (!(ok = wait(v_full + st, (jp / NV) & 1))) break;
           if (!(ok = wait(p_ready + (jp & 1), (jp >> 1) & 1))) break;
           tc_fence_after();
-          paged_pv_steps<3>(tO, sdesc_sw128(v_addr + st * L::TILE, BN * 128, 1024),
-                            sdesc_sw128(p_addr + (jp & 1) * L::P_BYTES, BN * 128, 1024), IDESC_O, i > 1 ? 1u : 0u);
-          mma_commit_warp(v_empty + st);
-          mma_commit_warp(o_done);
+          if (lane == 0) {
+            paged_steps(tO, sdesc_sw128(v_addr + st * L::TILE, BN * 128, 1024),
+                        sdesc_sw128(p_addr + (jp & 1) * L::P_BYTES, BN * 128, 1024), 32 * 128 / 16, IDESC_O,
+                        i > 1 ? 1u : 0u);
+            mma_commit(v_empty + st);
+            mma_commit(o_done);
+          }
+          __syncwarp();
         }
       }
     }
@@ -961,6 +965,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, PagedLayout<NCOL>::CTAS)
     if (more) load_ahead();
     bool ok = true;
     int j = 0;
+#pragma unroll 1
     while (ok && more) {
       sg = nx;
       const int group = gbase + sg.g, b = group / p.groups_per_row, t0 = (group - b * p.groups_per_row) * p.TQ;
@@ -1032,6 +1037,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, PagedLayout<NCOL>::CTAS)
       auto two = [](const float* at, int i) { return reinterpret_cast<const uint64_t*>(at)[i]; };
 #pragma unroll
       for (int i = 0; i < NCOL / 2; ++i) lp[i] = 0ull;
+#pragma unroll 1
       for (int i = 0; i < sg.n; ++i, ++j) {
         ok = __all_sync(0xffffffffu, mbar_wait(s_full + (j & 1), (j >> 1) & 1, p.status));
         tc_fence_after();
@@ -1044,59 +1050,53 @@ __global__ void __launch_bounds__(PAGED_THREADS, PagedLayout<NCOL>::CTAS)
         if (n0 < alo || n0 + BN - 1 > ahi) {
           const int row = n0 + r;
           vis = 0ull;
+#pragma unroll 1
           for (int tq = 0; tq < TQg; ++tq)
             if (row >= s_qlo[tq] && row <= s_qhi[tq]) vis |= head_bits << (tq * p.H);
           if (vis == all_cols) vis = ~0ull;
         }
         if (sc.w == 0.f) vis = 0ull;
-        // A value that no column may read is 0 in the product; where only some may (drafts that come before it do
-        // not), a NaN in it is taken out of the product and noted for those columns.
-        if (vis != ~0ull) {
-          if (ok) ok = mbar_wait(v_full + j % NV, (j / NV) & 1, p.status);
-          uint8_t* vr = sV + j % NV * L::TILE + r * 128;
-#pragma unroll 1
-          for (int ch = 0; ok && ch < 32; ++ch) {  // four channels each
-            uint32_t* at = reinterpret_cast<uint32_t*>(vr + (((ch >> 2) ^ (r & 7)) << 4) + (ch & 3) * 4);
-            const uint32_t w = *at;
-            const uint32_t nan = __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu);
-            if (vis == 0ull) {
-              *at = 0u;
-            } else if (nan != 0u) {
-              *at = w & ~nan;
-              *s_any_nan = 1;
-              const uint32_t bits = ((nan & 1u) | (nan >> 7 & 2u) | (nan >> 14 & 4u) | (nan >> 21 & 8u)) << (ch & 7) * 4;
-              for (int c = 0; c < ncols; ++c)
-                if ((vis >> c) & 1ull) atomicOr(s_nan + c * 4 + (ch >> 3), bits);
-            }
-          }
-        }
-        __syncwarp();
         // The maximum is lazy, as in the key-stream kernel: a column's base changes only when a score is PAGED_TOP past
-        // it. A segment's first tile sets the bases, each warp a quarter of them, to the maxima of its own 32 keys; a
-        // tile with a score past its column's bound is taken twice, that column's base being its maximum then. What
-        // is run once in a segment is kept short: such code is fetched anew each time. (A wait that failed is
-        // carried to the barriers, where all warps agree to stop.)
+        // it. A segment's first tile sets the bases: the warps with keys that all columns read share the columns, and
+        // set each to the maximum over their own 32 keys (no such key: to the tile's). A tile with a score past its
+        // column's bound is taken twice, that column's base being its maximum then. What is run once in a segment is
+        // kept short: such code is fetched anew each time. (A wait that failed is carried to the barriers, where all
+        // warps agree to stop.)
         const uint32_t sa = lane_addr + (j & 1) * L::S_COLS;
         auto score = [&](uint32_t hi, uint32_t lo) {
           return fmaf(fmaf(__uint_as_float(lo), 0.0625f, __uint_as_float(hi)), fk, sc.y);
         };
         if (i == 0) {
+          const int from = max(alo, n0), upto = min(ahi, n0 + BN - 1);
+          const bool shared = from <= upto;
+          const int w0 = (from - n0) >> 5, per = shared ? (NCOL / 8 + ((upto - n0) >> 5) - w0) / (((upto - n0) >> 5) - w0 + 1) * 8 : 0;
+          float* to = shared ? s_base : s_red + warp * NCOL;
+          const int c_end = !shared ? NCOL : n0 + 32 * warp > upto ? 0 : min(NCOL, (warp - w0 + 1) * per);
 #pragma unroll 1
-          for (int c = warp * (NCOL / 4); c < (warp + 1) * (NCOL / 4); c += 4) {
-            uint32_t x[4], y[4];
-            tmem_ld4x2(sa + c, sa + NCOL + c, x, y);
-            float m[4];
+          for (int c = shared ? max(0, warp - w0) * per : 0; c < c_end; c += 8) {
+            uint32_t x[8], y[8];
+            tmem_ld8x2(sa + c, sa + NCOL + c, x, y);
+            float m[8];
+            const uint32_t sees = static_cast<uint32_t>(vis >> c);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              m[k] = warp_max((vis >> (c + k)) & 1ull ? score(x[k], y[k]) : -INFINITY);
-              m[k] = m[k] == -INFINITY ? PAGED_UNSET : -m[k];
+            for (int k = 0; k < 8; ++k) m[k] = warp_max((sees >> k) & 1u ? score(x[k], y[k]) : -INFINITY);
+            if (lane < 8) {
+              float mine = m[0];
+#pragma unroll
+              for (int k = 1; k < 8; ++k) mine = lane == k ? m[k] : mine;
+              to[c + lane] = mine == -INFINITY ? PAGED_UNSET : -mine;
             }
-            if (lane == 0) *reinterpret_cast<float4*>(s_base + c) = make_float4(m[0], m[1], m[2], m[3]);
+          }
+          if (!shared) {
+            named_barrier(1, 128);
+            if (r < NCOL)
+              s_base[r] = fminf(fminf(s_red[r], s_red[NCOL + r]), fminf(s_red[2 * NCOL + r], s_red[3 * NCOL + r]));
           }
           if (r == 0) bulk_wait_read();  // the segment before has left P's buffers
           named_barrier(1, 128);
         }
         bool stop = false;
+#pragma unroll 1
         for (int pass = 0;; ++pass) {
           // the exponents s + lv - base
           if (L::IN_REGS && (pass != 0 || i == 0)) {
@@ -1140,10 +1140,11 @@ __global__ void __launch_bounds__(PAGED_THREADS, PagedLayout<NCOL>::CTAS)
             tmem_ld4x2(sa + c, sa + NCOL + c, x, y);
             const float4 base = *reinterpret_cast<const float4*>(s_base + c);
             const float past[4] = {base.x, base.y, base.z, base.w};
+            const uint32_t sees = static_cast<uint32_t>(vis >> c);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               const float v = score(x[k], y[k]);
-              if (((vis >> (c + k)) & 1ull) && v + past[k] > PAGED_TOP) atomicMax(s_top + c + k, ordered(v));
+              if (((sees >> k) & 1u) && v + past[k] > PAGED_TOP) atomicMax(s_top + c + k, ordered(v));
             }
           }
           stop = !named_barrier_and(1, 128, ok);
@@ -1186,6 +1187,39 @@ __global__ void __launch_bounds__(PAGED_THREADS, PagedLayout<NCOL>::CTAS)
           ok = false;
           break;
         }
+        // A value that no column may read is 0 in the product; where only some may (drafts that come before it do
+        // not), a NaN in it is taken out of the product and noted for those columns.
+        if (vis != ~0ull) {
+          if (ok) ok = mbar_wait(v_full + j % NV, (j / NV) & 1, p.status);
+          uint4* vr = reinterpret_cast<uint4*>(sV + j % NV * L::TILE + r * 128);
+          if (vis == 0ull && ok) {
+#pragma unroll
+            for (int i8 = 0; i8 < 8; ++i8) vr[i8 ^ (r & 7)] = make_uint4(0u, 0u, 0u, 0u);
+          }
+#pragma unroll 1
+          for (int i8 = 0; ok && vis != 0ull && i8 < 8; ++i8) {  // 16 channels each, others in each lane
+            const int at = i8 ^ (r & 7);
+            uint4 v = vr[at];
+            uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+            uint32_t any = 0u, bits = 0u;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t nan = __vcmpeq4(w[k] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+              w[k] &= ~nan;
+              any |= nan;
+              bits |= ((nan & 1u) | (nan >> 7 & 2u) | (nan >> 14 & 4u) | (nan >> 21 & 8u)) << 4 * k;
+            }
+            if (any != 0u) {
+              vr[at] = v;
+              *s_any_nan = 1;
+              const int ch = (at ^ (r & 7)) * 16;  // the first channel
+#pragma unroll 1
+              for (int c = 0; c < ncols; ++c)
+                if ((vis >> c) & 1ull) atomicOr(s_nan + c * 4 + (ch >> 5), bits << (ch & 31));
+            }
+          }
+        }
+        __syncwarp();
         // weights, their sums (a key on no page adds 0 times 0), and as fp16 pairs
         uint32_t h[NCOL / 2];
         const uint64_t iv = f2_pack(sc.z, sc.z);
@@ -1262,19 +1296,27 @@ __global__ void __launch_bounds__(PAGED_THREADS, PagedLayout<NCOL>::CTAS)
       // (a cluster's to be merged from there), and leaves as one bulk copy.
       const bool any_nan = *s_any_nan != 0, wide = !final || p.splits > 1;
 #pragma unroll 1
-      for (int c = 0; ok && c < NCOL; c += 4) {
-        uint32_t x[4], y[4], z[4];
-        tmem_ld4x3(tO + c, tO + NCOL + c, tO + 2 * NCOL + c, x, y, z);
-        const float4 l4 = *reinterpret_cast<const float4*>(s_l + c);
-        const float f[4] = {l4.x, l4.y, l4.z, l4.w};
+      for (int c = 0; ok && c < NCOL; c += 8) {
+        uint32_t x[8], y[8], z[8];
+        tmem_ld8x3(tO + c, tO + NCOL + c, tO + 2 * NCOL + c, x, y, z);
+        float o[8];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          float o = __uint_as_float(x[k]) + fmaf(__uint_as_float(z[k]), 0.03125f, __uint_as_float(y[k]));
-          if (any_nan && ((s_nan[(c + k) * 4 + (r >> 5)] >> lane) & 1u)) o = __int_as_float(0x7fffffff);
-          if (wide)
-            reinterpret_cast<float*>(sP)[(c + k) * C + r] = o;
-          else
-            reinterpret_cast<__nv_bfloat16*>(sP)[(c + k) * C + r] = __float2bfloat16_rn(o * f[k]);
+        for (int k = 0; k < 8; ++k)
+          o[k] = __uint_as_float(x[k]) + fmaf(__uint_as_float(z[k]), 0.03125f, __uint_as_float(y[k]));
+        if (any_nan) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if ((s_nan[(c + k) * 4 + (r >> 5)] >> lane) & 1u) o[k] = __int_as_float(0x7fffffff);
+        }
+        if (wide) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) reinterpret_cast<float*>(sP)[(c + k) * C + r] = o[k];
+        } else {
+          const float4 f0 = *reinterpret_cast<const float4*>(s_l + c), f1 = *reinterpret_cast<const float4*>(s_l + c + 4);
+          const float f[8] = {f0.x, f0.y, f0.z, f0.w, f1.x, f1.y, f1.z, f1.w};
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            reinterpret_cast<__nv_bfloat16*>(sP)[(c + k) * C + r] = __float2bfloat16_rn(o[k] * f[k]);
         }
       }
       if (p.splits <= 1) {
@@ -1313,12 +1355,15 @@ __global__ void __launch_bounds__(PAGED_THREADS, PagedLayout<NCOL>::CTAS)
 }
 
 // Balanced: groups in several CTAs, or in none. A warp a row (query, head),
-// four channels a lane; with SPREAD a row's parts go over the 8 warps of a CTA
-// and are added up in shared memory (one long row has a part in every CTA).
-template <bool SPREAD>
-__global__ void __launch_bounds__(256) paged_merge_kernel(const PagedParams p, int ncol) {
+// four channels a lane; with SPREAD (8 or 32) a row's parts go over that many
+// warps of a CTA and are added up in shared memory. One long row has a part in
+// every CTA: 8 warps take its 296 parts in 10 rounds of loads, 32 in 3; for
+// hundreds of rows of 22 parts CTAs of 32 warps cost more than they save (24 us a
+// call against 17).
+template <int SPREAD>
+__global__ void __launch_bounds__(SPREAD ? SPREAD * 32 : 256) paged_merge_kernel(const PagedParams p, int ncol) {
   griddep_wait();
-  constexpr int C = 128, WARPS = 8, STEP = SPREAD ? WARPS : 1;
+  constexpr int C = 128, WARPS = SPREAD ? SPREAD : 8, STEP = SPREAD ? WARPS : 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t row = SPREAD ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * WARPS + warp;
   if (row >= static_cast<int64_t>(p.B) * p.T * p.H) return;
@@ -1333,7 +1378,7 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedParams p, i
   float M = -INFINITY, L = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   // adds parts (exponents and sums ml, outputs o; a sum of 0: nothing was read, nothing was written)
-  constexpr int MOST = SPREAD ? WARPS : 4;
+  constexpr int MOST = 4;
   auto add = [&](const float2 (&ml)[MOST], const float4 (&o)[MOST]) {
     float top = M;
 #pragma unroll
@@ -1381,14 +1426,16 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedParams p, i
     M = -INFINITY;
     L = 0.f;
     acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float2 ml[WARPS];
-    float4 o[WARPS];
+    for (int w0 = 0; w0 < WARPS && w0 < info.y; w0 += MOST) {
+      float2 ml[MOST];
+      float4 o[MOST];
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      ml[w] = s_ml[w];
-      o[w] = s_acc[w][lane];
+      for (int k = 0; k < MOST; ++k) {
+        ml[k] = s_ml[w0 + k];
+        o[k] = s_acc[w0 + k][lane];
+      }
+      add(ml, o);
     }
-    add(ml, o);
   }
   float inv;
   const float lse = paged_total(M, L, p.sink, h, inv);

@@ -2007,9 +2007,12 @@ extern "C" int wpt_paged_attention(const void* q, const void* pages, int64_t pag
   if (rc || splits != 0) return rc;
   const int64_t rows = static_cast<int64_t>(B) * T * H;
   // parts of a group: about ctas / groups + 1
-  const bool spread = ctas > 7 * groups;
-  cudaError_t e = launch_dependent(spread ? wpt::paged_merge_kernel<true> : wpt::paged_merge_kernel<false>,
-                                   dim3(static_cast<unsigned>(spread ? rows : (rows + 7) / 8)), 256, 0, 1, s, p, ncol);
+  const int spread = ctas <= 7 * groups ? 0 : ctas > 31 * groups && rows <= 256 ? 32 : 8;
+  cudaError_t e = launch_dependent(spread == 0   ? wpt::paged_merge_kernel<0>
+                                   : spread == 8 ? wpt::paged_merge_kernel<8>
+                                                 : wpt::paged_merge_kernel<32>,
+                                   dim3(static_cast<unsigned>(spread ? rows : (rows + 7) / 8)), spread ? spread * 32 : 256,
+                                   0, 1, s, p, ncol);
   if (e != cudaSuccess) return cuda_fail(e, "paged_merge_kernel launch");
   return WPT_OK;
 }
