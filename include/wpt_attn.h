@@ -398,7 +398,7 @@ int wpt_paged_append(const void* src, int f32, int64_t src_stride_b, int64_t src
 
 /*
  * Attention over the 8-bit paged cache for few queries a row (C = 128, up to
- * 64 heads; any T is computed, 64 / H queries at a time): query t of row b
+ * 64 heads; any T): query t of row b
  * reads the row's entries max(0, p - window + 1) .. min(p, M S - 1), p =
  * positions[b, t] (window 0: no window), but for those on no page; q, out, lse
  * and sink as above. What other entries hold (NaN too) reaches no result.
@@ -406,10 +406,10 @@ int wpt_paged_append(const void* src, int f32, int64_t src_stride_b, int64_t src
  *   splits     how the work is split. 1 to 8: each query group's entries go to
  *              that many CTAs in equal runs, a thread-block cluster where more
  *              than one; ctas and scratch are not used. 0: all groups' entries
- *              in equal runs over `ctas` CTAs, for up to 256 groups (64 / H
- *              queries of a row each; 32 / H or 16 / H where T * H is no
- *              more), with scratch of wpt_paged_scratch_bytes bytes, 16-byte
- *              aligned.
+ *              in equal runs over `ctas` CTAs, for up to 256 groups (32 / H
+ *              queries of a row, 16 / H where T * H is no more; with more than
+ *              32 heads each query is two groups), with scratch of
+ *              wpt_paged_scratch_bytes bytes, 16-byte aligned.
  */
 size_t wpt_paged_scratch_bytes(int B, int T, int H, int splits, int ctas);
 int wpt_paged_attention(const void* q, const void* pages, int64_t page_stride, int64_t entry_stride,

@@ -69,7 +69,8 @@ def test_paged_attention_arguments(lib):
     for empty in (dict(B=0), dict(T=0)):
         assert _attend(lib, **empty) == lib.OK
     size = lib.lib().wpt_paged_scratch_bytes
-    assert size(2, 1, 32, 0, 10) == (2 + 10) * 32 * 520 + 16 and size(1, 5, 12, 0, 3) == 4 * 64 * 520 + 8
+    assert size(2, 1, 32, 0, 10) == (2 + 10) * 32 * 520 + 16 and size(1, 5, 12, 0, 3) == 6 * 32 * 520 + 24
+    assert size(3, 2, 33, 0, 1) == (12 + 1) * 32 * 520 + 96  # two groups for a query's heads
     assert size(1, 1, 1, 1, 1) == 0 and size(1, 1, 65, 0, 1) == 0 and size(0, 1, 1, 0, 1) == 0
 
 
@@ -95,8 +96,8 @@ def test_plans():
                 for N in (16, 128, 129, 1024, 4096, 8192, 32768, 262144, 2 ** 30):
                     for window in (0, 1, 128, 1024):
                         splits, ctas = ops._paged_plan_for(B, T, H, N, window, sms)
-                        ncol = 16 if T * H <= 16 else 32 if T * H <= 32 else 64
-                        groups, slots = B * math.ceil(T / (ncol // H)), sms * (1 if ncol == 64 else 2)
+                        ncol = 16 if T * H <= 16 else 32
+                        groups, slots = B * (math.ceil(T / (ncol // H)) if H <= 32 else 2 * T), 2 * sms
                         assert 0 <= splits <= 8
                         if splits > 1:
                             assert groups * splits <= slots

@@ -409,8 +409,11 @@ __global__ void __launch_bounds__(APPEND_THREADS, ROWS ? 8 : 1) paged_append_ker
 // scaling; the softmax's sum takes w 2^-lv. Sums, maxima and accumulators are
 // fp32.
 //
-// Work. A group is up to 64 columns (query, head) of a batch row, its tiles
-// those that its queries read. Balanced: every CTA works out the groups' tile
+// Work. A group is up to 32 columns (query, head) of a batch row, its tiles
+// those that its queries read. (Groups of 64 read each tile once for twice the
+// columns, but leave room for one CTA of them on an SM, whose four softmax warps
+// are what the time goes to: 45 queries of 24 heads over 1,261 keys 25 us against
+// 13, 59 of 32 in 13 rows over 1,073 51 against 41.) Balanced: every CTA works out the groups' tile
 // counts and takes an equal run of all tiles in a row, a part of one group or
 // of several (segments); a group in several CTAs leaves parts for
 // paged_merge_kernel. Otherwise a group's tiles go in equal runs to a cluster of
@@ -444,7 +447,9 @@ struct PagedParams {
   unsigned* status;
   int t64;
   unsigned M, S;                 // pages a row, entries a page
-  int B, T, H, P, window, TQ, groups_per_row, groups;
+  int B, T, H, P, window;
+  int TQ, HG, chunks;            // queries and heads of a group; groups that the heads of a query take (TQ is 1 then)
+  int groups_per_row, groups;
   int splits;                    // CTAs of a group, a cluster where > 1; 0: balanced, all groups' tiles over the grid
   float scale_log2;
 };
@@ -459,12 +464,10 @@ constexpr int PAGED_SEGMENT = 4;   // what a segment costs beside its tiles, in 
 template <int NCOL>
 struct PagedLayout {
   static constexpr int C = 128, BN = 128;
-  static constexpr int NK = NCOL == 64 ? 4 : 2, NV = NCOL == 64 ? 4 : 2;  // ring stages of keys and of values
-  static constexpr int CTAS = NCOL == 64 ? 1 : 2;                         // a SM
-  static constexpr bool IN_REGS = NCOL <= 32;                             // bases stay in registers
+  static constexpr int NK = 2, NV = 2;  // ring stages of keys and of values
   static constexpr int TILE = BN * C;
   static constexpr int Q_BYTES = 2 * NCOL * C;
-  static constexpr int P_BYTES = BN * (NCOL == 64 ? 256 : 128);
+  static constexpr int P_BYTES = BN * 128;
   static constexpr int OFF_K = ((Q_BYTES + 1023) / 1024) * 1024;
   static constexpr int OFF_V = OFF_K + NK * TILE;
   static constexpr int OFF_P = OFF_V + NV * TILE;
@@ -476,14 +479,14 @@ struct PagedLayout {
   static constexpr int OFF_SCALE = OFF_TOP + NCOL * 4;         // 2 tiles x 8 blocks x float4
   static constexpr int OFF_NAN = OFF_SCALE + 2 * 8 * 16;     // 4 words a column
   static constexpr int OFF_QLO = OFF_NAN + NCOL * 16;
-  static constexpr int OFF_QHI = OFF_QLO + 64 * 4;
-  static constexpr int OFF_TILES = OFF_QHI + 64 * 4;         // groups: tiles before each, and the first tile
+  static constexpr int OFF_QHI = OFF_QLO + 32 * 4;
+  static constexpr int OFF_TILES = OFF_QHI + 32 * 4;         // groups: tiles before each, and the first tile
   static constexpr int OFF_BAR = OFF_TILES + (2 * PAGED_GROUPS + 2) * 4;
   static constexpr int NBAR = 1 + 2 * NK + 2 * NV + 2 + 2 + 1;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
   static constexpr int BYTES = OFF_MISC + 64 + 1024;
   static constexpr int S_COLS = 2 * NCOL, O_COLS = 3 * NCOL;
-  static constexpr int TMEM_COLS = 2 * S_COLS + O_COLS <= 128 ? 128 : 2 * S_COLS + O_COLS <= 256 ? 256 : 512;
+  static constexpr int TMEM_COLS = 2 * S_COLS + O_COLS <= 128 ? 128 : 256;
 };
 
 constexpr int PAGED_THREADS = 256;
@@ -513,6 +516,27 @@ __device__ __forceinline__ void paged_steps(uint32_t d, uint64_t da, uint64_t db
 #pragma unroll
   for (int k = 0; k < 4; ++k) mma_f8(d, da + k * step, db + k * step, idesc, k > 0 ? 1u : accumulate);
 }
+
+// Group g: the batch row, its queries (query .. query + queries - 1 of the B T), their heads h0 .. h0 + heads - 1;
+// rows row0 .. row0 + columns - 1 of the (B T H, 128) queries and results.
+struct PagedGroup {
+  int b, queries, h0, heads, columns, query, row0;  // (B T H is under 2^31)
+  __device__ __forceinline__ PagedGroup(const PagedParams& p, int g) {
+    b = g / p.groups_per_row;
+    int at = g - b * p.groups_per_row;
+    h0 = 0;
+    if (p.chunks > 1) {
+      h0 = at % p.chunks * p.HG;
+      at /= p.chunks;
+    }
+    const int t0 = at * p.TQ;
+    queries = min(p.TQ, p.T - t0);
+    heads = min(p.HG, p.H - h0);
+    columns = queries * heads;
+    query = b * p.T + t0;
+    row0 = query * p.H + h0;
+  }
+};
 
 // The rows that a query at `pos` reads: lo .. hi of its batch row (hi < lo: none).
 __device__ __forceinline__ void paged_rows(const PagedParams& p, int64_t pos, int& lo, int& hi) {
@@ -573,10 +597,11 @@ __device__ __forceinline__ float paged_total(float M, float L, const float* sink
 // shared memory; CTA k owns columns k, k + S, ... (as stream_cluster_merge).
 template <int NCOL>
 __device__ __forceinline__ void paged_cluster_merge(const PagedParams& p, const float* s_base, const float* s_l,
-                                                    const float* s_o, float* s_w, int64_t row0, int ncols) {
+                                                    const float* s_o, float* s_w, const PagedGroup& group) {
   constexpr int C = 128;
   cluster_sync();
-  const int S = p.splits;
+  const int S = p.splits, ncols = group.columns;
+  const int64_t row0 = group.row0;
   const int rank = static_cast<int>(cluster_rank());
   const int mine = ncols > rank ? (ncols - rank + S - 1) / S : 0;
   const uint32_t am = smem_u32(s_base), al = smem_u32(s_l), ao = smem_u32(s_o);
@@ -602,7 +627,7 @@ __device__ __forceinline__ void paged_cluster_merge(const PagedParams& p, const 
       w[i] = li[i] != 0.f ? fast_exp2(mi[i] - M) : 0.f;
       L += li[i] != 0.f ? w[i] * li[i] : 0.f;
     }
-    s_w[cl * 9 + 8] = paged_total(M, L, p.sink, c % p.H, inv);
+    s_w[cl * 9 + 8] = paged_total(M, L, p.sink, group.h0 + c % p.HG, inv);
 #pragma unroll
     for (int i = 0; i < 8; ++i) s_w[cl * 9 + i] = li[i] != 0.f ? w[i] * inv : 0.f;
   }
@@ -635,7 +660,7 @@ __device__ __forceinline__ void paged_cluster_merge(const PagedParams& p, const 
 }
 
 template <int NCOL>
-__global__ void __launch_bounds__(PAGED_THREADS, PagedLayout<NCOL>::CTAS)
+__global__ void __launch_bounds__(PAGED_THREADS, 2)
     paged_kernel(const __grid_constant__ CUtensorMap tm, const PagedParams p) {
   using L = PagedLayout<NCOL>;
   constexpr int C = L::C, BN = L::BN, NK = L::NK, NV = L::NV;
@@ -709,12 +734,12 @@ __global__ void __launch_bounds__(PAGED_THREADS, PagedLayout<NCOL>::CTAS)
   // the groups' tiles: thread g counts group g's, a scan adds them up
   int count = 0;
   if (static_cast<int>(threadIdx.x) < gcount) {
-    const int g = gbase + threadIdx.x, b = g / p.groups_per_row, t0 = (g - b * p.groups_per_row) * p.TQ;
+    const PagedGroup group(p, gbase + threadIdx.x);
     int rlo = INT_MAX, rhi = -1;
 #pragma unroll 1
-    for (int t = t0; t < min(t0 + p.TQ, p.T); ++t) {
+    for (int t = 0; t < group.queries; ++t) {
       int lo, hi;
-      paged_rows(p, p.positions[static_cast<int64_t>(b) * p.T + t], lo, hi);
+      paged_rows(p, p.positions[group.query + t], lo, hi);
       if (hi >= lo) {
         rlo = min(rlo, lo);
         rhi = max(rhi, hi);
@@ -790,17 +815,15 @@ __global__ void __launch_bounds__(PAGED_THREADS, PagedLayout<NCOL>::CTAS)
 
   if (begin == end) {  // nothing to read (a cluster's share of that is merged below)
     if (p.splits == 1) {
-      const int b = gbase / p.groups_per_row, t0 = (gbase - b * p.groups_per_row) * p.TQ;
-      const int ncols = min(p.TQ, p.T - t0) * p.H;
-      const int64_t row0 = (static_cast<int64_t>(b) * p.T + t0) * p.H;
+      const PagedGroup group(p, gbase);
 #pragma unroll 1
-      for (int i = threadIdx.x; i < ncols * (C / 2); i += PAGED_THREADS)
-        reinterpret_cast<uint32_t*>(p.out + row0 * C)[i] = 0u;
-      if (static_cast<int>(threadIdx.x) < ncols)
-        p.lse[row0 + threadIdx.x] = p.sink != nullptr ? p.sink[threadIdx.x % p.H] : -INFINITY;
+      for (int i = threadIdx.x; i < group.columns * (C / 2); i += PAGED_THREADS)
+        reinterpret_cast<uint32_t*>(p.out + static_cast<int64_t>(group.row0) * C)[i] = 0u;
+      if (static_cast<int>(threadIdx.x) < group.columns)
+        p.lse[group.row0 + threadIdx.x] = p.sink != nullptr ? p.sink[group.h0 + threadIdx.x % p.HG] : -INFINITY;
     }
   } else if (warp == 5) {
-    if constexpr (L::CTAS == 2) setmaxnreg_dec<PAGED_REGS_OTHERS>();
+    setmaxnreg_dec<PAGED_REGS_OTHERS>();
     // ------------------------------------------------ keys and values by TMA
     const int rows = min(static_cast<int>(p.S), BN), per = BN / rows;  // entries of a box, boxes of a tile
     const int batch = 32 / per;                      // tiles whose page numbers the warp holds, a lane a box
@@ -840,7 +863,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, PagedLayout<NCOL>::CTAS)
       }
     }
   } else if (warp == 6) {
-    if constexpr (L::CTAS == 2) setmaxnreg_dec<PAGED_REGS_OTHERS>();
+    setmaxnreg_dec<PAGED_REGS_OTHERS>();
     // ------------------------------------- scales: a lane a block, four tiles at a time
     bool ok = true;
     int j = 0;
@@ -892,7 +915,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, PagedLayout<NCOL>::CTAS)
       }
     }
   } else if (warp == 4) {
-    if constexpr (L::CTAS == 2) setmaxnreg_dec<PAGED_REGS_OTHERS>();
+    setmaxnreg_dec<PAGED_REGS_OTHERS>();
     // --------------------------------------------------------- MMA issuer
     constexpr uint32_t IDESC_S = idesc_f8(128, 2 * NCOL, 0, 0, 0, 0);
     constexpr uint32_t IDESC_O = idesc_f8(128, 3 * NCOL, 0, 1, 1, 1);
@@ -937,30 +960,25 @@ __global__ void __launch_bounds__(PAGED_THREADS, PagedLayout<NCOL>::CTAS)
       }
     }
   } else if (warp == 7) {
-    if constexpr (L::CTAS == 2) setmaxnreg_dec<PAGED_REGS_OTHERS>();
+    setmaxnreg_dec<PAGED_REGS_OTHERS>();
   } else {
-    if constexpr (L::CTAS == 2) setmaxnreg_inc<PAGED_REGS_SOFTMAX>();
+    setmaxnreg_inc<PAGED_REGS_SOFTMAX>();
     const int r = threadIdx.x;
     const uint32_t lane_addr = tmem + (static_cast<uint32_t>(warp * 32) << 16);
     const uint32_t tO = lane_addr + 2 * L::S_COLS;
-    const uint64_t head_bits = p.H >= 64 ? ~0ull : ((1ull << p.H) - 1);
     // A segment's queries: each warp's columns (warp, warp + 4, ...), four channels a lane, and a lane's
     // positions, loaded while the segment before ends.
     uint2 ahead_q[NCOL / 4];
-    int64_t ahead_pos[2];
+    int64_t ahead_pos;
     Segments nx = sg;
     bool more = nx.next();
     auto load_ahead = [&]() {
-      const int group = gbase + nx.g, b = group / p.groups_per_row, t0 = (group - b * p.groups_per_row) * p.TQ;
-      const int TQg = min(p.TQ, p.T - t0), ncols = TQg * p.H;
-      const int64_t query = static_cast<int64_t>(b) * p.T + t0;
-      const __nv_bfloat16* q = p.q + query * p.H * C + lane * 4;
+      const PagedGroup group(p, gbase + nx.g);
+      const __nv_bfloat16* q = p.q + static_cast<int64_t>(group.row0) * C + lane * 4;
 #pragma unroll
       for (int i = 0; i < NCOL / 4; ++i)
-        if (warp + 4 * i < ncols) ahead_q[i] = *reinterpret_cast<const uint2*>(q + (warp + 4 * i) * C);
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-        if (lane + 32 * k < TQg) ahead_pos[k] = p.positions[query + lane + 32 * k];
+        if (warp + 4 * i < group.columns) ahead_q[i] = *reinterpret_cast<const uint2*>(q + (warp + 4 * i) * C);
+      if (lane < group.queries) ahead_pos = p.positions[group.query + lane];
     };
     if (more) load_ahead();
     bool ok = true;
@@ -968,24 +986,16 @@ __global__ void __launch_bounds__(PAGED_THREADS, PagedLayout<NCOL>::CTAS)
 #pragma unroll 1
     while (ok && more) {
       sg = nx;
-      const int group = gbase + sg.g, b = group / p.groups_per_row, t0 = (group - b * p.groups_per_row) * p.TQ;
-      const int TQg = min(p.TQ, p.T - t0), ncols = TQg * p.H;
-      const int64_t row0 = (static_cast<int64_t>(b) * p.T + t0) * p.H;
-      const uint64_t all_cols = ncols >= 64 ? ~0ull : ((1ull << ncols) - 1);
+      const PagedGroup group(p, gbase + sg.g);
+      const int ncols = group.columns;
+      const uint32_t head_bits = 0xffffffffu >> (32 - group.heads), all_cols = 0xffffffffu >> (32 - ncols);
       // each query's rows, and those that all of them read
       int alo = 0, ahi = INT_MAX;
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int tq = lane + 32 * k;
-        if (tq < TQg) {
-          int lo, hi;
-          paged_rows(p, ahead_pos[k], lo, hi);
-          if (warp == 0) {
-            s_qlo[tq] = lo;
-            s_qhi[tq] = hi;
-          }
-          alo = max(alo, lo);
-          ahi = min(ahi, hi);
+      if (lane < group.queries) {
+        paged_rows(p, ahead_pos, alo, ahi);
+        if (warp == 0) {
+          s_qlo[lane] = alo;
+          s_qhi[lane] = ahi;
         }
       }
       alo = __reduce_max_sync(0xffffffffu, alo);
@@ -1032,8 +1042,8 @@ __global__ void __launch_bounds__(PAGED_THREADS, PagedLayout<NCOL>::CTAS)
       mbar_arrive(q_full);
       named_barrier(1, 128);  // s_qlo, s_qhi; s_sum is read
 
-      // softmax: thread r = key r. Pairs of columns: minus bases (in registers, or shared memory), sums, exponents
-      uint64_t nb[L::IN_REGS ? NCOL / 2 : 1], lp[NCOL / 2], e[NCOL / 2];
+      // softmax: thread r = key r. Pairs of columns: minus bases, sums, exponents
+      uint64_t nb[NCOL / 2], lp[NCOL / 2], e[NCOL / 2];
       auto two = [](const float* at, int i) { return reinterpret_cast<const uint64_t*>(at)[i]; };
 #pragma unroll
       for (int i = 0; i < NCOL / 2; ++i) lp[i] = 0ull;
@@ -1046,16 +1056,16 @@ __global__ void __launch_bounds__(PAGED_THREADS, PagedLayout<NCOL>::CTAS)
         const uint64_t ks = f2_pack(fk, fk), lv = f2_pack(sc.y, sc.y);
         // which columns read this key; ~0 (padding columns too) where all do
         const int n0 = (sg.tile0 + i) * BN;
-        uint64_t vis = ~0ull;
+        uint32_t vis = ~0u;
         if (n0 < alo || n0 + BN - 1 > ahi) {
           const int row = n0 + r;
-          vis = 0ull;
+          vis = 0u;
 #pragma unroll 1
-          for (int tq = 0; tq < TQg; ++tq)
-            if (row >= s_qlo[tq] && row <= s_qhi[tq]) vis |= head_bits << (tq * p.H);
-          if (vis == all_cols) vis = ~0ull;
+          for (int tq = 0; tq < group.queries; ++tq)
+            if (row >= s_qlo[tq] && row <= s_qhi[tq]) vis |= head_bits << (tq * group.heads);
+          if (vis == all_cols) vis = ~0u;
         }
-        if (sc.w == 0.f) vis = 0ull;
+        if (sc.w == 0.f) vis = 0u;
         // The maximum is lazy, as in the key-stream kernel: a column's base changes only when a score is PAGED_TOP past
         // it. A segment's first tile sets the bases: the warps with keys that all columns read share the columns, and
         // set each to the maximum over their own 32 keys (no such key: to the tile's). A tile with a score past its
@@ -1077,7 +1087,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, PagedLayout<NCOL>::CTAS)
             uint32_t x[8], y[8];
             tmem_ld8x2(sa + c, sa + NCOL + c, x, y);
             float m[8];
-            const uint32_t sees = static_cast<uint32_t>(vis >> c);
+            const uint32_t sees = vis >> c;
 #pragma unroll
             for (int k = 0; k < 8; ++k) m[k] = warp_max((sees >> k) & 1u ? score(x[k], y[k]) : -INFINITY);
             if (lane < 8) {
@@ -1099,9 +1109,9 @@ __global__ void __launch_bounds__(PAGED_THREADS, PagedLayout<NCOL>::CTAS)
 #pragma unroll 1
         for (int pass = 0;; ++pass) {
           // the exponents s + lv - base
-          if (L::IN_REGS && (pass != 0 || i == 0)) {
+          if (pass != 0 || i == 0) {
 #pragma unroll
-            for (int k = 0; k < NCOL / 2; ++k) nb[L::IN_REGS ? k : 0] = two(s_base, k);
+            for (int k = 0; k < NCOL / 2; ++k) nb[k] = two(s_base, k);
           }
           const uint64_t low = f2_pack(0.0625f, 0.0625f);
 #pragma unroll
@@ -1111,18 +1121,17 @@ __global__ void __launch_bounds__(PAGED_THREADS, PagedLayout<NCOL>::CTAS)
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
               const int at = c0 / 2 + k;
-              const uint64_t nbase = L::IN_REGS ? nb[L::IN_REGS ? at : 0] : two(s_base, at);
               const uint64_t t = f2_fma(f2_pack(__uint_as_float(y[2 * k]), __uint_as_float(y[2 * k + 1])), low,
                                         f2_pack(__uint_as_float(x[2 * k]), __uint_as_float(x[2 * k + 1])));
-              e[at] = f2_fma(t, ks, f2_add(lv, nbase));
+              e[at] = f2_fma(t, ks, f2_add(lv, nb[at]));
             }
           }
-          if (vis != ~0ull) {
+          if (vis != ~0u) {
 #pragma unroll
             for (int k = 0; k < NCOL / 2; ++k) {
               float x, y;
               f2_unpack(e[k], x, y);
-              e[k] = f2_pack((vis >> (2 * k)) & 1ull ? x : -INFINITY, (vis >> (2 * k + 1)) & 1ull ? y : -INFINITY);
+              e[k] = f2_pack((vis >> (2 * k)) & 1u ? x : -INFINITY, (vis >> (2 * k + 1)) & 1u ? y : -INFINITY);
             }
           }
           if (pass == 1) break;
@@ -1140,7 +1149,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, PagedLayout<NCOL>::CTAS)
             tmem_ld4x2(sa + c, sa + NCOL + c, x, y);
             const float4 base = *reinterpret_cast<const float4*>(s_base + c);
             const float past[4] = {base.x, base.y, base.z, base.w};
-            const uint32_t sees = static_cast<uint32_t>(vis >> c);
+            const uint32_t sees = vis >> c;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               const float v = score(x[k], y[k]);
@@ -1189,15 +1198,15 @@ __global__ void __launch_bounds__(PAGED_THREADS, PagedLayout<NCOL>::CTAS)
         }
         // A value that no column may read is 0 in the product; where only some may (drafts that come before it do
         // not), a NaN in it is taken out of the product and noted for those columns.
-        if (vis != ~0ull) {
+        if (vis != ~0u) {
           if (ok) ok = mbar_wait(v_full + j % NV, (j / NV) & 1, p.status);
           uint4* vr = reinterpret_cast<uint4*>(sV + j % NV * L::TILE + r * 128);
-          if (vis == 0ull && ok) {
+          if (vis == 0u && ok) {
 #pragma unroll
             for (int i8 = 0; i8 < 8; ++i8) vr[i8 ^ (r & 7)] = make_uint4(0u, 0u, 0u, 0u);
           }
 #pragma unroll 1
-          for (int i8 = 0; ok && vis != 0ull && i8 < 8; ++i8) {  // 16 channels each, others in each lane
+          for (int i8 = 0; ok && vis != 0u && i8 < 8; ++i8) {  // 16 channels each, others in each lane
             const int at = i8 ^ (r & 7);
             uint4 v = vr[at];
             uint32_t* w = reinterpret_cast<uint32_t*>(&v);
@@ -1215,7 +1224,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, PagedLayout<NCOL>::CTAS)
               const int ch = (at ^ (r & 7)) * 16;  // the first channel
 #pragma unroll 1
               for (int c = 0; c < ncols; ++c)
-                if ((vis >> c) & 1ull) atomicOr(s_nan + c * 4 + (ch >> 5), bits << (ch & 31));
+                if ((vis >> c) & 1u) atomicOr(s_nan + c * 4 + (ch >> 5), bits << (ch & 31));
             }
           }
         }
@@ -1248,7 +1257,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, PagedLayout<NCOL>::CTAS)
 #pragma unroll
             for (int n = 0; n < 3; ++n) {
               const int at = n * NCOL + c0;  // the column's byte in the key's row
-              *reinterpret_cast<uint4*>(pj + (at >> 7) * (BN * 128) + sw128_offset(r, (at & 127) >> 4)) =
+              *reinterpret_cast<uint4*>(pj + sw128_offset(r, at >> 4)) =
                   make_uint4(part[n][0], part[n][1], part[n][2], part[n][3]);
             }
           }
@@ -1262,30 +1271,29 @@ __global__ void __launch_bounds__(PAGED_THREADS, PagedLayout<NCOL>::CTAS)
       if (ok) ok = __all_sync(0xffffffffu, mbar_wait(o_done, (j - 1) & 1, p.status));
       tc_fence_after();
       // per-column sums over the 128 keys
-#pragma unroll
-      for (int c32 = 0; c32 < (NCOL + 31) / 32; ++c32) {
+      {
         float tmp[32];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           tmp[2 * i] = tmp[2 * i + 1] = 0.f;
-          if (c32 * 16 + i < NCOL / 2) f2_unpack(lp[(c32 * 16 + i) % (NCOL / 2)], tmp[2 * i], tmp[2 * i + 1]);
+          if (i < NCOL / 2) f2_unpack(lp[i % (NCOL / 2)], tmp[2 * i], tmp[2 * i + 1]);
         }
         const float sum = transpose_reduce32(tmp, SumOp());
-        if (c32 * 32 + lane < NCOL) s_red[warp * NCOL + c32 * 32 + lane] = sum;
+        if (lane < NCOL) s_red[warp * NCOL + lane] = sum;
       }
       ok = named_barrier_and(1, 128, ok);
       // a whole group's result is final; else a part
       const bool final = balanced ? sg.whole : p.splits == 1;
-      const int64_t seg = static_cast<int64_t>(blockIdx.x) + group;
+      const int64_t seg = static_cast<int64_t>(blockIdx.x) + gbase + sg.g;
       if (r < NCOL) {
         const float l = (s_red[r] + s_red[NCOL + r]) + (s_red[2 * NCOL + r] + s_red[3 * NCOL + r]);
         if (p.splits > 1) {
           s_l[r] = ok ? l : 0.f;
         } else if (r < ncols && final) {
           float inv;
-          const float lse = paged_total(l != 0.f ? -s_base[r] : -INFINITY, l, p.sink, r % p.H, inv);
+          const float lse = paged_total(l != 0.f ? -s_base[r] : -INFINITY, l, p.sink, group.h0 + r % p.HG, inv);
           s_l[r] = inv;
-          if (ok) p.lse[row0 + r] = lse;
+          if (ok) p.lse[group.row0 + r] = lse;
         } else {
           s_l[r] = 1.f;
           if (r < ncols) p.part_ml[seg * NCOL + r] = ok ? make_float2(-s_base[r], l) : make_float2(-INFINITY, 0.f);
@@ -1326,7 +1334,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, PagedLayout<NCOL>::CTAS)
           if (wide)
             bulk_store(p.part_o + seg * NCOL * C, sP, ncols * C * 4);
           else
-            bulk_store(p.out + row0 * C, sP, ncols * C * 2);
+            bulk_store(p.out + static_cast<int64_t>(group.row0) * C, sP, ncols * C * 2);
           bulk_commit();
         }
       }
@@ -1348,9 +1356,8 @@ __global__ void __launch_bounds__(PAGED_THREADS, PagedLayout<NCOL>::CTAS)
     tmem_dealloc(tmem, L::TMEM_COLS);
   }
   if (p.splits > 1) {
-    const int b = gbase / p.groups_per_row, t0 = (gbase - b * p.groups_per_row) * p.TQ;
     paged_cluster_merge<NCOL>(p, s_base, s_l, reinterpret_cast<const float*>(sP), reinterpret_cast<float*>(sK),
-                              (static_cast<int64_t>(b) * p.T + t0) * p.H, min(p.TQ, p.T - t0) * p.H);
+                              PagedGroup(p, gbase));
   }
 }
 
@@ -1371,8 +1378,8 @@ __global__ void __launch_bounds__(SPREAD ? SPREAD * 32 : 256) paged_merge_kernel
   const int h = static_cast<int>(row - query * p.H);
   const int64_t b = query / p.T;
   const int t = static_cast<int>(query - b * p.T);
-  const int64_t group = b * p.groups_per_row + t / p.TQ;
-  const int col = (t % p.TQ) * p.H + h;
+  const int64_t group = b * p.groups_per_row + t / p.TQ * p.chunks + h / p.HG;
+  const int col = (t % p.TQ) * p.HG + h % p.HG;
   const int2 info = p.info[group];
   if (info.y == 1) return;  // one CTA had all of it
   float M = -INFINITY, L = 0.f;

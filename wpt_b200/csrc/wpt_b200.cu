@@ -1785,18 +1785,18 @@ int launch_append(const wpt::AppendParams& p, int interleaved, unsigned blocks, 
 template <int NCOL>
 int launch_paged(const CUtensorMap& tm, const wpt::PagedParams& p, int ctas, cudaStream_t s) {
   using L = wpt::PagedLayout<NCOL>;
-  static_assert(L::BYTES <= (L::CTAS == 2 ? 115712 : 232448), "paged attention kernel: too much shared memory");
+  static_assert(L::BYTES <= 115712, "paged attention kernel: too much shared memory");
   auto kernel = wpt::paged_kernel<NCOL>;
   if (int rc = allow_smem(kernel, L::BYTES)) return rc;
   // its register split draws on what the block was launched with: fewer would leave the increase waiting
   static std::atomic<int> regs{0};
-  if (L::CTAS == 2 && regs.load(std::memory_order_relaxed) == 0) {
+  if (regs.load(std::memory_order_relaxed) == 0) {
     cudaFuncAttributes fa;
     cudaError_t e = cudaFuncGetAttributes(&fa, kernel);
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncGetAttributes(paged_kernel)");
     regs.store(fa.numRegs, std::memory_order_relaxed);
   }
-  if (L::CTAS == 2 && regs.load(std::memory_order_relaxed) != wpt::PAGED_REGS)
+  if (regs.load(std::memory_order_relaxed) != wpt::PAGED_REGS)
     return fail(WPT_ERR_CUDA, "paged_kernel built with %d registers a thread, its register split needs %d",
                 regs.load(std::memory_order_relaxed), wpt::PAGED_REGS);
   const dim3 grid = p.splits == 0 ? dim3(ctas) : dim3(p.groups, p.splits);
@@ -1805,10 +1805,18 @@ int launch_paged(const CUtensorMap& tm, const wpt::PagedParams& p, int ctas, cud
   return WPT_OK;
 }
 
-int paged_columns(int T, int H) {
-  const int64_t cols = static_cast<int64_t>(T) * H;
-  return cols <= 16 ? 16 : cols <= 32 ? 32 : 64;
-}
+// Columns of a group, its queries and its heads: more than 32 heads are shared out evenly over several groups a query.
+struct PagedPlan {
+  int ncol, TQ, HG, chunks;
+  int64_t per_row;  // groups of a batch row
+  PagedPlan(int T, int H) {
+    ncol = static_cast<int64_t>(T) * H <= 16 ? 16 : 32;
+    chunks = (H + 31) / 32;
+    HG = (H + chunks - 1) / chunks;
+    TQ = chunks > 1 ? 1 : ncol / H;
+    per_row = (static_cast<int64_t>(T) + TQ - 1) / TQ * chunks;
+  }
+};
 
 bool page_size_ok(int S) { return S == 16 || S == 32 || S == 64 || (S >= 128 && S % 128 == 0); }
 
@@ -1928,9 +1936,9 @@ extern "C" int wpt_paged_append(const void* src, int f32, int64_t src_stride_b, 
 
 extern "C" size_t wpt_paged_scratch_bytes(int B, int T, int H, int splits, int ctas) {
   if (B < 1 || T < 1 || H < 1 || H > 64 || splits != 0 || ctas < 1) return 0;
-  const int ncol = paged_columns(T, H), TQ = ncol / H;
-  const size_t groups = static_cast<size_t>(B) * ((T + TQ - 1) / TQ);
-  return (groups + ctas) * ncol * (128 * 4 + 8) + groups * 8;
+  const PagedPlan plan(T, H);
+  const size_t groups = static_cast<size_t>(B) * plan.per_row;
+  return (groups + ctas) * plan.ncol * (128 * 4 + 8) + groups * 8;
 }
 
 extern "C" int wpt_paged_attention(const void* q, const void* pages, int64_t page_stride, int64_t entry_stride,
@@ -1949,8 +1957,9 @@ extern "C" int wpt_paged_attention(const void* q, const void* pages, int64_t pag
     return fail(WPT_ERR_INVALID, "a required pointer is NULL");
   if (!aligned16(q) || !aligned16(out) || (scratch && !aligned16(scratch)))
     return fail(WPT_ERR_INVALID, "q, out and scratch must be 16-byte aligned");
-  const int ncol = paged_columns(T, H), TQ = ncol / H;
-  const int64_t groups = static_cast<int64_t>(B) * ((T + TQ - 1) / TQ);
+  const PagedPlan plan(T, H);
+  const int ncol = plan.ncol;
+  const int64_t groups = static_cast<int64_t>(B) * plan.per_row;
   if (splits == 0) {
     if (!scratch || ctas < 1) return fail(WPT_ERR_INVALID, "a balanced call needs scratch and CTAs");
     if (groups > wpt::PAGED_GROUPS || groups * ((static_cast<int64_t>(M) * S + 127) / 128 + wpt::PAGED_SEGMENT) >= (int64_t(1) << 31) ||
@@ -1988,8 +1997,10 @@ extern "C" int wpt_paged_attention(const void* q, const void* pages, int64_t pag
   p.P = P;
   p.S = S;
   p.window = window;
-  p.TQ = TQ;
-  p.groups_per_row = (T + TQ - 1) / TQ;
+  p.TQ = plan.TQ;
+  p.HG = plan.HG;
+  p.chunks = plan.chunks;
+  p.groups_per_row = static_cast<int>(plan.per_row);
   p.groups = static_cast<int>(groups);
   p.splits = splits;
   p.scale_log2 = scale * wpt::LOG2E;
@@ -1998,12 +2009,7 @@ extern "C" int wpt_paged_attention(const void* q, const void* pages, int64_t pag
   p.part_ml = reinterpret_cast<float2*>(p.part_o + parts * ncol * 128);
   p.info = reinterpret_cast<int2*>(p.part_ml + parts * ncol);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  int rc;
-  switch (ncol) {
-    case 16: rc = launch_paged<16>(tm, p, ctas, s); break;
-    case 32: rc = launch_paged<32>(tm, p, ctas, s); break;
-    default: rc = launch_paged<64>(tm, p, ctas, s); break;
-  }
+  const int rc = ncol == 16 ? launch_paged<16>(tm, p, ctas, s) : launch_paged<32>(tm, p, ctas, s);
   if (rc || splits != 0) return rc;
   const int64_t rows = static_cast<int64_t>(B) * T * H;
   // parts of a group: about ctas / groups + 1

@@ -1032,14 +1032,14 @@ def _paged_plan(B, T, H, N, window, sms):
 
 
 def _paged_plan_for(B, T, H, N, window, sms):
-    cols = min(T * H, 64)
-    ncol = 16 if cols <= 16 else 32 if cols <= 32 else 64
-    TQ = ncol // H
-    groups = B * math.ceil(T / TQ)
+    ncol = 16 if T * H <= 16 else 32
+    chunks = math.ceil(H / 32)  # groups that a query's heads take
+    TQ = max(1, ncol // H)
+    groups = B * math.ceil(T / TQ) * chunks
     tiles = max(1, math.ceil(N / 128))
     if window:  # what neighbouring queries reach
         tiles = min(tiles, (window + TQ - 2) // 128 + 2)
-    slots = sms * (1 if ncol == 64 else 2)  # CTAs at a time
+    slots = 2 * sms  # CTAs at a time
     # few tiles for few groups: one launch, a group's tiles over a cluster
     splits = min(8, tiles, max(1, slots // groups))
     if tiles <= 4 * splits:
