@@ -91,6 +91,9 @@ APPENDS = [
     (2, 40, 32, 2, 144, 18, False, torch.bfloat16),  # nothing aligned
     (1, 300, 256, 2, 32, 30, True, torch.bfloat16),
     (1, 17, 128, 1, 512, 512, False, torch.float32),
+    (2, 20, 32, 2, 112, 28, False, torch.bfloat16),  # vectors of 2
+    (2, 20, 32, 2, 224, 46, True, torch.bfloat16),
+    (2, 20, 32, 2, 48, 36, False, torch.float32),
     (5, 0, 16, 2, 128, 64, False, torch.bfloat16),
 ]
 

@@ -71,6 +71,10 @@ CASES = [
     (2, 9, 4, 62, 34, 3, False, torch.bfloat16),   # nothing aligned
     (2, 9, 4, 62, 34, 3, True, torch.float32),
     (1, 5, 64, 130, 2, 127, False, torch.float32),
+    (2, 19, 5, 132, 52, None, False, torch.bfloat16),  # vectors of 2
+    (2, 19, 5, 102, 52, 6, True, torch.bfloat16),
+    (3, 5, 2, 22, 12, 2, False, torch.float32),
+    (3, 5, 2, 22, 14, 6, True, torch.float32),
     (4, 300, 16, 128, 64, None, False, torch.bfloat16),
     (1, 1200, 2, 256, 256, None, True, torch.bfloat16),
     (2, 3, 0, 128, 64, None, False, torch.bfloat16),
@@ -110,7 +114,7 @@ def test_strides(wb):
     f = wb.rotary_frequencies(64, device="cuda")
     positions = torch.arange(7).cuda()
     packed = torch.randn(2, 7, 6, 3 * 128, generator=g).bfloat16().cuda()
-    views = [packed[..., 128:256], packed[..., 1:129], packed[:, :, ::2, :128], packed[:, :, :, ::3],
+    views = [packed[..., 128:256], packed[..., 1:129], packed[..., 2:130], packed[:, :, ::2, :128], packed[:, :, :, ::3],
              packed.transpose(0, 1)[:, :1].transpose(0, 1)[..., :128].expand(2, 7, 6, 128),
              packed[:, :, :1, :128].expand(2, 7, 6, 128), packed[..., :128].permute(0, 2, 1, 3).contiguous().transpose(1, 2)]
     for x in views:
@@ -154,6 +158,17 @@ def test_gradient_of_shared_heads_and_sums(wb):
     assert (np.abs(_np(x.grad) - 7 * one) <= 7 * (2 * TURN + 8 * 2.0 ** -24 * 2)).all()
     with torch.no_grad():
         assert not wb.rotate(x, positions, f).requires_grad
+
+
+def test_second_derivative(wb):
+    """The gradient is a rotation too, of d_out: it can be differentiated again."""
+    g = torch.Generator().manual_seed(6)
+    f = wb.rotary_frequencies(16, device="cuda")
+    positions = torch.arange(3, 8).cuda()
+    x, d, v = (torch.randn(1, 5, 2, 24, generator=g).cuda().requires_grad_() for _ in range(3))
+    dx, = torch.autograd.grad(wb.rotate(x, positions, f, 4, True), x, d, create_graph=True)
+    dd, = torch.autograd.grad(dx, d, v)
+    _check(dd, v, positions[None], f, 4, True)
 
 
 def test_graph_and_streams(wb):

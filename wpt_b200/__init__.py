@@ -377,15 +377,15 @@ def rotary_frequencies(dims, base=10000.0, scaling=None, factor=1.0, original=No
 
 class _Rotate(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, positions, frequencies, start, interleaved, magnitude):
+    def forward(ctx, x, positions, frequencies, start, interleaved, magnitude, inverse):
         ctx.save_for_backward(positions, frequencies)
-        ctx.how = start, interleaved, magnitude
-        return ops.rotate(x, positions, frequencies, start, interleaved, magnitude)
+        ctx.how = start, interleaved, magnitude, not inverse
+        return ops.rotate(x, positions, frequencies, start, interleaved, magnitude, inverse)
 
     @staticmethod
     def backward(ctx, d_out):
-        positions, frequencies = ctx.saved_tensors
-        return ops.rotate(d_out, positions, frequencies, *ctx.how, inverse=True), None, None, None, None, None
+        turn = _Rotate.apply if _needs_grad(d_out) else ops.rotate  # a gradient to be differentiated again
+        return turn(d_out, *ctx.saved_tensors, *ctx.how), None, None, None, None, None, None
 
 
 def rotate(x, positions, frequencies, start=None, interleaved=False, magnitude=1.0):
@@ -399,7 +399,7 @@ def rotate(x, positions, frequencies, start=None, interleaved=False, magnitude=1
     returns a new tensor in x's dtype."""
     if not _needs_grad(x):
         return ops.rotate(x, positions, frequencies, start, interleaved, magnitude)
-    return _Rotate.apply(x, positions, frequencies, start, interleaved, magnitude)
+    return _Rotate.apply(x, positions, frequencies, start, interleaved, magnitude, False)
 
 
 # ---------------------------------------------------- the 8-bit paged cache

@@ -98,6 +98,24 @@ struct Vec<float, 4> {
   }
 };
 template <>
+struct Vec<__nv_bfloat16, 2> {
+  using Raw = uint32_t;
+  static __device__ __forceinline__ void widen(const Raw& r, float* x) {
+    x[0] = __uint_as_float(r << 16);
+    x[1] = __uint_as_float(r & 0xffff0000u);
+  }
+  static __device__ __forceinline__ Raw round(const float* x) { return pack_bf16(x[0], x[1]); }
+};
+template <>
+struct Vec<float, 2> {
+  using Raw = float2;
+  static __device__ __forceinline__ void widen(const Raw& r, float* x) {
+    x[0] = r.x;
+    x[1] = r.y;
+  }
+  static __device__ __forceinline__ Raw round(const float* x) { return make_float2(x[0], x[1]); }
+};
+template <>
 struct Vec<__nv_bfloat16, 1> {
   using Raw = __nv_bfloat16;
   static __device__ __forceinline__ void widen(const Raw& r, float* x) { x[0] = __bfloat162float(r); }
