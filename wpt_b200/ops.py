@@ -1040,9 +1040,14 @@ def _paged_plan_for(B, T, H, N, window, sms):
     if window:  # what neighbouring queries reach
         tiles = min(tiles, (window + TQ - 2) // 128 + 2)
     slots = 2 * sms  # CTAs at a time
-    # few tiles for few groups: one launch, a group's tiles over a cluster
-    splits = min(8, tiles, max(1, slots // groups))
-    if tiles <= 4 * splits:
+    # Few tiles a CTA: one launch, a group's tiles over a cluster. A cluster's CTAs share a GPC (on B200 8 of 16 to 20
+    # SMs), and more clusters than fit run in two waves: past two CTAs, 7/8 of the slots (33 clusters of 8 11.6 us, 34
+    # 19.0; 44 of 6 11.7, 46 20.1). Rows of uneven lengths wait for the longest there; balanced, all CTAs end together,
+    # but parts are written and merged in a second launch. Equal and ragged lengths (1/32 to all), us, cluster then
+    # balanced: 16 rows of 4,096 12.3, 12.4 and 11.5, 11.7, of 8,192 15.6, 14.0 and 14.5, 12.5; where clusters fill the
+    # SMs, 64 rows of 4,096 16.0, 19.6 and 15.3, 16.7, of 8,192 29.9, 33.8 and 22.7, 21.1.
+    splits = next(s for s in range(min(8, tiles), 0, -1) if s == 1 or groups * s <= (slots if s == 2 else slots * 7 // 8))
+    if tiles <= (10 if groups * splits > slots * 3 // 4 else 4) * splits:
         return splits, 1
     if groups <= 256 and groups * (math.ceil(N / 128) + 8) < 2 ** 31:
         return 0, min(slots, groups * tiles)
