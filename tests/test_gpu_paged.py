@@ -222,10 +222,10 @@ ATTENDS = [
     (2, 1, 16, 32, 5, 0, True),
     (3, 1, 32, 64, 9, 0, False),
     (5, 1, 12, 128, 3, 100, True),
-    (2, 1, 64, 256, 2, 0, False),
+    (2, 1, 64, 256, 2, 0, False),      # two groups a query
     (3, 4, 8, 16, 21, 0, True),        # 32 columns
-    (2, 5, 12, 32, 17, 0, True),       # 60 columns
-    (2, 9, 12, 64, 5, 37, False),      # two groups a row
+    (2, 5, 12, 32, 17, 0, True),       # three groups a row
+    (2, 9, 12, 64, 5, 37, False),      # five
     (1, 70, 1, 16, 12, 50, True),      # 70 queries of one head
     (4, 3, 21, 128, 7, 300, True),
     (40, 1, 32, 64, 11, 0, False),     # balanced over the CTAs
