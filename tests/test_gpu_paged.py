@@ -373,6 +373,36 @@ def test_scores_that_jump(wb):
         assert (np.abs(_np(got[0]) - ref) <= 2.0 ** -8 * np.abs(ref) + (2.0 ** -8.6 + 2 * SCORE + 2 * slack) * 8).all()
 
 
+@pytest.mark.parametrize("T,H", [(1, 16), (4, 8), (3, 12), (1, 64)])
+def test_heads_and_padding_of_other_sizes(wb, T, H):
+    """Heads whose queries are 2^-20 to 1 of the others', and padding queries of up to 2^120 next to live ones: each
+    column's result is as if it were alone. (Smaller queries' scores are off by less; the padding's own are not
+    looked at, but for being there.)"""
+    g = torch.Generator().manual_seed(23)
+    B, S, M = 4, 32, 9
+    pages, scales, table = _filled(B, M, S, 128, g)
+    q = _queries(B, T, H, g) * torch.exp2(torch.randint(-20, 1, (B, 1, H, 1), generator=g).float()).bfloat16()
+    q[2, :, H // 2] = 0
+    positions = torch.full((B, 1), M * S - T) + torch.arange(T)
+    cache = _cache(pages, scales)
+    dev = [t.cuda() for t in (pages, scales, table, positions)]
+    plain = wb.paged_attention(q.cuda(), *dev, 128 ** -0.5)
+    _check_attention(plain, q, cache, table, positions, 128 ** -0.5)
+    padded = q.clone()
+    padded[0, T - 1, H - 1] *= 2.0 ** 120
+    padded[1, 0, 0] = 2.0 ** 100
+    padded[3, :, ::2] *= 2.0 ** 30
+    got = wb.paged_attention(padded.cuda(), *dev, 128 ** -0.5)
+    same = (padded == q).all(-1)
+    assert same.sum() > 0
+    ref = torch.where(same[..., None], padded, 0).bfloat16()  # the padding's columns as zeros, which the check passes over
+    out, lse = got[0].clone(), got[1].clone()
+    zero = wb.paged_attention(ref.cuda(), *dev, 128 ** -0.5)
+    out[~same.cuda()], lse[~same.cuda()] = zero[0][~same.cuda()], zero[1][~same.cuda()]
+    _check_attention((out, lse), ref, cache, table, positions, 128 ** -0.5)
+    assert wb.device_status() == 0
+
+
 def test_scales_of_all_sizes(wb):
     """Blocks of zeros (scale 0, or the least), and blocks whose values are far larger or smaller than the others'."""
     g = torch.Generator().manual_seed(17)

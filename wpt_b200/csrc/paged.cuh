@@ -396,7 +396,10 @@ __global__ void __launch_bounds__(APPEND_THREADS, ROWS ? 8 : 1) paged_append_ker
 // columns of the same product, whose M (the streamed side) is read once:
 //   q (bf16, 8 significant bits), by a power of two that brings the group's
 //   largest value into 224 .. 448, is hi + lo / 16, both e4m3: exact down to
-//   2^-10 of that value, and within 2^-22.8 of it below.
+//   2^-10 of that value, and within 2^-22.8 of it below. Where a column's own
+//   largest value is under 2^-6 of the group's (a head that is off, or a
+//   padding query of anything next to it), each column has a power of two of
+//   its own, and a tile's scores are multiplied by them where they lie.
 //   a weight w = 2^x, as fp16 (11 significant bits) 3 e5m2 numbers, each the
 //   upper byte (e5m2 is fp16's) of what the ones before it leave, the last one
 //   times 32 and rounded: within 2^-8.6 w (2^-9, and fp16's 2^-11; a bf16
@@ -455,6 +458,7 @@ struct PagedParams {
 };
 
 constexpr float PAGED_TOP = 15.f;  // weights up to 2^15 (fp16 ends at 2^16)
+constexpr uint32_t PAGED_EVEN = 6u << 23;  // 2^6 between columns' largest values, up to which they share a power of two
 // Minus the base of a column that has read nothing: any score is past it.
 constexpr float PAGED_UNSET = 1e30f;
 
@@ -476,7 +480,8 @@ struct PagedLayout {
   static constexpr int OFF_ALPHA = OFF_RED + 4 * NCOL * 4;   // the factor of a rescaled column, 1 for others
   static constexpr int OFF_L = OFF_ALPHA + NCOL * 4;
   static constexpr int OFF_TOP = OFF_L + NCOL * 4;           // a column's largest exponent, where it is to be raised
-  static constexpr int OFF_SCALE = OFF_TOP + NCOL * 4;         // 2 tiles x 8 blocks x float4
+  static constexpr int OFF_POWER = OFF_TOP + NCOL * 4;       // a column's own power of two, where they are uneven
+  static constexpr int OFF_SCALE = OFF_POWER + NCOL * 4;       // 2 tiles x 8 blocks x float4
   static constexpr int OFF_NAN = OFF_SCALE + 2 * 8 * 16;     // 4 words a column
   static constexpr int OFF_QLO = OFF_NAN + NCOL * 16;
   static constexpr int OFF_QHI = OFF_QLO + 32 * 4;
@@ -675,6 +680,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, 2)
   float* s_alpha = reinterpret_cast<float*>(smem + L::OFF_ALPHA);
   float* s_l = reinterpret_cast<float*>(smem + L::OFF_L);
   int* s_top = reinterpret_cast<int*>(smem + L::OFF_TOP);
+  float* s_power = reinterpret_cast<float*>(smem + L::OFF_POWER);
   float4* s_scale = reinterpret_cast<float4*>(smem + L::OFF_SCALE);
   uint32_t* s_nan = reinterpret_cast<uint32_t*>(smem + L::OFF_NAN);
   int* s_qlo = reinterpret_cast<int*>(smem + L::OFF_QLO);
@@ -1001,34 +1007,30 @@ __global__ void __launch_bounds__(PAGED_THREADS, 2)
       alo = __reduce_max_sync(0xffffffffu, alo);
       ahi = __reduce_min_sync(0xffffffffu, ahi);
       // q: the group's largest value, then hi and lo rows. A query with an infinity or NaN has no result but NaN.
-      uint32_t top_q = 0u;
+      uint32_t col_q[NCOL / 4], top_q = 0u;
 #pragma unroll
       for (int i = 0; i < NCOL / 4; ++i) {
-        const int col = warp + 4 * i;
-        if (col >= ncols) ahead_q[i] = make_uint2(0u, 0u);
+        if (warp + 4 * i >= ncols) ahead_q[i] = make_uint2(0u, 0u);
         const uint2 raw = ahead_q[i];
+        col_q[i] = 0u;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const uint32_t bits = (((k & 2) ? raw.y : raw.x) << ((k & 1) ? 0 : 16)) & 0x7fff0000u;
-          top_q = max(top_q, bits < 0x7f800000u ? bits : 0u);
+          col_q[i] = max(col_q[i], bits < 0x7f800000u ? bits : 0u);
         }
+        top_q = max(top_q, col_q[i]);
       }
       top_q = __reduce_max_sync(0xffffffffu, top_q);
       if (lane == 0) s_sum[warp] = static_cast<int>(top_q);
       named_barrier(1, 128);
       top_q = max(max(s_sum[0], s_sum[1]), max(s_sum[2], s_sum[3]));
-      const int e_q = scale_exponent(top_q, -100);
-      const float inv_q = power_of_two(-e_q), factor = power_of_two(e_q) * p.scale_log2;
-#pragma unroll
-      for (int i = 0; i < NCOL / 4; ++i) {
-        const int col = warp + 4 * i;
-        const uint2 raw = ahead_q[i];
+      auto put_q = [&](int col, const uint2& raw, float inv) {  // a column's hi and lo rows, this lane's four channels
         float x[4] = {__uint_as_float(raw.x << 16), __uint_as_float(raw.x & 0xffff0000u),
                       __uint_as_float(raw.y << 16), __uint_as_float(raw.y & 0xffff0000u)};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const bool finite = (__float_as_uint(x[k]) & 0x7fffffffu) < 0x7f800000u;
-          x[k] = finite ? x[k] * inv_q : __int_as_float(0x7fffffff);
+          x[k] = finite ? x[k] * inv : __int_as_float(0x7fffffff);
         }
         const uint32_t hi = pack_e4m3x4(x[0], x[1], x[2], x[3]);
         const uint32_t u = unpack_e4m3x2(hi & 0xffffu), w = unpack_e4m3x2(hi >> 16);
@@ -1037,10 +1039,38 @@ __global__ void __launch_bounds__(PAGED_THREADS, 2)
         const uint32_t chunk = lane >> 2, in = (lane & 3) * 4;
         *reinterpret_cast<uint32_t*>(sQ + sw128_offset(col, chunk) + in) = hi;
         *reinterpret_cast<uint32_t*>(sQ + sw128_offset(NCOL + col, chunk) + in) = lo;
+      };
+      const int e_q = scale_exponent(top_q, -100);
+      const float inv_q = power_of_two(-e_q);
+      float factor = power_of_two(e_q) * p.scale_log2;
+      const uint32_t small = top_q > PAGED_EVEN ? top_q - PAGED_EVEN : 0u;
+      bool uneven = false;
+#pragma unroll
+      for (int i = 0; i < NCOL / 4; ++i) {
+        put_q(warp + 4 * i, ahead_q[i], inv_q);
+        uneven |= !__any_sync(0xffffffffu, col_q[i] >= small) && __any_sync(0xffffffffu, col_q[i] != 0u);
+      }
+      uneven = named_barrier_or(1, 128, uneven);  // s_qlo, s_qhi too; s_sum is read
+      if (uneven) {
+        factor = p.scale_log2;
+#pragma unroll 1
+        for (int col = warp; col < ncols; col += 4) {
+          const uint2 raw = *reinterpret_cast<const uint2*>(p.q + (static_cast<int64_t>(group.row0) + col) * C + lane * 4);
+          uint32_t top = 0u;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t bits = (((k & 2) ? raw.y : raw.x) << ((k & 1) ? 0 : 16)) & 0x7fff0000u;
+            top = max(top, bits < 0x7f800000u ? bits : 0u);
+          }
+          const int e_col = scale_exponent(__reduce_max_sync(0xffffffffu, top), -100);
+          put_q(col, raw, power_of_two(-e_col));
+          if (lane == 0) s_power[col] = power_of_two(e_col);
+        }
+        if (r >= ncols && r < NCOL) s_power[r] = 0.f;
+        named_barrier(1, 128);
       }
       fence_proxy_async();
       mbar_arrive(q_full);
-      named_barrier(1, 128);  // s_qlo, s_qhi; s_sum is read
 
       // softmax: thread r = key r. Pairs of columns: minus bases, sums, exponents
       uint64_t nb[NCOL / 2], lp[NCOL / 2], e[NCOL / 2];
@@ -1073,6 +1103,21 @@ __global__ void __launch_bounds__(PAGED_THREADS, 2)
         // kept short: such code is fetched anew each time. (A wait that failed is carried to the barriers, where all
         // warps agree to stop.)
         const uint32_t sa = lane_addr + (j & 1) * L::S_COLS;
+        if (uneven) {
+#pragma unroll 1
+          for (int c = 0; c < NCOL; c += 16) {
+            uint32_t x[16], y[16];
+            tmem_ld16x2(sa + c, sa + NCOL + c, x, y);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              x[k] = __float_as_uint(fmaf(__uint_as_float(y[k]), 0.0625f, __uint_as_float(x[k])) * s_power[c + k]);
+              y[k] = 0u;
+            }
+            tmem_st16(sa + c, x);
+            tmem_st16(sa + NCOL + c, y);
+          }
+          tmem_wait_st();
+        }
         auto score = [&](uint32_t hi, uint32_t lo) {
           return fmaf(fmaf(__uint_as_float(lo), 0.0625f, __uint_as_float(hi)), fk, sc.y);
         };
