@@ -402,7 +402,8 @@ int wpt_paged_append(const void* src, int f32, int64_t src_stride_b, int64_t src
  * reads the row's entries max(0, p - window + 1) .. min(p, M S - 1), p =
  * positions[b, t] (window 0: no window), but for those on no page; q, out, lse
  * and sink as above. What other entries hold (NaN too) reaches no result.
- * Value scales are 0, or 2^-60 to 2^60.
+ * Value scales are 0, or 2^-60 to 2^60 (where those of one row lie 2^112 and
+ * more apart, weights under 2^-6 of small values may be lost).
  *   splits     how the work is split. 1 to 8: each query group's entries go to
  *              that many CTAs in equal runs, a thread-block cluster where more
  *              than one; ctas and scratch are not used. 0: all groups' entries

@@ -127,8 +127,10 @@ constexpr int APPEND_THREADS = 128;
 // turned and widened to fp32, their largest value gives the scale, and they are
 // rounded. ROWS: a warp takes an entry, a lane a vector of it (with halves, the
 // other channels of its pairs come from the lane that loaded them), and the
-// entries stay in registers; else they go through shared memory. Bound by HBM for prompts; a step of one entry a row is a chain of
-// three loads (first, the page's number, its scale).
+// entries stay in registers; else they go through shared memory. Prompts (16
+// rows of 4,096, 2 x 128, all key channels turned: 25 us for 50 MB) are bound by
+// issue slots, 1,380 instructions for a warp's four entries; a step of one entry
+// a row (2.8 us) is a chain of three loads (first, the page's number, its scale).
 template <class T, int VE, bool INTERLEAVED, bool ROWS>
 __global__ void __launch_bounds__(APPEND_THREADS, ROWS ? 8 : 1) paged_append_kernel(const AppendParams p) {
   using V = Vec<T, VE>;
@@ -427,13 +429,14 @@ __global__ void __launch_bounds__(APPEND_THREADS, ROWS ? 8 : 1) paged_append_ker
 // TMA, a box for each page of a tile; warp 6 brings the scales. Two CTAs share
 // an SM (64 columns: one), so that one's exponents run under the other's loads.
 //
-// What bounds it: at 64 rows of 4,097 to 32,768 keys and 16 columns HBM and the
+// What bounds it: at 64 rows of 1,024 to 32,768 keys and 32 columns HBM and the
 // softmax warps' instructions about equally, 60 us for 278 MB (4.6 TB/s), of
-// which 5 are the merge; one row of 131,071 keys and 64 drafts of 10,000 keys are
-// chains of latencies: the groups' tiles, a page's number, its tile, the products,
-// the parts, the merge (26 and 17 us). A segment's fixed cost is code that is
-// fetched anew for it (the kernel is larger than the instruction cache), which is
-// why what runs once a segment is in loops that are not unrolled.
+// which 5 are the merge; one row of 262,144 keys (26 us) and 7 rows of 5 drafts
+// of 12 heads over up to 6,007 (16 us) are chains of latencies: the groups'
+// tiles, a page's number, its tile, the products, the parts, the merge. A
+// segment's fixed cost is code that is fetched anew for it (the kernel is larger
+// than the instruction cache), which is why what runs once a segment is in loops
+// that are not unrolled.
 struct PagedParams {
   const __nv_bfloat16* q;        // (B, T, H, 128) contiguous
   const float* scales;

@@ -186,7 +186,7 @@ struct RotateAt {
 // come out even (0, 1 or 2: all lanes then do the same work and have 2 to 4
 // loads in flight for each of two heads); else (-1) they are items of their own.
 // Bound by HBM: 8 x 4,096 tokens of 16 heads of 128, 64 turned (134 MB in, 134
-// out). A vector a thread, its partner from the lane that owns it (51 us there)
+// out) take 44 us, 6.1 TB/s. A vector a thread, its partner from the lane that owns it (51 us there)
 // or from L1 (67 us: it was read from L2 twice), was no faster.
 template <class T, int VE, bool INTERLEAVED, int COPIES>
 __global__ void __launch_bounds__(256) rotate_kernel(const RotateParams p) {
