@@ -571,6 +571,53 @@ def test_graphs_and_streams(wb):
         assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(after, dev))
 
 
+def test_two_streams_at_once(wb):
+    """Balanced calls (with scratch) and appends to different pools on two streams, over and over: what one alone gives."""
+    g = torch.Generator().manual_seed(24)
+    sides, runs = [torch.cuda.Stream() for _ in range(2)], []
+    for B, H, S, M in ((5, 16, 16, 200), (3, 24, 32, 150)):
+        pages, scales, table = _filled(B, M, S, 128, g)
+        dev = [t.cuda() for t in (pages, scales, table)]
+        q, new = _queries(B, 2, H, g).cuda(), torch.randn(B, 2, 256, generator=g).bfloat16().cuda()
+        first, counts = torch.randint(0, M * S - 2, (B,), generator=g).cuda(), torch.full((B,), 2).cuda()
+        wb.paged_append(*dev, new, first, counts)
+        positions = first[:, None] + torch.arange(2).cuda()
+        runs.append((dev, q, new, first, counts, positions, wb.paged_attention(q, *dev, positions, 128 ** -0.5)))
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for k, (side, (dev, q, new, first, counts, positions, _)) in enumerate(zip(sides, runs)):
+            with torch.cuda.stream(side):
+                wb.paged_append(*dev, new, first, counts)  # the same entries again
+                got[k].append(wb.paged_attention(q, *dev, positions, 128 ** -0.5))
+    torch.cuda.synchronize()
+    for outs, run in zip(got, runs):
+        for out in outs:
+            assert torch.equal(out[0], run[-1][0]) and torch.equal(out[1], run[-1][1])
+    assert wb.device_status() == 0
+
+
+def test_offsets_past_32_bits(wb):
+    """A pool of 5 GB: rows on its last pages, on its first, and on both."""
+    g = torch.Generator().manual_seed(25)
+    B, n, S, M, P = 3, 50, 64, 2, 327_680
+    pages, scales = wb.paged_cache(P, S, 128)
+    assert pages.numel() > 2 ** 32
+    table = torch.tensor([[P - 1, P - 2], [0, 1], [2, P - 3]])
+    new = torch.randn(B, n, 256, generator=g).bfloat16()
+    first, counts = torch.tensor([70, 0, 40]), torch.tensor([50, 50, 50])
+    wb.paged_append(pages, scales, table.cuda(), new.cuda(), first.cuda(), counts.cuda())
+    used = torch.tensor([P - 1, P - 2, 0, 1, 2, P - 3])
+    near = torch.tensor([[0, 1], [2, 3], [4, 5]])
+    few = pages.view(torch.uint8)[used.cuda()].view(torch.float8_e4m3fn), scales[used.cuda()]
+    empty = dict(values=np.zeros((6, S, 256)), scales=np.zeros((6, S // 16, 2)))
+    _check_append(few, empty, near, new, first, counts)
+    q, positions = _queries(B, 1, 8, g), (first + n - 1)[:, None]
+    got = wb.paged_attention(q.cuda(), pages, scales, table.cuda(), positions.cuda(), 128 ** -0.5)
+    _check_attention(got, q, _cache(*few), near, positions, 128 ** -0.5)
+    assert wb.device_status() == 0
+
+
 def test_refusals(wb):
     pages, scales = wb.paged_cache(4, 32, 128)
     table, p = torch.zeros(2, 3, dtype=torch.int32, device="cuda"), torch.zeros(2, 1, dtype=torch.int64, device="cuda")

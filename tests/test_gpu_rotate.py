@@ -171,6 +171,20 @@ def test_second_derivative(wb):
     _check(dd, v, positions[None], f, 4, True)
 
 
+def test_more_than_32_bits_of_elements(wb):
+    """2.2e9 elements: the ends are as in calls of their own."""
+    B, T, H, C = 33, 8192, 64, 128
+    x = torch.empty(B, T, H, C, dtype=torch.bfloat16, device="cuda")
+    assert x.numel() > 2 ** 31
+    x[0], x[-1] = torch.randn(2, T, H, C, device="cuda")
+    f = wb.rotary_frequencies(40, device="cuda")
+    positions = torch.arange(T, device="cuda") + 5
+    y = wb.rotate(x, positions, f, 20)
+    for b in (0, B - 1):
+        assert torch.equal(y[b:b + 1], wb.rotate(x[b:b + 1], positions, f, 20))
+    _check(y[-1:, -3:], x[-1:, -3:], positions[None, -3:], f, 20, False)
+
+
 def test_graph_and_streams(wb):
     f = wb.rotary_frequencies(64, device="cuda")
     x = torch.randn(2, 9, 4, 128).bfloat16().cuda()

@@ -439,7 +439,7 @@ def paged_attention(q, pages, scales, table, positions, scale, window=0, sink=No
     entries 0 .. position (given a window, the last `window` of them), with
     sink (H,) in each head's denominator. Entries on no page are not read, and
     what they and entries past the position hold reaches no result. Made for few
-    queries a row (decode, drafts); any number is computed, 64 / H at a time.
+    queries a row (decode, drafts); any number is computed, 32 / H at a time.
     Returns (out (B, T, H, 128) bf16, lse (B, T, H) fp32); 0 and -inf (or the
     sink) for a query without entries. Not differentiable."""
     _bf16_only(q)
