@@ -442,8 +442,7 @@ def paged_attention(q, pages, scales, table, positions, scale, window=0, sink=No
     queries a row (decode, drafts); any number is computed, 32 / H at a time.
     Returns (out (B, T, H, 128) bf16, lse (B, T, H) fp32); 0 and -inf (or the
     sink) for a query without entries. Not differentiable."""
-    _bf16_only(q)
-    return ops.paged_attention(q, pages, scales, table, _positions(positions, q.shape[0]), scale, window, sink)
+    return ops.paged_attention(q, pages, scales, table, positions, scale, window, sink)
 
 
 # ------------------------------------------------------------- installation

@@ -921,7 +921,7 @@ _PAGE_LAYOUTS = {}  # what _pages found for shapes, strides and types that it ha
 
 
 def _pages(pages, scales, table):
-    """Checks a paged cache's tensors; (P, S, C, M)."""
+    """Checks a paged cache's tensors; (P, S, C, B, M)."""
     ps, pt, ss, st, ts = pages.shape, pages.stride(), scales.shape, scales.stride(), table.shape
     key = ps, pt, ss, st, ts, pages.dtype, scales.dtype, table.dtype
     found = _PAGE_LAYOUTS.get(key)
@@ -952,7 +952,7 @@ def _page_layout(ps, pt, ss, st, ts, pages_dtype, scales_dtype, table_dtype):
         raise ValueError("scales must be contiguous within a page")
     if (P | S | ts[1] | ts[1] * S) >> 31:
         raise NotImplementedError(f"{P} pages of {S} entries, {ts[1]} a row: past the library's 32-bit arguments")
-    return P, S, C2 // 2, ts[1]
+    return P, S, C2 // 2, ts[0], ts[1]
 
 
 def _table_rows(table):
@@ -987,11 +987,11 @@ def paged_append(pages, scales, table, new, first, counts, frequencies=None, pos
             first.device == device and counts.device == device and
             (frequencies is None or frequencies.device == device) and (positions is None or positions.device == device)):
         _one_device(pages, scales, table, new, first, counts, frequencies, positions)
-    P, S, C, M = _pages(pages, scales, table)
+    P, S, C, B, M = _pages(pages, scales, table)
     f32 = new.dtype is torch.float32
     if not f32 and new.dtype is not torch.bfloat16:
         raise NotImplementedError(f"the append kernel takes bfloat16 or float32 entries; got {new.dtype}")
-    B, shape = table.shape[0], new.shape
+    shape = new.shape
     if len(shape) != 3 or shape[0] != B or shape[2] != 2 * C or first.shape != (B,) or counts.shape != (B,):
         raise ValueError(f"entries {tuple(shape)} for a table of {B} rows and pages of 2 x {C}, with first "
                          f"{tuple(first.shape)} and counts {tuple(counts.shape)}")
@@ -1031,6 +1031,15 @@ def _paged_plan(B, T, H, N, window, sms):
     return plan
 
 
+def _paged_scratch(B, T, H, ctas):
+    """The scratch of a balanced call in bf16 elements, remembered per shape."""
+    key = ("paged scratch", B, T, H, ctas)
+    size = _PLAN_CACHE.get(key)
+    if size is None:
+        size = _PLAN_CACHE[key] = (_lib.lib().wpt_paged_scratch_bytes(B, T, H, 0, ctas) + 1) // 2
+    return size
+
+
 def _paged_plan_for(B, T, H, N, window, sms):
     ncol = 16 if T * H <= 16 else 32
     chunks = math.ceil(H / 32)  # groups that a query's heads take
@@ -1064,12 +1073,12 @@ def paged_attention(q, pages, scales, table, positions, scale, window=0, sink=No
     if not (q.is_cuda and pages.device == device and scales.device == device and table.device == device and
             positions.device == device and (sink is None or sink.device == device)):
         _one_device(q, pages, scales, table, positions, sink)
-    P, S, C, M = _pages(pages, scales, table)
+    P, S, C, rows, M = _pages(pages, scales, table)
     _bf16(q)
-    shape = q.shape
-    if len(shape) != 4 or shape[3] != C or table.shape[0] != shape[0] or positions.shape != shape[:2]:
-        raise ValueError(f"queries {tuple(shape)} with pages of 2 x {C}, a table of {table.shape[0]} rows and "
-                         f"positions {tuple(positions.shape)}")
+    shape, at = q.shape, positions.shape
+    if len(shape) != 4 or shape[3] != C or rows != shape[0] or at[-1:] != shape[1:2] or \
+            not (len(at) == 1 or len(at) == 2 and at[0] in (1, rows)):
+        raise ValueError(f"queries {tuple(shape)} with pages of 2 x {C}, a table of {rows} rows and positions {tuple(at)}")
     B, T, H, _ = shape
     if sink is not None and sink.shape != (H,):
         raise ValueError(f"sink must be {(H,)}; got {tuple(sink.shape)}")
@@ -1081,7 +1090,7 @@ def paged_attention(q, pages, scales, table, positions, scale, window=0, sink=No
     window = min(window, 2 ** 31 - 1)  # past every table
     if not q.is_contiguous() or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
-    positions = _rows(positions)
+    positions = _rows(positions if len(at) == 2 and at[0] == B else positions.expand(B, -1))
     table = _table_rows(table)
     if sink is not None and (sink.dtype is not torch.float32 or not sink.is_contiguous()):
         sink = sink.float().contiguous()
@@ -1093,7 +1102,7 @@ def paged_attention(q, pages, scales, table, positions, scale, window=0, sink=No
     lib = _lib.lib()
     scratch = None
     if splits == 0:
-        scratch = torch.empty(lib.wpt_paged_scratch_bytes(B, T, H, splits, ctas), dtype=torch.uint8, device=device)
+        scratch = q.new_empty(_paged_scratch(B, T, H, ctas))
     ps = pages.stride()
     _call(device, lib.wpt_paged_attention,
           (q.data_ptr(), pages.data_ptr(), ps[0], ps[1], scales.data_ptr(), scales.stride(0), table.data_ptr(),
