@@ -73,6 +73,7 @@ struct AppendParams {
   int B, n, C, M, P, dims, start;
   int blocks;                      // grid blocks a row
   int turn_rows, turn_pairs;       // APPEND_THREADS / (dims / 2), and the rest
+  int vecs, inv_vecs;              // ROWS: vectors of a key, and 65536 / vecs + 1
   float magnitude;
 };
 
@@ -109,14 +110,21 @@ struct TurnedVector {
         u[2 * k + 1] = b;
       }
     } else {
+      const float sign = front ? -1.f : 1.f;
 #pragma unroll
       for (int k = 0; k < VE; ++k) {  // x_a cos - x_b sin, or x_b cos + x_a sin
-        const float s = front ? -sn[k] : sn[k];
-        u[k] = __fadd_rn(__fmul_rn(u[k], cs[k]), __fmul_rn(z[k], s));
+        u[k] = __fmaf_rn(__fmul_rn(z[k], sn[k]), sign, __fmul_rn(u[k], cs[k]));
       }
     }
   }
 };
+
+// max(|x|, |y|, m), NaN ignored
+__device__ __forceinline__ float max_abs(float x, float y, float m) {
+  float r;
+  asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(m));
+  return r;
+}
 
 constexpr int APPEND_THREADS = 128;
 
@@ -125,12 +133,13 @@ constexpr int APPEND_THREADS = 128;
 // (a table in shared memory: 16 x dims / 2 pairs, where the lanes that turn
 // would each compute 8 a token while the others wait), the new entries are
 // turned and widened to fp32, their largest value gives the scale, and they are
-// rounded. ROWS: a warp takes an entry, a lane a vector of it (with halves, the
-// other channels of its pairs come from the lane that loaded them), and the
-// entries stay in registers; else they go through shared memory. Prompts (16
-// rows of 4,096, 2 x 128, all key channels turned: 25 us for 50 MB) are bound by
-// issue slots, 1,380 instructions for a warp's four entries; a step of one entry
-// a row (2.8 us) is a chain of three loads (first, the page's number, its scale).
+// rounded. ROWS: a warp takes four entries, their keys and values apart, so that
+// all its lanes turn or none; a lane has a vector (with halves, the other
+// channels of its pairs come from the lane that loaded them), and the entries
+// stay in registers; else they go through shared memory. Prompts (16 rows of
+// 4,096, 2 x 128, all key channels turned: 23 us for 50 MB) are bound by issue
+// slots, a third of them for angles; a step of one entry a row (2.8 us) is a
+// chain of three loads (first, the page's number, its scale).
 template <class T, int VE, bool INTERLEAVED, bool ROWS>
 __global__ void __launch_bounds__(APPEND_THREADS, ROWS ? 8 : 1) paged_append_kernel(const AppendParams p) {
   using V = Vec<T, VE>;
@@ -163,14 +172,24 @@ __global__ void __launch_bounds__(APPEND_THREADS, ROWS ? 8 : 1) paged_append_ker
   const int64_t row0 = lo - first;  // the first new entry's number
   const T* src = static_cast<const T*>(p.src) + b * p.ssb + row0 * p.ssn;
   const int half = p.dims >> 1;
-  constexpr int MINE = PAGE_BLOCK / WARPS;  // ROWS: entries of a warp: warp, warp + WARPS, ...
-  const int ca = lane * VE;             // and the lane's first channel
-  const bool some = ca < 2 * p.C;
-  Raw raw[MINE];
+  // ROWS: a warp has 4 entries, 32 / vecs of them at a time, first their keys, then their values
+  constexpr int MINE = PAGE_BLOCK / WARPS, GROUPS = 2;
+  const int sub = lane * p.inv_vecs >> 16, vec = lane - sub * p.vecs, each = (32 * p.inv_vecs) >> 16;
+  auto entry_of = [&](int g) {  // this lane's of group g, `live` or more: none
+    const int e = g * each + sub;
+    return sub < each && e < MINE ? MINE * warp + e : PAGE_BLOCK;
+  };
+  Raw raw[GROUPS][2];
   if constexpr (ROWS) {
 #pragma unroll
-    for (int q = 0; q < MINE; ++q)
-      if (some && warp + WARPS * q < live) raw[q] = *reinterpret_cast<const Raw*>(src + (warp + WARPS * q) * p.ssn + ca);
+    for (int g = 0; g < GROUPS; ++g) {
+      const int i = entry_of(g);
+      if (i < live) {
+        const T* x = src + i * p.ssn + vec * VE;
+        raw[g][0] = *reinterpret_cast<const Raw*>(x);
+        raw[g][1] = *reinterpret_cast<const Raw*>(x + p.C);
+      }
+    }
   }
   float2* s_turn = reinterpret_cast<float2*>(s_all);
   float* s_val = s_all + PAGE_BLOCK * p.dims;
@@ -207,40 +226,49 @@ __global__ void __launch_bounds__(APPEND_THREADS, ROWS ? 8 : 1) paged_append_ker
   }
   if (p.dims > 0) __syncthreads();
 
-  // turned and widened values, and the bits of the largest absolute ones (NaN's above all)
+  // turned and widened values, and the bits of the largest absolute ones of keys and values
   uint32_t amax[2] = {0u, 0u};
   auto note = [](float v, uint32_t& m) { m = max(m, __float_as_uint(v) & 0x7fffffffu); };
-  float u[ROWS ? MINE : 1][VE];
+  float u[ROWS ? 2 * GROUPS : 1][VE];
   if constexpr (ROWS) {
-    const TurnedVector<VE, INTERLEAVED> tv(ca < p.C ? lane : -1 - p.dims, p.start, p.dims);
-    uint32_t m = 0u;
+    const TurnedVector<VE, INTERLEAVED> tv(vec, p.start, p.dims);
+    float most[2] = {0.f, 0.f};
 #pragma unroll
-    for (int q = 0; q < MINE; ++q) {
-      if (warp + WARPS * q >= live) break;  // the whole warp
-      Raw z = raw[q];
-      if constexpr (!INTERLEAVED) z = V::from_lane(raw[q], lane + tv.partner);
-      V::widen(raw[q], u[q]);
-      if (tv.turned) {
-        float c[VE], sn[VE], cs[VE];
-        V::widen(z, c);
-        const float4* at = reinterpret_cast<const float4*>(s_turn + (warp + WARPS * q) * half + tv.pair);
-#pragma unroll
-        for (int k = 0; k < (INTERLEAVED ? VE / 2 : VE); k += 2) {
-          const float4 t = at[k / 2];
-          sn[k] = t.x;
-          cs[k] = t.y;
-          sn[k + 1] = t.z;
-          cs[k + 1] = t.w;
-        }
-        tv.turn(u[q], c, sn, cs);
+    for (int g = 0; g < GROUPS; ++g) {
+      if (MINE * warp + g * each >= live || g * each >= MINE) break;  // the whole warp
+      const int i = entry_of(g);
+      Raw z = raw[g][0];
+      if constexpr (!INTERLEAVED) {
+        if (p.dims > 0) z = V::from_lane(raw[g][0], lane + tv.partner);
       }
-      if (some) {
+      if (i < live) {
+        float(&key)[VE] = u[2 * g];
+        float(&value)[VE] = u[ROWS ? 2 * g + 1 : 0];
+        V::widen(raw[g][0], key);
+        V::widen(raw[g][1], value);
+        if (tv.turned) {
+          float c[VE], sn[VE], cs[VE];
+          V::widen(z, c);
+          const float4* at = reinterpret_cast<const float4*>(s_turn + i * half + tv.pair);
 #pragma unroll
-        for (int k = 0; k < VE; ++k) note(u[q][k], m);
+          for (int k = 0; k < (INTERLEAVED ? VE / 2 : VE); k += 2) {
+            const float4 t = at[k / 2];
+            sn[k] = t.x;
+            cs[k] = t.y;
+            sn[k + 1] = t.z;
+            cs[k + 1] = t.w;
+          }
+          tv.turn(key, c, sn, cs);
+        }
+#pragma unroll
+        for (int k = 0; k < VE; k += 2) {
+          most[0] = max_abs(key[k], key[k + 1], most[0]);
+          most[1] = max_abs(value[k], value[k + 1], most[1]);
+        }
       }
     }
-    amax[0] = ca < p.C ? m : 0u;
-    amax[1] = ca < p.C ? 0u : m;
+    amax[0] = __float_as_uint(most[0]);
+    amax[1] = __float_as_uint(most[1]);
   } else {
     // items: pairs (with VE > 1, vectors of them), then the channels that do not turn
     constexpr bool ONE = INTERLEAVED && VE > 1;  // an item is one vector of whole pairs
@@ -299,63 +327,64 @@ __global__ void __launch_bounds__(APPEND_THREADS, ROWS ? 8 : 1) paged_append_ker
     for (int h = 0; h < 2; ++h) amax[h] = __reduce_max_sync(0xffffffffu, s_red[lane % WARPS][h]);
   };
   largest();
-  // infinities, NaN and values past 448 * 2^60 do not count (seldom: looked at again without them), and become NaN
-  const bool huge = max(amax[0], amax[1]) > SCALE_TOP_BITS;
-  auto fits = [](float v) { return (__float_as_uint(v) & 0x7fffffffu) <= SCALE_TOP_BITS; };
-  if (huge) {
+  // infinities and values past 448 * 2^60 do not count (seldom: looked at again without them), and become NaN
+  if (max(amax[0], amax[1]) > SCALE_TOP_BITS) {
     amax[0] = amax[1] = 0u;
-    uint32_t m = 0u;
+    auto again = [&](float& v, uint32_t& m) {
+      if ((__float_as_uint(v) & 0x7fffffffu) <= SCALE_TOP_BITS)
+        note(v, m);
+      else
+        v = __int_as_float(0x7fffffff);
+    };
     if constexpr (ROWS) {
 #pragma unroll
-      for (int q = 0; q < MINE; ++q)
-        if (some && warp + WARPS * q < live) {
+      for (int g = 0; g < GROUPS; ++g)
+        if (entry_of(g) < live) {
 #pragma unroll
           for (int k = 0; k < VE; ++k) {
-            if (fits(u[q][k]))
-              note(u[q][k], m);
-            else
-              u[q][k] = __int_as_float(0x7fffffff);
+            again(u[2 * g][k], amax[0]);
+            again(u[ROWS ? 2 * g + 1 : 0][k], amax[1]);
           }
         }
-      amax[0] = ca < p.C ? m : 0u;
-      amax[1] = ca < p.C ? 0u : m;
     } else {
-      for (int at = tid; at < live * 2 * p.C; at += APPEND_THREADS) {
-        float& v = s_val[slot0 * 2 * p.C + at];
-        if (fits(v))
-          note(v, amax[at % (2 * p.C) < p.C ? 0 : 1]);
-        else
-          v = __int_as_float(0x7fffffff);
-      }
+      for (int at = tid; at < live * 2 * p.C; at += APPEND_THREADS)
+        again(s_val[slot0 * 2 * p.C + at], amax[at % (2 * p.C) < p.C ? 0 : 1]);
     }
     __syncthreads();  // s_red has been read
     largest();
   }
   float scale[2], inv[2];
-  bool grown[2];
+  bool grown[2] = {true, true};
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    scale[h] = power_of_two(scale_exponent(amax[h], SCALE_LEAST));
-    grown[h] = old[h] < scale[h];
-    if (!grown[h]) scale[h] = old[h];
-    inv[h] = 1.f / scale[h];
+    const int e = scale_exponent(amax[h], SCALE_LEAST);
+    scale[h] = power_of_two(e);
+    inv[h] = power_of_two(-e);
+    if (older && !(old[h] < scale[h])) {
+      grown[h] = false;
+      scale[h] = old[h];
+      inv[h] = 1.f / old[h];
+    }
   }
   if constexpr (ROWS) {
-    if (some) {
-      const float f = ca >= p.C ? inv[1] : inv[0];
 #pragma unroll
-      for (int q = 0; q < MINE; ++q)
-        if (warp + WARPS * q < live) {
+    for (int g = 0; g < GROUPS; ++g) {
+      const int i = entry_of(g);
+      if (i < live) {
+        uint8_t* to = rows + (slot0 + i) * p.psr + vec * VE;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float(&x)[VE] = u[ROWS ? 2 * g + h : 0];
           uint32_t out4[VE / 4];
 #pragma unroll
           for (int k = 0; k < VE; k += 4)
-            out4[k / 4] = pack_e4m3x4(u[q][k] * f, u[q][k + 1] * f, u[q][k + 2] * f, u[q][k + 3] * f);
-          uint8_t* to = rows + (slot0 + warp + WARPS * q) * p.psr + ca;
+            out4[k / 4] = pack_e4m3x4(x[k] * inv[h], x[k + 1] * inv[h], x[k + 2] * inv[h], x[k + 3] * inv[h]);
           if constexpr (VE == 8)
-            *reinterpret_cast<uint2*>(to) = make_uint2(out4[0], out4[VE / 4 - 1]);
+            *reinterpret_cast<uint2*>(to + h * p.C) = make_uint2(out4[0], out4[VE / 4 - 1]);
           else
-            *reinterpret_cast<uint32_t*>(to) = out4[0];
+            *reinterpret_cast<uint32_t*>(to + h * p.C) = out4[0];
         }
+      }
     }
   } else {
     const int quads = p.C / 2;

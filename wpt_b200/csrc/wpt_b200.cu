@@ -1929,6 +1929,8 @@ extern "C" int wpt_paged_append(const void* src, int f32, int64_t src_stride_b, 
   p.dims = dims;
   p.start = start;
   p.magnitude = magnitude;
+  p.vecs = C / ve;
+  p.inv_vecs = 65536 / p.vecs + 1;
   p.turn_rows = dims > 0 ? wpt::APPEND_THREADS / (dims / 2) : 0;
   p.turn_pairs = dims > 0 ? wpt::APPEND_THREADS % (dims / 2) : 0;
   p.blocks = (n - 1) / wpt::PAGE_BLOCK + 2;  // n entries reach into that many blocks at most
