@@ -384,7 +384,7 @@ class _Rotate(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, d_out):
-        turn = _Rotate.apply if _needs_grad(d_out) else ops.rotate  # a gradient to be differentiated again
+        turn = _Rotate.apply if d_out.requires_grad else ops.rotate  # a gradient to be differentiated again
         return turn(d_out, *ctx.saved_tensors, *ctx.how), None, None, None, None, None, None
 
 
@@ -397,7 +397,7 @@ def rotate(x, positions, frequencies, start=None, interleaved=False, magnitude=1
     copied. A pair is channels i and i + dims / 2 of them, or 2 i and 2 i + 1
     (interleaved). Angles are exact at far positions. Differentiable in x;
     returns a new tensor in x's dtype."""
-    if not _needs_grad(x):
+    if not (x.requires_grad and torch.is_grad_enabled()):
         return ops.rotate(x, positions, frequencies, start, interleaved, magnitude)
     return _Rotate.apply(x, positions, frequencies, start, interleaved, magnitude, False)
 
