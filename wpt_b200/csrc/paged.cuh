@@ -814,15 +814,10 @@ __global__ void __launch_bounds__(PAGED_THREADS, 2)
   // no more runs than tiles, so that every CTA from a group's first to its last has a part of it
   const int parts = balanced ? max(1, min(static_cast<int>(gridDim.x), all)) : p.splits;
   const int part_of = balanced ? min(static_cast<int>(blockIdx.x), parts) : blockIdx.y;
-  const int begin = static_cast<int>(static_cast<int64_t>(all) * part_of / parts);
-  const int end = part_of < parts ? static_cast<int>(static_cast<int64_t>(all) * (part_of + 1) / parts) : begin;
-  if (balanced && blockIdx.x == 0 && static_cast<int>(threadIdx.x) < gcount) {
-    // parts of group g: from the CTA whose run holds its first tile to the one that holds its last
-    const int before = upto - count + aside;
-    auto holder = [&](int64_t tile) { return static_cast<int>(((tile + 1) * parts + all - 1) / all) - 1; };
-    p.info[threadIdx.x] = count == 0 ? make_int2(0, 0)
-                                     : make_int2(holder(before) + threadIdx.x, holder(upto - 1) - holder(before) + 1);
-  }
+  // (all * part_of / parts without 64 bits: parts are under 2^16)
+  const unsigned share = static_cast<unsigned>(all) / parts, rest = all - share * parts;
+  const int begin = share * part_of + rest * part_of / parts;
+  const int end = part_of < parts ? share * (part_of + 1) + rest * (part_of + 1) / parts : begin;
   __syncthreads();
   const uint32_t tmem = *s_tmem;
   griddep_launch();
@@ -851,6 +846,16 @@ __global__ void __launch_bounds__(PAGED_THREADS, 2)
   };
   Segments sg{s_before, s_first, aside, begin, end, 0, 0, 0, false};
 
+  if (balanced && blockIdx.x == 0 && warp == 7) {
+    // parts of group g, for the merge: from the CTA whose run holds its first tile to the one that holds its last
+    auto holder = [&](int64_t tile) { return static_cast<int>(((tile + 1) * parts + all - 1) / all) - 1; };
+#pragma unroll 1
+    for (int g = lane; g < gcount; g += 32) {
+      const int before = s_before[g], last = s_before[g + 1];
+      const int from = last > before ? holder(before + aside) : 0;
+      p.info[g] = last > before ? make_int2(from + g, holder(last - 1) - from + 1) : make_int2(0, 0);
+    }
+  }
   if (begin == end) {  // nothing to read (a cluster's share of that is merged below)
     if (p.splits == 1) {
       const PagedGroup group(p, gbase);

@@ -1976,7 +1976,7 @@ extern "C" int wpt_paged_attention(const void* q, const void* pages, int64_t pag
   if (splits == 0) {
     if (!scratch || ctas < 1) return fail(WPT_ERR_INVALID, "a balanced call needs scratch and CTAs");
     if (groups > wpt::PAGED_GROUPS || groups * ((static_cast<int64_t>(M) * S + 127) / 128 + wpt::PAGED_SEGMENT) >= (int64_t(1) << 31) ||
-        ctas > (1 << 20))
+        ctas >= (1 << 16))
       return fail(WPT_ERR_UNSUPPORTED, "a balanced call takes up to %d query groups (got %lld) and 2^31 tiles",
                   wpt::PAGED_GROUPS, static_cast<long long>(groups));
   }
