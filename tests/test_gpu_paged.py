@@ -94,6 +94,12 @@ APPENDS = [
     (2, 20, 32, 2, 112, 28, False, torch.bfloat16),  # vectors of 2
     (2, 20, 32, 2, 224, 46, True, torch.bfloat16),
     (2, 20, 32, 2, 48, 36, False, torch.float32),
+    (2, 40, 32, 2, 144, 64, False, torch.bfloat16),  # more than 16 vectors a key
+    (2, 40, 32, 2, 256, 256, True, torch.bfloat16),
+    (3, 21, 16, 3, 128, 64, False, torch.float32),
+    (1, 40, 32, 2, 304, 64, False, torch.bfloat16),  # more than 32
+    (5, 19, 64, 1, 16, 16, False, torch.bfloat16),   # 2: all entries of a warp at a time
+    (2, 19, 64, 1, 80, 0, False, torch.bfloat16),    # 10: three, then one
     (5, 0, 16, 2, 128, 64, False, torch.bfloat16),
 ]
 

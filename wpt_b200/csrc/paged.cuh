@@ -140,8 +140,8 @@ constexpr int APPEND_THREADS = 128;
 // 4,096, 2 x 128, all key channels turned: 23 us for 50 MB) are bound by issue
 // slots, a third of them for angles; a step of one entry a row (2.8 us) is a
 // chain of three loads (first, the page's number, its scale).
-template <class T, int VE, bool INTERLEAVED, bool ROWS>
-__global__ void __launch_bounds__(APPEND_THREADS, ROWS ? 8 : 1) paged_append_kernel(const AppendParams p) {
+template <class T, int VE, bool INTERLEAVED, int ROWS>
+__global__ void __launch_bounds__(APPEND_THREADS, ROWS == 2 ? 8 : ROWS == 4 ? 4 : 1) paged_append_kernel(const AppendParams p) {
   using V = Vec<T, VE>;
   using Raw = typename V::Raw;
   constexpr int WARPS = APPEND_THREADS / 32;
@@ -172,8 +172,8 @@ __global__ void __launch_bounds__(APPEND_THREADS, ROWS ? 8 : 1) paged_append_ker
   const int64_t row0 = lo - first;  // the first new entry's number
   const T* src = static_cast<const T*>(p.src) + b * p.ssb + row0 * p.ssn;
   const int half = p.dims >> 1;
-  // ROWS: a warp has 4 entries, 32 / vecs of them at a time, first their keys, then their values
-  constexpr int MINE = PAGE_BLOCK / WARPS, GROUPS = 2;
+  // ROWS: a warp has 4 entries, 32 / vecs of them at a time (a group; up to ROWS), first their keys, then their values
+  constexpr int MINE = PAGE_BLOCK / WARPS, GROUPS = ROWS > 0 ? ROWS : 1;
   const int sub = lane * p.inv_vecs >> 16, vec = lane - sub * p.vecs, each = (32 * p.inv_vecs) >> 16;
   auto entry_of = [&](int g) {  // this lane's of group g, `live` or more: none
     const int e = g * each + sub;
