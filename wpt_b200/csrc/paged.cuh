@@ -519,7 +519,7 @@ struct PagedLayout {
   static constexpr int OFF_QHI = OFF_QLO + 32 * 4;
   static constexpr int OFF_TILES = OFF_QHI + 32 * 4;         // groups: tiles before each, and the first tile
   static constexpr int OFF_BAR = OFF_TILES + (2 * PAGED_GROUPS + 2) * 4;
-  static constexpr int NBAR = 1 + 2 * NK + 2 * NV + 2 + 2 + 1;
+  static constexpr int NBAR = 1 + 2 * NK + 2 * NV + 2 + 2 + 1 + 1;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
   static constexpr int BYTES = OFF_MISC + 64 + 1024;
   static constexpr int S_COLS = 2 * NCOL, O_COLS = 3 * NCOL;
@@ -726,6 +726,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, 2)
   uint64_t* s_full = v_empty + NV;  // a tile's scores, and its scales
   uint64_t* p_ready = s_full + 2;
   uint64_t* o_done = p_ready + 2;
+  uint64_t* o_final = o_done + 1;   // a segment's last product has completed: a phase a segment
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC);
   int* s_any_nan = reinterpret_cast<int*>(smem + L::OFF_MISC + 4);
   int* s_sum = reinterpret_cast<int*>(smem + L::OFF_MISC + 8);  // 8 warps; later the largest |q| of four
@@ -761,6 +762,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, 2)
         mbar_init(p_ready + s, 128);
       }
       mbar_init(o_done, 1);
+      mbar_init(o_final, 1);
       fence_mbar_init();
       *s_any_nan = 0;
     }
@@ -997,6 +999,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, 2)
                         i > 1 ? 1u : 0u);
             mma_commit(v_empty + st);
             mma_commit(o_done);
+            if (i == sg.n) mma_commit(o_final);
           }
           __syncwarp();
         }
@@ -1025,7 +1028,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, 2)
     };
     if (more) load_ahead();
     bool ok = true;
-    int j = 0;
+    int j = 0, nseg = 0;
 #pragma unroll 1
     while (ok && more) {
       sg = nx;
@@ -1254,6 +1257,8 @@ __global__ void __launch_bounds__(PAGED_THREADS, 2)
 #pragma unroll
           for (int k = 0; k < NCOL / 2; ++k) lp[k] = f2_mul(lp[k], two(s_alpha, k));
           if (i > 0) {
+            // (its parity tells the product before this tile's from the one before that, which is complete: this tile's
+            // scores were issued after it)
             ok = __all_sync(0xffffffffu, mbar_wait(o_done, (j - 1) & 1, p.status));
             if (ok) {
               tc_fence_after();
@@ -1350,7 +1355,11 @@ __global__ void __launch_bounds__(PAGED_THREADS, 2)
       }
       more = nx.next();
       if (more) load_ahead();
-      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(o_done, (j - 1) & 1, p.status));
+      // o_done's parity cannot name the last product here: the last tile's scores vouch for the products up to two tiles
+      // before it, whose phase has the same parity, and the two after may still wait for their values. o_final completes
+      // once a segment, and every one of its phases is waited for.
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(o_final, nseg & 1, p.status));
+      ++nseg;
       tc_fence_after();
       // per-column sums over the 128 keys
       {
