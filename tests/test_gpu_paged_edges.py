@@ -2,10 +2,12 @@
 against oracle/paged.py in float64. Its tolerances and checks are used where a
 test says nothing else."""
 
+import math
+
 import pytest
 import torch
 
-from test_gpu_paged import _cache, _check_attention, _filled, _queries, wb  # noqa: F401
+from test_gpu_paged import SCORE, _cache, _check_attention, _filled, _queries, wb  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -24,4 +26,65 @@ def test_results_wait_for_a_segments_last_product(wb, tiles, monkeypatch):  # no
     for _ in range(30):
         again = wb.paged_attention(*dev, 128 ** -0.5)
         assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
+    assert wb.device_status() == 0
+
+
+def _dominated(N, at, share, deviation, g, H=8, S=64):
+    """A row of N entries of which those at `at` take `share` of each head's weight while their values are 0, as a
+    text's first tokens may: (q (1, 1, H, 128), pages, scales, out and log-sum in 64 bits, sum w|v|). Half of the
+    channels' values are positive, so that a weight that is lost shows in full. All on the GPU."""
+    k, v = (torch.randn(N, 128, generator=g).cuda() for _ in range(2))
+    v[:, ::2] = v[:, ::2].abs()
+    k[:, 0] = 0
+    k[at] = 0
+    k[at, 0], v[at] = 8.0, 0.0
+    held, scales = [], []
+    for x in (k, v):
+        top = x.view(-1, 16 * 128).abs().amax(1)
+        s = torch.exp2(torch.ceil(torch.log2(top.double() / 448))).float()
+        held.append((x.view(-1, 16, 128) / s[:, None, None]).to(torch.float8_e4m3fn).view(N, 128))
+        scales.append(s)
+    keys, values = (h.double() * s.double().repeat_interleave(16)[:, None] for h, s in zip(held, scales))
+    q = (torch.randn(1, 1, H, 128, generator=g) * deviation).cuda()
+    q[..., 0] = 0
+    q = q.bfloat16()
+    rest = torch.logsumexp(q[0, 0].double() @ keys.t() * 128 ** -0.5, 1)
+    q[0, 0, :, 0] = ((rest + math.log(share / (1 - share) / len(at))) * 128 ** 0.5 / 8).bfloat16()
+    z = q[0, 0].double() @ keys.t() * 128 ** -0.5
+    lse = torch.logsumexp(z, 1)
+    w = torch.exp(z - lse[:, None])
+    assert (w[:, at].sum(1) > share - 0.1 * (1 - share) ** 0.5).all()
+    pages = torch.cat([h.view(torch.uint8) for h in held], 1).view(N // S, S, 256).view(torch.float8_e4m3fn)
+    return q, pages, torch.stack(scales, 1).view(N // S, S // 16, 2), w @ values, lse, w @ values.abs()
+
+
+def _check_dominated(got, ref, lse, around):
+    """As near as weights and results in bf16 are: nothing here grows with the row."""
+    out = got[0].double()
+    assert ((out - ref).abs() <= 2.0 ** -8 * ref.abs() + (2.0 ** -8.6 + 2 * SCORE) * around).all()
+    # a scale of the whole result is seen much finer: by the weights' mean error, here under 2^-10
+    some = around[:, ::2] > 0
+    kept = (out[:, ::2][some].sum() / ref[:, ::2][some].sum()).item()
+    assert abs(kept - 1) <= 2.0 ** -10 + 2 * SCORE, kept
+    assert ((got[1].double() - lse).abs() <= SCORE + 2.0 ** -22 * lse.abs()).all()
+
+
+@pytest.mark.parametrize("at", [[0], [5], [0, 1, 2, 3], [77], [127, 128], [20000]])
+@pytest.mark.parametrize("N,deviation,share", [(2048, 1.0, 0.98), (32768, 1.0, 0.98), (32768, 2.0, 0.98), (32768, 2.0, 0.999),
+                                               (131072, 1.0, 0.98), (262144, 2.0, 0.98)])
+def test_keys_that_take_nearly_all_of_the_weight(wb, N, deviation, share, at):  # noqa: F811
+    """Their rows' other weights keep their precision, in runs of whole rows (more than 256 groups), of clusters and in
+    balanced ones."""
+    if at[0] >= N:
+        pytest.skip("past the row")
+    g = torch.Generator().manual_seed(31)
+    q, pages, scales, ref, lse, around = _dominated(N, at, share, deviation, g)
+    table = torch.randperm(N // 64, generator=g).cuda()
+    pages, scales = pages[torch.argsort(table)], scales[torch.argsort(table)]
+    for rows in (1, 6, 260):
+        got = wb.paged_attention(q.expand(rows, -1, -1, -1), pages, scales, table.int().expand(rows, -1),
+                                 torch.tensor([N - 1]).cuda(), 128 ** -0.5)
+        assert (got[0] == got[0][:1]).all() and (got[1] == got[1][:1]).all() or rows == 6  # (balanced runs differ)
+        for b in (0, rows - 1):
+            _check_dominated((got[0][b, 0], got[1][b, 0]), ref, lse, around)
     assert wb.device_status() == 0

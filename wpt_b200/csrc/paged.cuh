@@ -433,11 +433,20 @@ __global__ void __launch_bounds__(APPEND_THREADS, ROWS == 2 ? 8 : ROWS == 4 ? 4 
 //   its own, and a tile's scores are multiplied by them where they lie.
 //   a weight w = 2^x, as fp16 (11 significant bits) 3 e5m2 numbers, each the
 //   upper byte (e5m2 is fp16's) of what the ones before it leave, the last one
-//   times 32 and rounded: within 2^-8.6 w (2^-9, and fp16's 2^-11; a bf16
-//   weight's is 2^-8), and 2^-22 where w is small. 1 is the largest weight of
-//   the keys that set a column's base (32 or more of the first tile), 2^15 the
-//   largest that fits: a column is rescaled when a score passes its base by 15
-//   (base 2), and a run of n keys may lose n 2^-22 of its largest weight.
+//   times 32 and rounded to nearest: within 2^-8.6 w (2^-9, and fp16's 2^-11; a
+//   bf16 weight's is 2^-8), and 2^-22 where w is small. 2^15 is the largest
+//   weight that fits. So what 2^-22 is worth hangs on a column's base, the
+//   exponent that stands for a weight of 1, and a key that takes nearly all of
+//   the weight (while its value may be next to nothing) must not set it:
+//     the first base is the maximum over 32 keys of the first tile, but not more
+//     than 8 (base 2) above the least of the maxima over each eight of them;
+//     a score 15 above its base raises it, to 12 below that score.
+//   A weight under 2^-34 of that of a key that raised the base, or under 2^-14 of
+//   the largest of such eight keys, adds nothing to O (all add to the sum). With
+//   bases at the maxima themselves, one key of 0.98 of the weight whose value is 0
+//   and 32,768 or 262,144 others in one run: off by 20% and 73% of the result;
+//   with these 0.18% (the result's own rounding) and 0.21%. Price: 64 rows 59.4
+//   us (59.1), scores of four times the deviation 125 (107).
 // Scales. A key's scale multiplies its score. A value's scale 2^lv joins the
 // exponent, w = 2^(s + lv - m), m the running maximum of s + lv, so O needs no
 // scaling; the softmax's sum takes w 2^-lv. Sums, maxima and accumulators are
@@ -489,7 +498,9 @@ struct PagedParams {
   float scale_log2;
 };
 
-constexpr float PAGED_TOP = 15.f;  // weights up to 2^15 (fp16 ends at 2^16)
+constexpr float PAGED_TOP = 15.f;    // weights up to 2^15 (fp16 ends at 2^16)
+constexpr float PAGED_LIFT = 12.f;   // how far a raised base stays below the score that raised it
+constexpr float PAGED_APART = 8.f;   // and a first one at most above the least of four maxima
 constexpr uint32_t PAGED_EVEN = 6u << 23;  // 2^6 between columns' largest values, up to which they share a power of two
 // Minus the base of a column that has read nothing: any score is past it.
 constexpr float PAGED_UNSET = 1e30f;
@@ -597,15 +608,17 @@ __device__ __forceinline__ int ordered(float x) {
   return i ^ ((i >> 31) & 0x7fffffff);
 }
 __device__ __forceinline__ float unordered(int i) { return __int_as_float(i ^ ((i >> 31) & 0x7fffffff)); }
-__device__ __forceinline__ float warp_max(float x) {  // NaN ignored
-  float r;
-  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
-  return r;
-}
 __device__ __forceinline__ uint32_t half2_times32(uint32_t h) {
   uint32_t r;
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(h), "r"(0x50005000u));
   return r;
+}
+// two fp16 pairs as four e5m2, to nearest even
+__device__ __forceinline__ uint32_t pack_e5m2x4(uint32_t ab, uint32_t cd) {
+  uint16_t lo, hi;
+  asm("cvt.rn.satfinite.e5m2x2.f16x2 %0, %1;" : "=h"(lo) : "r"(ab));
+  asm("cvt.rn.satfinite.e5m2x2.f16x2 %0, %1;" : "=h"(hi) : "r"(cd));
+  return lo | (static_cast<uint32_t>(hi) << 16);
 }
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   uint32_t r;
@@ -1138,8 +1151,8 @@ __global__ void __launch_bounds__(PAGED_THREADS, 2)
         if (sc.w == 0.f) vis = 0u;
         // The maximum is lazy, as in the key-stream kernel: a column's base changes only when a score is PAGED_TOP past
         // it. A segment's first tile sets the bases: the warps with keys that all columns read share the columns, and
-        // set each to the maximum over their own 32 keys (no such key: to the tile's). A tile with a score past its
-        // column's bound is taken twice, that column's base being its maximum then. What is run once in a segment is
+        // set each by their own 32 keys (no such key: by the tile's). A tile with a score past its column's bound is
+        // taken twice, that column's base being PAGED_LIFT below its maximum then. What is run once in a segment is
         // kept short: such code is fetched anew each time. (A wait that failed is carried to the barriers, where all
         // warps agree to stop.)
         const uint32_t sa = lane_addr + (j & 1) * L::S_COLS;
@@ -1174,13 +1187,24 @@ __global__ void __launch_bounds__(PAGED_THREADS, 2)
             float m[8];
             const uint32_t sees = vis >> c;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) m[k] = warp_max((sees >> k) & 1u ? score(x[k], y[k]) : -INFINITY);
-            if (lane < 8) {
-              float mine = m[0];
+            for (int k = 0; k < 8; ++k) m[k] = (sees >> k) & 1u ? score(x[k], y[k]) : -INFINITY;
+            // the maximum over each eight lanes, column c + lane % 8's in m[0]; the largest and the least of the four
+            // (of those that read a key)
 #pragma unroll
-              for (int k = 1; k < 8; ++k) mine = lane == k ? m[k] : mine;
-              to[c + lane] = mine == -INFINITY ? PAGED_UNSET : -mine;
+            for (int step = 4; step > 0; step >>= 1)
+#pragma unroll
+              for (int k = 0; k < step; ++k) {
+                const bool up = (lane & step) != 0;
+                const float other = __shfl_xor_sync(0xffffffffu, up ? m[k] : m[k + step], step);
+                m[k] = fmaxf(up ? m[k + step] : m[k], other);
+              }
+            float most = m[0], least = m[0] == -INFINITY ? INFINITY : m[0];
+#pragma unroll
+            for (int step = 8; step < 32; step <<= 1) {
+              most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, step));
+              least = fminf(least, __shfl_xor_sync(0xffffffffu, least, step));
             }
+            if (lane < 8) to[c + lane] = most == -INFINITY ? PAGED_UNSET : -fminf(most, least + PAGED_APART);
           }
           if (!shared) {
             named_barrier(1, 128);
@@ -1246,7 +1270,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, 2)
           if (r < NCOL) {
             float a = 1.f;
             if (s_top[r] != INT_MIN) {
-              const float base = -unordered(s_top[r]);
+              const float base = PAGED_LIFT - unordered(s_top[r]);
               if (s_base[r] != PAGED_UNSET) a = fast_exp2(base - s_base[r]);  // else nothing was added up
               s_base[r] = base;
               s_top[r] = INT_MIN;
@@ -1339,7 +1363,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, 2)
               uint32_t x = h[c0 / 2 + 2 * k], y = h[c0 / 2 + 2 * k + 1];
 #pragma unroll
               for (int n = 0; n < 2; ++n) part[n][k] = __byte_perm(e5m2_part(x), e5m2_part(y), 0x7531);
-              part[2][k] = __byte_perm(half2_times32(x) + 0x00800080u, half2_times32(y) + 0x00800080u, 0x7531);
+              part[2][k] = pack_e5m2x4(half2_times32(x), half2_times32(y));
             }
 #pragma unroll
             for (int n = 0; n < 3; ++n) {
