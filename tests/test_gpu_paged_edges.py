@@ -88,3 +88,29 @@ def test_keys_that_take_nearly_all_of_the_weight(wb, N, deviation, share, at):  
         for b in (0, rows - 1):
             _check_dominated((got[0][b, 0], got[1][b, 0]), ref, lse, around)
     assert wb.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64, torch.bfloat16, torch.bool])
+def test_positions_that_are_not_whole_are_refused(wb, dtype):  # noqa: F811
+    """Cut off, a fractional position would be another one."""
+    pages, scales = wb.paged_cache(4, 32, 128)
+    table, at = torch.zeros(2, 3, dtype=torch.int32, device="cuda"), torch.zeros(2, 1, dtype=torch.int64, device="cuda")
+    q, new = torch.zeros(2, 1, 4, 128, device="cuda").bfloat16(), torch.ones(2, 1, 256, device="cuda")
+    f, one = wb.rotary_frequencies(64, device="cuda"), torch.ones(2, dtype=torch.int64, device="cuda")
+    for positions in (at, at[0], at[:, :0].expand(2, 0)):
+        x = q[:, :positions.shape[-1]]
+        assert wb.rotate(x, positions, f).shape == x.shape
+        with pytest.raises(ValueError, match="whole"):
+            wb.rotate(x, positions.to(dtype), f)
+    with pytest.raises(ValueError, match="whole"):
+        wb.paged_attention(q, pages, scales, table, at.to(dtype), 1.0)
+    with pytest.raises(ValueError, match="whole"):
+        wb.paged_attention(q, pages, scales, table, at[0].to(dtype), 1.0)
+    for bad in (dict(first=at[:, 0].to(dtype)), dict(counts=one.to(dtype)), dict(positions=at.to(dtype), frequencies=f)):
+        with pytest.raises(ValueError, match="whole"):
+            wb.paged_append(**(dict(pages=pages, scales=scales, table=table, new=new, first=at[:, 0], counts=one) | bad))
+    assert not pages.view(torch.uint8).any()
+    for small in (torch.int32, torch.uint8):  # whole numbers of other types are taken
+        assert torch.equal(wb.rotate(q, at.to(small), f), wb.rotate(q, at, f))
+        wb.paged_append(pages.clone(), scales.clone(), table, new, at[:, 0].to(small), one.to(small), f, at.to(small))
+    assert wb.device_status() == 0

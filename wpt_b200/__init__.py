@@ -391,7 +391,8 @@ class _Rotate(torch.autograd.Function):
 def rotate(x, positions, frequencies, start=None, interleaved=False, magnitude=1.0):
     """Rotary positions (attention.py:59, which turns the last 64 channels of a
     window layer's queries and keys): x (B, T, C) or (B, T, H, C), bf16 or fp32,
-    at positions (T,) or (B, T), with the pairs of the channels start .. start +
+    at whole positions (T,) or (B, T) (fractional ones go into the frequencies;
+    floating types are refused), with the pairs of the channels start .. start +
     dims - 1 of each head (default: the last ones; dims = 2 len(frequencies))
     turned by position * frequencies and multiplied by magnitude, the others
     copied. A pair is channels i and i + dims / 2 of them, or 2 i and 2 i + 1
@@ -418,7 +419,8 @@ def paged_append(pages, scales, table, new, first, counts, frequencies=None, pos
     """cache_append for a paged cache (cache.py:110-128), in place: row b's new
     entries new[b, :counts[b]] ((B, n, 2 C), bf16 or fp32) become its entries
     first[b] .., entry i being entry i % S of page table[b, i // S] (table
-    (B, M) int32 or int64, -1 for none; the pages written to are the row's own).
+    (B, M) int32 or int64, -1 for none; the pages written to are the row's own;
+    first, counts and positions are whole numbers, floating types are refused).
     With frequencies, the keys are turned on the way as rotate turns them, at
     positions (B, n) or, by default, at their places first[b] + i.
 
@@ -435,7 +437,7 @@ def paged_append(pages, scales, table, new, first, counts, frequencies=None, pos
 
 def paged_attention(q, pages, scales, table, positions, scale, window=0, sink=None):
     """forward_with_lse over the 8-bit paged cache: q (B, T, H, 128) bf16, up
-    to 64 heads, at positions (T,) or (B, T); query t of row b reads the row's
+    to 64 heads, at whole positions (T,) or (B, T); query t of row b reads the row's
     entries 0 .. position (given a window, the last `window` of them), with
     sink (H,) in each head's denominator. Entries on no page are not read, and
     what they and entries past the position hold reaches no result. Made for few

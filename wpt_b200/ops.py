@@ -830,6 +830,17 @@ def cache_reorder(tables, parents, lengths, first=None):
 PAGE_BLOCK = 16  # cached entries that share a scale
 
 
+def _whole(x, what):
+    """x (...) contiguous int64. Numbers of a type that is not whole are
+    refused: cut off, they would be other positions."""
+    dtype = x.dtype
+    if dtype is not torch.int64:
+        if dtype.is_floating_point or dtype.is_complex or dtype is torch.bool:
+            raise ValueError(f"{what} must be whole numbers; got {dtype}")
+        x = x.to(torch.int64)
+    return x if x.is_contiguous() else x.contiguous()
+
+
 def rotary_frequencies(dims, base=10000.0, scaling=None, factor=1.0, original=None, low=1.0, high=32.0, device=None):
     """(dims / 2,) float64 angles a position, base ** (-2 i / dims), for rotate
     and paged_append. For a context `factor` times as long as the `original` one:
@@ -899,7 +910,7 @@ def rotate(x, positions, frequencies, start=None, interleaved=False, magnitude=1
         raise NotImplementedError(f"x of {tuple(shape)}: past the library's 32-bit arguments")
     frequencies, dims, start = _frequencies(frequencies, C, start)
     if positions.dtype is not torch.int64 or positions.stride(-1) != 1:
-        positions = positions.to(torch.int64).contiguous()
+        positions = _whole(positions, "positions")
     if x.is_contiguous():
         y = torch.empty_like(x)
     else:
@@ -1001,8 +1012,8 @@ def paged_append(pages, scales, table, new, first, counts, frequencies=None, pos
     if (B | n) >> 31:
         raise NotImplementedError(f"entries {tuple(new.shape)}: past the library's 32-bit arguments")
     frequencies, dims, start = _frequencies(frequencies, C, start)
-    first, counts = _rows(first), _rows(counts)
-    positions = None if positions is None else _rows(positions)
+    first, counts = _whole(first, "first"), _whole(counts, "counts")
+    positions = None if positions is None else _whole(positions, "positions")
     table = _table_rows(table)
     if new.stride(2) != 1:
         new = new.contiguous()
@@ -1090,7 +1101,7 @@ def paged_attention(q, pages, scales, table, positions, scale, window=0, sink=No
     window = min(window, 2 ** 31 - 1)  # past every table
     if not q.is_contiguous() or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
-    positions = _rows(positions if len(at) == 2 and at[0] == B else positions.expand(B, -1))
+    positions = _whole(positions if len(at) == 2 and at[0] == B else positions.expand(B, -1), "positions")
     table = _table_rows(table)
     if sink is not None and (sink.dtype is not torch.float32 or not sink.is_contiguous()):
         sink = sink.float().contiguous()
