@@ -114,3 +114,30 @@ def test_positions_that_are_not_whole_are_refused(wb, dtype):  # noqa: F811
         assert torch.equal(wb.rotate(q, at.to(small), f), wb.rotate(q, at, f))
         wb.paged_append(pages.clone(), scales.clone(), table, new, at[:, 0].to(small), one.to(small), f, at.to(small))
     assert wb.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotation_in_forward_mode(wb, interleaved, dtype):  # noqa: F811
+    """A dual tensor's tangent is turned as its value is, leaf or not, and the tangent's gradient back."""
+    from torch.autograd import forward_ad
+
+    g = torch.Generator().manual_seed(32)
+    x, v, d = (torch.randn(2, 7, 3, 96, generator=g).to(dtype).cuda() for _ in range(3))
+    positions, f = torch.randint(0, 5000, (2, 7), generator=g).cuda(), wb.rotary_frequencies(48, device="cuda")
+    how = (positions, f, 16, interleaved, 0.75)
+    value, turned = wb.rotate(x, *how), wb.rotate(v, *how)
+    for leaf in (False, True):
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(x.clone().requires_grad_(leaf), v)
+            y = forward_ad.unpack_dual(wb.rotate(dual, *how))
+            assert torch.equal(y.primal, value) and torch.equal(y.tangent, turned)
+            plain = wb.rotate(x, *how)  # no tangent: none comes out
+            assert forward_ad.unpack_dual(plain).tangent is None and torch.equal(plain, value)
+            if leaf:
+                tangent = v.clone().requires_grad_()
+                y = forward_ad.unpack_dual(wb.rotate(forward_ad.make_dual(x, tangent), *how))
+                back, = torch.autograd.grad(y.tangent, tangent, d)
+                assert torch.equal(back, wb.ops.rotate(d, *how, inverse=True))
+    y = wb.rotate(x.requires_grad_(), *how)
+    assert torch.equal(torch.autograd.grad(y, x, d)[0], wb.ops.rotate(d, *how, inverse=True))

@@ -41,6 +41,7 @@ tensor-core kernels too, from the saved output and log-sum-exp.
 """
 
 import torch
+from torch.autograd import forward_ad
 
 from . import ops
 from ._lib import LibraryMissing, device_status  # noqa: F401
@@ -379,6 +380,8 @@ class _Rotate(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, positions, frequencies, start, interleaved, magnitude, inverse):
         ctx.save_for_backward(positions, frequencies)
+        if forward_ad._current_level >= 0:
+            ctx.save_for_forward(positions, frequencies)
         ctx.how = start, interleaved, magnitude, not inverse
         return ops.rotate(x, positions, frequencies, start, interleaved, magnitude, inverse)
 
@@ -386,6 +389,12 @@ class _Rotate(torch.autograd.Function):
     def backward(ctx, d_out):
         turn = _Rotate.apply if d_out.requires_grad else ops.rotate  # a gradient to be differentiated again
         return turn(d_out, *ctx.saved_tensors, *ctx.how), None, None, None, None, None, None
+
+    @staticmethod
+    def jvp(ctx, d_x, *_):
+        start, interleaved, magnitude, forward = ctx.how
+        turn = _Rotate.apply if d_x.requires_grad else ops.rotate
+        return turn(d_x, *ctx.saved_tensors, start, interleaved, magnitude, not forward)
 
 
 def rotate(x, positions, frequencies, start=None, interleaved=False, magnitude=1.0):
@@ -396,9 +405,9 @@ def rotate(x, positions, frequencies, start=None, interleaved=False, magnitude=1
     dims - 1 of each head (default: the last ones; dims = 2 len(frequencies))
     turned by position * frequencies and multiplied by magnitude, the others
     copied. A pair is channels i and i + dims / 2 of them, or 2 i and 2 i + 1
-    (interleaved). Angles are exact at far positions. Differentiable in x;
-    returns a new tensor in x's dtype."""
-    if not (x.requires_grad and torch.is_grad_enabled()):
+    (interleaved). Angles are exact at far positions. Differentiable in x, in
+    reverse and forward mode; returns a new tensor in x's dtype."""
+    if not (x.requires_grad and torch.is_grad_enabled()) and forward_ad._current_level < 0:
         return ops.rotate(x, positions, frequencies, start, interleaved, magnitude)
     return _Rotate.apply(x, positions, frequencies, start, interleaved, magnitude, False)
 
