@@ -7,7 +7,8 @@ import math
 import pytest
 import torch
 
-from test_gpu_paged import SCORE, _cache, _check_attention, _filled, _queries, wb  # noqa: F401
+from oracle import paged as op
+from test_gpu_paged import SCORE, _cache, _check_attention, _filled, _np, _queries, wb  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -141,3 +142,37 @@ def test_rotation_in_forward_mode(wb, interleaved, dtype):  # noqa: F811
                 assert torch.equal(back, wb.ops.rotate(d, *how, inverse=True))
     y = wb.rotate(x.requires_grad_(), *how)
     assert torch.equal(torch.autograd.grad(y, x, d)[0], wb.ops.rotate(d, *how, inverse=True))
+
+
+@pytest.mark.parametrize("size", [2.0 ** 28, 2.0 ** 33, 2.0 ** 60, 2.0 ** 104])
+@pytest.mark.parametrize("which", ["some", "all"])
+def test_queries_of_any_size(wb, which, size):  # noqa: F811
+    """Heads and drafts of very large queries, all of them or next to ordinary and to tiny ones: their scores are
+    finite, so all weight is the largest one's, and the others are as if alone."""
+    g = torch.Generator().manual_seed(33)
+    B, T, H, S, M = 2, 2, 8, 32, 12
+    pages, scales, table = _filled(B, M, S, 128, g)
+    q = _queries(B, T, H, g)
+    large = torch.full((B, T, H), which == "all")
+    large[0, 0, 3] = large[1, :, 5] = True
+    if which == "some":
+        q[0, 1, 0] = (q[0, 1, 0].float() * 2.0 ** -100).bfloat16()
+    q[large] = (q[large].float() * size).bfloat16()
+    positions = torch.full((B, 1), M * S - T) + torch.arange(T)
+    cache = _cache(pages, scales)
+    for window in (0, 200):
+        args = [t.cuda() for t in (pages, scales, table, positions)]
+        got = wb.paged_attention(q.cuda(), *args, 128 ** -0.5, window=window)
+        out, lse = got[0].float().cpu(), got[1].cpu()
+        ref, top = (torch.from_numpy(t) for t in op.attention(_np(q), cache, table.numpy(), positions.numpy(),
+                                                               128 ** -0.5, window))
+        assert out.isfinite().all() and lse.isfinite().all()
+        # one key's value, its weight held to 2^-8.6, and the result's rounding; its score to 128 truncations of 2^-23 of
+        # a sum that is 32 times it at most
+        assert ((out - ref)[large].abs() <= (2.0 ** -8.6 + 2.0 ** -8) * ref[large].abs()).all()
+        assert ((lse - top)[large].abs() <= 128 * 2.0 ** -23 * 32 * top[large].abs()).all()
+        plain = torch.where(large[..., None], 0, q).bfloat16()  # the others, with zeros in the large ones' place
+        zero = wb.paged_attention(plain.cuda(), *args, 128 ** -0.5, window=window)
+        out, lse = torch.where(large[..., None], zero[0].cpu().float(), out), torch.where(large, zero[1].cpu(), lse)
+        _check_attention((out, lse), plain, cache, table, positions, 128 ** -0.5, window)
+    assert wb.device_status() == 0

@@ -503,7 +503,7 @@ constexpr float PAGED_LIFT = 12.f;   // how far a raised base stays below the sc
 constexpr float PAGED_APART = 8.f;   // and a first one at most above the least of four maxima
 constexpr uint32_t PAGED_EVEN = 6u << 23;  // 2^6 between columns' largest values, up to which they share a power of two
 // Minus the base of a column that has read nothing: any score is past it.
-constexpr float PAGED_UNSET = 1e30f;
+constexpr float PAGED_UNSET = 3e38f;
 
 constexpr int PAGED_GROUPS = 256;  // of a balanced call, at most
 constexpr int PAGED_SEGMENT = 4;   // what a segment costs beside its tiles, in tiles
@@ -1217,7 +1217,8 @@ __global__ void __launch_bounds__(PAGED_THREADS, 2)
         bool stop = false;
 #pragma unroll 1
         for (int pass = 0;; ++pass) {
-          // the exponents s + lv - base
+          // the exponents s + lv - base, the scores rounded as where they set bases: else half a unit in the last place of
+          // a score of 2^28 is 2^4 and more of exponent
           if (pass != 0 || i == 0) {
 #pragma unroll
             for (int k = 0; k < NCOL / 2; ++k) nb[k] = two(s_base, k);
@@ -1232,7 +1233,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, 2)
               const int at = c0 / 2 + k;
               const uint64_t t = f2_fma(f2_pack(__uint_as_float(y[2 * k]), __uint_as_float(y[2 * k + 1])), low,
                                         f2_pack(__uint_as_float(x[2 * k]), __uint_as_float(x[2 * k + 1])));
-              e[at] = f2_fma(t, ks, f2_add(lv, nb[at]));
+              e[at] = f2_add(f2_fma(t, ks, lv), nb[at]);
             }
           }
           if (vis != ~0u) {
