@@ -144,7 +144,7 @@ def test_rotation_in_forward_mode(wb, interleaved, dtype):  # noqa: F811
     assert torch.equal(torch.autograd.grad(y, x, d)[0], wb.ops.rotate(d, *how, inverse=True))
 
 
-@pytest.mark.parametrize("size", [2.0 ** 28, 2.0 ** 33, 2.0 ** 60, 2.0 ** 104])
+@pytest.mark.parametrize("size", [2.0 ** 28, 2.0 ** 33, 2.0 ** 60, 2.0 ** 104, 2.0 ** 117, 2.0 ** 122])
 @pytest.mark.parametrize("which", ["some", "all"])
 def test_queries_of_any_size(wb, which, size):  # noqa: F811
     """Heads and drafts of very large queries, all of them or next to ordinary and to tiny ones: their scores are

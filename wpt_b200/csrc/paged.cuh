@@ -1105,7 +1105,10 @@ __global__ void __launch_bounds__(PAGED_THREADS, 2)
       }
       uneven = named_barrier_or(1, 128, uneven);  // s_qlo, s_qhi too; s_sum is read
       if (uneven) {
-        factor = p.scale_log2;
+        // (what is over 2^90 stays in the factor, where it meets the key's scale: 2^24 times a column's power of two may
+        // be past fp32 although the score is not)
+        const int high = max(0, e_q - 90);
+        factor = power_of_two(high) * p.scale_log2;
 #pragma unroll 1
         for (int col = warp; col < ncols; col += 4) {
           const uint2 raw = *reinterpret_cast<const uint2*>(p.q + (static_cast<int64_t>(group.row0) + col) * C + lane * 4);
@@ -1117,7 +1120,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, 2)
           }
           const int e_col = scale_exponent(__reduce_max_sync(0xffffffffu, top), -100);
           put_q(col, raw, power_of_two(-e_col));
-          if (lane == 0) s_power[col] = power_of_two(e_col);
+          if (lane == 0) s_power[col] = power_of_two(max(e_col - high, -126));
         }
         if (r >= ncols && r < NCOL) s_power[r] = 0.f;
         named_barrier(1, 128);
