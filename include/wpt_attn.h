@@ -386,9 +386,11 @@ int wpt_rotate(const void* x, int64_t x_stride_b, int64_t x_stride_t, int64_t x_
  * scales are the least powers of two, 2^-60 at least, that bring its values
  * within 448; a block with earlier entries of the row (before first[b]) keeps
  * a larger scale, and where its scale grows the earlier entries are rounded
- * again. Infinities and values past 448 * 2^60 are held as NaN. Entries
- * outside the table or on no page are not written and set the status word's
- * shape bit (bit 1). C a multiple of 16 up to 512.
+ * again. Entries after the new ones in their last block keep their bytes under
+ * a scale that may have changed: they are to be appended again. Infinities and
+ * values past 448 * 2^60 are held as NaN. Entries outside the table or on no
+ * page are not written and set the status word's shape bit (bit 1); with M or P
+ * 0 nothing is launched and none is set. C a multiple of 16 up to 512.
  */
 int wpt_paged_append(const void* src, int f32, int64_t src_stride_b, int64_t src_stride_n, void* pages,
                      int64_t page_stride, int64_t entry_stride, float* scales, int64_t scales_stride, const void* table,

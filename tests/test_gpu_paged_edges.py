@@ -8,7 +8,8 @@ import pytest
 import torch
 
 from oracle import paged as op
-from test_gpu_paged import SCORE, _cache, _check_attention, _filled, _np, _queries, wb  # noqa: F401
+from test_gpu_paged import (SCORE, _cache, _check_append, _check_attention, _filled, _np, _queries,  # noqa: F401
+                             wb)
 
 pytestmark = pytest.mark.gpu
 
@@ -176,3 +177,38 @@ def test_queries_of_any_size(wb, which, size):  # noqa: F811
         out, lse = torch.where(large[..., None], zero[0].cpu().float(), out), torch.where(large, zero[1].cpu(), lse)
         _check_attention((out, lse), plain, cache, table, positions, 128 ** -0.5, window)
     assert wb.device_status() == 0
+
+
+def test_what_an_append_reports(wb):  # noqa: F811
+    """The status word's shape bit for each way to miss the table, and none for calls that miss nothing; without any
+    page at all a call writes and reports nothing."""
+    g = torch.Generator().manual_seed(35)
+    pages, scales, _ = _filled(4, 2, 32, 32, g)
+    pages, scales = pages.cuda(), scales.cuda()
+    table = torch.tensor([[0, 1]], device="cuda")
+    new = torch.randn(1, 3, 64, generator=g).cuda()
+    for first, count, want in ((2 ** 62, 3, 2), (-2 ** 62, 3, 2), (64, 1, 2), (63, 2, 2), (61, 3, 0), (-3, 3, 2), (-3, 2 ** 62, 2),
+                               (-1, 2, 2), (0, 0, 0), (70, 0, 0), (0, -5, 0), (-9, -5, 0), (61, 2 ** 62, 0), (62, 2 ** 62, 2)):
+        wb.paged_append(pages.clone(), scales.clone(), table, new, torch.tensor([first]).cuda(), torch.tensor([count]).cuda())
+        assert wb.device_status() == want, (first, count)
+    one, at = torch.ones(1, dtype=torch.int64, device="cuda"), torch.zeros(1, dtype=torch.int64, device="cuda")
+    for missing in (-1, 10, 2 ** 40):
+        wb.paged_append(pages.clone(), scales.clone(), torch.tensor([[missing, 1]]).cuda(), new, at, one)
+        assert wb.device_status() == 2
+    wb.paged_append(pages[:0], scales[:0], table, new, at, one)
+    wb.paged_append(pages, scales, table[:, :0], new, at, one)
+    assert wb.device_status() == 0
+
+
+def test_entries_after_an_append_keep_their_bytes(wb):  # noqa: F811
+    """An append inside a text: what follows in its last block keeps its bytes, other blocks their scales too."""
+    g = torch.Generator().manual_seed(36)
+    pages, scales, table = _filled(1, 3, 32, 64, g)
+    new, first, counts = 50 * torch.randn(1, 20, 128, generator=g), torch.tensor([21]), torch.tensor([20])
+    cache = _cache(pages, scales)
+    got = wb.paged_append(*(t.cuda() for t in (pages, scales, table, new, first, counts)))
+    _check_append(got, cache, table, new, first, counts)
+    before, after = (t.view(torch.uint8)[table[0].long()].view(96, 128) for t in (pages, got[0].cpu()))
+    assert torch.equal(before[:16], after[:16]) and torch.equal(before[41:], after[41:])
+    changed = (scales[table[0].long()] != got[1].cpu()[table[0].long()]).view(6, 2).all(1)
+    assert changed.tolist() == [False, True, True, False, False, False]

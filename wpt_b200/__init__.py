@@ -436,10 +436,15 @@ def paged_append(pages, scales, table, new, first, counts, frequencies=None, pos
     A block's scales are the least powers of two that bring its values within
     e4m3's 448 (2^-60 at least); a block that already holds entries of the row
     before first[b] keeps its scale if that is larger, else its earlier
-    entries are rounded again to the new one. Infinities, and values past 448 *
-    2^60, are held as NaN. Entries outside the table or on no page are not
-    written (device_status's bit 1). One launch, no host synchronisation.
-    Returns (pages, scales). Not differentiable."""
+    entries are rounded again to the new one. The new entries are taken to be the
+    row's last: what follows them in their last block keeps its bytes under a
+    scale that may have changed, so it has to be appended again before it is read
+    (refused drafts are). A scale never shrinks while a block is continued, so a
+    refused draft of far larger values leaves its steps to the block. Infinities,
+    and values past 448 * 2^60, are held as NaN. Entries outside the table or on
+    no page are not written (device_status's bit 1; a table or a pool without any
+    page makes the call return at once, with no bit). One launch, no host
+    synchronisation. Returns (pages, scales). Not differentiable."""
     return ops.paged_append(pages, scales, table, new, first, counts, frequencies, positions, start, interleaved,
                             magnitude)
 

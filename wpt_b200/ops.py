@@ -991,8 +991,10 @@ def paged_append(pages, scales, table, new, first, counts, frequencies=None, pos
     rotate does, by positions (B, n) (default: their places first[b] + i). A
     block's scales become the least powers of two that hold its values; where it
     holds earlier entries of the row, not less than they were, and those are
-    rounded again where a scale grows. Places outside the table or on no page
-    (-1) are not written and set the status word's shape bit."""
+    rounded again where a scale grows. What follows the new entries in their last
+    block keeps its bytes, not its scale. Places outside the table or on no page
+    (-1) are not written and set the status word's shape bit (with no page at all
+    nothing is launched and it is not set)."""
     device = pages.device
     if not (pages.is_cuda and scales.device == device and table.device == device and new.device == device and
             first.device == device and counts.device == device and
