@@ -212,3 +212,29 @@ def test_entries_after_an_append_keep_their_bytes(wb):  # noqa: F811
     assert torch.equal(before[:16], after[:16]) and torch.equal(before[41:], after[41:])
     changed = (scales[table[0].long()] != got[1].cpu()[table[0].long()]).view(6, 2).all(1)
     assert changed.tolist() == [False, True, True, False, False, False]
+
+
+def test_unread_entries_without_a_window(wb):  # noqa: F811
+    """NaN in keys, values and scales of whatever no query reads, as recycled pages may hold: past the positions, in
+    rows that read nothing, behind a missing page, and on pages of no row."""
+    g = torch.Generator().manual_seed(34)
+    B, H, S, M = 5, 16, 32, 12
+    for T, at in ((1, [200, 0, -1, 383, 5000]), (3, [[200, 201, 202], [0, 1, 2], [-1, -1, 7], [90, 17, 383], [63, 64, -5]])):
+        pages, scales, table = _filled(B, M, S, 128, g)
+        positions = torch.tensor(at).view(B, T)
+        table[3, 2] = -1
+        clean = _cache(pages, scales)
+        read = torch.arange(M * S) <= positions.max(1).values[:, None]
+        mine = torch.zeros(pages.shape[0], S, dtype=torch.bool)
+        for b in range(B):
+            for i in range(M):
+                if table[b, i] >= 0:
+                    mine[table[b, i]] |= read[b, i * S:(i + 1) * S]
+        dirty, bad = pages.clone(), scales.clone()
+        dirty.view(torch.uint8)[~mine] = 0x7F
+        bad[~mine.view(-1, S // 16, 16).any(-1)] = math.nan
+        assert bad.isnan().any() and not bad.isnan().all()
+        q = _queries(B, T, H, g)
+        got = wb.paged_attention(*(t.cuda() for t in (q, dirty, bad, table, positions)), 128 ** -0.5)
+        _check_attention(got, q, clean, table, positions, 128 ** -0.5)
+    assert wb.device_status() == 0
