@@ -364,7 +364,8 @@ int wpt_cache_append(const void* src, int64_t src_stride_b, int64_t src_stride_n
  * channels i and i + dims / 2 of them, or with `interleaved` 2 i and 2 i + 1;
  * the others are copied. inverse: by -t (the gradient of x from that of y).
  *   frequencies  (dims / 2,) radians a position, fp64 with frequencies_f64,
- *                else fp32; finite. Angles are taken modulo a turn exactly.
+ *                else fp32; finite. A turn's multiples are taken off exactly:
+ *                an angle is off by 2^-52 |p f| + 2^-62 |p| + 2^-29 at most.
  */
 int wpt_rotate(const void* x, int64_t x_stride_b, int64_t x_stride_t, int64_t x_stride_h, const int64_t* positions,
                int64_t positions_stride_b, const void* frequencies, int frequencies_f64, void* y, int f32, int B, int T,

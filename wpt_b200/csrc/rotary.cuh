@@ -12,12 +12,15 @@
 // Angles. A position is whole, so p f in turns, modulo a turn, is a product
 // of whole numbers that wraps: f / (2 pi) as a fraction of 2^64 (turn_of), times
 // p, modulo 2^64 (turn_sincos). The product is exact at any position, where
-// p f in fp32 is off by 2^-24 p f radians (0.03 at a million); what is left
-// is the rounding of f / (2 pi) to double, 2^-53 p f. The nearest quarter turn is
-// taken off in whole numbers too, and sine and cosine of the rest, |x| <= pi /
-// 4, are their Taylor series: to x^9 and x^10, whose next terms are under
-// 1.8e-9 and 1.2e-10 there (the math library's function, made for any
-// argument, took five times the instructions).
+// p f in fp32 is off by 2^-24 p f radians (0.03 at a million). What is left, in
+// radians: 2^-52 p f, since f / (2 pi) is rounded to double twice (the constant
+// and the product); 2 pi 2^-65 p, since its fraction of a turn is rounded to
+// 2^-64 (2e-13 at a million positions, 2e-7 at 2^40: what grows for slow pairs);
+// and 2 pi 2^-32, of which the phase is cut. The nearest quarter turn is taken off
+// in whole numbers too, and sine and cosine of the rest, |x| <= pi / 4, are
+// their Taylor series: to x^9 and x^10, whose next terms are under 1.8e-9 and
+// 1.2e-10 there (the math library's function, made for any argument, took five
+// times the instructions).
 #pragma once
 
 #include <cstdint>
@@ -26,11 +29,13 @@
 
 namespace wpt {
 
-// A frequency (radians a position) in 2^-64 turns a position.
+// A frequency (radians a position) in 2^-64 turns a position. (By its size: 1
+// less a small number would keep 2^-54 of it.)
 __device__ __forceinline__ uint64_t turn_of(double f) {
-  double t = f * 0.15915494309189535;  // 1 / (2 pi)
+  double t = fabs(f) * 0.15915494309189535;  // 1 / (2 pi)
   t -= floor(t);
-  return __double2ull_rz(t * 18446744073709551616.0);
+  const uint64_t turn = __double2ull_rn(t * 18446744073709551616.0);
+  return f < 0.0 ? 0 - turn : turn;
 }
 
 // sin and cos of position p at `turn` 2^-64 turns a position.
