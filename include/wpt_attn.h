@@ -407,10 +407,10 @@ int wpt_paged_append(const void* src, int f32, int64_t src_stride_b, int64_t src
  * and sink as above. What other entries hold (NaN too) reaches no result.
  * Value scales are 0, or 2^-60 to 2^60 (where those of one row lie 2^112 and
  * more apart, weights under 2^-6 of small values may be lost).
- * Weights are within 2^-8.6 of their own down to 2^-25 of a run's largest;
- * what is under 2^-34 of it adds nothing to out (lse has it all), nor what is
- * under 2^-22 of it where four and more keys hold 2^-8 of it each: a run of n
- * keys may lose n 2^-22 of such keys' weight, whatever splits says.
+ * A weight in out is off by at most 2^-8.6 of itself or, where that is more, by
+ * 2^-21.8 of the largest of its run; by 2^-33.8 of it where that one alone stands
+ * 2^15 and more above the run's first keys (lse has all of it). A run of n keys
+ * may so lose n 2^-21.8 of the weight of keys that share the top.
  *   splits     how the work is split. 1 to 8: each query group's entries go to
  *              that many CTAs in equal runs, a thread-block cluster where more
  *              than one; ctas and scratch are not used. 0: all groups' entries

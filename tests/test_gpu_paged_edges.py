@@ -4,6 +4,7 @@ test says nothing else."""
 
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -238,3 +239,31 @@ def test_unread_entries_without_a_window(wb):  # noqa: F811
         got = wb.paged_attention(*(t.cuda() for t in (q, dirty, bad, table, positions)), 128 ** -0.5)
         _check_attention(got, q, clean, table, positions, 128 ** -0.5)
     assert wb.device_status() == 0
+
+
+@pytest.mark.parametrize("H", [1, 16, 32])
+def test_each_weight(wb, H):  # noqa: F811
+    """Key i's value is 1 in channel i and 0 elsewhere, so the result is the weights themselves, from the largest (some
+    keys near it in each eight of the first 32, so that it sets the base) down to 2^-28 of it."""
+    g = torch.Generator().manual_seed(37)
+    S, M, C = 32, 4, 128
+    pages = torch.zeros(M, S, 2 * C)
+    pages[:, :, 0] = 14 * torch.rand(M, S, generator=g)  # scores, in units of q's: weights down to e^-14 q
+    pages[0, 0, 0], pages[0, 4::8, 0] = 14.0, 13.0
+    for i in range(C):
+        pages[i // S, i % S, C + i] = 1.0
+    pages = pages.to(torch.float8_e4m3fn)
+    scales, table = torch.ones(M, S // 16, 2), torch.arange(M).int()[None]
+    q = torch.zeros(1, 1, H, C)
+    q[..., 0] = 128 ** 0.5 * torch.linspace(0.7, 1.4, H)
+    q, positions = q.bfloat16(), torch.tensor([[C - 1]])
+    out, _ = wb.paged_attention(*(t.cuda() for t in (q, pages, scales, table, positions)), 128 ** -0.5)
+    z = (_np(q)[0, 0, :, :1] * _np(pages)[:, :, 0].reshape(1, C)) * 128 ** -0.5
+    w = np.exp(z - z.max(1, keepdims=True))
+    total = w.sum(1, keepdims=True)
+    # a score is one product of up to 20 and its exponent's roundings: 1e-5; the result's own rounding is half a step of
+    # bf16, which keeps 8 bits: torch.finfo(torch.bfloat16).eps / 2 = 2^-8
+    tol = np.maximum(2.0 ** -8.6 * w, 2.0 ** -21.8) / total
+    off = np.abs(_np(out)[0, 0] - w / total)
+    assert (off <= tol + (2.0 ** -8 + 1e-5) * (w / total + tol)).all(), (off / tol).max()
+    assert w.min() < 2.0 ** -14

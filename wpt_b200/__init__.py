@@ -457,10 +457,9 @@ def paged_attention(q, pages, scales, table, positions, scale, window=0, sink=No
     sink (H,) in each head's denominator. Entries on no page are not read, and
     what they and entries past the position hold reaches no result. Made for few
     queries a row (decode, drafts); any number is computed, 32 / H at a time.
-    Weights have a bfloat16's precision down to 2^-25 of the row's largest (keys
-    that take nearly all of it, as a text's first may, cost the others nothing);
-    under 2^-34 of it, or 2^-22 where several keys share the top, they add
-    nothing to out.
+    A weight in out is off by 2^-8.6 of itself or, where that is more, by 2^-21.8
+    of the row's largest; by 2^-33.8 of it where that one stands 2^15 and more
+    above the others (a text's first token, say, that takes nearly all of it).
     Returns (out (B, T, H, 128) bf16, lse (B, T, H) fp32); 0 and -inf (or the
     sink) for a query without entries. Not differentiable."""
     return ops.paged_attention(q, pages, scales, table, positions, scale, window, sink)

@@ -432,12 +432,13 @@ __global__ void __launch_bounds__(APPEND_THREADS, ROWS == 2 ? 8 : ROWS == 4 ? 4 
 //   padding query of anything next to it), each column has a power of two of
 //   its own, and a tile's scores are multiplied by them where they lie.
 //   a weight w = 2^x, as fp16 (11 significant bits) 3 e5m2 numbers, each the
-//   upper byte (e5m2 is fp16's) of what the ones before it leave, the last one
-//   times 32 and rounded to nearest: within 2^-8.6 w (2^-9, and fp16's 2^-11; a
-//   bf16 weight's is 2^-8), and 2^-22 where w is small. 2^15 is the largest
-//   weight that fits. So what 2^-22 is worth hangs on a column's base, the
-//   exponent that stands for a weight of 1, and a key that takes nearly all of
-//   the weight (while its value may be next to nothing) must not set it:
+//   upper byte (e5m2 is fp16's) of what the ones before it leave, the second times
+//   4 and the last times 32 and rounded to nearest: within 2^-8.6 w (2^-9, and
+//   fp16's 2^-11; a bf16 weight's is 2^-8), or 2^-21.8 where w is under 2^-13 (2^-20
+//   were the second part not enlarged: under 2^-16 it would hold nothing). 2^15
+//   is the largest weight that fits. So what 2^-22 is worth hangs on a column's
+//   base, the exponent that stands for a weight of 1, and a key that takes nearly
+//   all of the weight (while its value may be next to nothing) must not set it:
 //     the first base is the maximum over 32 keys of the first tile, but not more
 //     than 8 (base 2) above the least of the maxima over each eight of them;
 //     a score 15 above its base raises it, to 12 below that score.
@@ -445,8 +446,8 @@ __global__ void __launch_bounds__(APPEND_THREADS, ROWS == 2 ? 8 : ROWS == 4 ? 4 
 //   the largest of such eight keys, adds nothing to O (all add to the sum). With
 //   bases at the maxima themselves, one key of 0.98 of the weight whose value is 0
 //   and 32,768 or 262,144 others in one run: off by 20% and 73% of the result;
-//   with these 0.18% (the result's own rounding) and 0.21%. Price: 64 rows 59.4
-//   us (59.1), scores of four times the deviation 125 (107).
+//   with these 0.18% (the result's own rounding) and 0.21%. Price: 64 rows 59.7
+//   us (59.1), scores of four times the deviation 126 (107).
 // Scales. A key's scale multiplies its score. A value's scale 2^lv joins the
 // exponent, w = 2^(s + lv - m), m the running maximum of s + lv, so O needs no
 // scaling; the softmax's sum takes w 2^-lv. Sums, maxima and accumulators are
@@ -608,9 +609,10 @@ __device__ __forceinline__ int ordered(float x) {
   return i ^ ((i >> 31) & 0x7fffffff);
 }
 __device__ __forceinline__ float unordered(int i) { return __int_as_float(i ^ ((i >> 31) & 0x7fffffff)); }
-__device__ __forceinline__ uint32_t half2_times32(uint32_t h) {
+template <uint32_t POWER>  // fp16: both halves times it
+__device__ __forceinline__ uint32_t half2_times(uint32_t h) {
   uint32_t r;
-  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(h), "r"(0x50005000u));
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(h), "r"(POWER * 0x10001u));
   return r;
 }
 // two fp16 pairs as four e5m2, to nearest even
@@ -1365,9 +1367,11 @@ __global__ void __launch_bounds__(PAGED_THREADS, 2)
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               uint32_t x = h[c0 / 2 + 2 * k], y = h[c0 / 2 + 2 * k + 1];
-#pragma unroll
-              for (int n = 0; n < 2; ++n) part[n][k] = __byte_perm(e5m2_part(x), e5m2_part(y), 0x7531);
-              part[2][k] = pack_e5m2x4(half2_times32(x), half2_times32(y));
+              part[0][k] = __byte_perm(e5m2_part(x), e5m2_part(y), 0x7531);
+              x = half2_times<0x4400>(x);  // 4
+              y = half2_times<0x4400>(y);
+              part[1][k] = __byte_perm(e5m2_part(x), e5m2_part(y), 0x7531);
+              part[2][k] = pack_e5m2x4(half2_times<0x4800>(x), half2_times<0x4800>(y));  // 8
             }
 #pragma unroll
             for (int n = 0; n < 3; ++n) {
@@ -1429,7 +1433,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, 2)
         float o[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          o[k] = __uint_as_float(x[k]) + fmaf(__uint_as_float(z[k]), 0.03125f, __uint_as_float(y[k]));
+          o[k] = fmaf(fmaf(__uint_as_float(z[k]), 0.125f, __uint_as_float(y[k])), 0.25f, __uint_as_float(x[k]));
         if (any_nan) {
 #pragma unroll
           for (int k = 0; k < 8; ++k)
