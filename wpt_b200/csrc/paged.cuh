@@ -466,11 +466,11 @@ __global__ void __launch_bounds__(APPEND_THREADS, ROWS == 2 ? 8 : ROWS == 4 ? 4 
 // Warps 0-3 prepare q, then take thread r = key r of a tile of 128 (as the
 // key-stream kernel's do); warp 4 issues products; warp 5 brings K and V by
 // TMA, a box for each page of a tile; warp 6 brings the scales. Two CTAs share
-// an SM (64 columns: one), so that one's exponents run under the other's loads.
+// an SM, so that one's exponents run under the other's loads.
 //
 // What bounds it: at 64 rows of 1,024 to 32,768 keys and 32 columns HBM and the
-// softmax warps' instructions about equally, 60 us for 278 MB (4.6 TB/s), of
-// which 5 are the merge; one row of 262,144 keys (26 us) and 7 rows of 5 drafts
+// softmax warps' instructions about equally, 61 us for 278 MB (4.5 TB/s), of
+// which 5 are the merge; one row of 262,144 keys (27 us) and 7 rows of 5 drafts
 // of 12 heads over up to 6,007 (16 us) are chains of latencies: the groups'
 // tiles, a page's number, its tile, the products, the parts, the merge. A
 // segment's fixed cost is code that is fetched anew for it (the kernel is larger
@@ -540,7 +540,7 @@ struct PagedLayout {
 
 constexpr int PAGED_THREADS = 256;
 // Registers: the softmax warps hold a column's score, sum, factor and base
-// each, the others little. 128 threads of 192 and 128 of 64 are the 256 of 128
+// each, the others little. 128 threads of 200 and 128 of 56 are the 256 of 128
 // that a block of two on an SM is launched with.
 constexpr int PAGED_REGS = 128, PAGED_REGS_SOFTMAX = 200, PAGED_REGS_OTHERS = 56;
 
